@@ -298,6 +298,25 @@ int mxa_rms_norm_q8_k(const float *x, const float *weight, float eps, int n_toke
 int mxa_silu_mul_q8_k(const float *gate, const float *up, long long ld, int n_tokens, int dim,
                       float *out, void *workspace, size_t workspace_bytes, void *stream);
 
+/* The residual stream between two blocks in one launch: with block output x and stream r,
+ *   u = x, or with post_weight x * post_weight / sqrt(mean(x^2) + post_eps)
+ *   hidden = r + scale * gate * u
+ *   out = hidden * weight / sqrt(mean(hidden^2) + eps), of hidden as it was stored
+ * over n_tokens rows of dim values (1 .. 32768), in float32, hidden and out each rounded once. x,
+ * post_weight, gate, weight and out are bfloat16 (bf16 != 0) or float32, residual and hidden bfloat16
+ * (residual_bf16 != 0, with bf16 only) or float32. Rows of x, residual and gate are ldx, ldr and ldg values
+ * apart (0: one row for all); gate is NULL, or has a value for each column (gate_step 1) or one for a row
+ * (gate_step 0); post_weight is NULL or dim values. hidden and out are contiguous and overlap no input.
+ * workspace: NULL, or (dim a multiple of 256) written with the Q8_K blocks of out, mxa_quantize_q8_k's
+ * layout. Pointers need their elements' alignment, the workspace 16 bytes.
+ * The steps around the block of the reference's decoder layers, whose norms are RMSNorm.forward
+ * (app/architectures/layers.py:72-81), and the next projections' quantization. */
+int mxa_add_rms_norm_q8_k(const void *x, long long ldx, const void *residual, long long ldr,
+                          const void *post_weight, float post_eps, const void *gate, long long ldg,
+                          int gate_step, float scale, const void *weight, float eps, int n_tokens,
+                          int dim, int bf16, int residual_bf16, void *hidden, void *out,
+                          void *workspace, size_t workspace_bytes, void *stream);
+
 /* Q8_K activation quantization of x (n_tokens, in_features) into the workspace layout
  * q int8 (n_tokens, K) | d fp32 (n_tokens, K/256) | bsums int16 (n_tokens, K/256, 16), each
  * part starting on a 256-byte boundary (see mxa_workspace_bytes).

@@ -36,6 +36,7 @@ EXPORTS = (
     "mxa_quantize_q8_k",
     "mxa_rms_norm_q8_k",
     "mxa_silu_mul_q8_k",
+    "mxa_add_rms_norm_q8_k",
     "mxa_dequantize",
     "mxa_dequant_rows",
     "mxa_embed_rows",
@@ -56,6 +57,7 @@ _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _sz = ctypes.c_size_t
 _ll = ctypes.c_longlong
+_f = ctypes.c_float
 
 _lib: ctypes.CDLL | None = None
 
@@ -133,6 +135,9 @@ def load() -> ctypes.CDLL:
     lib.mxa_silu_mul_q8_k_bf16.restype = _i
     lib.mxa_silu_mul_q8_k.argtypes = [_vp, _vp, _ll, _i, _i, _vp, _vp, _sz, _vp]
     lib.mxa_silu_mul_q8_k.restype = _i
+    lib.mxa_add_rms_norm_q8_k.argtypes = [_vp, _ll, _vp, _ll, _vp, _f, _vp, _ll, _i, _f, _vp, _f, _i, _i, _i, _i,
+                                          _vp, _vp, _vp, _sz, _vp]
+    lib.mxa_add_rms_norm_q8_k.restype = _i
     lib.mxa_dequantize.argtypes = [_i, _vp, _ll, _vp, _vp]
     lib.mxa_dequantize.restype = _i
     lib.mxa_dequant_rows.argtypes = [_i, _vp, _ll, _vp, _i, _i, _vp, _vp]

@@ -573,6 +573,31 @@ int mxa_silu_mul_q8_k_bf16(const void* gate, const void* up, long long ld, int n
   return check_launch();
 }
 
+int mxa_add_rms_norm_q8_k(const void* x, long long ldx, const void* residual, long long ldr,
+                          const void* post_weight, float post_eps, const void* gate, long long ldg,
+                          int gate_step, float scale, const void* weight, float eps, int n_tokens,
+                          int dim, int bf16, int residual_bf16, void* hidden, void* out,
+                          void* workspace, size_t workspace_bytes, void* stream) {
+  const uintptr_t xa = bf16 ? 2 : 4, ra = residual_bf16 ? 2 : 4;
+  if (x == nullptr || residual == nullptr || weight == nullptr || hidden == nullptr || out == nullptr ||
+      n_tokens <= 0 || dim <= 0 || ldx < 0 || ldr < 0 || ldg < 0 || (gate_step != 0 && gate_step != 1) ||
+      (residual_bf16 && !bf16) || !aligned(x, xa) || !aligned(weight, xa) || !aligned(post_weight, xa) ||
+      !aligned(gate, xa) || !aligned(out, xa) || !aligned(residual, ra) || !aligned(hidden, ra) ||
+      !aligned(workspace, 16))
+    return MXA_ERR_UNSUPPORTED;
+  mxa::ActBuffers a{};
+  if (workspace != nullptr) {
+    if (dim % mxa::QK != 0) return MXA_ERR_UNSUPPORTED;
+    if (workspace_bytes < mxa::act_bytes(n_tokens, dim)) return MXA_ERR_WORKSPACE;
+    a = mxa::act_layout(workspace, n_tokens, dim);
+  }
+  if (mxa::launch_add_rms_norm(x, ldx, residual, ldr, post_weight, post_eps, gate, ldg, gate_step, scale,
+                               weight, eps, bf16 != 0, residual_bf16 != 0, n_tokens, dim, hidden, out,
+                               workspace != nullptr ? &a : nullptr, (hipStream_t)stream) != 0)
+    return MXA_ERR_UNSUPPORTED;
+  return check_launch();
+}
+
 int mxa_dequantize(int ggml_type, const void* blocks, long long n_blocks, float* out,
                    void* stream) {
   if (!known_type(ggml_type) || blocks == nullptr || out == nullptr || n_blocks <= 0)

@@ -95,6 +95,16 @@ int launch_rms_norm_q8k_bf16(const uint16_t* x, const uint16_t* w, float eps, ui
 int launch_silu_mul_q8k_bf16(const uint16_t* gate, const uint16_t* up, long long ld, uint16_t* out,
                              const ActBuffers& a, int m_rows, int k, hipStream_t stream);
 
+// The residual stream between two blocks (mxa_norm.hip): h = r + scale * gate * u, u = x or its RMSNorm with
+// `post`, and n = RMSNorm of h with w, over rows of k <= kNormMaxValues values; x, post, gate, w and n bfloat16
+// (xbf16) or float32, r and h bfloat16 (rbf16, with xbf16 only) or float32; ldx, ldr, ldg row strides, gstep the
+// gate's column stride (0 or 1). q: n's Q8_K blocks (k a multiple of 256), or nullptr. -1 for other arguments.
+constexpr int kNormMaxValues = 32768;
+int launch_add_rms_norm(const void* x, long long ldx, const void* r, long long ldr, const void* post,
+                        float post_eps, const void* gate, long long ldg, int gstep, float scale, const void* w,
+                        float eps, bool xbf16, bool rbf16, int rows, int k, void* h, void* n,
+                        const ActBuffers* q, hipStream_t stream);
+
 // Reads bytes (a multiple of 16) at src once and discards them; may write one word to sink.
 void launch_stream_read(const void* src, long long bytes, uint32_t* sink, hipStream_t stream);
 

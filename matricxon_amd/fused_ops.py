@@ -11,6 +11,8 @@ weights on the GPU:
   reference runs for them (layers.py:53-57, 77-81), each elementwise result rounded to bfloat16
   where torch rounds it. Each also writes the Q8_K blocks of its result in the same kernel and
   hands them to the packed projections that read that result.
+* `HipFusedOps.add_rms_norm(residual, x, weight, eps, ...)`: the stream between two blocks, a block's output
+  (normed or not, gated, scaled) added and the sum normed for the next block, handed on the same way.
 * `project_shared(owner, names, x)`: `owner.<name>(x)` for each name, as one
   `mxa_gemm_multi` call when every module is a `DevicePackedLinear` over the same input (the
   device side of app/architectures/shared_projection.py:33-43).
@@ -83,6 +85,11 @@ def _handled(*tensors: torch.Tensor) -> bool:
         t.dtype == dt and t.device.type == "cuda" for t in tensors)
 
 
+def _broadcasts(shape: torch.Size, to: torch.Size) -> bool:
+    """Whether a tensor of `shape` expands to `to`."""
+    return len(shape) <= len(to) and all(a in (1, b) for a, b in zip(reversed(shape), reversed(to)))
+
+
 class HipFusedOps:
     """`FusedOps` (app/native/fused_ops.py:128-150) for GPU tensors: `configure` / `active`
     select it, and each method returns None for inputs it does not handle."""
@@ -112,6 +119,31 @@ class HipFusedOps:
             out = out.view(x.shape)
         HANDOFF.offer(out, ws)
         return out
+
+    def add_rms_norm(self, residual: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, eps: float, *,
+                     post_weight: torch.Tensor | None = None, post_eps: float | None = None,
+                     gate: torch.Tensor | None = None, scale: float = 1.0, q8k: bool = True
+                     ) -> tuple[torch.Tensor, torch.Tensor] | None:
+        """The residual stream between two blocks, one launch: (hidden, normed) with
+        hidden = residual + scale * gate * u, u = x or RMSNorm(x; post_weight, post_eps), and
+        normed = RMSNorm(hidden; weight, eps), whose Q8_K blocks the next projections claim (`q8k`, rows of whole
+        256-value blocks). `gate` broadcasts to x: one value, one a channel, one a token, or all. The stream may
+        be float32 beside a bfloat16 block; the weights and the gate have x's dtype, post_eps is eps unless given.
+        Float32 steps; hidden and normed are each rounded once (rms_norm's bfloat16 steps round twice, as torch's
+        do). None for what it does not take: CPU tensors, other dtypes or shapes, rows of more than 32768 values."""
+        k = x.shape[-1] if x.dim() else 0
+        others = [t for t in (weight, post_weight, gate) if t is not None]
+        if (not _handled(x, *others) or residual.dtype not in (torch.float32, x.dtype)
+                or residual.shape != x.shape or any(t.device != x.device for t in (residual, *others))
+                or not 1 <= k <= HipGemm.NORM_MAX_VALUES or x.numel() == 0
+                or any(w.shape != (k,) for w in (weight, post_weight) if w is not None)
+                or (gate is not None and not _broadcasts(gate.shape, x.shape))):
+            return None
+        hidden, out, ws = self._gemm.add_rms_norm_q8k(residual, x, weight, eps, post_weight, post_eps, gate, scale,
+                                                      q8k)
+        if ws is not None:
+            HANDOFF.offer(out, ws)
+        return hidden, out
 
     def silu_mul(self, gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor | None:
         """silu(gate) * up elementwise (layers.py:53-57)."""

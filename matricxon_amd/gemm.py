@@ -9,6 +9,7 @@ the packed weight is a device uint8 tensor instead of an mmap'd memoryview, x an
 device, and the call is asynchronous on torch's current HIP stream (no host sync).
 """
 
+import contextlib
 import ctypes
 import logging
 
@@ -34,6 +35,14 @@ def _stream(device: torch.device) -> int:
         return torch.cuda.current_stream(device).cuda_stream
     index = device.index
     return _RAW_STREAM(torch.cuda.current_device() if index is None else index)
+
+
+def _on(device: torch.device):
+    """A context in which `device` is the current one: a launch goes to the current device, whatever device its
+    tensors and its stream belong to. Nothing where it is already, as it mostly is."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 def _al256(n: int) -> int:
@@ -70,6 +79,12 @@ def _rows16(t: torch.Tensor, k: int) -> torch.Tensor:
     if t.is_contiguous() and t.data_ptr() % 16 == 0:
         return t
     return _aligned16(t.detach().reshape(-1, k).contiguous())
+
+
+def _rows_of(t: torch.Tensor, k: int) -> torch.Tensor:
+    """`t` (..., k) as (rows, k) with unit column stride: a view where its rows are evenly spaced."""
+    t2 = t.detach() if t.dim() == 2 else t.detach().reshape(-1, k)
+    return t2 if t2.stride(1) == 1 or k == 1 else t2.contiguous()
 
 
 def _weight_arrays(items: list[tuple[int, torch.Tensor, int]], outs: list[int]):
@@ -410,6 +425,58 @@ class HipGemm:
                                                   ws.data_ptr(), ws.numel(), _stream(x.device))
         self._check(status, "mxa_rms_norm_q8_k_bf16", 15)
         return out, ws
+
+    NORM_MAX_VALUES = 32768  # the longest row of add_rms_norm_q8k
+
+    def add_rms_norm_q8k(self, residual: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, eps: float,
+                         post_weight: torch.Tensor | None = None, post_eps: float | None = None,
+                         gate: torch.Tensor | None = None, scale: float = 1.0, want_q8k: bool = True
+                         ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+        """The residual stream between two blocks in one launch (`mxa_add_rms_norm_q8_k`): (hidden, out,
+        workspace) with hidden = residual + scale * gate * u, u = x or RMSNorm(x; post_weight, post_eps), in
+        residual's dtype, out = RMSNorm(hidden; weight, eps) in x's, and the workspace the Q8_K blocks of out
+        (None where they are not wanted or the rows are not whole blocks). x and residual (..., K), of float32 or
+        bfloat16 each, residual not narrower than x; weight and post_weight (K,) and gate, which broadcasts to x,
+        in x's dtype. K up to NORM_MAX_VALUES."""
+        _require_device_tensor("x", x)
+        dev, dt, k = x.device, x.dtype, x.shape[-1] if x.dim() else 0
+        if dt not in (torch.float32, torch.bfloat16) or residual.dtype not in (torch.float32, dt):
+            raise ValueError(f"x must be float32 or bfloat16 and residual float32 or x's dtype, got {dt} and "
+                             f"{residual.dtype}")
+        if not 1 <= k <= self.NORM_MAX_VALUES or residual.shape != x.shape or residual.device != dev:
+            raise ValueError(f"x and residual must be (..., K) on one device, K in 1..{self.NORM_MAX_VALUES}, got "
+                             f"{tuple(x.shape)} and {tuple(residual.shape)}")
+        for name, w in (("weight", weight), ("post_weight", post_weight)):
+            if w is not None and (w.shape != (k,) or w.dtype != dt or w.device != dev):
+                raise ValueError(f"{name} must be ({k},) {dt} on {dev}")
+        x2, r2 = _rows_of(x, k), _rows_of(residual, k)
+        weight = weight.contiguous()
+        post = None if post_weight is None else post_weight.contiguous()
+        g2, ldg, gstep = None, 0, 0
+        if gate is not None:
+            if gate.dtype != dt or gate.device != dev:
+                raise ValueError(f"gate must be {dt} on {dev}")
+            g2 = gate.expand(x.shape).reshape(-1, k)  # RuntimeError where it does not broadcast
+            if g2.stride(1) > 1 and k > 1:
+                g2 = g2.contiguous()
+            ldg, gstep = g2.stride(0), min(g2.stride(1), 1) if k > 1 else 0
+        m = x2.shape[0]
+        hidden = torch.empty(x.shape, dtype=residual.dtype, device=dev)
+        out = torch.empty(x.shape, dtype=dt, device=dev)
+        ws = None
+        if want_q8k and k % 256 == 0:
+            ws = torch.empty(q8k_bytes(m, k), dtype=torch.uint8, device=dev)
+        if m == 0:
+            return hidden, out, ws
+        with _on(dev):
+            status = self._lib.mxa_add_rms_norm_q8_k(
+                x2.data_ptr(), x2.stride(0), r2.data_ptr(), r2.stride(0), None if post is None else post.data_ptr(),
+                float(eps if post_eps is None else post_eps), None if g2 is None else g2.data_ptr(), ldg, gstep,
+                float(scale), weight.data_ptr(), float(eps), m, k, int(dt == torch.bfloat16),
+                int(residual.dtype == torch.bfloat16), hidden.data_ptr(), out.data_ptr(),
+                None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _stream(dev))
+        self._check(status, "mxa_add_rms_norm_q8_k", 15)
+        return hidden, out, ws
 
     def silu_mul_q8k(self, gate: torch.Tensor, up: torch.Tensor,
                      want_out: bool = True) -> tuple[torch.Tensor | None, torch.Tensor]:
