@@ -317,6 +317,25 @@ int mxa_add_rms_norm_q8_k(const void *x, long long ldx, const void *residual, lo
                           int dim, int bf16, int residual_bf16, void *hidden, void *out,
                           void *workspace, size_t workspace_bytes, void *stream);
 
+/* Rotary positions of q (q_heads heads) and k (k_heads; 0: k, k_strides and k_out are not read) in one launch.
+ * Token t (of n_tokens) is step t % seq_len of sequence t / seq_len; its row of head h starts at
+ * strides[0] * sequence + strides[1] * step + strides[2] * h elements (HOST arrays of 3), head_dim values in
+ * a row; the outputs are contiguous (n_tokens, heads, head_dim) and overlap no input. Of a head the first
+ * rotary_dim values turn: pair i, elements (i, i + rotary_dim / 2) or interleaved (2i, 2i + 1), by
+ * position * turns[i] full turns (DEVICE float64, rotary_dim / 2: the angle per position / 2 pi), times
+ * scale; the others are copied. The position of a token is positions[pos_batch * sequence + pos_token *
+ * step], DEVICE int32 or int64. Values float32 or bfloat16 (bf16 != 0), each rounded once from float32. Any
+ * position: the angle is reduced in float64. head_dim and rotary_dim even, head_dim <= MXA_ROPE_MAX_DIM.
+ * The reference's CPU libraries fuse the same step (app/native/src/mx_fused_ops.c); its GPU layers run it
+ * in torch operations. */
+#define MXA_ROPE_MAX_DIM 1024
+#define MXA_ROPE_MAX_HEADS 65536
+int mxa_rope(const void *q, const long long *q_strides, int q_heads, const void *k,
+             const long long *k_strides, int k_heads, const void *positions, int positions_int64,
+             long long pos_batch, long long pos_token, const double *turns, int n_tokens, int seq_len,
+             int head_dim, int rotary_dim, int interleaved, float scale, int bf16, void *q_out,
+             void *k_out, void *stream);
+
 /* Q8_K activation quantization of x (n_tokens, in_features) into the workspace layout
  * q int8 (n_tokens, K) | d fp32 (n_tokens, K/256) | bsums int16 (n_tokens, K/256, 16), each
  * part starting on a 256-byte boundary (see mxa_workspace_bytes).

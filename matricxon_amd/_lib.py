@@ -37,6 +37,7 @@ EXPORTS = (
     "mxa_rms_norm_q8_k",
     "mxa_silu_mul_q8_k",
     "mxa_add_rms_norm_q8_k",
+    "mxa_rope",
     "mxa_dequantize",
     "mxa_dequant_rows",
     "mxa_embed_rows",
@@ -138,6 +139,9 @@ def load() -> ctypes.CDLL:
     lib.mxa_add_rms_norm_q8_k.argtypes = [_vp, _ll, _vp, _ll, _vp, _f, _vp, _ll, _i, _f, _vp, _f, _i, _i, _i, _i,
                                           _vp, _vp, _vp, _sz, _vp]
     lib.mxa_add_rms_norm_q8_k.restype = _i
+    lib.mxa_rope.argtypes = [_vp, _vp, _i, _vp, _vp, _i, _vp, _i, _ll, _ll, _vp, _i, _i, _i, _i, _i, _f, _i, _vp, _vp,
+                             _vp]
+    lib.mxa_rope.restype = _i
     lib.mxa_dequantize.argtypes = [_i, _vp, _ll, _vp, _vp]
     lib.mxa_dequantize.restype = _i
     lib.mxa_dequant_rows.argtypes = [_i, _vp, _ll, _vp, _i, _i, _vp, _vp]

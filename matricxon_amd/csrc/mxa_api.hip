@@ -598,6 +598,26 @@ int mxa_add_rms_norm_q8_k(const void* x, long long ldx, const void* residual, lo
   return check_launch();
 }
 
+int mxa_rope(const void* q, const long long* q_strides, int q_heads, const void* k, const long long* k_strides,
+             int k_heads, const void* positions, int positions_int64, long long pos_batch, long long pos_token,
+             const double* turns, int n_tokens, int seq_len, int head_dim, int rotary_dim, int interleaved,
+             float scale, int bf16, void* q_out, void* k_out, void* stream) {
+  const uintptr_t ea = bf16 ? 2 : 4;
+  if (q == nullptr || q_strides == nullptr || q_out == nullptr || positions == nullptr || turns == nullptr ||
+      q_heads < 1 || k_heads < 0 || q_heads > MXA_ROPE_MAX_HEADS || k_heads > MXA_ROPE_MAX_HEADS ||
+      n_tokens < 1 || seq_len < 1 || head_dim < 2 || head_dim > MXA_ROPE_MAX_DIM || head_dim % 2 != 0 ||
+      rotary_dim < 2 || rotary_dim > head_dim || rotary_dim % 2 != 0 || !aligned(q, ea) || !aligned(q_out, ea) ||
+      !aligned(positions, positions_int64 ? 8 : 4) || !aligned(turns, 8))
+    return MXA_ERR_UNSUPPORTED;
+  if (k_heads > 0 && (k == nullptr || k_strides == nullptr || k_out == nullptr || !aligned(k, ea) || !aligned(k_out, ea)))
+    return MXA_ERR_UNSUPPORTED;
+  if (mxa::launch_rope(q, q_strides, q_heads, k, k_strides, k_heads, positions, positions_int64 != 0, pos_batch,
+                       pos_token, turns, n_tokens, seq_len, head_dim, rotary_dim, interleaved != 0, scale,
+                       bf16 != 0, q_out, k_out, (hipStream_t)stream) != 0)
+    return MXA_ERR_UNSUPPORTED;
+  return check_launch();
+}
+
 int mxa_dequantize(int ggml_type, const void* blocks, long long n_blocks, float* out,
                    void* stream) {
   if (!known_type(ggml_type) || blocks == nullptr || out == nullptr || n_blocks <= 0)

@@ -105,6 +105,14 @@ int launch_add_rms_norm(const void* x, long long ldx, const void* r, long long l
                         float eps, bool xbf16, bool rbf16, int rows, int k, void* h, void* n,
                         const ActBuffers* q, hipStream_t stream);
 
+// Rotary positions (mxa_rope.hip) of q and k (k_heads 0: q alone), rows of dim values at strides (batch, token,
+// head) in elements, to contiguous (token, head, dim) outputs; token t is step t % seq of sequence t / seq.
+// rot <= dim values of a head turn, pair i by pos * turns[i] full turns; rot and dim even.
+int launch_rope(const void* q, const long long* q_strides, int q_heads, const void* k, const long long* k_strides,
+                int k_heads, const void* pos, bool pos64, long long pos_batch, long long pos_tok,
+                const double* turns, int n_tokens, int seq, int dim, int rot, bool interleaved, float mscale,
+                bool bf16, void* q_out, void* k_out, hipStream_t stream);
+
 // Reads bytes (a multiple of 16) at src once and discards them; may write one word to sink.
 void launch_stream_read(const void* src, long long bytes, uint32_t* sink, hipStream_t stream);
 

@@ -478,6 +478,62 @@ class HipGemm:
         self._check(status, "mxa_add_rms_norm_q8_k", 15)
         return hidden, out, ws
 
+    ROPE_MAX_DIM = 1024
+    ROPE_MAX_HEADS = 65536
+
+    def rope(self, q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, turns: torch.Tensor,
+             rotary_dim: int, interleaved: bool, scale: float) -> tuple[torch.Tensor, torch.Tensor | None]:
+        """Rotary positions of q and k in one launch (`mxa_rope`), `turns` (rotary_dim / 2) float64 on their device;
+        `matricxon_amd.rotary.HipRotary` is the face of it."""
+        _require_device_tensor("q", q)
+        dev, dt, nd, dim = q.device, q.dtype, q.dim(), q.shape[-1] if q.dim() else 0
+        if dt not in (torch.float32, torch.bfloat16) or nd not in (3, 4):
+            raise ValueError(f"q must be float32 or bfloat16 (T, heads, head_dim) or (B, T, heads, head_dim), got {dt} "
+                             f"{tuple(q.shape)}")
+        if dim % 2 or not rotary_dim <= dim <= self.ROPE_MAX_DIM or not 1 <= q.shape[-2] <= self.ROPE_MAX_HEADS:
+            raise ValueError(f"head_dim must be even, {rotary_dim}..{self.ROPE_MAX_DIM}, and 1..{self.ROPE_MAX_HEADS} "
+                             f"heads, got {tuple(q.shape)}")
+        if k is not None and (k.dtype != dt or k.device != dev or k.dim() != nd or k.shape[-1] != dim
+                              or k.shape[:-2] != q.shape[:-2] or not 1 <= k.shape[-2] <= self.ROPE_MAX_HEADS):
+            raise ValueError(f"k must be {dt} on {dev} and have q's shape but for the heads, got {k.dtype} "
+                             f"{tuple(k.shape)} on {k.device} for q {tuple(q.shape)}")
+        if turns.dtype != torch.float64 or turns.shape != (rotary_dim // 2,) or turns.device != dev:
+            raise ValueError(f"turns must be ({rotary_dim // 2},) float64 on {dev}")
+        if positions.dtype not in (torch.int32, torch.int64) or positions.device != dev:
+            raise ValueError(f"positions must be int32 or int64 on {dev}, got {positions.dtype} on {positions.device}")
+        lead = q.shape[:-2]
+        if positions.dim() == 0 or positions.shape[-1] != lead[-1] or (
+                positions.dim() != 1 and (positions.dim() != nd - 2 or positions.shape[0] not in (1, lead[0]))):
+            raise ValueError(f"positions must be {tuple(lead)} or {tuple(lead[-1:])}, got {tuple(positions.shape)}")
+        seq = lead[-1]
+        n_tokens = seq if nd == 3 else lead[0] * seq
+        ps = positions.stride()
+        pos_batch = 0 if positions.dim() == 1 or positions.shape[0] == 1 else ps[0]
+        heads, strides, outs, held = [], [], [], []
+        for x in (q, k):
+            if x is None:
+                heads.append(0), strides.append(None), outs.append(None), held.append(None)
+                continue
+            x = x.detach()
+            if x.stride(-1) != 1:
+                x = x.contiguous()
+            st = x.stride()
+            heads.append(x.shape[-2])
+            strides.append((ctypes.c_longlong * 3)(st[0] if nd == 4 else 0, st[-3], st[-2]))
+            outs.append(torch.empty(x.shape, dtype=dt, device=dev))
+            held.append(x)
+        if n_tokens == 0:
+            return outs[0], outs[1]
+        with _on(dev):
+            status = self._lib.mxa_rope(
+                held[0].data_ptr(), strides[0], heads[0], None if k is None else held[1].data_ptr(), strides[1],
+                heads[1], positions.data_ptr(), int(positions.dtype == torch.int64), pos_batch, ps[-1],
+                turns.data_ptr(), n_tokens, seq, dim, int(rotary_dim), int(interleaved), float(scale),
+                int(dt == torch.bfloat16), outs[0].data_ptr(), None if k is None else outs[1].data_ptr(),
+                _stream(dev))
+        self._check(status, "mxa_rope", 0)
+        return outs[0], outs[1]
+
     def silu_mul_q8k(self, gate: torch.Tensor, up: torch.Tensor,
                      want_out: bool = True) -> tuple[torch.Tensor | None, torch.Tensor]:
         """silu(gate) * up over (..., K) on the device, in float32: (out (M, K) or None,
