@@ -263,6 +263,46 @@ int mxa_moe_combine(const float *down, const int32_t *rows, const int32_t *ids,
                     const float *weights, int n_tokens, int top_k, int n_embd, int round_bf16,
                     float *out, void *stream);
 
+/* mxa_moe_combine that leaves out the slots of a negative id (their down rows and weights count for nothing,
+ * whatever they hold): tokens with fewer than top_k experts, as mxa_moe_topk routes them. */
+int mxa_moe_combine_masked(const float *down, const int32_t *rows, const int32_t *ids,
+                           const float *weights, int n_tokens, int top_k, int n_embd, int round_bf16,
+                           float *out, void *stream);
+
+/* Routing of MoE tokens from router logits (n_tokens, n_experts), float32 or bfloat16 (logits_bf16 != 0): ids
+ * and weights (n_tokens, top_k), DEVICE int32 and float32. Slot i of a token is its i-th largest logit, ties to
+ * the lowest id; its weight is exp(logit - max) over the sum of those of all experts (norm_topk 0) or of the
+ * chosen ones (norm_topk 1), times scale. A logit of -inf is an expert that the token may not take: where
+ * fewer than top_k are left the slots behind them get id -1 and weight 0 (all of them for a token with
+ * none). NaN counts as the largest logit and makes its token's weights NaN. n_experts <= 256, top_k <= 64
+ * and <= n_experts; else -1. The router's softmax and top-k before `QuantizedMoEExperts.forward`
+ * (app/architectures/moe_experts.py:29-89). */
+int mxa_moe_topk(const void *logits, int logits_bf16, int n_tokens, int n_experts, int top_k,
+                 int norm_topk, float scale, int32_t *ids, float *weights, void *stream);
+
+/* Workspace of mxa_moe_layer; 0 where it does not take the layer: gate_type (gate and up) and down_type of Q4_K,
+ * Q6_K, Q8_0; n_tokens 1 .. 8, top_k <= 16, n_tokens * top_k <= 64, n_experts <= 256; n_embd and ffn_len
+ * multiples of 256 up to 16384. Depends on the current device. */
+size_t mxa_moe_layer_workspace_bytes(int gate_type, int down_type, int n_experts, int top_k, int n_tokens,
+                                     int n_embd, int ffn_len, int bf16);
+
+/* A whole mixture-of-experts layer of packed experts for a few tokens, in two launches: the routing of
+ * mxa_moe_topk, silu(gate_e x) * (up_e x) of each token's experts, down_e of that, and their weighted sum
+ * in ascending expert id. x (n_tokens, n_embd) bfloat16 (bf16 != 0) or float32, 16-byte aligned; expert e at
+ * gate and up + e * gate_stride (ffn_len rows) and down + e * down_stride (n_embd rows), 16-byte aligned
+ * bases and strides; ids and weights (n_tokens, top_k) are written as mxa_moe_topk writes them; out (n_tokens,
+ * n_embd) float32 or bfloat16 (out_bf16 != 0). The steps, roundings and bits are those of mxa_gemm_moe(_bf16)
+ * for gate and up, mxa_silu_mul_q8_k(_bf16), mxa_gemm_moe for down and mxa_moe_combine_masked
+ * (round_bf16 = bf16), then the cast to out's type; with reciprocal != 0 the codes of the Q8_K blocks are
+ * rint(v * (127 * (1 / amax))) in place of rint(v * (127 / amax)), as an emulation in torch computes them
+ * (its 127.0 / amax is that product), which differ where v * 127 / amax is next to a half. Replaces the per-expert loop of
+ * `QuantizedMoEExperts.forward` (app/architectures/moe_experts.py:81-88) with its routing. */
+int mxa_moe_layer(int gate_type, int down_type, const void *gate, const void *up, long long gate_stride,
+                  const void *down, long long down_stride, int n_experts, const void *x, int bf16,
+                  const void *logits, int logits_bf16, int top_k, int norm_topk, float scale, int n_tokens,
+                  int n_embd, int ffn_len, int reciprocal, int32_t *ids, float *weights, void *out,
+                  int out_bf16, void *workspace, size_t workspace_bytes, void *stream);
+
 /* Up to 4 packed weights sharing one input (q/k/v, gate/up): one activation quantization, then
  * each weight's output columns written after the previous weight's, y (n_tokens, sum outs).
  * `types`, `ws` (device pointers) and `outs` are HOST arrays of n entries.

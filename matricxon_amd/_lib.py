@@ -31,6 +31,10 @@ EXPORTS = (
     "mxa_gemm_moe_pairs_bf16",
     "mxa_moe_route",
     "mxa_moe_combine",
+    "mxa_moe_combine_masked",
+    "mxa_moe_topk",
+    "mxa_moe_layer",
+    "mxa_moe_layer_workspace_bytes",
     "mxa_gemm_multi",
     "mxa_gemm_multi_q8k",
     "mxa_quantize_q8_k",
@@ -110,6 +114,15 @@ def load() -> ctypes.CDLL:
     lib.mxa_moe_route.restype = _i
     lib.mxa_moe_combine.argtypes = [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp]
     lib.mxa_moe_combine.restype = _i
+    lib.mxa_moe_combine_masked.argtypes = lib.mxa_moe_combine.argtypes
+    lib.mxa_moe_combine_masked.restype = _i
+    lib.mxa_moe_topk.argtypes = [_vp, _i, _i, _i, _i, _i, _f, _vp, _vp, _vp]
+    lib.mxa_moe_topk.restype = _i
+    lib.mxa_moe_layer_workspace_bytes.argtypes = [_i] * 8
+    lib.mxa_moe_layer_workspace_bytes.restype = _sz
+    lib.mxa_moe_layer.argtypes = [_i, _i, _vp, _vp, _ll, _vp, _ll, _i, _vp, _i, _vp, _i, _i, _i, _f, _i, _i, _i, _i, _vp,
+                                  _vp, _vp, _i, _vp, _sz, _vp]
+    lib.mxa_moe_layer.restype = _i
     lib.mxa_gemm_multi.argtypes = [_i, _vp, _vp, _vp, _vp, _vp, _i, _i, _vp, _sz, _vp]
     lib.mxa_gemm_multi.restype = _i
     lib.mxa_gemm_multi_q8k.argtypes = [_i, _vp, _vp, _vp, _vp, _i, _i, _vp, _sz, _vp]

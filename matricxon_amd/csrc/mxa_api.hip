@@ -487,8 +487,59 @@ int mxa_moe_combine(const float* down, const int32_t* rows, const int32_t* ids,
                     float* out, void* stream) {
   if (down == nullptr || ids == nullptr || weights == nullptr || out == nullptr)
     return MXA_ERR_UNSUPPORTED;
-  if (mxa::launch_moe_combine(down, rows, ids, weights, n_tokens, top_k, n_embd, round_bf16 != 0,
+  if (mxa::launch_moe_combine(down, rows, ids, weights, n_tokens, top_k, n_embd, round_bf16 != 0, 0,
                               out, (hipStream_t)stream) != 0)
+    return MXA_ERR_UNSUPPORTED;
+  return check_launch();
+}
+
+int mxa_moe_combine_masked(const float* down, const int32_t* rows, const int32_t* ids, const float* weights,
+                           int n_tokens, int top_k, int n_embd, int round_bf16, float* out, void* stream) {
+  if (down == nullptr || ids == nullptr || weights == nullptr || out == nullptr)
+    return MXA_ERR_UNSUPPORTED;
+  if (mxa::launch_moe_combine(down, rows, ids, weights, n_tokens, top_k, n_embd, round_bf16 != 0, 1,
+                              out, (hipStream_t)stream) != 0)
+    return MXA_ERR_UNSUPPORTED;
+  return check_launch();
+}
+
+int mxa_moe_topk(const void* logits, int logits_bf16, int n_tokens, int n_experts, int top_k, int norm_topk,
+                 float scale, int32_t* ids, float* weights, void* stream) {
+  if (logits == nullptr || ids == nullptr || weights == nullptr || !aligned(logits, logits_bf16 ? 2 : 4) ||
+      !aligned(ids, 4) || !aligned(weights, 4))
+    return MXA_ERR_UNSUPPORTED;
+  if (mxa::launch_moe_topk(logits, logits_bf16 != 0, n_tokens, n_experts, top_k, norm_topk != 0, scale, ids, weights,
+                           (hipStream_t)stream) != 0)
+    return MXA_ERR_UNSUPPORTED;
+  return check_launch();
+}
+
+size_t mxa_moe_layer_workspace_bytes(int gate_type, int down_type, int n_experts, int top_k, int n_tokens, int n_embd,
+                                     int ffn_len, int bf16) {
+  if (!mxa::moe_layer_supported(gate_type, down_type, n_experts, top_k, n_tokens, n_embd, ffn_len)) return 0;
+  return mxa::moe_layer_workspace(n_tokens, top_k, n_embd, ffn_len, bf16 != 0);
+}
+
+int mxa_moe_layer(int gate_type, int down_type, const void* gate, const void* up, long long gate_stride,
+                  const void* down, long long down_stride, int n_experts, const void* x, int bf16, const void* logits,
+                  int logits_bf16, int top_k, int norm_topk, float scale, int n_tokens, int n_embd, int ffn_len,
+                  int reciprocal, int32_t* ids, float* weights, void* out, int out_bf16, void* workspace, size_t workspace_bytes,
+                  void* stream) {
+  const size_t need = mxa_moe_layer_workspace_bytes(gate_type, down_type, n_experts, top_k, n_tokens, n_embd, ffn_len, bf16);
+  if (need == 0 || gate == nullptr || up == nullptr || down == nullptr || x == nullptr || logits == nullptr ||
+      ids == nullptr || weights == nullptr || out == nullptr || !aligned(gate, 16) || !aligned(up, 16) ||
+      !aligned(down, 16) || !aligned(x, 16) || !aligned(logits, logits_bf16 ? 2 : 4) || !aligned(ids, 4) ||
+      !aligned(weights, 4) || !aligned(out, out_bf16 ? 2 : 4) || !aligned(workspace, 16))
+    return MXA_ERR_UNSUPPORTED;
+  const long long gate_row = (long long)mxa_row_bytes(gate_type, n_embd), down_row = (long long)mxa_row_bytes(down_type, ffn_len);
+  if (gate_stride < gate_row * ffn_len || down_stride < down_row * n_embd || gate_stride % 16 != 0 || down_stride % 16 != 0)
+    return MXA_ERR_UNSUPPORTED;
+  if (workspace == nullptr || workspace_bytes < need) return MXA_ERR_WORKSPACE;
+  if (mxa::launch_moe_layer(gate_type, down_type, (const uint8_t*)gate, (const uint8_t*)up, gate_stride, gate_row,
+                            (const uint8_t*)down, down_stride, down_row, n_experts, x, bf16 != 0, logits,
+                            logits_bf16 != 0, top_k, norm_topk != 0, scale, n_tokens, n_embd, ffn_len, reciprocal != 0, ids, weights,
+                            out_bf16 ? mxa::YOut::bf16(out) : mxa::YOut::f32((float*)out), workspace,
+                            (hipStream_t)stream) != 0)
     return MXA_ERR_UNSUPPORTED;
   return check_launch();
 }

@@ -32,8 +32,9 @@ inline size_t act_bytes(int m_rows, int k) {
 // correctly rounded divisions, q = clamp(round-half-even(x * iscale), +-127) (lrintf in the
 // default rounding mode is v_rndne_f32), and bsums are the sums of q over 16 values. Writes the
 // lane's 16 q at qblk + 16p, its bsum at bsblk[p] and, from part 0, d. All 16 lanes must be active.
+// reciprocal: iscale = 127 * (1 / amax), which torch's `127.0 / amax` evaluates to.
 __device__ __forceinline__ void q8k_part16(const float (&v)[16], int p, int8_t* qblk, int16_t* bsblk,
-                                           float* dp) {
+                                           float* dp, bool reciprocal = false) {
   float amax = 0.0f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(v[i]));
@@ -42,7 +43,7 @@ __device__ __forceinline__ void q8k_part16(const float (&v)[16], int p, int8_t* 
 #pragma unroll
   for (int i = 0; i < 16; ++i) qv[i] = 0;
   if (amax != 0.0f) {
-    const float iscale = 127.0f / amax;
+    const float iscale = reciprocal ? 127.0f * (1.0f / amax) : 127.0f / amax;
 #pragma unroll
     for (int i = 0; i < 16; ++i) qv[i] = (int)fminf(fmaxf(rintf(v[i] * iscale), -127.0f), 127.0f);
   }
@@ -245,7 +246,7 @@ int launch_moe_lpb(int type, const uint8_t* w, long long row_bytes, long long ex
 // out[t] (n_tokens x n_embd fp32) = the routing-weighted sum of token t's expert outputs:
 // down row rows[t top_k + k] (rows == nullptr: row t top_k + k) of slot k, times weights[t top_k
 // + k], slots in ascending ids[t top_k + k] (ties in slot order), bf16 != 0: each down value
-// rounded to bfloat16 first. top_k <= kMoeMaxTopK; -1 otherwise.
+// rounded to bfloat16 first; masked != 0: slots of a negative id are left out. top_k <= kMoeMaxTopK; -1 otherwise.
 constexpr int kMoeMaxTopK = 16;
 // MoE routing (one workgroup, stable counting sort): up to kMoeRouteMaxExperts experts and
 // kMoeRouteMaxPairs (token, slot) pairs; -1 otherwise.
@@ -256,7 +257,22 @@ int launch_moe_route(const void* ids, bool ids64, int n_tokens, int top_k, int n
                      hipStream_t stream);
 int launch_moe_combine(const float* down, const int32_t* rows, const int32_t* ids,
                        const float* weights, int n_tokens, int top_k, int n_embd, int bf16,
-                       float* out, hipStream_t stream);
+                       int masked, float* out, hipStream_t stream);
+
+// The routing of MoE tokens from router logits (mxa_moe_layer.hip): ids and softmax weights of the top_k largest,
+// ties to the lowest id; id -1 and weight 0 where only logits of -inf are left. -1 for other sizes.
+int launch_moe_topk(const void* logits, bool bf16, int n_tokens, int n_experts, int top_k, bool norm_topk, float scale,
+                    int32_t* ids, float* wts, hipStream_t stream);
+// A whole layer of packed experts for up to kMoeLayerMaxTokens tokens (mxa_moe_layer.hip), from router logits to the
+// weighted sum, in two launches; ws of moe_layer_workspace bytes. -1 where it does not apply.
+constexpr int kMoeLayerMaxTokens = 8;
+bool moe_layer_supported(int gate_type, int down_type, int n_experts, int top_k, int n_tokens, int n_embd, int ffn);
+size_t moe_layer_workspace(int n_tokens, int top_k, int n_embd, int ffn, bool bf16);
+int launch_moe_layer(int gate_type, int down_type, const uint8_t* gate, const uint8_t* up, long long gate_stride,
+                     long long gate_row, const uint8_t* down, long long down_stride, long long down_row, int n_experts,
+                     const void* x, bool bf16, const void* logits, bool logits_bf16, int top_k, bool norm_topk,
+                     float scale, int n_tokens, int n_embd, int ffn, bool reciprocal, int32_t* ids, float* wts,
+                     YOut out, void* ws, hipStream_t stream);
 
 // Batched decode (m_rows <= 16) on the matrix cores with the weight rows streamed into LDS by
 // coalesced copies, one persistent workgroup per CU: Q4_K, Q6_K, Q8_0 on Q8_K activations in the

@@ -23,7 +23,7 @@ __device__ __forceinline__ float round_bf16(float f) {
 __global__ __launch_bounds__(256) void moe_combine_kernel(
     const float* __restrict__ down, const int32_t* __restrict__ rows,
     const int32_t* __restrict__ ids, const float* __restrict__ wts, int top_k, int n_embd,
-    int bf16, float* __restrict__ out) {
+    int bf16, int masked, float* __restrict__ out) {
   __shared__ int ord[kMoeMaxTopK];
   const int t = blockIdx.y, j = blockIdx.x * 256 + threadIdx.x;
   const int32_t* tid = ids + (size_t)t * top_k;
@@ -38,6 +38,7 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(
   float acc = 0.0f;
   for (int i = 0; i < top_k; ++i) {
     const size_t p = (size_t)t * top_k + ord[i];
+    if (masked && ids[p] < 0) continue;  // a slot without an expert: its down row says nothing
     const size_t r = rows != nullptr ? (size_t)rows[p] : p;
     float v = down[r * n_embd + j];
     if (bf16) v = round_bf16(v);
@@ -162,11 +163,11 @@ int launch_moe_route(const void* ids, bool ids64, int n_tokens, int top_k, int n
 
 int launch_moe_combine(const float* down, const int32_t* rows, const int32_t* ids,
                        const float* weights, int n_tokens, int top_k, int n_embd, int bf16,
-                       float* out, hipStream_t stream) {
+                       int masked, float* out, hipStream_t stream) {
   if (n_tokens < 1 || n_tokens > 65535 || top_k < 1 || top_k > kMoeMaxTopK || n_embd < 1)
     return -1;
   hipLaunchKernelGGL(moe_combine_kernel, dim3((n_embd + 255) / 256, n_tokens), dim3(256), 0,
-                     stream, down, rows, ids, weights, top_k, n_embd, bf16, out);
+                     stream, down, rows, ids, weights, top_k, n_embd, bf16, masked, out);
   return 0;
 }
 

@@ -726,14 +726,48 @@ class HipGemm:
         self._check(status, "mxa_moe_route", 0)
         return offsets, pair_tok, rows, ids32
 
+    MOE_MAX_TOP_K = 16
+
+    def moe_topk(self, logits: torch.Tensor, top_k: int, norm_topk: bool = True, scale: float = 1.0
+                 ) -> tuple[torch.Tensor, torch.Tensor]:
+        """The routing of MoE tokens from their router logits (n_tokens, n_experts), float32 or bfloat16, in one
+        launch (`mxa_moe_topk`): (ids int32, weights float32), (n_tokens, top_k) each, largest logit first, ties to
+        the lowest id, weights the softmax over all experts or (`norm_topk`) over the chosen ones, times `scale`. A
+        logit of -inf is no expert: slots without one have id -1 and weight 0."""
+        _require_device_tensor("logits", logits)
+        self._check_router(logits, logits.shape[0] if logits.dim() == 2 else 0, logits.shape[-1], top_k)
+        dev, n_tokens = logits.device, logits.shape[0]
+        logits = logits.detach().contiguous()
+        ids = torch.empty((n_tokens, top_k), dtype=torch.int32, device=dev)
+        weights = torch.empty((n_tokens, top_k), dtype=torch.float32, device=dev)
+        if n_tokens == 0:
+            return ids, weights
+        with _on(dev):
+            status = self._lib.mxa_moe_topk(logits.data_ptr(), int(logits.dtype == torch.bfloat16), n_tokens,
+                                            logits.shape[1], top_k, int(bool(norm_topk)), float(scale),
+                                            ids.data_ptr(), weights.data_ptr(), _stream(dev))
+        self._check(status, "mxa_moe_topk", 0)
+        return ids, weights
+
+    def _check_router(self, logits: torch.Tensor, n_tokens: int, n_experts: int, top_k: int) -> None:
+        if logits.dim() != 2 or tuple(logits.shape) != (n_tokens, n_experts) or \
+                logits.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"router logits must be float32 or bfloat16 ({n_tokens}, {n_experts}), got {logits.dtype} "
+                             f"{tuple(logits.shape)}")
+        if not 1 <= top_k <= min(n_experts, self.MOE_MAX_TOP_K) or n_experts > self.MOE_ROUTE_MAX_EXPERTS:
+            raise ValueError(f"top_k must be 1..min(n_experts, {self.MOE_MAX_TOP_K}) of up to "
+                             f"{self.MOE_ROUTE_MAX_EXPERTS} experts, got {top_k} of {n_experts}")
+
     def moe_combine(self, down: torch.Tensor, ids: torch.Tensor, weights: torch.Tensor,
-                    rows: torch.Tensor | None = None, round_bf16: bool = False) -> torch.Tensor:
+                    rows: torch.Tensor | None = None, round_bf16: bool = False,
+                    masked: bool = False) -> torch.Tensor:
         """The weighted combine of MoE expert outputs in one launch (`mxa_moe_combine`): row t of
         the result (n_tokens, n_embd) float32 adds, in ascending expert id of token t's slots
         (`ids` (n_tokens, top_k) int32; equal ids in slot order), down row rows[t, k] (`rows`
         int32 like `ids`, or None for row t * top_k + k) times weights[t, k] (float32), from a
         float zero; `round_bf16` rounds each down value to bfloat16 first, as the module's cast
-        to a bfloat16 layer dtype does. The combine of QuantizedMoEExperts.forward
+        to a bfloat16 layer dtype does. `masked` leaves out slots of a negative id
+        (`mxa_moe_combine_masked`). The combine of QuantizedMoEExperts.forward
         (app/architectures/moe_experts.py:81-88), bit for bit."""
         _require_device_tensor("down", down)
         device = down.device
@@ -749,7 +783,8 @@ class HipGemm:
                 raise ValueError(f"{name} must be a contiguous {dt} ({n_tokens}, {top_k}) tensor "
                                  f"on {device}")
         out = torch.empty((n_tokens, down.shape[1]), dtype=torch.float32, device=device)
-        status = self._lib.mxa_moe_combine(
+        combine = self._lib.mxa_moe_combine_masked if masked else self._lib.mxa_moe_combine
+        status = combine(
             down.data_ptr(), rows.data_ptr() if rows is not None else None, ids.data_ptr(),
             weights.data_ptr(), n_tokens, top_k, down.shape[1], int(bool(round_bf16)),
             out.data_ptr(), _stream(device))

@@ -16,7 +16,7 @@ from collections.abc import Callable
 import torch
 from torch import nn
 
-from .gemm import HipGemm, q8k_bytes
+from .gemm import HipGemm, _on, _stream, q8k_bytes
 
 
 def route_pairs(top_k_idx: torch.Tensor, num_experts: int) -> tuple[torch.Tensor, torch.Tensor,
@@ -55,6 +55,8 @@ def combine_in_expert_order(contrib: torch.Tensor, order: torch.Tensor, top_k_id
 
 
 _IQ4_XS = 23  # float activations: no Q8_K blocks
+_LAYER_MAX_TOKENS = 8  # tokens of mxa_moe_layer
+_GROUPED_MAX_TOKENS = 32768  # tokens of one routing and one combine launch
 
 
 def _is_silu(fn) -> bool:
@@ -91,6 +93,11 @@ class HipPackedMoEExperts(nn.Module):
         self._pairs = all(int(t) != 23 and k // 256 in (4, 8, 16, 32, 56, 64) and
                           self._gemm.row_bytes(int(t), k) % 16 == 0
                           for t, k in ((gate_type, n_embd), (up_type, n_embd), (down_type, ffn_len)))
+        # what mxa_moe_layer takes besides its sizes; its workspace by (tokens, top_k, device), 0 where it declines
+        self._layer_ok = (gate_type == up_type and _is_silu(activation) and dtype in (torch.float32, torch.bfloat16)
+                          and all(w.is_contiguous() and w.data_ptr() % 16 == 0 and w.stride(0) % 16 == 0
+                                  for w in (gate, up, down)))
+        self._layer_bytes: dict[tuple[int, int, torch.device], int] = {}
         self.register_buffer("gate_packed", gate, persistent=False)
         self.register_buffer("up_packed", up, persistent=False)
         self.register_buffer("down_packed", down, persistent=False)
@@ -103,6 +110,99 @@ class HipPackedMoEExperts(nn.Module):
             out = self._one_token(x, top_k_weights, top_k_idx)
             if out is not None:
                 return out
+        return self._grouped(x, top_k_weights, top_k_idx)
+
+    def forward_logits(self, x: torch.Tensor, logits: torch.Tensor, top_k: int, norm_topk: bool = True,
+                       scale: float = 1.0, q8k_scale: str = "divide"
+                       ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """The whole layer from the router's logits (n_tokens, num_experts), float32 or bfloat16: (out like x, ids
+        int32, weights float32, the last two (n_tokens, top_k)). A token takes its top_k largest logits, ties to the
+        lowest id, weighted by the softmax over all experts or (`norm_topk`) over the chosen ones, times `scale`. A
+        logit of -inf masks its expert; a slot without an expert has id -1 and weight 0 and adds nothing, so that a
+        token of -inf alone (padding) gets a row of zeros, whatever x holds there. `forward` on those ids and weights
+        gives the same bits.
+
+        Up to eight tokens (and 64 pairs) of Q4_K, Q6_K or Q8_0 experts, gate and up of one type, with a SiLU: two
+        launches (`mxa_moe_layer`). Otherwise the routing in one launch, then the grouped projections.
+
+        `q8k_scale` "reciprocal" takes the codes of the activations' blocks as rint(v * (127 * (1 / amax))), which is
+        what torch evaluates for `127.0 / amax`, for layers that were tuned or are checked against such an emulation;
+        a code differs from the default's rint(v * (127 / amax)) only next to a half (one in some 2500 for bfloat16
+        activations), but a layer's later roundings make 0.5% of the output of it. More than eight tokens then run
+        eight at a time, and a layer that the two launches do not take is refused (ValueError)."""
+        if q8k_scale not in ("divide", "reciprocal"):
+            raise ValueError(f'q8k_scale must be "divide" or "reciprocal", got {q8k_scale!r}')
+        reciprocal = q8k_scale == "reciprocal"
+        g = self._gemm
+        n_tokens = x.shape[0] if x.dim() == 2 else -1
+        if n_tokens < 0 or x.shape[1] != self.n_embd or x.device != self.gate_packed.device:
+            raise ValueError(f"x must be (n_tokens, {self.n_embd}) on {self.gate_packed.device}, got {tuple(x.shape)} "
+                             f"on {x.device}")
+        g._check_router(logits, n_tokens, self.num_experts, top_k)
+        if logits.device != x.device or self.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"router logits on {x.device} and a float32 or bfloat16 layer, got {logits.device} and "
+                             f"{self.dtype}")
+        res = self._few_tokens(x, logits, top_k, norm_topk, scale, reciprocal)
+        if res is not None:
+            return res
+        if reciprocal and n_tokens > 0:
+            step = max(1, min(_LAYER_MAX_TOKENS, 64 // top_k))
+            parts = [self._few_tokens(x[i : i + step], logits[i : i + step], top_k, norm_topk, scale, True)
+                     for i in range(0, n_tokens, step)]
+            if None in parts:
+                raise ValueError("reciprocal code scales need a layer of Q4_K, Q6_K or Q8_0 experts, gate and up of "
+                                 "one type, rows of up to 16384 values and a SiLU")
+            return tuple(torch.cat(p) for p in zip(*parts))
+        ids, weights = g.moe_topk(logits, top_k, norm_topk, scale)
+        if n_tokens == 0:
+            return torch.empty_like(x), ids, weights
+        step = _GROUPED_MAX_TOKENS
+        outs = [self._grouped(x[i : i + step], weights[i : i + step], ids[i : i + step], masked=True)
+                for i in range(0, n_tokens, step)]
+        return outs[0] if len(outs) == 1 else torch.cat(outs), ids, weights
+
+    def _few_tokens(self, x: torch.Tensor, logits: torch.Tensor, top_k: int, norm_topk: bool, scale: float,
+                    reciprocal: bool = False
+                    ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor] | None:
+        """`forward_logits` in two launches, or None where they do not take the layer."""
+        n_tokens, dev = x.shape[0], x.device
+        if not 1 <= n_tokens <= _LAYER_MAX_TOKENS or not self._layer_ok:
+            return None
+        lib, bf16 = self._gemm._lib, self.dtype == torch.bfloat16
+        gt, _, dt = self.types
+        with _on(dev):
+            key = (n_tokens, top_k, dev)
+            ws_bytes = self._layer_bytes.get(key)
+            if ws_bytes is None:
+                ws_bytes = self._layer_bytes[key] = lib.mxa_moe_layer_workspace_bytes(
+                    gt, dt, self.num_experts, top_k, n_tokens, self.n_embd, self.ffn_len, int(bf16))
+            if ws_bytes == 0:
+                return None
+            xs = x.detach() if x.dtype == self.dtype else x.detach().to(self.dtype)
+            if not xs.is_contiguous() or xs.data_ptr() % 16 != 0:
+                xs = xs.clone(memory_format=torch.contiguous_format)
+            logits = logits.detach().contiguous()
+            gate, up, down = self.gate_packed, self.up_packed, self.down_packed
+            out = torch.empty(x.shape, dtype=x.dtype if x.dtype == torch.bfloat16 else torch.float32, device=dev)
+            ids = torch.empty((n_tokens, top_k), dtype=torch.int32, device=dev)
+            weights = torch.empty((n_tokens, top_k), dtype=torch.float32, device=dev)
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+            status = lib.mxa_moe_layer(
+                gt, dt, gate.data_ptr(), up.data_ptr(), gate.stride(0), down.data_ptr(), down.stride(0),
+                self.num_experts, xs.data_ptr(), int(bf16), logits.data_ptr(), int(logits.dtype == torch.bfloat16),
+                top_k, int(bool(norm_topk)), float(scale), n_tokens, self.n_embd, self.ffn_len, int(reciprocal),
+                ids.data_ptr(), weights.data_ptr(), out.data_ptr(), int(out.dtype == torch.bfloat16), ws.data_ptr(), ws_bytes,
+                _stream(dev))
+        if status == -1:
+            return None
+        self._gemm._check(status, "mxa_moe_layer", gt)
+        return (out if out.dtype == x.dtype else out.to(x.dtype)), ids, weights
+
+    def _grouped(self, x: torch.Tensor, top_k_weights: torch.Tensor, top_k_idx: torch.Tensor,
+                 masked: bool = False) -> torch.Tensor:
+        """The grouped launches for any number of tokens; `masked`: slots of a negative id add nothing."""
+        n_tokens, n_embd = x.shape
+        top_k = top_k_idx.shape[1]
         g = self._gemm
         fused = self._fused_combine(top_k_weights)
         if fused and self.num_experts <= g.MOE_ROUTE_MAX_EXPERTS and \
@@ -153,7 +253,7 @@ class HipPackedMoEExperts(nn.Module):
             act = self.activation(gate.to(self.dtype)) * up.to(self.dtype)
             down = g.matmul_moe(dt, self.down_packed, act, offsets, bound, n_embd, self.ffn_len)
         if order is None:
-            return self._combine(down, rows, ids32, top_k_weights).to(x.dtype)
+            return self._combine(down, rows, ids32, top_k_weights, masked).to(x.dtype)
         if fused:
             # down row of pair p = its place in the sorted order
             rows = torch.empty_like(order)
@@ -172,7 +272,7 @@ class HipPackedMoEExperts(nn.Module):
                 and self.dtype in (torch.float32, torch.bfloat16))
 
     def _combine(self, down: torch.Tensor, rows: torch.Tensor | None, top_k_idx: torch.Tensor,
-                 top_k_weights: torch.Tensor) -> torch.Tensor:
+                 top_k_weights: torch.Tensor, masked: bool = False) -> torch.Tensor:
         """float32 (n_tokens, n_embd): the reference's `down.to(dtype) * weight` contributions
         `index_add_`ed in ascending expert order, in one launch."""
         shape = top_k_idx.shape
@@ -181,7 +281,7 @@ class HipPackedMoEExperts(nn.Module):
         if rows is not None:
             rows = rows.to(torch.int32).reshape(shape).contiguous()
         return self._gemm.moe_combine(down, ids, top_k_weights.contiguous(), rows,
-                                      round_bf16=self.dtype == torch.bfloat16)
+                                      round_bf16=self.dtype == torch.bfloat16, masked=masked)
 
     def _one_token(self, x: torch.Tensor, top_k_weights: torch.Tensor,
                    top_k_idx: torch.Tensor) -> torch.Tensor | None:
