@@ -342,7 +342,9 @@ def _own_moe(s):
 
         layer = s["plan"] = HipPackedMoEExperts(s["gate"], s["up"], s["down"], case["type"], case["type"], case["down"],
                                                 case["embd"], case["ffn"], torch.nn.functional.silu, torch.bfloat16)
-    return layer.forward_logits(s["x"], s["logits"], case["top_k"], norm_topk=case["norm_topk"], scale=case["scale"])
+    # the codes' scales as the plain form's torch operations round them
+    return layer.forward_logits(s["x"], s["logits"], case["top_k"], norm_topk=case["norm_topk"], scale=case["scale"],
+                                q8k_scale="reciprocal")
 
 
 def run(state):
