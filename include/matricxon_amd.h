@@ -282,11 +282,11 @@ int mxa_moe_topk(const void *logits, int logits_bf16, int n_tokens, int n_expert
 
 /* Workspace of mxa_moe_layer; 0 where it does not take the layer: gate_type (gate and up) and down_type of Q4_K,
  * Q6_K, Q8_0; n_tokens 1 .. 8, top_k <= 16, n_tokens * top_k <= 64, n_experts <= 256; n_embd and ffn_len
- * multiples of 256 up to 16384. Depends on the current device. */
+ * multiples of 256 up to 16384. Host-only. */
 size_t mxa_moe_layer_workspace_bytes(int gate_type, int down_type, int n_experts, int top_k, int n_tokens,
                                      int n_embd, int ffn_len, int bf16);
 
-/* A whole mixture-of-experts layer of packed experts for a few tokens, in two launches: the routing of
+/* A whole mixture-of-experts layer of packed experts for a few tokens, in two launches and the combine: the routing of
  * mxa_moe_topk, silu(gate_e x) * (up_e x) of each token's experts, down_e of that, and their weighted sum
  * in ascending expert id. x (n_tokens, n_embd) bfloat16 (bf16 != 0) or float32, 16-byte aligned; expert e at
  * gate and up + e * gate_stride (ffn_len rows) and down + e * down_stride (n_embd rows), 16-byte aligned

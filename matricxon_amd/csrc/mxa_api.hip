@@ -488,7 +488,7 @@ int mxa_moe_combine(const float* down, const int32_t* rows, const int32_t* ids,
   if (down == nullptr || ids == nullptr || weights == nullptr || out == nullptr)
     return MXA_ERR_UNSUPPORTED;
   if (mxa::launch_moe_combine(down, rows, ids, weights, n_tokens, top_k, n_embd, round_bf16 != 0, 0,
-                              out, (hipStream_t)stream) != 0)
+                              mxa::YOut::f32(out), (hipStream_t)stream) != 0)
     return MXA_ERR_UNSUPPORTED;
   return check_launch();
 }
@@ -498,7 +498,7 @@ int mxa_moe_combine_masked(const float* down, const int32_t* rows, const int32_t
   if (down == nullptr || ids == nullptr || weights == nullptr || out == nullptr)
     return MXA_ERR_UNSUPPORTED;
   if (mxa::launch_moe_combine(down, rows, ids, weights, n_tokens, top_k, n_embd, round_bf16 != 0, 1,
-                              out, (hipStream_t)stream) != 0)
+                              mxa::YOut::f32(out), (hipStream_t)stream) != 0)
     return MXA_ERR_UNSUPPORTED;
   return check_launch();
 }

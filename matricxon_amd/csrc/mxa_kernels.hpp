@@ -257,7 +257,7 @@ int launch_moe_route(const void* ids, bool ids64, int n_tokens, int top_k, int n
                      hipStream_t stream);
 int launch_moe_combine(const float* down, const int32_t* rows, const int32_t* ids,
                        const float* weights, int n_tokens, int top_k, int n_embd, int bf16,
-                       int masked, float* out, hipStream_t stream);
+                       int masked, YOut out, hipStream_t stream);
 
 // The routing of MoE tokens from router logits (mxa_moe_layer.hip): ids and softmax weights of the top_k largest,
 // ties to the lowest id; id -1 and weight 0 where only logits of -inf are left. -1 for other sizes.

@@ -23,7 +23,7 @@ __device__ __forceinline__ float round_bf16(float f) {
 __global__ __launch_bounds__(256) void moe_combine_kernel(
     const float* __restrict__ down, const int32_t* __restrict__ rows,
     const int32_t* __restrict__ ids, const float* __restrict__ wts, int top_k, int n_embd,
-    int bf16, int masked, float* __restrict__ out) {
+    int bf16, int masked, YOut out) {
   __shared__ int ord[kMoeMaxTopK];
   const int t = blockIdx.y, j = blockIdx.x * 256 + threadIdx.x;
   const int32_t* tid = ids + (size_t)t * top_k;
@@ -44,7 +44,7 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(
     if (bf16) v = round_bf16(v);
     acc = acc + v * wts[p];
   }
-  out[(size_t)t * n_embd + j] = acc;
+  out.put((size_t)t * n_embd + j, acc);
 }
 
 // Routing of the (token, slot) pairs by expert, one workgroup: a stable counting sort. Pair
@@ -163,7 +163,7 @@ int launch_moe_route(const void* ids, bool ids64, int n_tokens, int top_k, int n
 
 int launch_moe_combine(const float* down, const int32_t* rows, const int32_t* ids,
                        const float* weights, int n_tokens, int top_k, int n_embd, int bf16,
-                       int masked, float* out, hipStream_t stream) {
+                       int masked, YOut out, hipStream_t stream) {
   if (n_tokens < 1 || n_tokens > 65535 || top_k < 1 || top_k > kMoeMaxTopK || n_embd < 1)
     return -1;
   hipLaunchKernelGGL(moe_combine_kernel, dim3((n_embd + 255) / 256, n_tokens), dim3(256), 0,

@@ -1,26 +1,36 @@
-// A mixture-of-experts layer of packed experts for a few tokens, from the router's logits, in two launches:
+// A mixture-of-experts layer of packed experts for a few tokens, from the router's logits, in two launches and the
+// combine:
 //
-//   ids, w  = the top_k largest logits of a token and their softmax weights         (both launches need them)
-//   act_p   = silu(gate_e x_t) * (up_e x_t)        for each pair p = (token t, expert e = ids[p])   first launch
-//   y_t     = sum over the token's pairs, experts ascending, of w_p * (down_e act_p)                second launch
+//   ids, w  = the top_k largest logits of a token and their softmax weights
+//   act_p   = silu(gate_e x_t) * (up_e x_t)    for each pair p = (token t, expert e = ids[p])     first launch
+//   down_p  = down_e act_p                                                                       second launch
+//   y_t     = sum over the token's pairs, experts ascending, of w_p * down_p                      mxa_moe.hip
 //
 // with the steps of the grouped path (mxa_gemm_moe, mxa_silu_mul_q8_k, mxa_moe_combine): x and act as Q8_K blocks,
 // gate, up, silu, their product and each down row rounded to bfloat16 in a bfloat16 layer, the sum in float32. The
 // block arithmetic (mxa_lpb.hpp), the folds and the order of the sum are the same, so the bits are.
 //
 // Bound: the routed experts' packed bytes, read once each. A work item is one expert with up to MAXM of its pairs
-// (experts of more are read again), and the workgroups (one a CU) are shared out evenly over the items, each taking
-// a contiguous range of the expert's rows. Every workgroup routes for itself: a wave per token finds the top_k of up
-// to 256 logits with one wave-wide maximum a slot, which costs less than a launch that does it once. No host sync,
-// no sort, no gather.
+// (experts of more are read again), and the workgroups (one a CU) are shared out over the items, each taking a
+// contiguous range of the expert's rows. Every workgroup routes for itself: a wave per token finds the top_k of up to
+// 256 logits, which costs less than a launch that does it once. No host sync, no sort, no gather.
 //
 // A workgroup's first W waves own rows: a wave copies the packed bytes of R = 64 / nb rows (gate's and up's) into
-// its LDS stage (global_load_lds_dwordx4, coalesced, no registers), waits for its own copies only, computes a block
-// per lane and folds a row per lane. The other waves turn the item's activations into Q8_K in LDS meanwhile; their
-// loads are issued before the copies, behind which they would otherwise queue.
+// its LDS stages (global_load_lds_dwordx4, coalesced, no registers), waits for its own copies only, computes a block
+// per lane and folds a row per lane; a stage is requested again as soon as its blocks are computed. The other waves
+// turn the item's activations into Q8_K in LDS meanwhile; their loads are issued before the copies, behind which
+// they would otherwise queue (with one token x's before the routing).
 //
-// The second launch's items share output rows: each writes its down rows, and the last workgroup to finish a range
-// of rows (a counter per range, cleared by the first launch) adds them up.
+// What bounds it, MI355X, kernel alone with weights that no cache holds: 8 experts top 2 of 4096 x 14336 (Q4_K, Q6_K
+// down), one token, gate and up 27 us for 132 MB (4.9 TB/s; a read of as many bytes 21), of which 3 us before the
+// first copy and 3 after the last; down 29 us for 96 MB (3.3 TB/s), the LDS holding 11 rows of 56 blocks, which
+// wait and compute in turn. Eight tokens: 104 and 139 us, 4.5 and 2.5 TB/s: each further pair of an expert adds to
+// the part of a wave's turn in which its stage is not in flight. 64 experts top 8 of 2048 x 1024, one token: 11.7
+// and 8.2 us, latency from end to end (logits, routing, activations, weights, block arithmetic).
+//
+// Adding the pairs up in the second launch, by the last workgroup to finish a range of rows, was slower than the
+// combine's launch: the fences that such a hand-over needs between XCDs cost the weights' stream more (down 62.8
+// against 29.3 + 4.4 us, one token of 8 experts top 2, 4096 x 14336 with Q6_K down).
 #include "mxa_kernels.hpp"
 #include "mxa_lpb.hpp"
 
@@ -30,6 +40,7 @@ namespace mxa {
 namespace {
 
 constexpr int kLayerLds = 160 * 1024;
+constexpr int kLayerWaves = 16, kLayerStagers = 4;  // waves of a workgroup; of them without rows, at least
 constexpr int kLayerMaxPairs = 64;  // a lane per pair
 constexpr int kActStride = QK + kActPad;
 
@@ -42,9 +53,7 @@ struct LayerArgs {
   int32_t* ids;
   float* wts;
   void* act;         // first launch: act (pairs, n); second: down rows (pairs, n) float32
-  int32_t* counters;   // a finished-items count per range of rows
   const void* logits;
-  uintptr_t out;       // second launch: YOut of (tokens, n)
   int n, k, nb, R, W;
   int n_experts, top_k, n_tokens;
   int logits_bf16, norm_topk, xbf16;
@@ -52,7 +61,7 @@ struct LayerArgs {
   float scale;
 };
 
-// Maximum over the wave, in every lane.
+// Reductions over the wave, in every lane: DPP within rows of 16, then the four rows.
 __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
 #define MXA_DPP_UMAX(ctrl) v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xF, 0xF, false))
   MXA_DPP_UMAX(0xB1);
@@ -63,57 +72,96 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
   const auto at = [&](int l) { return (uint32_t)__builtin_amdgcn_readlane((int)v, l); };
   return max(max(at(0), at(16)), max(at(32), at(48)));
 }
+__device__ __forceinline__ float lane_value(float v, int l) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+  v = quad_sum(v);
+  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x141, 0xF, 0xF, false));
+  v += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x140, 0xF, 0xF, false));
+  return (lane_value(v, 0) + lane_value(v, 16)) + (lane_value(v, 32) + lane_value(v, 48));
+}
 
-// The top_k experts of one token by a wave: lane i < top_k gets slot i's id and weight (id -1, weight 0 where no
-// expert is left: a logit of -inf is no expert). Larger logits first, ties to the lowest id, NaN above all (its
-// token's weights are NaN).
+// The top_k experts of one token by a wave: put(slot, id, weight) is called for every slot by one lane (id -1, weight
+// 0 where no expert is left: a logit of -inf is no expert). Larger logits first, ties to the lowest id, NaN above all
+// (its token's weights are NaN). A lane holds logits lane + 64 j.
+//
+// Up to 64 logits: each lane counts the logits that go before its own, broadcast one by one, which no step waits for
+// (64 logits, 8 slots: 0.5 us; a maximum over the wave per slot 1.5). More: a maximum per slot.
+template <class Put>
 __device__ __forceinline__ void route_token(const void* logits, bool bf16, long long first, int n_experts, int top_k,
-                                            bool norm_topk, float scale, int& id, float& wt) {
+                                            bool norm_topk, float scale, bool weights, Put put) {
   const int lane = threadIdx.x & 63;
   float v[4];
-  uint32_t key[4];
+  uint32_t key[4];  // ordered as the logits, 0 for no expert
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const int e = 4 * lane + j;
+    const int e = lane + 64 * j;
     v[j] = -__builtin_inff();
     if (e < n_experts)
       v[j] = bf16 ? bf16_to_float(((const uint16_t*)logits)[first + e]) : ((const float*)logits)[first + e];
     const uint32_t u = __builtin_bit_cast(uint32_t, v[j] + 0.0f);  // -0 as +0
     key[j] = (u & 0x7FFFFFFFu) > 0x7F800000u ? 0xFFFFFFFFu : u == 0xFF800000u ? 0u : (u >> 31) ? ~u : u | 0x80000000u;
   }
-  id = -1;
-  float mine = -__builtin_inff(), top = 0.0f;
-  for (int i = 0; i < top_k; ++i) {
-    uint32_t best = key[0];
-    int at = 0;
-    float val = v[0];
+  int slot = top_k, id = lane, live;  // this lane's slot (top_k or more: none) and its expert
+  float mine = v[0], top;
+  if (n_experts <= 64) {
+    live = __popcll(__ballot(key[0] != 0));
+    int before = 0;
 #pragma unroll
-    for (int j = 1; j < 4; ++j)
-      if (key[j] > best) best = key[j], at = j, val = v[j];
-    const uint32_t most = wave_umax(best);
-    if (most == 0) break;  // uniform
-    const int owner = __builtin_ctzll(__ballot(best == most));
-    const int e = 4 * owner + __builtin_amdgcn_readlane(at, owner);
-    const float l = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, val), owner));
-    if (i == 0) top = l;
-    if (lane == i) id = e, mine = l;
-    if (lane == owner) {
+    for (int l = 0; l < 64; ++l)  // lanes past the experts hold key 0
+      before += (uint32_t)__builtin_amdgcn_readlane((int)key[0], l) > key[0] - (l < lane ? 1u : 0u);
+    if (key[0] != 0) slot = before;  // o >= key where an equal lower id goes before, o > key else; key 0 has no slot
+    top = live > 0 ? lane_value(v[0], __builtin_ctzll(__ballot(slot == 0))) : 0.0f;
+  } else {
+    top = 0.0f;
+    for (live = 0; live < top_k; ++live) {
+      uint32_t best = key[0];
+      int at = 0;
+      float val = v[0];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (j == at) key[j] = 0;
+      for (int j = 1; j < 4; ++j)
+        if (key[j] > best) best = key[j], at = j, val = v[j];
+      const uint32_t most = wave_umax(best);
+      if (most == 0) break;  // uniform
+      // the lowest id of that logit: the lowest j, then the lowest lane
+      int j = 0;
+      uint64_t with = __ballot(key[0] == most);
+#pragma unroll
+      for (int i = 1; i < 4; ++i)
+        if (with == 0) with = __ballot(key[i] == most), j = i;
+      const int owner = __builtin_ctzll(with);
+      const float l = lane_value(val, owner);  // its best: no lower j of its own has that logit
+      if (live == 0) top = l;
+      if (lane == live) slot = live, id = owner + 64 * j, mine = l;
+      if (lane == owner) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i == j) key[i] = 0;
+      }
     }
   }
-  const float p = id >= 0 ? expf(mine - top) : 0.0f;
-  float s = p;
-  if (!norm_topk) {
-    s = 0.0f;
+  if (lane >= live && lane < top_k) put(lane, -1, 0.0f);
+  float wt = 0.0f;
+  if (weights) {
+    const float p = slot < top_k ? expf(mine - top) : 0.0f;
+    float s = p;
+    if (!norm_topk) {
+      s = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (v[j] != -__builtin_inff()) s += expf(v[j] - top);
+      for (int j = 0; j < 4; ++j)
+        if (v[j] != -__builtin_inff()) s += expf(v[j] - top);
+    }
+    wt = p / wave_sum(s) * scale;
   }
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o);
-  wt = id >= 0 ? p / s * scale : 0.0f;
+  if (slot < top_k) put(slot, id, wt);
+}
+
+// A barrier for what the waves wrote to LDS: loads in flight stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 // The number of work items of the pairs whose experts the lanes hold (e < 0: none): MAXM pairs of one expert each, in
@@ -145,64 +193,87 @@ constexpr int layer_region_bytes(int blocks) {
 // Activations of `rows` rows in LDS: q (272 bytes a block), bsums, d; and the routing.
 constexpr int layer_row_act(int nb) { return nb * (kActStride + 32 + 4); }
 constexpr int layer_act_bytes(int rows, int nb) { return (rows * layer_row_act(nb) + 15) / 16 * 16; }
-constexpr int kLayerFixed = 2 * 4 * kLayerMaxPairs + 16;
+constexpr int kLayerFixed = 4 * kLayerMaxPairs;
 
 template <int TYPE, int MAXM, bool GATEUP>
-__global__ __launch_bounds__(MAXM == 1 ? 1024 : 512) void moe_layer_kernel(LayerArgs a) {
+__global__ __launch_bounds__(64 * kLayerWaves) void moe_layer_kernel(LayerArgs a) {
   using L = Lpb<TYPE>;
   constexpr int kMats = GATEUP ? 2 : 1;
+  constexpr bool kReg = MAXM == 1 && TYPE != T_Q6_K;  // Q6_K's arithmetic leaves no registers
   extern __shared__ __align__(16) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 63, wg = blockIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
   const int pairs = a.n_tokens * a.top_k, W = a.W, nb = a.nb;
-  int* const sid = (int*)smem;  // the pairs' experts, then their weights or places
-  float* const swt = (float*)(smem + 4 * kLayerMaxPairs);
-  int* const flag = (int*)(smem + 8 * kLayerMaxPairs);
+  int* const sid = (int*)smem;  // the pairs' experts
   uint8_t* const acts = smem + kLayerFixed;
   int8_t* const aq = (int8_t*)acts;  // row m, block b at (m nb + b) 272
   int16_t* const abs_ = (int16_t*)(acts + MAXM * nb * kActStride);
   float* const ad = (float*)(acts + MAXM * nb * (kActStride + 32));
+  const bool rows_wave = wave < W;
+
+  // Activations to Q8_K, by the waves that own no rows: 16 lanes a block, four blocks a wave at a time, the first
+  // eight of a wave requested before the weights
+  const int step = 4 * (waves - W), p16 = lane & 15;
+  int g = 4 * (wave - W) + (lane >> 4);
+  uint4 first[4] = {}, second[4] = {};
+  const auto fetch = [&](int total, int g, long long row, int b, uint4 (&raw)[4]) __attribute__((always_inline)) {
+    if (g >= total) return;
+    const uint4* src = (const uint4*)((const uint8_t*)a.x + (row * a.k + b * QK + 16 * p16) * (a.xbf16 ? 2 : 4));
+    raw[0] = src[0], raw[1] = src[1];
+    if (!a.xbf16) raw[2] = src[2], raw[3] = src[3];
+  };
+  constexpr bool kOneToken = GATEUP && MAXM == 1;  // its row is known before its experts are
+  if (kOneToken && !rows_wave) {
+    fetch(nb, g, 0, g, first);
+    fetch(nb, g + step, 0, g + step, second);
+  }
 
   // the pairs' experts
+  int e_lane = -1;
   if constexpr (GATEUP) {
     for (int t = wave; t < a.n_tokens; t += waves) {
-      int id;
-      float wt;
       route_token(a.logits, a.logits_bf16 != 0, (long long)t * a.n_experts, a.n_experts, a.top_k, a.norm_topk != 0,
-                  a.scale, id, wt);
-      if (lane < a.top_k) {
-        sid[t * a.top_k + lane] = id;
-        if (wg == 0) a.ids[t * a.top_k + lane] = id, a.wts[t * a.top_k + lane] = wt;
-      }
+                  a.scale, wg == 0, [&](int slot, int id, float wt) {
+                    sid[t * a.top_k + slot] = id;
+                    if (wg == 0) a.ids[t * a.top_k + slot] = id, a.wts[t * a.top_k + slot] = wt;
+                  });
     }
-    if (wg == 0)
-      for (int i = tid; i < (int)gridDim.x; i += blockDim.x) a.counters[i] = 0;
-    __syncthreads();
+    lds_barrier();
+    if (lane < pairs) e_lane = sid[lane];
   } else {
-    if (wave == 0 && lane < pairs) {
-      sid[lane] = a.ids[lane];
-      swt[lane] = a.wts[lane];
-    }
-    __syncthreads();
+    if (lane < pairs) e_lane = a.ids[lane];
   }
-  const int e_lane = lane < pairs ? sid[lane] : -1;
   uint64_t same, leaders;
   const int bits = a.n_experts > 1 ? 32 - __builtin_clz(a.n_experts - 1) : 0;
   const int items = count_items<MAXM>(e_lane, bits, same, leaders);
-  const YOut out{a.out};
-  if (items == 0) {  // no token has an expert
-    if constexpr (!GATEUP)
-      for (long long i = (long long)wg * blockDim.x + tid; i < (long long)a.n_tokens * a.n;
-           i += (long long)gridDim.x * blockDim.x)
-        out.put(i, 0.0f);
-    return;
+  if (items == 0) return;  // no token has an expert
+  // The item of this workgroup, its leading pair, and the workgroup's place among the item's. The workgroups are
+  // shared out by the items' costs: a set of rows takes a third longer for each further pair (8 tokens of 8 experts
+  // top 2, 4096 x 14336: one pair 58 us, four 117 with equal shares).
+  int lead, part, wpi;
+  if constexpr (MAXM == 1) {
+    wpi = (int)gridDim.x / items;
+    const int item = wg / wpi;
+    part = wg - item * wpi;
+    if (item >= items) return;
+    uint64_t rest = leaders;
+    for (int i = 0; i < item; ++i) rest &= rest - 1;
+    lead = __builtin_ctzll(rest);
+  } else {
+    const bool leads = (leaders >> lane) & 1;
+    const int cost = leads ? 2 + min(MAXM, __popcll(same & ~((1ull << lane) - 1ull))) : 0;
+    int upto = cost;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int x = __shfl_up(upto, off, 64);
+      if (lane >= off) upto += x;
+    }
+    const int all = __builtin_amdgcn_readlane(upto, 63), grid = (int)gridDim.x;
+    const int from = (upto - cost) * grid / all, to = upto * grid / all;  // at least two each: launch_moe_layer
+    lead = __builtin_ctzll(__ballot(leads && wg >= from && wg < to));
+    wpi = __builtin_amdgcn_readlane(to - from, lead);
+    part = wg - __builtin_amdgcn_readlane(from, lead);
   }
-  const int wpi = (int)gridDim.x / items, item = wg / wpi, part = wg - item * wpi;
-  if (item >= items) return;
-  // the item's leading pair (the item-th set bit of the leaders), its expert and pairs
-  uint64_t rest = leaders;
-  for (int i = 0; i < item; ++i) rest &= rest - 1;
-  const int lead = __builtin_ctzll(rest);
   const int expert = __builtin_amdgcn_readlane(e_lane, lead);
   const uint64_t own = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)same, lead) |
                        (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(same >> 32), lead) << 32;
@@ -216,47 +287,40 @@ __global__ __launch_bounds__(MAXM == 1 ? 1024 : 512) void moe_layer_kernel(Layer
   uint64_t left = mine;
   const int p0 = next(left), p1 = next(left), p2 = next(left), p3 = next(left);
   static_assert(MAXM <= 4, "an item's pairs");
-  const auto pair = [=](int m) __attribute__((always_inline)) { return m == 0 ? p0 : m == 1 ? p1 : m == 2 ? p2 : p3; };  // pair m < M
+  const auto pair = [=](int m) __attribute__((always_inline)) {
+    return p0 + (m > 0 ? p1 - p0 : 0) + (m > 1 ? p2 - p1 : 0) + (m > 2 ? p3 - p2 : 0);
+  };  // pair m < M
 
   const int R = a.R, sets = (a.n + R - 1) / R;
-  const int lo = (int)((long long)part * sets / wpi), hi = (int)((long long)(part + 1) * sets / wpi);
+  const int lo = part * sets / wpi, hi = (part + 1) * sets / wpi;  // below 2^8 * 2^14
   const int blocks = R * nb, stage = layer_stage_bytes<TYPE>(blocks);
   uint8_t* const region = acts + layer_act_bytes(MAXM, nb) + (size_t)wave * layer_region_bytes<TYPE, MAXM, GATEUP>(blocks);
   float* const Vbuf = (float*)(region + kMats * stage);  // [matrix][row m][64]
   float* const Dbuf = Vbuf + kMats * MAXM * 64;          // [matrix][64]
-  const bool rows_wave = wave < W;
   const uintptr_t base0 = (uintptr_t)a.w0 + (uintptr_t)((long long)expert * a.stride);
   const uintptr_t base1 = (uintptr_t)a.w1 + (uintptr_t)((long long)expert * a.stride);
   const uint32_t lane16 = 16u * (uint32_t)lane;
 
-  // the packed bytes of set s's rows into the stage, from the 16-byte word that holds the first
-  const auto issue = [&](int s) {
-    const int n0 = s * R, nrows = min(R, a.n - n0);
-#pragma unroll
-    for (int t = 0; t < kMats; ++t) {
-      const uintptr_t src = (t == 0 ? base0 : base1) + (uintptr_t)n0 * (uintptr_t)a.row_bytes;
-      const uint32_t bytes = (uint32_t)nrows * (uint32_t)a.row_bytes + (uint32_t)(src & 15);
-      const void* from = (const void*)(src & ~(uintptr_t)15);
-      const uint32_t to = lds_addr(region) + (uint32_t)(t * stage);
-      for (uint32_t c = 0; c < bytes; c += 1024)
-        if (c + lane16 < bytes) copy16_to_lds_s_nt(from, c + lane16, to + c);
-    }
+  // The packed bytes of set s's rows of matrix t into its stage, from the 16-byte word that holds the first, and the
+  // copies that takes (none past the last set).
+  const auto span = [&](int s, int t, uintptr_t& from) __attribute__((always_inline)) {
+    const int n0 = s * R;
+    const uintptr_t src = (t == 0 ? base0 : base1) + (uintptr_t)n0 * (uintptr_t)a.row_bytes;
+    from = src & ~(uintptr_t)15;
+    return s < hi ? (uint32_t)min(R, a.n - n0) * (uint32_t)a.row_bytes + (uint32_t)(src & 15) : 0u;
+  };
+  const auto issue = [&](int s, int t) __attribute__((always_inline)) {
+    uintptr_t from;
+    const uint32_t bytes = span(s, t, from), to = lds_addr(region) + (uint32_t)(t * stage);
+    for (uint32_t c = 0; c < bytes; c += 1024)
+      if (c + lane16 < bytes) copy16_to_lds_s_nt((const void*)from, c + lane16, to + c);
+    return (int)((bytes + 1023) / 1024);
   };
 
-  // the item's activation rows to Q8_K, by the waves that own no rows: 16 lanes a block, four blocks a wave at a
-  // time, the first eight a wave requested before the weights
-  const int stagers = waves - W, total = M * nb, p16 = lane & 15;
-  const auto source = [&](int g) __attribute__((always_inline)) {  // block g's 16 values of this lane
-    const int m = g / nb, b = g - m * nb;
-    int row = MAXM == 1 ? lead : pair(m);
-    if constexpr (GATEUP) row /= a.top_k;
-    return (long long)row * a.k + b * QK + 16 * p16;
-  };
-  const auto fetch = [&](int g, uint4 (&raw)[4]) __attribute__((always_inline)) {
-    if (g >= total) return;
-    const uint4* src = (const uint4*)((const uint8_t*)a.x + source(g) * (a.xbf16 ? 2 : 4));
-    raw[0] = src[0], raw[1] = src[1];
-    if (!a.xbf16) raw[2] = src[2], raw[3] = src[3];
+  const int total = M * nb;
+  const auto fetch_pair = [&](int g, uint4 (&raw)[4]) __attribute__((always_inline)) {  // block g of the item's rows
+    const int m = MAXM == 1 ? 0 : g / nb, p = MAXM == 1 ? lead : pair(m);
+    fetch(total, g, GATEUP ? p / a.top_k : p, g - m * nb, raw);
   };
   const auto quantize = [&](int g, const uint4 (&raw)[4]) __attribute__((always_inline)) {
     if (g >= total) return;  // uniform over the block's 16 lanes
@@ -272,27 +336,31 @@ __global__ __launch_bounds__(MAXM == 1 ? 1024 : 512) void moe_layer_kernel(Layer
     }
     q8k_part16(v, p16, aq + (size_t)g * kActStride, abs_ + 16 * g, ad + g, a.reciprocal != 0);
   };
-  int s = lo + wave;
+  int s = lo + wave, behind = 0;  // copies issued behind those of the matrix that is waited for next
   if (rows_wave) {
-    __syncthreads();  // the activations are requested
-    if (s < hi) issue(s);
+    __builtin_amdgcn_s_barrier();  // the activations are requested
+    // no load of this wave's is in flight: said here, or the compiler, which sees the other waves' loads into the
+    // same registers, waits for every copy before it issues the next
+    wait_vmcnt(0);
+    issue(s, 0);
+    if constexpr (GATEUP) behind = issue(s, 1);
   } else {
-    const int step = 4 * stagers;
-    int g = 4 * (wave - W) + (lane >> 4);
-    uint4 first[4] = {}, second[4] = {};
-    fetch(g, first);
-    fetch(g + step, second);
-    __syncthreads();
+    if (!kOneToken) {
+      fetch_pair(g, first);
+      fetch_pair(g + step, second);
+    }
+    __builtin_amdgcn_sched_barrier(0);  // not sunk below the barrier
+    __builtin_amdgcn_s_barrier();
     for (;;) {
       quantize(g, first);
       quantize(g + step, second);
       g += 2 * step;
       if (__ballot(g < total) == 0) break;
-      fetch(g, first);
-      fetch(g + step, second);
+      fetch_pair(g, first);
+      fetch_pair(g + step, second);
     }
   }
-  __syncthreads();  // the activations are in LDS
+  lds_barrier();  // the activations are in LDS
 
   if (rows_wave) {
     const int b = lane % nb;
@@ -305,31 +373,61 @@ __global__ __launch_bounds__(MAXM == 1 ? 1024 : 512) void moe_layer_kernel(Layer
     for (; s < hi; s += W) {
       const int n0 = s * R, nrows = min(R, a.n - n0);
       const int jl = min(lane, nrows * nb - 1);  // lanes past the rows redo the last block
-      wait_vmcnt(0);
+      ActRegs areg;  // the lane's activation block, for both matrices (again for every set: held across them it spills)
+      if constexpr (kReg) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) areg.q[i] = ab[0].q16(16 * i);
+        areg.bs[0] = ab[0].bs8(0);
+        areg.bs[1] = ab[0].bs8(1);
+      }
 #pragma unroll 1  // one copy of the block arithmetic
       for (int t = 0; t < kMats; ++t) {
+        // Copies land in order: a matrix is computed while the other one's are in flight. (A store of the last set's
+        // fold behind them makes this wait for one copy more than it has to.)
+        wait_vmcnt(behind);
         // bases are 16-byte aligned; only Q6_K rows can start between 16-byte words
         const int delta = TYPE == T_Q6_K ? (int)(((uintptr_t)n0 * (uintptr_t)a.row_bytes) & 15) : 0;
         float V[MAXM], D;
-        L::template compute<MAXM, ActBlock>(region + t * stage, delta + jl * L::kBytes, ab, M, V, D);
+        if constexpr (kReg)
+          L::template compute<1, ActRegs>(region + t * stage, delta + jl * L::kBytes, &areg, 1, V, D);
+        else
+          L::template compute<MAXM, ActBlock>(region + t * stage, delta + jl * L::kBytes, ab, M, V, D);
 #pragma unroll
         for (int m = 0; m < MAXM; ++m)
           if (m < M) Vbuf[(t * MAXM + m) * 64 + lane] = V[m];
         if (L::kHasD) Dbuf[t * 64 + lane] = D;
+        __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the stage has been read
+        wave_sync();
+        const int n = issue(s + W, t);
+        if constexpr (GATEUP) behind = n;
       }
-      __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the stage has been read
-      wave_sync();
-      if (s + W < hi) issue(s + W);
       for (int f = lane; f < R * M; f += 64) {  // row f % R of activation row f / R
         const int fr = f % R, fm = f / R;
         if (fr >= nrows) continue;
         const float* xd = ad + fm * nb;
         float acc[2] = {0.0f, 0.0f};
-        for (int i = 0; i < nb; ++i)
+        const float* vr = Vbuf + fm * 64 + fr * nb;
+        const float* dr = Dbuf + fr * nb;
+        constexpr int kC = 8;  // operands read before they are folded
+        for (int i = 0; i < nb; i += kC) {
+          float xx[kC], vv[kMats][kC], dd[kMats][kC];
 #pragma unroll
-          for (int t = 0; t < kMats; ++t)
-            acc[t] = L::fold(acc[t], xd[i], Vbuf[(t * MAXM + fm) * 64 + fr * nb + i],
-                             L::kHasD ? Dbuf[t * 64 + fr * nb + i] : 0.0f);
+          for (int j = 0; j < kC; ++j) {
+            const int c = min(i + j, nb - 1);
+            xx[j] = xd[c];
+#pragma unroll
+            for (int t = 0; t < kMats; ++t) {
+              vv[t][j] = vr[t * MAXM * 64 + c];
+              dd[t][j] = L::kHasD ? dr[t * 64 + c] : 0.0f;
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < kC; ++j)
+            if (i + j < nb) {
+#pragma unroll
+              for (int t = 0; t < kMats; ++t) acc[t] = L::fold(acc[t], xx[j], vv[t][j], dd[t][j]);
+            }
+        }
         const int p = MAXM == 1 ? lead : pair(fm);
         const long long at = (long long)p * a.n + n0 + fr;
         if constexpr (GATEUP) {
@@ -347,68 +445,28 @@ __global__ __launch_bounds__(MAXM == 1 ? 1024 : 512) void moe_layer_kernel(Layer
       wave_sync();  // the block values are read before the next set's are written
     }
   }
-  if constexpr (!GATEUP) {
-    // the range's last item adds the items' rows up
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's rows are written
-    __syncthreads();
-    if (tid == 0) {
-      __threadfence();
-      *flag = atomicAdd(a.counters + part, 1);
-    }
-    __syncthreads();
-    if (*flag != items - 1) return;
-    __threadfence();
-    // a token's slots in ascending expert, those without one last (and not read)
-    int* const place = (int*)acts;
-    __syncthreads();
-    if (wave == 0 && lane < pairs) {
-      const int t = lane / a.top_k, e = sid[lane];
-      int rank = 0, live = 0;
-      for (int i = t * a.top_k; i < (t + 1) * a.top_k; ++i) {
-        const int o = sid[i];
-        rank += o >= 0 && (e < 0 || o < e || (o == e && i < lane));
-        live += o >= 0;
-      }
-      if (e >= 0) place[t * a.top_k + rank] = lane;
-      if (lane == t * a.top_k) place[kLayerMaxPairs + t] = live;
-    }
-    __syncthreads();
-    const int r0 = lo * R, nr = min(a.n, hi * R) - r0;
-    const float* down = (const float*)a.act;
-    for (int i = tid; i < nr * a.n_tokens; i += blockDim.x) {
-      const int t = i / nr, r = r0 + i - t * nr, live = place[kLayerMaxPairs + t];
-      float acc = 0.0f;
-      for (int j = 0; j < live; ++j) {
-        const int p = place[t * a.top_k + j];
-        float v = down[(long long)p * a.n + r];
-        if (a.xbf16) v = bf16_to_float(bf16_rne(v));
-        acc = acc + v * swt[p];
-      }
-      out.put((long long)t * a.n + r, acc);
-    }
-  }
 }
 
 // The routing alone: a wave per token.
 __global__ __launch_bounds__(256) void moe_topk_kernel(const void* __restrict__ logits, int bf16, int n_tokens,
                                                        int n_experts, int top_k, int norm_topk, float scale,
                                                        int32_t* __restrict__ ids, float* __restrict__ wts) {
-  const int lane = threadIdx.x & 63, t = (int)blockIdx.x * 4 + ((int)threadIdx.x >> 6);
+  const int t = (int)blockIdx.x * 4 + ((int)threadIdx.x >> 6);
   if (t >= n_tokens) return;
-  int id;
-  float wt;
-  route_token(logits, bf16 != 0, (long long)t * n_experts, n_experts, top_k, norm_topk != 0, scale, id, wt);
-  if (lane < top_k) ids[(long long)t * top_k + lane] = id, wts[(long long)t * top_k + lane] = wt;
+  route_token(logits, bf16 != 0, (long long)t * n_experts, n_experts, top_k, norm_topk != 0, scale, true,
+              [&](int slot, int id, float wt) {
+                ids[(long long)t * top_k + slot] = id;
+                wts[(long long)t * top_k + slot] = wt;
+              });
 }
 
 // Rows per wave, row waves and LDS for a matrix of rows of nb blocks; false when not one wave's rows fit.
 template <int TYPE, int MAXM, bool GATEUP>
 bool layer_shape(int nb, int& R, int& W, int& lds) {
-  constexpr int kWaves = MAXM == 1 ? 16 : 8, kStagers = MAXM == 1 ? 4 : 2;
   R = 64 / nb;
   const int region = layer_region_bytes<TYPE, MAXM, GATEUP>(R * nb);
   const int act = kLayerFixed + layer_act_bytes(MAXM, nb);
-  W = min(kWaves - kStagers, (kLayerLds - act) / region);
+  W = min(kLayerWaves - kLayerStagers, (kLayerLds - act) / region);
   lds = act + W * region;
   return W >= 1;
 }
@@ -419,30 +477,49 @@ int launch_layer(LayerArgs a, int grid, hipStream_t stream) {
   if (!layer_shape<TYPE, MAXM, GATEUP>(a.nb, a.R, a.W, lds)) return -1;
   auto kern = moe_layer_kernel<TYPE, MAXM, GATEUP>;
   allow_lds((const void*)kern, kLayerLds);
-  hipLaunchKernelGGL(kern, dim3(grid), dim3(MAXM == 1 ? 1024 : 512), lds, stream, a);
+  hipLaunchKernelGGL(kern, dim3(grid), dim3(64 * kLayerWaves), lds, stream, a);
   return 0;
 }
 
-template <bool GATEUP>
-bool layer_fits(int type, int nb, bool one) {
-  int R, W, lds;
+// Pairs of an item: one for one token; for more, four, or two where four rows of activations take the LDS of the
+// waves' stages (down on 56-block rows, eight tokens: 143 us with four, 139 with two).
+constexpr int kLayerLongRow = 32;
+inline int layer_pairs(bool one, int nb) { return one ? 1 : nb > kLayerLongRow ? 2 : 4; }
+
+// f.template operator()<TYPE, MAXM>() of a type and a number of pairs; -1 for another type.
+template <class F>
+int with_layer_kernel(int type, int pairs, F f) {
   switch (type) {
-    case T_Q4_K: return one ? layer_shape<T_Q4_K, 1, GATEUP>(nb, R, W, lds) : layer_shape<T_Q4_K, 4, GATEUP>(nb, R, W, lds);
-    case T_Q6_K: return one ? layer_shape<T_Q6_K, 1, GATEUP>(nb, R, W, lds) : layer_shape<T_Q6_K, 4, GATEUP>(nb, R, W, lds);
-    case T_Q8_0: return one ? layer_shape<T_Q8_0, 1, GATEUP>(nb, R, W, lds) : layer_shape<T_Q8_0, 4, GATEUP>(nb, R, W, lds);
-    default: return false;
+#define MXA_LAYER(t) \
+  case t: return pairs == 1 ? f.template operator()<t, 1>() : pairs == 2 ? f.template operator()<t, 2>() : f.template operator()<t, 4>();
+    MXA_LAYER(T_Q4_K)
+    MXA_LAYER(T_Q6_K)
+    MXA_LAYER(T_Q8_0)
+#undef MXA_LAYER
+    default: return -1;
   }
 }
 
 template <bool GATEUP>
-int launch_layer_type(int type, bool one, const LayerArgs& a, int grid, hipStream_t stream) {
-  switch (type) {
-    case T_Q4_K: return one ? launch_layer<T_Q4_K, 1, GATEUP>(a, grid, stream) : launch_layer<T_Q4_K, 4, GATEUP>(a, grid, stream);
-    case T_Q6_K: return one ? launch_layer<T_Q6_K, 1, GATEUP>(a, grid, stream) : launch_layer<T_Q6_K, 4, GATEUP>(a, grid, stream);
-    case T_Q8_0: return one ? launch_layer<T_Q8_0, 1, GATEUP>(a, grid, stream) : launch_layer<T_Q8_0, 4, GATEUP>(a, grid, stream);
-    default: return -1;
+struct LayerFits {
+  int nb;
+  template <int TYPE, int MAXM>
+  int operator()() const {
+    int R, W, lds;
+    return layer_shape<TYPE, MAXM, GATEUP>(nb, R, W, lds) ? 0 : -1;
   }
-}
+};
+
+template <bool GATEUP>
+struct LaunchLayer {
+  const LayerArgs& a;
+  int grid;
+  hipStream_t stream;
+  template <int TYPE, int MAXM>
+  int operator()() const {
+    return launch_layer<TYPE, MAXM, GATEUP>(a, grid, stream);
+  }
+};
 
 }  // namespace
 
@@ -452,12 +529,14 @@ bool moe_layer_supported(int gate_type, int down_type, int n_experts, int top_k,
       n_embd < QK || ffn < QK || n_embd > 64 * QK || ffn > 64 * QK)
     return false;
   const bool one = n_tokens == 1;
-  return layer_fits<true>(gate_type, n_embd / QK, one) && layer_fits<false>(down_type, ffn / QK, one);
+  const int kb = n_embd / QK, fb = ffn / QK;
+  return with_layer_kernel(gate_type, layer_pairs(one, kb), LayerFits<true>{kb}) == 0 &&
+         with_layer_kernel(down_type, layer_pairs(one, fb), LayerFits<false>{fb}) == 0;
 }
 
 size_t moe_layer_workspace(int n_tokens, int top_k, int n_embd, int ffn, bool bf16) {
   const size_t pairs = (size_t)n_tokens * top_k;
-  return align256(pairs * ffn * (bf16 ? 2 : 4)) + align256(pairs * n_embd * 4) + align256((size_t)cu_count() * 4);
+  return align256(pairs * ffn * (bf16 ? 2 : 4)) + align256(pairs * n_embd * 4);
 }
 
 int launch_moe_layer(int gate_type, int down_type, const uint8_t* gate, const uint8_t* up, long long gate_stride,
@@ -466,18 +545,20 @@ int launch_moe_layer(int gate_type, int down_type, const uint8_t* gate, const ui
                      float scale, int n_tokens, int n_embd, int ffn, bool reciprocal, int32_t* ids, float* wts,
                      YOut out, void* ws, hipStream_t stream) {
   const int grid = cu_count();
-  if (!moe_layer_supported(gate_type, down_type, n_experts, top_k, n_tokens, n_embd, ffn) || grid < n_tokens * top_k)
+  // a workgroup for every item, by their costs of 3 to 6
+  if (!moe_layer_supported(gate_type, down_type, n_experts, top_k, n_tokens, n_embd, ffn) || grid < 2 * n_tokens * top_k)
     return -1;
   const size_t pairs = (size_t)n_tokens * top_k;
   uint8_t* const act = (uint8_t*)ws;
   uint8_t* const rows = act + align256(pairs * ffn * (bf16 ? 2 : 4));
-  int32_t* const counters = (int32_t*)(rows + align256(pairs * n_embd * 4));
-  LayerArgs a{gate, up, gate_stride, gate_row, x, ids, wts, act, counters, logits, 0, ffn, n_embd, n_embd / QK, 0, 0,
+  LayerArgs a{gate, up, gate_stride, gate_row, x, ids, wts, act, logits, ffn, n_embd, n_embd / QK, 0, 0,
               n_experts, top_k, n_tokens, logits_bf16 ? 1 : 0, norm_topk ? 1 : 0, bf16 ? 1 : 0, reciprocal ? 1 : 0, scale};
-  if (launch_layer_type<true>(gate_type, n_tokens == 1, a, grid, stream) != 0) return -1;
-  a.w0 = down, a.w1 = nullptr, a.stride = down_stride, a.row_bytes = down_row, a.x = act, a.act = rows, a.out = out.v;
+  const bool one = n_tokens == 1;
+  if (with_layer_kernel(gate_type, layer_pairs(one, a.nb), LaunchLayer<true>{a, grid, stream}) != 0) return -1;
+  a.w0 = down, a.w1 = nullptr, a.stride = down_stride, a.row_bytes = down_row, a.x = act, a.act = rows;
   a.n = n_embd, a.k = ffn, a.nb = ffn / QK;
-  return launch_layer_type<false>(down_type, n_tokens == 1, a, grid, stream);
+  if (with_layer_kernel(down_type, layer_pairs(one, a.nb), LaunchLayer<false>{a, grid, stream}) != 0) return -1;
+  return launch_moe_combine((const float*)rows, nullptr, ids, wts, n_tokens, top_k, n_embd, bf16 ? 1 : 0, 1, out, stream);
 }
 
 int launch_moe_topk(const void* logits, bool bf16, int n_tokens, int n_experts, int top_k, bool norm_topk, float scale,

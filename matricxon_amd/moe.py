@@ -122,14 +122,14 @@ class HipPackedMoEExperts(nn.Module):
         token of -inf alone (padding) gets a row of zeros, whatever x holds there. `forward` on those ids and weights
         gives the same bits.
 
-        Up to eight tokens (and 64 pairs) of Q4_K, Q6_K or Q8_0 experts, gate and up of one type, with a SiLU: two
-        launches (`mxa_moe_layer`). Otherwise the routing in one launch, then the grouped projections.
+        Up to eight tokens (and 64 pairs) of Q4_K, Q6_K or Q8_0 experts, gate and up of one type, with a SiLU: one
+        library call, two launches over the weights and the sum (`mxa_moe_layer`). Otherwise the routing in one launch, then the grouped projections.
 
         `q8k_scale` "reciprocal" takes the codes of the activations' blocks as rint(v * (127 * (1 / amax))), which is
         what torch evaluates for `127.0 / amax`, for layers that were tuned or are checked against such an emulation;
         a code differs from the default's rint(v * (127 / amax)) only next to a half (one in some 2500 for bfloat16
         activations), but a layer's later roundings make 0.5% of the output of it. More than eight tokens then run
-        eight at a time, and a layer that the two launches do not take is refused (ValueError)."""
+        eight at a time, and a layer that this call does not take is refused (ValueError)."""
         if q8k_scale not in ("divide", "reciprocal"):
             raise ValueError(f'q8k_scale must be "divide" or "reciprocal", got {q8k_scale!r}')
         reciprocal = q8k_scale == "reciprocal"
@@ -164,7 +164,7 @@ class HipPackedMoEExperts(nn.Module):
     def _few_tokens(self, x: torch.Tensor, logits: torch.Tensor, top_k: int, norm_topk: bool, scale: float,
                     reciprocal: bool = False
                     ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor] | None:
-        """`forward_logits` in two launches, or None where they do not take the layer."""
+        """`forward_logits` in one library call, or None where it does not take the layer."""
         n_tokens, dev = x.shape[0], x.device
         if not 1 <= n_tokens <= _LAYER_MAX_TOKENS or not self._layer_ok:
             return None
