@@ -131,16 +131,18 @@ class HipFusedOps:
         be float32 beside a bfloat16 block; the weights and the gate have x's dtype, post_eps is eps unless given.
         Float32 steps; hidden and normed are each rounded once (rms_norm's bfloat16 steps round twice, as torch's
         do). None for what it does not take: CPU tensors, other dtypes or shapes, rows of more than 32768 values."""
-        k = x.shape[-1] if x.dim() else 0
-        others = [t for t in (weight, post_weight, gate) if t is not None]
-        if (not _handled(x, *others) or residual.dtype not in (torch.float32, x.dtype)
-                or residual.shape != x.shape or any(t.device != x.device for t in (residual, *others))
-                or not 1 <= k <= HipGemm.NORM_MAX_VALUES or x.numel() == 0
-                or any(w.shape != (k,) for w in (weight, post_weight) if w is not None)
-                or (gate is not None and not _broadcasts(gate.shape, x.shape))):
+        shape, dt, dev = x.shape, x.dtype, x.device
+        k = shape[-1] if shape else 0
+        if (dev.type != "cuda" or (dt is not torch.bfloat16 and dt is not torch.float32) or residual.shape != shape
+                or (residual.dtype is not dt and residual.dtype is not torch.float32) or residual.device != dev
+                or not 1 <= k <= HipGemm.NORM_MAX_VALUES or x.numel() == 0):
             return None
-        hidden, out, ws = self._gemm.add_rms_norm_q8k(residual, x, weight, eps, post_weight, post_eps, gate, scale,
-                                                      q8k)
+        for w in (weight,) if post_weight is None else (weight, post_weight):
+            if w.dtype is not dt or w.shape != (k,) or w.device != dev:
+                return None
+        if gate is not None and (gate.dtype is not dt or gate.device != dev or not _broadcasts(gate.shape, shape)):
+            return None
+        hidden, out, ws = self._gemm._add_rms_norm(residual, x, weight, eps, post_weight, post_eps, gate, scale, q8k)
         if ws is not None:
             HANDOFF.offer(out, ws)
         return hidden, out

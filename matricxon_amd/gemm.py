@@ -9,7 +9,6 @@ the packed weight is a device uint8 tensor instead of an mmap'd memoryview, x an
 device, and the call is asynchronous on torch's current HIP stream (no host sync).
 """
 
-import contextlib
 import ctypes
 import logging
 
@@ -37,12 +36,10 @@ def _stream(device: torch.device) -> int:
     return _RAW_STREAM(torch.cuda.current_device() if index is None else index)
 
 
-def _on(device: torch.device):
-    """A context in which `device` is the current one: a launch goes to the current device, whatever device its
-    tensors and its stream belong to. Nothing where it is already, as it mostly is."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def _elsewhere(device: torch.device) -> bool:
+    """Whether `device` is not the current one: a launch goes to the current device, whatever device its tensors and
+    its stream belong to."""
+    return device.index is not None and device.index != torch._C._cuda_getDevice()
 
 
 def _al256(n: int) -> int:
@@ -81,10 +78,26 @@ def _rows16(t: torch.Tensor, k: int) -> torch.Tensor:
     return _aligned16(t.detach().reshape(-1, k).contiguous())
 
 
-def _rows_of(t: torch.Tensor, k: int) -> torch.Tensor:
-    """`t` (..., k) as (rows, k) with unit column stride: a view where its rows are evenly spaced."""
-    t2 = t.detach() if t.dim() == 2 else t.detach().reshape(-1, k)
-    return t2 if t2.stride(1) == 1 or k == 1 else t2.contiguous()
+def _rows_of(t: torch.Tensor, k: int) -> tuple[torch.Tensor, int]:
+    """`t` (..., k) as rows of adjacent values, in place where they are evenly spaced, and their stride."""
+    t2 = t.detach().reshape(-1, k)
+    if t2.stride(1) != 1 and k > 1:
+        t2 = t2.contiguous()
+    return t2, t2.stride(0)
+
+
+_Strides3 = ctypes.c_longlong * 3
+
+
+def _head_strides(x: torch.Tensor, nd: int) -> tuple[torch.Tensor, ctypes.Array]:
+    """x (T, heads, dim) or (B, T, heads, dim) with adjacent values in a head (a copy where they are not), without its
+    history, and its strides of a sequence, a step and a head as the library takes them."""
+    x = x.detach()
+    st = x.stride()
+    if st[-1] != 1:
+        x = x.contiguous()
+        st = x.stride()
+    return x, _Strides3(0, st[0], st[1]) if nd == 3 else _Strides3(st[0], st[1], st[2])
 
 
 def _weight_arrays(items: list[tuple[int, torch.Tensor, int]], outs: list[int]):
@@ -449,33 +462,49 @@ class HipGemm:
         for name, w in (("weight", weight), ("post_weight", post_weight)):
             if w is not None and (w.shape != (k,) or w.dtype != dt or w.device != dev):
                 raise ValueError(f"{name} must be ({k},) {dt} on {dev}")
-        x2, r2 = _rows_of(x, k), _rows_of(residual, k)
-        weight = weight.contiguous()
-        post = None if post_weight is None else post_weight.contiguous()
-        g2, ldg, gstep = None, 0, 0
+        if gate is not None and (gate.dtype != dt or gate.device != dev):
+            raise ValueError(f"gate must be {dt} on {dev}")
+        return self._add_rms_norm(residual, x, weight, eps, post_weight, post_eps, gate, scale, want_q8k)
+
+    def _add_rms_norm(self, residual: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, eps: float,
+                      post_weight: torch.Tensor | None, post_eps: float | None, gate: torch.Tensor | None,
+                      scale: float, want_q8k: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
+        """The library call of `add_rms_norm_q8k` on checked operands."""
+        dev = x.device
+        if _elsewhere(dev):
+            with torch.cuda.device(dev):
+                return self._add_rms_norm(residual, x, weight, eps, post_weight, post_eps, gate, scale, want_q8k)
+        k = x.shape[-1]
+        m = x.numel() // k
+        x2, ldx = (x, k) if x.is_contiguous() else _rows_of(x, k)
+        r2, ldr = (residual, k) if residual.is_contiguous() else _rows_of(residual, k)
+        if not weight.is_contiguous():
+            weight = weight.contiguous()
+        post = 0
+        if post_weight is not None:
+            post_weight = post_weight.contiguous()
+            post = post_weight.data_ptr()
+        gate_ptr, ldg, gstep = 0, 0, 0
         if gate is not None:
-            if gate.dtype != dt or gate.device != dev:
-                raise ValueError(f"gate must be {dt} on {dev}")
-            g2 = gate.expand(x.shape).reshape(-1, k)  # RuntimeError where it does not broadcast
-            if g2.stride(1) > 1 and k > 1:
-                g2 = g2.contiguous()
-            ldg, gstep = g2.stride(0), min(g2.stride(1), 1) if k > 1 else 0
-        m = x2.shape[0]
-        hidden = torch.empty(x.shape, dtype=residual.dtype, device=dev)
-        out = torch.empty(x.shape, dtype=dt, device=dev)
-        ws = None
+            gate = gate.expand(x.shape).reshape(-1, k)  # RuntimeError where it does not broadcast
+            if gate.stride(1) > 1 and k > 1:
+                gate = gate.contiguous()
+            gate_ptr, ldg, gstep = gate.data_ptr(), gate.stride(0), min(gate.stride(1), 1) if k > 1 else 0
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+        hidden = torch.empty_like(residual, memory_format=torch.contiguous_format)
+        ws, ws_ptr, ws_bytes = None, 0, 0
         if want_q8k and k % 256 == 0:
-            ws = torch.empty(q8k_bytes(m, k), dtype=torch.uint8, device=dev)
+            ws_bytes = q8k_bytes(m, k)
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+            ws_ptr = ws.data_ptr()
         if m == 0:
             return hidden, out, ws
-        with _on(dev):
-            status = self._lib.mxa_add_rms_norm_q8_k(
-                x2.data_ptr(), x2.stride(0), r2.data_ptr(), r2.stride(0), None if post is None else post.data_ptr(),
-                float(eps if post_eps is None else post_eps), None if g2 is None else g2.data_ptr(), ldg, gstep,
-                float(scale), weight.data_ptr(), float(eps), m, k, int(dt == torch.bfloat16),
-                int(residual.dtype == torch.bfloat16), hidden.data_ptr(), out.data_ptr(),
-                None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), _stream(dev))
-        self._check(status, "mxa_add_rms_norm_q8_k", 15)
+        status = self._lib.mxa_add_rms_norm_q8_k(
+            x2.data_ptr(), ldx, r2.data_ptr(), ldr, post, float(eps if post_eps is None else post_eps), gate_ptr, ldg,
+            gstep, float(scale), weight.data_ptr(), float(eps), m, k, x.dtype is torch.bfloat16, residual.dtype is torch.bfloat16,
+            hidden.data_ptr(), out.data_ptr(), ws_ptr, ws_bytes, _stream(dev))
+        if status != 0:
+            self._check(status, "mxa_add_rms_norm_q8_k", 15)
         return hidden, out, ws
 
     ROPE_MAX_DIM = 1024
@@ -505,34 +534,29 @@ class HipGemm:
         if positions.dim() == 0 or positions.shape[-1] != lead[-1] or (
                 positions.dim() != 1 and (positions.dim() != nd - 2 or positions.shape[0] not in (1, lead[0]))):
             raise ValueError(f"positions must be {tuple(lead)} or {tuple(lead[-1:])}, got {tuple(positions.shape)}")
+        if _elsewhere(dev):
+            with torch.cuda.device(dev):
+                return self.rope(q, k, positions, turns, rotary_dim, interleaved, scale)
         seq = lead[-1]
         n_tokens = seq if nd == 3 else lead[0] * seq
         ps = positions.stride()
-        pos_batch = 0 if positions.dim() == 1 or positions.shape[0] == 1 else ps[0]
-        heads, strides, outs, held = [], [], [], []
-        for x in (q, k):
-            if x is None:
-                heads.append(0), strides.append(None), outs.append(None), held.append(None)
-                continue
-            x = x.detach()
-            if x.stride(-1) != 1:
-                x = x.contiguous()
-            st = x.stride()
-            heads.append(x.shape[-2])
-            strides.append((ctypes.c_longlong * 3)(st[0] if nd == 4 else 0, st[-3], st[-2]))
-            outs.append(torch.empty(x.shape, dtype=dt, device=dev))
-            held.append(x)
+        pos_batch = 0 if len(ps) == 1 or positions.shape[0] == 1 else ps[0]
+        q, q_strides = _head_strides(q, nd)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        k_heads, k_ptr, k_strides, k_out, k_out_ptr = 0, 0, None, None, 0
+        if k is not None:
+            k, k_strides = _head_strides(k, nd)
+            k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+            k_heads, k_ptr, k_out_ptr = k.shape[-2], k.data_ptr(), k_out.data_ptr()
         if n_tokens == 0:
-            return outs[0], outs[1]
-        with _on(dev):
-            status = self._lib.mxa_rope(
-                held[0].data_ptr(), strides[0], heads[0], None if k is None else held[1].data_ptr(), strides[1],
-                heads[1], positions.data_ptr(), int(positions.dtype == torch.int64), pos_batch, ps[-1],
-                turns.data_ptr(), n_tokens, seq, dim, int(rotary_dim), int(interleaved), float(scale),
-                int(dt == torch.bfloat16), outs[0].data_ptr(), None if k is None else outs[1].data_ptr(),
-                _stream(dev))
-        self._check(status, "mxa_rope", 0)
-        return outs[0], outs[1]
+            return q_out, k_out
+        status = self._lib.mxa_rope(
+            q.data_ptr(), q_strides, q.shape[-2], k_ptr, k_strides, k_heads, positions.data_ptr(),
+            positions.dtype is torch.int64, pos_batch, ps[-1], turns.data_ptr(), n_tokens, seq, dim, rotary_dim,
+            interleaved, scale, dt is torch.bfloat16, q_out.data_ptr(), k_out_ptr, _stream(dev))
+        if status != 0:
+            self._check(status, "mxa_rope", 0)
+        return q_out, k_out
 
     def silu_mul_q8k(self, gate: torch.Tensor, up: torch.Tensor,
                      want_out: bool = True) -> tuple[torch.Tensor | None, torch.Tensor]:
@@ -742,10 +766,12 @@ class HipGemm:
         weights = torch.empty((n_tokens, top_k), dtype=torch.float32, device=dev)
         if n_tokens == 0:
             return ids, weights
-        with _on(dev):
-            status = self._lib.mxa_moe_topk(logits.data_ptr(), int(logits.dtype == torch.bfloat16), n_tokens,
-                                            logits.shape[1], top_k, int(bool(norm_topk)), float(scale),
-                                            ids.data_ptr(), weights.data_ptr(), _stream(dev))
+        if _elsewhere(dev):
+            with torch.cuda.device(dev):
+                return self.moe_topk(logits, top_k, norm_topk, scale)
+        status = self._lib.mxa_moe_topk(logits.data_ptr(), int(logits.dtype == torch.bfloat16), n_tokens,
+                                        logits.shape[1], top_k, int(bool(norm_topk)), float(scale),
+                                        ids.data_ptr(), weights.data_ptr(), _stream(dev))
         self._check(status, "mxa_moe_topk", 0)
         return ids, weights
 

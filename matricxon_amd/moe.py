@@ -16,7 +16,7 @@ from collections.abc import Callable
 import torch
 from torch import nn
 
-from .gemm import HipGemm, _on, _stream, q8k_bytes
+from .gemm import HipGemm, _elsewhere, _stream, q8k_bytes
 
 
 def route_pairs(top_k_idx: torch.Tensor, num_experts: int) -> tuple[torch.Tensor, torch.Tensor,
@@ -93,11 +93,11 @@ class HipPackedMoEExperts(nn.Module):
         self._pairs = all(int(t) != 23 and k // 256 in (4, 8, 16, 32, 56, 64) and
                           self._gemm.row_bytes(int(t), k) % 16 == 0
                           for t, k in ((gate_type, n_embd), (up_type, n_embd), (down_type, ffn_len)))
-        # what mxa_moe_layer takes besides its sizes; its workspace by (tokens, top_k, device), 0 where it declines
+        # what mxa_moe_layer takes besides its sizes; its workspace by (tokens, top_k), 0 where it declines
         self._layer_ok = (gate_type == up_type and _is_silu(activation) and dtype in (torch.float32, torch.bfloat16)
                           and all(w.is_contiguous() and w.data_ptr() % 16 == 0 and w.stride(0) % 16 == 0
                                   for w in (gate, up, down)))
-        self._layer_bytes: dict[tuple[int, int, torch.device], int] = {}
+        self._layer_bytes: dict[tuple[int, int], int] = {}
         self.register_buffer("gate_packed", gate, persistent=False)
         self.register_buffer("up_packed", up, persistent=False)
         self.register_buffer("down_packed", down, persistent=False)
@@ -168,35 +168,39 @@ class HipPackedMoEExperts(nn.Module):
         n_tokens, dev = x.shape[0], x.device
         if not 1 <= n_tokens <= _LAYER_MAX_TOKENS or not self._layer_ok:
             return None
+        if _elsewhere(dev):
+            with torch.cuda.device(dev):
+                return self._few_tokens(x, logits, top_k, norm_topk, scale, reciprocal)
         lib, bf16 = self._gemm._lib, self.dtype == torch.bfloat16
         gt, _, dt = self.types
-        with _on(dev):
-            key = (n_tokens, top_k, dev)
-            ws_bytes = self._layer_bytes.get(key)
-            if ws_bytes is None:
-                ws_bytes = self._layer_bytes[key] = lib.mxa_moe_layer_workspace_bytes(
-                    gt, dt, self.num_experts, top_k, n_tokens, self.n_embd, self.ffn_len, int(bf16))
-            if ws_bytes == 0:
-                return None
-            xs = x.detach() if x.dtype == self.dtype else x.detach().to(self.dtype)
-            if not xs.is_contiguous() or xs.data_ptr() % 16 != 0:
-                xs = xs.clone(memory_format=torch.contiguous_format)
-            logits = logits.detach().contiguous()
-            gate, up, down = self.gate_packed, self.up_packed, self.down_packed
-            out = torch.empty(x.shape, dtype=x.dtype if x.dtype == torch.bfloat16 else torch.float32, device=dev)
-            ids = torch.empty((n_tokens, top_k), dtype=torch.int32, device=dev)
-            weights = torch.empty((n_tokens, top_k), dtype=torch.float32, device=dev)
-            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-            status = lib.mxa_moe_layer(
-                gt, dt, gate.data_ptr(), up.data_ptr(), gate.stride(0), down.data_ptr(), down.stride(0),
-                self.num_experts, xs.data_ptr(), int(bf16), logits.data_ptr(), int(logits.dtype == torch.bfloat16),
-                top_k, int(bool(norm_topk)), float(scale), n_tokens, self.n_embd, self.ffn_len, int(reciprocal),
-                ids.data_ptr(), weights.data_ptr(), out.data_ptr(), int(out.dtype == torch.bfloat16), ws.data_ptr(), ws_bytes,
-                _stream(dev))
+        ws_bytes = self._layer_bytes.get((n_tokens, top_k))
+        if ws_bytes is None:
+            ws_bytes = self._layer_bytes[n_tokens, top_k] = lib.mxa_moe_layer_workspace_bytes(
+                gt, dt, self.num_experts, top_k, n_tokens, self.n_embd, self.ffn_len, bf16)
+        if ws_bytes == 0:
+            return None
+        xs = x if x.dtype is self.dtype else x.detach().to(self.dtype)
+        if not xs.is_contiguous() or xs.data_ptr() % 16 != 0:
+            xs = xs.clone(memory_format=torch.contiguous_format)
+        if not logits.is_contiguous():
+            logits = logits.contiguous()
+        gate, up, down = self.gate_packed, self.up_packed, self.down_packed
+        out_bf16 = x.dtype is torch.bfloat16
+        out = torch.empty_like(x, dtype=torch.bfloat16 if out_bf16 else torch.float32,
+                               memory_format=torch.contiguous_format)
+        ids = torch.empty((n_tokens, top_k), dtype=torch.int32, device=dev)
+        weights = torch.empty((n_tokens, top_k), dtype=torch.float32, device=dev)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        status = lib.mxa_moe_layer(
+            gt, dt, gate.data_ptr(), up.data_ptr(), gate.stride(0), down.data_ptr(), down.stride(0), self.num_experts,
+            xs.data_ptr(), bf16, logits.data_ptr(), logits.dtype is torch.bfloat16, top_k, bool(norm_topk), float(scale),
+            n_tokens, self.n_embd, self.ffn_len, reciprocal, ids.data_ptr(), weights.data_ptr(), out.data_ptr(), out_bf16,
+            ws.data_ptr(), ws_bytes, _stream(dev))
         if status == -1:
             return None
-        self._gemm._check(status, "mxa_moe_layer", gt)
-        return (out if out.dtype == x.dtype else out.to(x.dtype)), ids, weights
+        if status != 0:
+            self._gemm._check(status, "mxa_moe_layer", gt)
+        return (out if out.dtype is x.dtype else out.to(x.dtype)), ids, weights
 
     def _grouped(self, x: torch.Tensor, top_k_weights: torch.Tensor, top_k_idx: torch.Tensor,
                  masked: bool = False) -> torch.Tensor:
