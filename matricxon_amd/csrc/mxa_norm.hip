@@ -14,6 +14,10 @@
 // alignment beyond their elements' (a row of odd length starts anywhere), and the last one of a row may be
 // short. Rows of up to 512 values take one wave each, four rows to a workgroup, with no barrier; longer
 // rows a workgroup.
+//
+// Bound: memory from some 1000 rows on (4096 x 4096 bfloat16 with both norms 29.9 us for the 134 MB of x, r, h and
+// n and the 19 MB of blocks: 5.1 TB/s, what a large copy reaches), below that the latency of the loads and the two
+// reductions (1 x 4096: 3.6 us).
 #include "mxa_kernels.hpp"
 
 #pragma clang fp contract(off)
@@ -67,8 +71,8 @@ __device__ __forceinline__ void load8(const void* p, long long i, int count, flo
   }
 }
 
-// Stores v as p's type and leaves in v what was stored.
-template <bool BF16>
+// Stores v as p's type (ONCE: past the caches, for what is not read again soon) and leaves in v what was stored.
+template <bool BF16, bool ONCE>
 __device__ __forceinline__ void store8(void* p, long long i, int count, float (&v)[8]) {
   if constexpr (BF16) {
     h16x8 t;
@@ -78,7 +82,11 @@ __device__ __forceinline__ void store8(void* p, long long i, int count, float (&
       v[e] = bf16_to_float(t[e]);
     }
     if (count == 8) {
-      *(h16x8*)((uint16_t*)p + i) = t;
+      h16x8* to = (h16x8*)((uint16_t*)p + i);
+      if constexpr (ONCE)
+        __builtin_nontemporal_store(t, to);
+      else
+        *to = t;
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -86,8 +94,15 @@ __device__ __forceinline__ void store8(void* p, long long i, int count, float (&
     }
   } else {
     if (count == 8) {
-      *(f32x4u*)((float*)p + i) = f32x4u{v[0], v[1], v[2], v[3]};
-      *(f32x4u*)((float*)p + i + 4) = f32x4u{v[4], v[5], v[6], v[7]};
+      const f32x4u t0{v[0], v[1], v[2], v[3]}, t1{v[4], v[5], v[6], v[7]};
+      f32x4u* to = (f32x4u*)((float*)p + i);
+      if constexpr (ONCE) {
+        __builtin_nontemporal_store(t0, to);
+        __builtin_nontemporal_store(t1, (f32x4u*)((float*)p + i + 4));
+      } else {
+        *to = t0;
+        *(f32x4u*)((float*)p + i + 4) = t1;
+      }
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
@@ -134,7 +149,7 @@ __device__ __forceinline__ void q8k_part8(const float (&v)[8], int lane, bool st
 }
 
 // Thread t of a row's T holds vectors t + T j, j < P.
-template <bool XB, bool RB, bool POST, int P>
+template <bool XB, bool RB, bool POST, int P, bool ONCE>
 __global__ __launch_bounds__(kNormMaxThreads) void add_rms_norm_kernel(NormArgs a, int T, int8_t* __restrict__ q,
                                                                        float* __restrict__ d,
                                                                        int16_t* __restrict__ bsums) {
@@ -201,7 +216,7 @@ __global__ __launch_bounds__(kNormMaxThreads) void add_rms_norm_kernel(NormArgs 
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) h[j][e] = fmaf(a.scale, u[j][e], h[j][e]);
-    store8<RB>(a.h, (long long)row * k + i, count[j], h[j]);
+    store8<RB, ONCE>(a.h, (long long)row * k + i, count[j], h[j]);
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (e < count[j]) s = fmaf(h[j][e], h[j][e], s);
@@ -216,7 +231,7 @@ __global__ __launch_bounds__(kNormMaxThreads) void add_rms_norm_kernel(NormArgs 
       load8<XB>(a.w, i, count[j], w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) h[j][e] = h[j][e] * scale * w[e];
-      store8<XB>(a.n, (long long)row * k + i, count[j], h[j]);
+      store8<XB, ONCE>(a.n, (long long)row * k + i, count[j], h[j]);
     }
     if (q != nullptr) {  // every lane of the wave: k is a multiple of 256, a half wave holds a block or nothing
       const size_t b = (size_t)row * nb + (i >> 8);
@@ -228,10 +243,13 @@ __global__ __launch_bounds__(kNormMaxThreads) void add_rms_norm_kernel(NormArgs 
 template <bool XB, bool RB, bool POST>
 void launch_norm(const NormArgs& a, const ActBuffers* q, hipStream_t stream) {
   const int nv = (a.k + 7) / 8;
-  // Few rows: as many threads a row as there are vectors. Many rows: two vectors a thread, half the waves
-  // and reductions for the same bytes in flight.
+  // Few rows: as many threads a row as there are vectors. Many rows: two vectors a thread, half the waves and
+  // reductions for the same bytes in flight, and h and n past the caches, which they would not survive in (bfloat16
+  // rows of 4096 with a norm on both sides, kernel alone: 4096 rows one vector a thread 37.1 us, two 35.8, two past
+  // the caches 29.9, four 45.8; 1024 rows 13.1 and 11.9 past the caches; 256 rows one vector 6.2 and 5.8).
+  const bool many = a.rows > 512;
   const int fewest = (nv + kNormMaxThreads - 1) / kNormMaxThreads;
-  const int want = a.rows > 512 && nv >= 128 ? 2 : 1;
+  const int want = many && nv >= 128 ? 2 : 1;
   const int p = max(fewest, want) <= 1 ? 1 : max(fewest, want) <= 2 ? 2 : 4;
   const int T = ((nv + p - 1) / p + 63) / 64 * 64;
   const int waves = T == 64 ? 4 : T / 64;
@@ -239,9 +257,12 @@ void launch_norm(const NormArgs& a, const ActBuffers* q, hipStream_t stream) {
   int8_t* qq = q != nullptr ? q->q : nullptr;
   float* qd = q != nullptr ? q->d : nullptr;
   int16_t* qb = q != nullptr ? q->bsums : nullptr;
-  auto kern = p == 1 ? add_rms_norm_kernel<XB, RB, POST, 1>
-            : p == 2 ? add_rms_norm_kernel<XB, RB, POST, 2>
-                     : add_rms_norm_kernel<XB, RB, POST, 4>;
+  auto kern = many ? (p == 1 ? add_rms_norm_kernel<XB, RB, POST, 1, true>
+                      : p == 2 ? add_rms_norm_kernel<XB, RB, POST, 2, true>
+                               : add_rms_norm_kernel<XB, RB, POST, 4, true>)
+                   : (p == 1 ? add_rms_norm_kernel<XB, RB, POST, 1, false>
+                      : p == 2 ? add_rms_norm_kernel<XB, RB, POST, 2, false>
+                               : add_rms_norm_kernel<XB, RB, POST, 4, false>);
   hipLaunchKernelGGL(kern, grid, block, 0, stream, a, T, qq, qd, qb);
 }
 

@@ -14,6 +14,9 @@
 // A thread keeps one place of the heads (a vector of V pairs, or of V / 2 pairs interleaved) and walks over the
 // (token, head) rows of its workgroup, a batch of rows requested before the first is computed; the first batch is
 // requested before the angles.
+//
+// Bound: memory from some 500 tokens on (4096 tokens of 32 + 8 bfloat16 heads of 128: 15.5 us for 84 MB, 5.4 TB/s, a
+// large copy's rate), below that latency: the positions and the table, then sine and cosine (one token 3.1 us).
 #include "mxa_kernels.hpp"
 
 #pragma clang fp contract(off)
@@ -62,8 +65,8 @@ __device__ __forceinline__ T narrow(float v) {
     return v;
 }
 
-// T the element type; V values of a vector (an even number for interleaved pairs).
-template <class T, bool INTER, int V>
+// T the element type; V values of a vector (an even number for interleaved pairs); ONCE: stored past the caches.
+template <class T, bool INTER, int V, bool ONCE>
 __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a, int TP, int C, int CR, int HP) {
   extern __shared__ __align__(16) float trig[];  // cos of (token, pair), then sin
   union Piece {
@@ -97,9 +100,15 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a, int TP, 
       if constexpr (!INTER) y.v = *(const typename Vec<T, V>::type*)(src + half + c * V);
     }
   };
+  const auto put = [&](T* to, const Piece& p) __attribute__((always_inline)) {
+    if constexpr (ONCE)
+      __builtin_nontemporal_store(p.v, (typename Vec<T, V>::type*)to);
+    else
+      *(typename Vec<T, V>::type*)to = p.v;
+  };
   const auto store = [&](T* dst, int t, int c, Piece& x, Piece& y) {
     if (c >= CR) {
-      *(typename Vec<T, V>::type*)(dst + a.rot + (c - CR) * V) = x.v;
+      put(dst + a.rot + (c - CR) * V, x);
       return;
     }
     if constexpr (INTER) {
@@ -118,9 +127,9 @@ __global__ __launch_bounds__(kRopeThreads) void rope_kernel(RopeArgs a, int TP, 
         x.e[i] = narrow<T>(fmaf(u, co, -(v * si)));
         y.e[i] = narrow<T>(fmaf(u, si, v * co));
       }
-      *(typename Vec<T, V>::type*)(dst + half + c * V) = y.v;
+      put(dst + half + c * V, y);
     }
-    *(typename Vec<T, V>::type*)(dst + c * V) = x.v;
+    put(dst + c * V, x);
   };
 
   bool angles = false;
@@ -164,10 +173,16 @@ void launch_rope_v(const RopeArgs& a, hipStream_t stream) {
   const int C = CR + (a.dim - a.rot) / V;
   const int HP = max(1, kRopeThreads / C);  // heads side by side in a workgroup
   const int H = a.q.heads + a.k.heads;
-  // few tokens: the heads of one token over several workgroups, a row a thread; many: four tokens each
-  const int TP = a.n_tokens >= 1024 ? 4 : 1;
-  const int split = a.n_tokens >= 1024 ? 1 : (H + HP - 1) / HP;
-  hipLaunchKernelGGL((rope_kernel<T, INTER, V>), dim3((a.n_tokens + TP - 1) / TP, split), dim3(kRopeThreads),
+  // Up to 512 tokens the heads of one token over several workgroups, a row a thread (32 + 8 bfloat16 heads of 128,
+  // kernel alone: 300 tokens 5.0 us, a workgroup a token 5.4; 700 tokens 7.0 and 6.3). More: a workgroup a token, or
+  // as many tokens each as leave about a thousand workgroups, what the CUs hold at once (1500 tokens by one 11.2, by
+  // two 10.2, by four 11.6; 4096 by two 19.6, by four 17.3, by eight 19.6), stored past the caches, which the heads
+  // of so many tokens would not survive in (700 tokens 6.3 and 6.0, 1500 10.2 and 8.4, 4096 17.3 and 15.5).
+  const bool many = a.n_tokens > 512;
+  const int TP = many ? min(8, (a.n_tokens + 1023) / 1024) : 1;
+  const int split = many ? 1 : (H + HP - 1) / HP;
+  auto kern = many ? rope_kernel<T, INTER, V, true> : rope_kernel<T, INTER, V, false>;
+  hipLaunchKernelGGL(kern, dim3((a.n_tokens + TP - 1) / TP, split), dim3(kRopeThreads),
                      (size_t)TP * a.rot * sizeof(float), stream, a, TP, C, CR, HP);
 }
 

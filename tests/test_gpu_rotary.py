@@ -87,7 +87,7 @@ def test_far_positions(gpu, scaling, start) -> None:
     check(rot, k, k2, pos)
 
 
-@pytest.mark.parametrize("t", [1, 3, 1023, 1024, 1027])
+@pytest.mark.parametrize("t", [1, 3, 512, 513, 1023, 1024, 1027, 2051, 9001])
 @pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
 def test_columns_of_a_fused_projection(gpu, t, dt) -> None:
     """q and k as columns of one q | k | v buffer; token counts on both sides of the kernel's token tiles."""
