@@ -286,7 +286,7 @@ int mxa_moe_topk(const void *logits, int logits_bf16, int n_tokens, int n_expert
 size_t mxa_moe_layer_workspace_bytes(int gate_type, int down_type, int n_experts, int top_k, int n_tokens,
                                      int n_embd, int ffn_len, int bf16);
 
-/* A whole mixture-of-experts layer of packed experts for a few tokens, in two launches and the combine: the routing of
+/* A whole mixture-of-experts layer of packed experts for a few tokens, in two launches (three past 16 pairs): the routing of
  * mxa_moe_topk, silu(gate_e x) * (up_e x) of each token's experts, down_e of that, and their weighted sum
  * in ascending expert id. x (n_tokens, n_embd) bfloat16 (bf16 != 0) or float32, 16-byte aligned; expert e at
  * gate and up + e * gate_stride (ffn_len rows) and down + e * down_stride (n_embd rows), 16-byte aligned

@@ -1,10 +1,9 @@
-// A mixture-of-experts layer of packed experts for a few tokens, from the router's logits, in two launches and the
-// combine:
+// A mixture-of-experts layer of packed experts for a few tokens, from the router's logits, in two launches:
 //
 //   ids, w  = the top_k largest logits of a token and their softmax weights
 //   act_p   = silu(gate_e x_t) * (up_e x_t)    for each pair p = (token t, expert e = ids[p])     first launch
 //   down_p  = down_e act_p                                                                       second launch
-//   y_t     = sum over the token's pairs, experts ascending, of w_p * down_p                      mxa_moe.hip
+//   y_t     = sum over the token's pairs, experts ascending, of w_p * down_p   second, or for many pairs mxa_moe.hip's
 //
 // with the steps of the grouped path (mxa_gemm_moe, mxa_silu_mul_q8_k, mxa_moe_combine): x and act as Q8_K blocks,
 // gate, up, silu, their product and each down row rounded to bfloat16 in a bfloat16 layer, the sum in float32. The
@@ -28,9 +27,10 @@
 // the part of a wave's turn in which its stage is not in flight. 64 experts top 8 of 2048 x 1024, one token: 11.7
 // and 8.2 us, latency from end to end (logits, routing, activations, weights, block arithmetic).
 //
-// Adding the pairs up in the second launch, by the last workgroup to finish a range of rows, was slower than the
-// combine's launch: the fences that such a hand-over needs between XCDs cost the weights' stream more (down 62.8
-// against 29.3 + 4.4 us, one token of 8 experts top 2, 4096 x 14336 with Q6_K down).
+// The sum needs every pair's rows in one place. Up to 16 pairs the second launch's workgroups take rows, each through
+// all items, and add up in LDS. For more they take items, and the combine is a launch of its own (4 to 5 us): adding up
+// by the last workgroup to finish a range of rows was slower, the fences that such a hand-over needs between XCDs cost
+// the weights' stream more (down 62.8 against 29.3 + 4.4 us, one token of 8 experts top 2, 4096 x 14336).
 #include "mxa_kernels.hpp"
 #include "mxa_lpb.hpp"
 
@@ -181,6 +181,91 @@ __device__ __forceinline__ int count_items(int e, int bits, uint64_t& same, uint
   return __popcll(leaders);
 }
 
+// The expert and the pairs of the item that lane `lead` leads: the lanes of `mine`, the first M of them.
+struct LayerItem {
+  int expert, M, p0, p1, p2, p3;
+  __device__ __forceinline__ int pair(int m) const {  // m < M
+    return p0 + (m > 0 ? p1 - p0 : 0) + (m > 1 ? p2 - p1 : 0) + (m > 2 ? p3 - p2 : 0);
+  }
+};
+template <int MAXM>
+__device__ __forceinline__ LayerItem layer_item(int lead, int e_lane, uint64_t same) {
+  static_assert(MAXM <= 4, "an item's pairs");
+  const uint64_t own = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)same, lead) |
+                       (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(same >> 32), lead) << 32;
+  uint64_t left = own & ~((1ull << lead) - 1ull);
+  const auto next = [&]() __attribute__((always_inline)) {  // the next pair, -1 past the last
+    const int p = left != 0 ? __builtin_ctzll(left) : -1;
+    left &= left - 1;
+    return p;
+  };
+  LayerItem it;
+  it.expert = __builtin_amdgcn_readlane(e_lane, lead);
+  it.M = min(MAXM, __popcll(left));
+  it.p0 = next(), it.p1 = next(), it.p2 = next(), it.p3 = next();
+  return it;
+}
+
+// The lane's 16 of 256 activations from value `at` of x, and their Q8_K block part.
+__device__ __forceinline__ void fetch16(const LayerArgs& a, long long at, uint4 (&raw)[4]) {
+  const uint4* src = (const uint4*)((const uint8_t*)a.x + at * (a.xbf16 ? 2 : 4));
+  raw[0] = src[0], raw[1] = src[1];
+  if (!a.xbf16) raw[2] = src[2], raw[3] = src[3];
+}
+__device__ __forceinline__ void quantize16(const LayerArgs& a, const uint4 (&raw)[4], int p16, int8_t* q, int16_t* bs,
+                                           float* d) {
+  float v[16];
+  const uint32_t r[16] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w,
+                          raw[2].x, raw[2].y, raw[2].z, raw[2].w, raw[3].x, raw[3].y, raw[3].z, raw[3].w};
+  if (a.xbf16) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[2 * i] = bf16_to_float(r[i]), v[2 * i + 1] = bf16_to_float(r[i] >> 16);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __builtin_bit_cast(float, r[i]);
+  }
+  q8k_part16(v, p16, q, bs, d, a.reciprocal != 0);
+}
+
+// `bytes` packed bytes at src, with those before them in src's 16-byte word, to LDS address `to`; the copies it took.
+__device__ __forceinline__ int copy_rows(uintptr_t src, uint32_t bytes, uint32_t to) {
+  const uint32_t lane16 = 16u * (threadIdx.x & 63), end = bytes + (uint32_t)(src & 15);
+  const void* from = (const void*)(src & ~(uintptr_t)15);
+  for (uint32_t c = 0; c < end; c += 1024)
+    if (c + lane16 < end) copy16_to_lds_s_nt(from, c + lane16, to + c);
+  return (int)((end + 1023) / 1024);
+}
+
+// The fold of one row's nb block values in order, of MATS matrices at once (their values v and scales d `vstep` and
+// 64 apart); xd the activation row's scales.
+template <int TYPE, int MATS>
+__device__ __forceinline__ void fold_row(int nb, const float* xd, const float* v, int vstep, const float* d,
+                                         float (&acc)[MATS]) {
+  using L = Lpb<TYPE>;
+  constexpr int kC = 8;  // operands read before they are folded
+#pragma unroll
+  for (int t = 0; t < MATS; ++t) acc[t] = 0.0f;
+  for (int i = 0; i < nb; i += kC) {
+    float xx[kC], vv[MATS][kC], dd[MATS][kC];
+#pragma unroll
+    for (int j = 0; j < kC; ++j) {
+      const int c = min(i + j, nb - 1);
+      xx[j] = xd[c];
+#pragma unroll
+      for (int t = 0; t < MATS; ++t) {
+        vv[t][j] = v[t * vstep + c];
+        dd[t][j] = L::kHasD ? d[t * 64 + c] : 0.0f;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kC; ++j)
+      if (i + j < nb) {
+#pragma unroll
+        for (int t = 0; t < MATS; ++t) acc[t] = L::fold(acc[t], xx[j], vv[t][j], dd[t][j]);
+      }
+  }
+}
+
 template <int TYPE>
 constexpr int layer_stage_bytes(int blocks) {  // Q6_K rows start on any even byte
   return (blocks * Lpb<TYPE>::kBytes + (TYPE == T_Q6_K ? 15 : 0) + 1023) / 1024 * 1024;
@@ -217,10 +302,7 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_layer_kernel(LayerArgs a
   int g = 4 * (wave - W) + (lane >> 4);
   uint4 first[4] = {}, second[4] = {};
   const auto fetch = [&](int total, int g, long long row, int b, uint4 (&raw)[4]) __attribute__((always_inline)) {
-    if (g >= total) return;
-    const uint4* src = (const uint4*)((const uint8_t*)a.x + (row * a.k + b * QK + 16 * p16) * (a.xbf16 ? 2 : 4));
-    raw[0] = src[0], raw[1] = src[1];
-    if (!a.xbf16) raw[2] = src[2], raw[3] = src[3];
+    if (g < total) fetch16(a, row * a.k + b * QK + 16 * p16, raw);
   };
   constexpr bool kOneToken = GATEUP && MAXM == 1;  // its row is known before its experts are
   if (kOneToken && !rows_wave) {
@@ -274,22 +356,8 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_layer_kernel(LayerArgs a
     wpi = __builtin_amdgcn_readlane(to - from, lead);
     part = wg - __builtin_amdgcn_readlane(from, lead);
   }
-  const int expert = __builtin_amdgcn_readlane(e_lane, lead);
-  const uint64_t own = (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)same, lead) |
-                       (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(same >> 32), lead) << 32;
-  const uint64_t mine = own & ~((1ull << lead) - 1ull);  // this item's pairs: up to MAXM from the leader on
-  const int M = min(MAXM, __popcll(mine));
-  const auto next = [](uint64_t& left) {  // its lowest bit's place, -1 past the last
-    const int p = left != 0 ? __builtin_ctzll(left) : -1;
-    left &= left - 1;
-    return p;
-  };
-  uint64_t left = mine;
-  const int p0 = next(left), p1 = next(left), p2 = next(left), p3 = next(left);
-  static_assert(MAXM <= 4, "an item's pairs");
-  const auto pair = [=](int m) __attribute__((always_inline)) {
-    return p0 + (m > 0 ? p1 - p0 : 0) + (m > 1 ? p2 - p1 : 0) + (m > 2 ? p3 - p2 : 0);
-  };  // pair m < M
+  const LayerItem it = layer_item<MAXM>(lead, e_lane, same);
+  const int M = it.M;
 
   const int R = a.R, sets = (a.n + R - 1) / R;
   const int lo = part * sets / wpi, hi = (part + 1) * sets / wpi;  // below 2^8 * 2^14
@@ -297,44 +365,23 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_layer_kernel(LayerArgs a
   uint8_t* const region = acts + layer_act_bytes(MAXM, nb) + (size_t)wave * layer_region_bytes<TYPE, MAXM, GATEUP>(blocks);
   float* const Vbuf = (float*)(region + kMats * stage);  // [matrix][row m][64]
   float* const Dbuf = Vbuf + kMats * MAXM * 64;          // [matrix][64]
-  const uintptr_t base0 = (uintptr_t)a.w0 + (uintptr_t)((long long)expert * a.stride);
-  const uintptr_t base1 = (uintptr_t)a.w1 + (uintptr_t)((long long)expert * a.stride);
-  const uint32_t lane16 = 16u * (uint32_t)lane;
-
-  // The packed bytes of set s's rows of matrix t into its stage, from the 16-byte word that holds the first, and the
-  // copies that takes (none past the last set).
-  const auto span = [&](int s, int t, uintptr_t& from) __attribute__((always_inline)) {
-    const int n0 = s * R;
-    const uintptr_t src = (t == 0 ? base0 : base1) + (uintptr_t)n0 * (uintptr_t)a.row_bytes;
-    from = src & ~(uintptr_t)15;
-    return s < hi ? (uint32_t)min(R, a.n - n0) * (uint32_t)a.row_bytes + (uint32_t)(src & 15) : 0u;
-  };
+  const uintptr_t base0 = (uintptr_t)a.w0 + (uintptr_t)((long long)it.expert * a.stride);
+  const uintptr_t base1 = (uintptr_t)a.w1 + (uintptr_t)((long long)it.expert * a.stride);
+  // The packed bytes of set s's rows of matrix t into its stage, and the copies that takes (none past the last set).
   const auto issue = [&](int s, int t) __attribute__((always_inline)) {
-    uintptr_t from;
-    const uint32_t bytes = span(s, t, from), to = lds_addr(region) + (uint32_t)(t * stage);
-    for (uint32_t c = 0; c < bytes; c += 1024)
-      if (c + lane16 < bytes) copy16_to_lds_s_nt((const void*)from, c + lane16, to + c);
-    return (int)((bytes + 1023) / 1024);
+    if (s >= hi) return 0;
+    const int n0 = s * R;
+    return copy_rows((t == 0 ? base0 : base1) + (uintptr_t)n0 * (uintptr_t)a.row_bytes,
+                     (uint32_t)min(R, a.n - n0) * (uint32_t)a.row_bytes, lds_addr(region) + (uint32_t)(t * stage));
   };
 
   const int total = M * nb;
   const auto fetch_pair = [&](int g, uint4 (&raw)[4]) __attribute__((always_inline)) {  // block g of the item's rows
-    const int m = MAXM == 1 ? 0 : g / nb, p = MAXM == 1 ? lead : pair(m);
+    const int m = MAXM == 1 ? 0 : g / nb, p = MAXM == 1 ? lead : it.pair(m);
     fetch(total, g, GATEUP ? p / a.top_k : p, g - m * nb, raw);
   };
-  const auto quantize = [&](int g, const uint4 (&raw)[4]) __attribute__((always_inline)) {
-    if (g >= total) return;  // uniform over the block's 16 lanes
-    float v[16];
-    const uint32_t r[16] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w,
-                            raw[2].x, raw[2].y, raw[2].z, raw[2].w, raw[3].x, raw[3].y, raw[3].z, raw[3].w};
-    if (a.xbf16) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[2 * i] = bf16_to_float(r[i]), v[2 * i + 1] = bf16_to_float(r[i] >> 16);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) v[i] = __builtin_bit_cast(float, r[i]);
-    }
-    q8k_part16(v, p16, aq + (size_t)g * kActStride, abs_ + 16 * g, ad + g, a.reciprocal != 0);
+  const auto quantize = [&](int g, const uint4 (&raw)[4]) __attribute__((always_inline)) {  // uniform over 16 lanes
+    if (g < total) quantize16(a, raw, p16, aq + (size_t)g * kActStride, abs_ + 16 * g, ad + g);
   };
   int s = lo + wave, behind = 0;  // copies issued behind those of the matrix that is waited for next
   if (rows_wave) {
@@ -404,31 +451,9 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_layer_kernel(LayerArgs a
       for (int f = lane; f < R * M; f += 64) {  // row f % R of activation row f / R
         const int fr = f % R, fm = f / R;
         if (fr >= nrows) continue;
-        const float* xd = ad + fm * nb;
-        float acc[2] = {0.0f, 0.0f};
-        const float* vr = Vbuf + fm * 64 + fr * nb;
-        const float* dr = Dbuf + fr * nb;
-        constexpr int kC = 8;  // operands read before they are folded
-        for (int i = 0; i < nb; i += kC) {
-          float xx[kC], vv[kMats][kC], dd[kMats][kC];
-#pragma unroll
-          for (int j = 0; j < kC; ++j) {
-            const int c = min(i + j, nb - 1);
-            xx[j] = xd[c];
-#pragma unroll
-            for (int t = 0; t < kMats; ++t) {
-              vv[t][j] = vr[t * MAXM * 64 + c];
-              dd[t][j] = L::kHasD ? dr[t * 64 + c] : 0.0f;
-            }
-          }
-#pragma unroll
-          for (int j = 0; j < kC; ++j)
-            if (i + j < nb) {
-#pragma unroll
-              for (int t = 0; t < kMats; ++t) acc[t] = L::fold(acc[t], xx[j], vv[t][j], dd[t][j]);
-            }
-        }
-        const int p = MAXM == 1 ? lead : pair(fm);
+        float acc[kMats];
+        fold_row<TYPE, kMats>(nb, ad + fm * nb, Vbuf + fm * 64 + fr * nb, MAXM * 64, Dbuf + fr * nb, acc);
+        const int p = MAXM == 1 ? lead : it.pair(fm);
         const long long at = (long long)p * a.n + n0 + fr;
         if constexpr (GATEUP) {
           if (a.xbf16) {
@@ -444,6 +469,165 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_layer_kernel(LayerArgs a
       }
       wave_sync();  // the block values are read before the next set's are written
     }
+  }
+}
+
+// Bytes of the second launch's LDS besides its waves' regions when it adds the pairs up itself: the pairs' weights and
+// places, each token's pairs, the activations of all pairs, and their down values of the workgroup's `rows` rows.
+constexpr int kSumFixed = (2 * kLayerMaxPairs + kMoeLayerMaxTokens) * 4;
+constexpr int layer_sum_bytes(int pairs, int nb, int rows) {
+  return kSumFixed + layer_act_bytes(pairs, nb) + (pairs * rows * 4 + 15) / 16 * 16;
+}
+
+// The second launch where all pairs' activations fit LDS: a workgroup takes a range of `rows` output rows through every
+// item (a wave an item's R rows at a time, as above), keeps the down values in LDS and adds them up.
+template <int TYPE, int MAXM>
+__global__ __launch_bounds__(64 * kLayerWaves) void moe_down_sum_kernel(LayerArgs a, YOut out, int rows) {
+  using L = Lpb<TYPE>;
+  constexpr bool kReg = MAXM == 1 && TYPE != T_Q6_K;
+  extern __shared__ __align__(16) uint8_t smem[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
+  const int pairs = a.n_tokens * a.top_k, W = a.W, nb = a.nb, R = a.R;
+  float* const swt = (float*)smem;
+  int* const place = (int*)smem + kLayerMaxPairs;  // a token's pairs, experts ascending
+  int* const live = place + kLayerMaxPairs;        // how many they are
+  uint8_t* const acts = smem + kSumFixed;
+  int8_t* const aq = (int8_t*)acts;  // pair p, block b at (p nb + b) 272
+  int16_t* const abs_ = (int16_t*)(acts + pairs * nb * kActStride);
+  float* const ad = (float*)(acts + pairs * nb * (kActStride + 32));
+  float* const down = (float*)(acts + layer_act_bytes(pairs, nb));  // (pairs, rows)
+  const int r0 = (int)blockIdx.x * rows, nr = min(rows, a.n - r0);
+  if (nr <= 0) return;
+
+  int e_lane = -1;
+  float w_lane = 0.0f;
+  if (lane < pairs) e_lane = a.ids[lane], w_lane = a.wts[lane];
+  uint64_t same, leaders;
+  const int bits = a.n_experts > 1 ? 32 - __builtin_clz(a.n_experts - 1) : 0;
+  const int items = count_items<MAXM>(e_lane, bits, same, leaders);
+  const int sets = (nr + R - 1) / R, tasks = items * sets;
+  const int blocks = R * nb, stage = layer_stage_bytes<TYPE>(blocks);
+  uint8_t* const region =
+      acts + layer_sum_bytes(pairs, nb, rows) - kSumFixed + (size_t)wave * layer_region_bytes<TYPE, MAXM, false>(blocks);
+  float* const Vbuf = (float*)(region + stage);
+  float* const Dbuf = Vbuf + MAXM * 64;
+  const auto lead_of = [&](int task) __attribute__((always_inline)) {
+    uint64_t rest = leaders;
+    for (int i = task / sets; i > 0; --i) rest &= rest - 1;
+    return (int)__builtin_ctzll(rest);
+  };
+  const auto issue = [&](int task) __attribute__((always_inline)) {
+    if (task >= tasks) return;
+    const int n0 = r0 + task % sets * R, expert = __builtin_amdgcn_readlane(e_lane, lead_of(task));
+    copy_rows((uintptr_t)a.w0 + (uintptr_t)((long long)expert * a.stride) + (uintptr_t)n0 * (uintptr_t)a.row_bytes,
+              (uint32_t)min(R, r0 + nr - n0) * (uint32_t)a.row_bytes, lds_addr(region));
+  };
+
+  int task = wave;
+  if (wave < W) {
+    __builtin_amdgcn_s_barrier();  // the activations are requested
+    wait_vmcnt(0);  // as in moe_layer_kernel
+    issue(task);
+  } else {
+    // every pair's row, those without an expert (which nothing has written) left out
+    const int step = 4 * (waves - W), p16 = lane & 15, total = pairs * nb;
+    int g = 4 * (wave - W) + (lane >> 4);
+    uint4 first[4] = {}, second[4] = {};
+    const auto wanted = [&](int g) __attribute__((always_inline)) {
+      const int e = __shfl(e_lane, min(g / nb, pairs - 1));  // every lane: a lane reads what another one holds
+      return g < total && e >= 0;
+    };
+    const auto fetch = [&](int g, bool on, uint4 (&raw)[4]) __attribute__((always_inline)) {
+      if (on) fetch16(a, (long long)(g / nb) * a.k + g % nb * QK + 16 * p16, raw);
+    };
+    const auto quantize = [&](int g, bool on, const uint4 (&raw)[4]) __attribute__((always_inline)) {
+      if (on) quantize16(a, raw, p16, aq + (size_t)g * kActStride, abs_ + 16 * g, ad + g);
+    };
+    bool on1 = wanted(g), on2 = wanted(g + step);
+    fetch(g, on1, first);
+    fetch(g + step, on2, second);
+    __builtin_amdgcn_sched_barrier(0);  // not sunk below the barrier
+    __builtin_amdgcn_s_barrier();
+    if (wave == W && lane < pairs) {  // the sum's order
+      const int t = lane / a.top_k;
+      int rank = 0, n = 0;
+      for (int i = t * a.top_k; i < (t + 1) * a.top_k; ++i) {
+        const int o = a.ids[i];
+        rank += o >= 0 && (o < e_lane || (o == e_lane && i < lane));
+        n += o >= 0;
+      }
+      if (e_lane >= 0) place[t * a.top_k + rank] = lane;
+      live[t] = n;
+      swt[lane] = w_lane;
+    }
+    for (;;) {
+      quantize(g, on1, first);
+      quantize(g + step, on2, second);
+      g += 2 * step;
+      if (__ballot(g < total) == 0) break;
+      on1 = wanted(g), on2 = wanted(g + step);
+      fetch(g, on1, first);
+      fetch(g + step, on2, second);
+    }
+  }
+  lds_barrier();  // the activations are in LDS
+
+  if (wave < W) {
+    const int b = lane % nb;
+    for (; task < tasks; task += W) {
+      const int n0 = task % sets * R, nrows = min(R, nr - n0);  // rows of the workgroup's
+      const LayerItem it = layer_item<MAXM>(lead_of(task), e_lane, same);
+      const int M = it.M, jl = min(lane, nrows * nb - 1);
+      ActBlock ab[MAXM];
+#pragma unroll
+      for (int m = 0; m < MAXM; ++m) {
+        const int g = it.pair(m < M ? m : 0) * nb + b;
+        ab[m] = ActBlock{aq + (size_t)g * kActStride, abs_ + 16 * g, 0.0f, nullptr};
+      }
+      ActRegs areg;
+      if constexpr (kReg) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) areg.q[i] = ab[0].q16(16 * i);
+        areg.bs[0] = ab[0].bs8(0);
+        areg.bs[1] = ab[0].bs8(1);
+      }
+      wait_vmcnt(0);
+      const int delta = TYPE == T_Q6_K ? (int)(((uintptr_t)(r0 + n0) * (uintptr_t)a.row_bytes) & 15) : 0;
+      float V[MAXM], D;
+      if constexpr (kReg)
+        L::template compute<1, ActRegs>(region, delta + jl * L::kBytes, &areg, 1, V, D);
+      else
+        L::template compute<MAXM, ActBlock>(region, delta + jl * L::kBytes, ab, M, V, D);
+#pragma unroll
+      for (int m = 0; m < MAXM; ++m)
+        if (m < M) Vbuf[m * 64 + lane] = V[m];
+      if (L::kHasD) Dbuf[lane] = D;
+      __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the stage has been read
+      wave_sync();
+      issue(task + W);
+      for (int f = lane; f < R * M; f += 64) {
+        const int fr = f % R, fm = f / R;
+        if (fr >= nrows) continue;
+        const int p = it.pair(fm);
+        float acc[1];
+        fold_row<TYPE, 1>(nb, ad + p * nb, Vbuf + fm * 64 + fr * nb, 0, Dbuf + fr * nb, acc);
+        down[p * rows + n0 + fr] = acc[0];
+      }
+      wave_sync();  // the block values are read before the next set's are written
+    }
+  }
+  lds_barrier();  // the down values are in LDS
+  for (int i = tid; i < nr * a.n_tokens; i += blockDim.x) {
+    const int t = i / nr, r = i - t * nr, n = live[t];
+    float acc = 0.0f;
+    for (int j = 0; j < n; ++j) {
+      const int p = place[t * a.top_k + j];
+      float v = down[p * rows + r];
+      if (a.xbf16) v = bf16_to_float(bf16_rne(v));
+      acc = acc + v * swt[p];
+    }
+    out.put((long long)t * a.n + r0 + r, acc);
   }
 }
 
@@ -479,6 +663,23 @@ int launch_layer(LayerArgs a, int grid, hipStream_t stream) {
   allow_lds((const void*)kern, kLayerLds);
   hipLaunchKernelGGL(kern, dim3(grid), dim3(64 * kLayerWaves), lds, stream, a);
   return 0;
+}
+
+// The same of the second launch that adds up: `rows` output rows a workgroup, at least kSumWaves waves of them, and up
+// to kSumPairs pairs: a workgroup quantizes the activations of all of them. Both launches from start to end, adding up
+// and with the combine's launch: one token of 8 experts top 2 (4096 x 14336) 59.0 and 61.9 us, of 64 top 8 (2048 x
+// 1024) 23.6 and 27.8, of 5 top 1 (4096 x 4096) 20.6 and 26.6; 12 pairs (16 top 4, 2048 x 1536) 28.9 and 30.4; 24
+// pairs (40 top 8, 1536 x 512) 33.3 and 33.5, (32 top 3, 2560 x 768) 44.4 and 43.4; 32 and 64 pairs of 64 top 8 46.1
+// and 42.5, 66.4 and 55.2.
+constexpr int kSumWaves = 8, kSumPairs = 16;
+template <int TYPE, int MAXM>
+bool layer_sum_shape(int nb, int pairs, int rows, int& R, int& W, int& lds) {
+  R = min(64 / nb, rows);
+  const int region = layer_region_bytes<TYPE, MAXM, false>(R * nb);
+  const int fixed = layer_sum_bytes(pairs, nb, rows);
+  W = min(kLayerWaves - kLayerStagers, (kLayerLds - fixed) / region);
+  lds = fixed + W * region;
+  return pairs <= kSumPairs && fixed < kLayerLds && W >= kSumWaves;
 }
 
 // Pairs of an item: one for one token; for more, four, or two where four rows of activations take the LDS of the
@@ -521,6 +722,23 @@ struct LaunchLayer {
   }
 };
 
+struct LaunchSum {  // -1 for many pairs, and where its LDS leaves too few waves
+  LayerArgs a;
+  YOut out;
+  int grid;
+  hipStream_t stream;
+  template <int TYPE, int MAXM>
+  int operator()() {
+    const int rows = (a.n + grid - 1) / grid;
+    int lds;
+    if (!layer_sum_shape<TYPE, MAXM>(a.nb, a.n_tokens * a.top_k, rows, a.R, a.W, lds)) return -1;
+    auto kern = moe_down_sum_kernel<TYPE, MAXM>;
+    allow_lds((const void*)kern, kLayerLds);
+    hipLaunchKernelGGL(kern, dim3((a.n + rows - 1) / rows), dim3(64 * kLayerWaves), lds, stream, a, out, rows);
+    return 0;
+  }
+};
+
 }  // namespace
 
 bool moe_layer_supported(int gate_type, int down_type, int n_experts, int top_k, int n_tokens, int n_embd, int ffn) {
@@ -557,6 +775,7 @@ int launch_moe_layer(int gate_type, int down_type, const uint8_t* gate, const ui
   if (with_layer_kernel(gate_type, layer_pairs(one, a.nb), LaunchLayer<true>{a, grid, stream}) != 0) return -1;
   a.w0 = down, a.w1 = nullptr, a.stride = down_stride, a.row_bytes = down_row, a.x = act, a.act = rows;
   a.n = n_embd, a.k = ffn, a.nb = ffn / QK;
+  if (with_layer_kernel(down_type, layer_pairs(one, a.nb), LaunchSum{a, out, grid, stream}) == 0) return 0;
   if (with_layer_kernel(down_type, layer_pairs(one, a.nb), LaunchLayer<false>{a, grid, stream}) != 0) return -1;
   return launch_moe_combine((const float*)rows, nullptr, ids, wts, n_tokens, top_k, n_embd, bf16 ? 1 : 0, 1, out, stream);
 }
