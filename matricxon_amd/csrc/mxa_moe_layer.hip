@@ -21,11 +21,11 @@
 // they would otherwise queue (with one token x's before the routing).
 //
 // What bounds it, MI355X, kernel alone with weights that no cache holds: 8 experts top 2 of 4096 x 14336 (Q4_K, Q6_K
-// down), one token, gate and up 27 us for 132 MB (4.9 TB/s; a read of as many bytes 21), of which 3 us before the
-// first copy and 3 after the last; down 29 us for 96 MB (3.3 TB/s), the LDS holding 11 rows of 56 blocks, which
-// wait and compute in turn. Eight tokens: 104 and 139 us, 4.5 and 2.5 TB/s: each further pair of an expert adds to
+// down), one token, gate and up 28 us for 132 MB (4.7 TB/s; a read of as many bytes 21), of which 3 us before the
+// first copy and 3 after the last; down 28.5 us for 96 MB (3.4 TB/s), the LDS holding 11 rows of 56 blocks, which
+// wait and compute in turn. Eight tokens: 99 and 100 us, 4.8 and 3.5 TB/s: each further pair of an expert adds to
 // the part of a wave's turn in which its stage is not in flight. 64 experts top 8 of 2048 x 1024, one token: 11.7
-// and 8.2 us, latency from end to end (logits, routing, activations, weights, block arithmetic).
+// and 11.5 us, latency from end to end (logits, routing, activations, weights, block arithmetic).
 //
 // The sum needs every pair's rows in one place. Up to 16 pairs the second launch's workgroups take rows, each through
 // all items, and add up in LDS. For more they take items, and the combine is a launch of its own (4 to 5 us): adding up
@@ -206,26 +206,71 @@ __device__ __forceinline__ LayerItem layer_item(int lead, int e_lane, uint64_t s
   return it;
 }
 
-// The lane's 16 of 256 activations from value `at` of x, and their Q8_K block part.
-__device__ __forceinline__ void fetch16(const LayerArgs& a, long long at, uint4 (&raw)[4]) {
-  const uint4* src = (const uint4*)((const uint8_t*)a.x + at * (a.xbf16 ? 2 : 4));
-  raw[0] = src[0], raw[1] = src[1];
-  if (!a.xbf16) raw[2] = src[2], raw[3] = src[3];
-}
-__device__ __forceinline__ void quantize16(const LayerArgs& a, const uint4 (&raw)[4], int p16, int8_t* q, int16_t* bs,
-                                           float* d) {
-  float v[16];
-  const uint32_t r[16] = {raw[0].x, raw[0].y, raw[0].z, raw[0].w, raw[1].x, raw[1].y, raw[1].z, raw[1].w,
-                          raw[2].x, raw[2].y, raw[2].z, raw[2].w, raw[3].x, raw[3].y, raw[3].z, raw[3].w};
-  if (a.xbf16) {
+// Activations to Q8_K by the waves that own no rows, 16 lanes a block. A buffer holds a lane's 16 values of a float32
+// block, or of two bfloat16 blocks; block(i) gives the lane's i-th block: whether there is one, the value of x that the
+// lane's part starts at, and where its codes, sums and scale go.
+struct ActPart {
+  bool on;
+  long long at;
+  int8_t* q;
+  int16_t* bs;
+  float* d;
+};
+template <int BUFS, class Block>
+__device__ __forceinline__ void fetch_acts(const LayerArgs& a, int i0, Block block, uint4 (&raw)[BUFS][4]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[2 * i] = bf16_to_float(r[i]), v[2 * i + 1] = bf16_to_float(r[i] >> 16);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __builtin_bit_cast(float, r[i]);
+  for (int j = 0; j < BUFS; ++j) {
+    const ActPart p = block(i0 + (a.xbf16 ? 2 * j : j));
+    if (p.on) {
+      const uint4* src = (const uint4*)((const uint8_t*)a.x + p.at * (a.xbf16 ? 2 : 4));
+      raw[j][0] = src[0], raw[j][1] = src[1];
+      if (!a.xbf16) raw[j][2] = src[2], raw[j][3] = src[3];
+    }
+    if (a.xbf16) {
+      const ActPart p2 = block(i0 + 2 * j + 1);
+      if (p2.on) {
+        const uint4* src = (const uint4*)((const uint8_t*)a.x + p2.at * 2);
+        raw[j][2] = src[0], raw[j][3] = src[1];
+      }
+    }
   }
-  q8k_part16(v, p16, q, bs, d, a.reciprocal != 0);
 }
+__device__ __forceinline__ void widen_bf16x16(uint4 lo, uint4 hi, float (&v)[16]) {
+  const uint32_t r[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[2 * i] = bf16_to_float(r[i]), v[2 * i + 1] = bf16_to_float(r[i] >> 16);
+}
+template <int BUFS, class Block>
+__device__ __forceinline__ void quantize_acts(const LayerArgs& a, int i0, Block block, const uint4 (&raw)[BUFS][4]) {
+  const int p16 = threadIdx.x & 15;
+#pragma unroll
+  for (int j = 0; j < BUFS; ++j) {
+    const ActPart p = block(i0 + (a.xbf16 ? 2 * j : j));
+    if (p.on) {  // uniform over the block's 16 lanes
+      float v[16];
+      if (a.xbf16) {
+        widen_bf16x16(raw[j][0], raw[j][1], v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[4 * i] = __builtin_bit_cast(float, raw[j][i].x), v[4 * i + 1] = __builtin_bit_cast(float, raw[j][i].y);
+          v[4 * i + 2] = __builtin_bit_cast(float, raw[j][i].z), v[4 * i + 3] = __builtin_bit_cast(float, raw[j][i].w);
+        }
+      }
+      q8k_part16(v, p16, p.q, p.bs, p.d, a.reciprocal != 0);
+    }
+    if (a.xbf16) {
+      const ActPart p2 = block(i0 + 2 * j + 1);
+      if (p2.on) {
+        float v[16];
+        widen_bf16x16(raw[j][2], raw[j][3], v);
+        q8k_part16(v, p16, p2.q, p2.bs, p2.d, a.reciprocal != 0);
+      }
+    }
+  }
+}
+// Buffers of a wave: what it requests before the weights (what is left comes behind them).
+constexpr int kLayerBufs = 2;
 
 // `bytes` packed bytes at src, with those before them in src's 16-byte word, to LDS address `to`; the copies it took.
 __device__ __forceinline__ int copy_rows(uintptr_t src, uint32_t bytes, uint32_t to) {
@@ -236,33 +281,45 @@ __device__ __forceinline__ int copy_rows(uintptr_t src, uint32_t bytes, uint32_t
   return (int)((end + 1023) / 1024);
 }
 
-// The fold of one row's nb block values in order, of MATS matrices at once (their values v and scales d `vstep` and
-// 64 apart); xd the activation row's scales.
+// Rows of block values and of scales in LDS start on 16 bytes: their stride in floats.
+__host__ __device__ constexpr int layer_fold_row(int nb) { return (nb + 3) / 4 * 4; }
+
+// The fold of one row's nb block values in order, of MATS matrices at once (their values v `vstep`, their scales d
+// `dstep` apart); xd the activation row's scales. Four blocks a read: few lanes fold, and an instruction costs what it
+// costs a whole wave (56 blocks one at a time, their places clamped to the row's end, took 3 us).
 template <int TYPE, int MATS>
-__device__ __forceinline__ void fold_row(int nb, const float* xd, const float* v, int vstep, const float* d,
+__device__ __forceinline__ void fold_row(int nb, const float* xd, const float* v, int vstep, const float* d, int dstep,
                                          float (&acc)[MATS]) {
   using L = Lpb<TYPE>;
-  constexpr int kC = 8;  // operands read before they are folded
+  constexpr int kQuads = 2;  // read before the first is folded
 #pragma unroll
   for (int t = 0; t < MATS; ++t) acc[t] = 0.0f;
-  for (int i = 0; i < nb; i += kC) {
-    float xx[kC], vv[MATS][kC], dd[MATS][kC];
+  for (int i = 0; i < nb; i += 4 * kQuads) {
+    float4 xx[kQuads], vv[MATS][kQuads], dd[MATS][kQuads];
 #pragma unroll
-    for (int j = 0; j < kC; ++j) {
-      const int c = min(i + j, nb - 1);
-      xx[j] = xd[c];
+    for (int q = 0; q < kQuads; ++q) {
+      const int c = i + 4 * q;
+      if (c >= nb) break;
+      xx[q] = *(const float4*)(xd + c);
 #pragma unroll
       for (int t = 0; t < MATS; ++t) {
-        vv[t][j] = v[t * vstep + c];
-        dd[t][j] = L::kHasD ? d[t * 64 + c] : 0.0f;
+        vv[t][q] = *(const float4*)(v + t * vstep + c);
+        if (L::kHasD) dd[t][q] = *(const float4*)(d + t * dstep + c);
       }
     }
 #pragma unroll
-    for (int j = 0; j < kC; ++j)
-      if (i + j < nb) {
+    for (int q = 0; q < kQuads; ++q) {
+      const int c = i + 4 * q;
 #pragma unroll
-        for (int t = 0; t < MATS; ++t) acc[t] = L::fold(acc[t], xx[j], vv[t][j], dd[t][j]);
+      for (int j = 0; j < 4; ++j) {
+        if (c + j >= nb) break;
+#pragma unroll
+        for (int t = 0; t < MATS; ++t) {
+          const auto at = [&](const float4& f) { return j == 0 ? f.x : j == 1 ? f.y : j == 2 ? f.z : f.w; };
+          acc[t] = L::fold(acc[t], at(xx[q]), at(vv[t][q]), L::kHasD ? at(dd[t][q]) : 0.0f);
+        }
       }
+    }
   }
 }
 
@@ -271,12 +328,13 @@ constexpr int layer_stage_bytes(int blocks) {  // Q6_K rows start on any even by
   return (blocks * Lpb<TYPE>::kBytes + (TYPE == T_Q6_K ? 15 : 0) + 1023) / 1024 * 1024;
 }
 template <int TYPE, int MAXM, bool GATEUP>
-constexpr int layer_region_bytes(int blocks) {
+constexpr int layer_region_bytes(int R, int nb) {
   constexpr int kMats = GATEUP ? 2 : 1;
-  return kMats * (layer_stage_bytes<TYPE>(blocks) + 64 * 4 * (MAXM + (Lpb<TYPE>::kHasD ? 1 : 0)));
+  return kMats * (layer_stage_bytes<TYPE>(R * nb) +
+                  R * layer_fold_row(nb) * 4 * (MAXM + (Lpb<TYPE>::kHasD ? 1 : 0)));
 }
 // Activations of `rows` rows in LDS: q (272 bytes a block), bsums, d; and the routing.
-constexpr int layer_row_act(int nb) { return nb * (kActStride + 32 + 4); }
+constexpr int layer_row_act(int nb) { return nb * (kActStride + 32) + 4 * layer_fold_row(nb); }
 constexpr int layer_act_bytes(int rows, int nb) { return (rows * layer_row_act(nb) + 15) / 16 * 16; }
 constexpr int kLayerFixed = 4 * kLayerMaxPairs;
 
@@ -296,19 +354,18 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_layer_kernel(LayerArgs a
   float* const ad = (float*)(acts + MAXM * nb * (kActStride + 32));
   const bool rows_wave = wave < W;
 
-  // Activations to Q8_K, by the waves that own no rows: 16 lanes a block, four blocks a wave at a time, the first
-  // eight of a wave requested before the weights
-  const int step = 4 * (waves - W), p16 = lane & 15;
-  int g = 4 * (wave - W) + (lane >> 4);
-  uint4 first[4] = {}, second[4] = {};
-  const auto fetch = [&](int total, int g, long long row, int b, uint4 (&raw)[4]) __attribute__((always_inline)) {
-    if (g < total) fetch16(a, row * a.k + b * QK + 16 * p16, raw);
+  constexpr int kBufs = kLayerBufs;
+  const int step = 4 * (waves - W), p16 = lane & 15, g0 = 4 * (wave - W) + (lane >> 4);
+  uint4 raw[kBufs][4] = {};
+  const auto part_of = [&](int g, int total, long long row, int b, int d_at) __attribute__((always_inline)) {
+    return ActPart{g < total, row * a.k + b * QK + 16 * p16, aq + (size_t)g * kActStride, abs_ + 16 * g, ad + d_at};
   };
   constexpr bool kOneToken = GATEUP && MAXM == 1;  // its row is known before its experts are
-  if (kOneToken && !rows_wave) {
-    fetch(nb, g, 0, g, first);
-    fetch(nb, g + step, 0, g + step, second);
-  }
+  const auto token_block = [&](int i) __attribute__((always_inline)) {
+    const int g = g0 + step * i;
+    return part_of(g, nb, 0, g, g);
+  };
+  if (kOneToken && !rows_wave) fetch_acts(a, 0, token_block, raw);
 
   // the pairs' experts
   int e_lane = -1;
@@ -330,8 +387,8 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_layer_kernel(LayerArgs a
   const int items = count_items<MAXM>(e_lane, bits, same, leaders);
   if (items == 0) return;  // no token has an expert
   // The item of this workgroup, its leading pair, and the workgroup's place among the item's. The workgroups are
-  // shared out by the items' costs: a set of rows takes a third longer for each further pair (8 tokens of 8 experts
-  // top 2, 4096 x 14336: one pair 58 us, four 117 with equal shares).
+  // shared out by the items' costs, a set of rows taking about a third longer for each further pair (with equal shares
+  // of 8 tokens of 8 experts top 2, 4096 x 14336, an item of one pair was done after 58 us, one of four after 117).
   int lead, part, wpi;
   if constexpr (MAXM == 1) {
     wpi = (int)gridDim.x / items;
@@ -362,9 +419,11 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_layer_kernel(LayerArgs a
   const int R = a.R, sets = (a.n + R - 1) / R;
   const int lo = part * sets / wpi, hi = (part + 1) * sets / wpi;  // below 2^8 * 2^14
   const int blocks = R * nb, stage = layer_stage_bytes<TYPE>(blocks);
-  uint8_t* const region = acts + layer_act_bytes(MAXM, nb) + (size_t)wave * layer_region_bytes<TYPE, MAXM, GATEUP>(blocks);
-  float* const Vbuf = (float*)(region + kMats * stage);  // [matrix][row m][64]
-  float* const Dbuf = Vbuf + kMats * MAXM * 64;          // [matrix][64]
+  uint8_t* const region =
+      acts + layer_act_bytes(MAXM, nb) + (size_t)wave * layer_region_bytes<TYPE, MAXM, GATEUP>(R, nb);
+  const int fold = layer_fold_row(nb), fold_set = R * fold;
+  float* const Vbuf = (float*)(region + kMats * stage);  // [matrix][activation row][row][fold]
+  float* const Dbuf = Vbuf + kMats * MAXM * fold_set;    // [matrix][row][fold]
   const uintptr_t base0 = (uintptr_t)a.w0 + (uintptr_t)((long long)it.expert * a.stride);
   const uintptr_t base1 = (uintptr_t)a.w1 + (uintptr_t)((long long)it.expert * a.stride);
   // The packed bytes of set s's rows of matrix t into its stage, and the copies that takes (none past the last set).
@@ -376,14 +435,11 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_layer_kernel(LayerArgs a
   };
 
   const int total = M * nb;
-  const auto fetch_pair = [&](int g, uint4 (&raw)[4]) __attribute__((always_inline)) {  // block g of the item's rows
-    const int m = MAXM == 1 ? 0 : g / nb, p = MAXM == 1 ? lead : it.pair(m);
-    fetch(total, g, GATEUP ? p / a.top_k : p, g - m * nb, raw);
+  const auto item_block = [&](int i) __attribute__((always_inline)) {  // of the item's rows
+    const int g = g0 + step * i, m = MAXM == 1 ? 0 : g / nb, p = MAXM == 1 ? lead : it.pair(m);
+    return part_of(g, total, GATEUP ? p / a.top_k : p, g - m * nb, m * fold + g - m * nb);
   };
-  const auto quantize = [&](int g, const uint4 (&raw)[4]) __attribute__((always_inline)) {  // uniform over 16 lanes
-    if (g < total) quantize16(a, raw, p16, aq + (size_t)g * kActStride, abs_ + 16 * g, ad + g);
-  };
-  int s = lo + wave, behind = 0;  // copies issued behind those of the matrix that is waited for next
+  int s = lo + wave, behind = 0;  // copies issued behind those of the stage that is waited for next
   if (rows_wave) {
     __builtin_amdgcn_s_barrier();  // the activations are requested
     // no load of this wave's is in flight: said here, or the compiler, which sees the other waves' loads into the
@@ -392,25 +448,21 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_layer_kernel(LayerArgs a
     issue(s, 0);
     if constexpr (GATEUP) behind = issue(s, 1);
   } else {
-    if (!kOneToken) {
-      fetch_pair(g, first);
-      fetch_pair(g + step, second);
-    }
+    if (!kOneToken) fetch_acts(a, 0, item_block, raw);
     __builtin_amdgcn_sched_barrier(0);  // not sunk below the barrier
     __builtin_amdgcn_s_barrier();
-    for (;;) {
-      quantize(g, first);
-      quantize(g + step, second);
-      g += 2 * step;
-      if (__ballot(g < total) == 0) break;
-      fetch_pair(g, first);
-      fetch_pair(g + step, second);
+    const int per = a.xbf16 ? 2 * kBufs : kBufs;
+    for (int i = 0;;) {
+      quantize_acts(a, i, item_block, raw);
+      i += per;
+      if (__ballot(g0 + step * i < total) == 0) break;
+      fetch_acts(a, i, item_block, raw);
     }
   }
   lds_barrier();  // the activations are in LDS
 
   if (rows_wave) {
-    const int b = lane % nb;
+    const int b = lane % nb, to = lane / nb * fold + b;  // the lane's block, and its place in the folds
     ActBlock ab[MAXM];
 #pragma unroll
     for (int m = 0; m < MAXM; ++m) {
@@ -429,7 +481,7 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_layer_kernel(LayerArgs a
       }
 #pragma unroll 1  // one copy of the block arithmetic
       for (int t = 0; t < kMats; ++t) {
-        // Copies land in order: a matrix is computed while the other one's are in flight. (A store of the last set's
+        // Copies land in order: a stage is computed while the other one's are in flight. (A store of the last set's
         // fold behind them makes this wait for one copy more than it has to.)
         wait_vmcnt(behind);
         // bases are 16-byte aligned; only Q6_K rows can start between 16-byte words
@@ -441,8 +493,8 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_layer_kernel(LayerArgs a
           L::template compute<MAXM, ActBlock>(region + t * stage, delta + jl * L::kBytes, ab, M, V, D);
 #pragma unroll
         for (int m = 0; m < MAXM; ++m)
-          if (m < M) Vbuf[(t * MAXM + m) * 64 + lane] = V[m];
-        if (L::kHasD) Dbuf[t * 64 + lane] = D;
+          if (m < M && lane < blocks) Vbuf[(t * MAXM + m) * fold_set + to] = V[m];
+        if (L::kHasD && lane < blocks) Dbuf[t * fold_set + to] = D;
         __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the stage has been read
         wave_sync();
         const int n = issue(s + W, t);
@@ -452,7 +504,8 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_layer_kernel(LayerArgs a
         const int fr = f % R, fm = f / R;
         if (fr >= nrows) continue;
         float acc[kMats];
-        fold_row<TYPE, kMats>(nb, ad + fm * nb, Vbuf + fm * 64 + fr * nb, MAXM * 64, Dbuf + fr * nb, acc);
+        fold_row<TYPE, kMats>(nb, ad + fm * fold, Vbuf + fm * fold_set + fr * fold, MAXM * fold_set, Dbuf + fr * fold,
+                              fold_set, acc);
         const int p = MAXM == 1 ? lead : it.pair(fm);
         const long long at = (long long)p * a.n + n0 + fr;
         if constexpr (GATEUP) {
@@ -509,9 +562,10 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_down_sum_kernel(LayerArg
   const int sets = (nr + R - 1) / R, tasks = items * sets;
   const int blocks = R * nb, stage = layer_stage_bytes<TYPE>(blocks);
   uint8_t* const region =
-      acts + layer_sum_bytes(pairs, nb, rows) - kSumFixed + (size_t)wave * layer_region_bytes<TYPE, MAXM, false>(blocks);
-  float* const Vbuf = (float*)(region + stage);
-  float* const Dbuf = Vbuf + MAXM * 64;
+      acts + layer_sum_bytes(pairs, nb, rows) - kSumFixed + (size_t)wave * layer_region_bytes<TYPE, MAXM, false>(R, nb);
+  const int fold = layer_fold_row(nb), fold_set = R * fold;
+  float* const Vbuf = (float*)(region + stage);  // [activation row][row][fold]
+  float* const Dbuf = Vbuf + MAXM * fold_set;
   const auto lead_of = [&](int task) __attribute__((always_inline)) {
     uint64_t rest = leaders;
     for (int i = task / sets; i > 0; --i) rest &= rest - 1;
@@ -531,22 +585,16 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_down_sum_kernel(LayerArg
     issue(task);
   } else {
     // every pair's row, those without an expert (which nothing has written) left out
-    const int step = 4 * (waves - W), p16 = lane & 15, total = pairs * nb;
-    int g = 4 * (wave - W) + (lane >> 4);
-    uint4 first[4] = {}, second[4] = {};
-    const auto wanted = [&](int g) __attribute__((always_inline)) {
-      const int e = __shfl(e_lane, min(g / nb, pairs - 1));  // every lane: a lane reads what another one holds
-      return g < total && e >= 0;
+    constexpr int kBufs = kLayerBufs;
+    const int step = 4 * (waves - W), p16 = lane & 15, g0 = 4 * (wave - W) + (lane >> 4), total = pairs * nb;
+    uint4 raw[kBufs][4] = {};
+    const auto block = [&](int i) __attribute__((always_inline)) {
+      const int g = g0 + step * i, p = min(g / nb, pairs - 1);
+      const int e = __shfl(e_lane, p);  // every lane: a lane reads what another one holds
+      return ActPart{g < total && e >= 0, (long long)p * a.k + (g - p * nb) * QK + 16 * p16,
+                     aq + (size_t)g * kActStride, abs_ + 16 * g, ad + p * fold + g - p * nb};
     };
-    const auto fetch = [&](int g, bool on, uint4 (&raw)[4]) __attribute__((always_inline)) {
-      if (on) fetch16(a, (long long)(g / nb) * a.k + g % nb * QK + 16 * p16, raw);
-    };
-    const auto quantize = [&](int g, bool on, const uint4 (&raw)[4]) __attribute__((always_inline)) {
-      if (on) quantize16(a, raw, p16, aq + (size_t)g * kActStride, abs_ + 16 * g, ad + g);
-    };
-    bool on1 = wanted(g), on2 = wanted(g + step);
-    fetch(g, on1, first);
-    fetch(g + step, on2, second);
+    fetch_acts(a, 0, block, raw);
     __builtin_amdgcn_sched_barrier(0);  // not sunk below the barrier
     __builtin_amdgcn_s_barrier();
     if (wave == W && lane < pairs) {  // the sum's order
@@ -561,20 +609,18 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_down_sum_kernel(LayerArg
       live[t] = n;
       swt[lane] = w_lane;
     }
-    for (;;) {
-      quantize(g, on1, first);
-      quantize(g + step, on2, second);
-      g += 2 * step;
-      if (__ballot(g < total) == 0) break;
-      on1 = wanted(g), on2 = wanted(g + step);
-      fetch(g, on1, first);
-      fetch(g + step, on2, second);
+    const int per = a.xbf16 ? 2 * kBufs : kBufs;
+    for (int i = 0;;) {
+      quantize_acts(a, i, block, raw);
+      i += per;
+      if (__ballot(g0 + step * i < total) == 0) break;
+      fetch_acts(a, i, block, raw);
     }
   }
   lds_barrier();  // the activations are in LDS
 
   if (wave < W) {
-    const int b = lane % nb;
+    const int b = lane % nb, to = lane / nb * fold + b;
     for (; task < tasks; task += W) {
       const int n0 = task % sets * R, nrows = min(R, nr - n0);  // rows of the workgroup's
       const LayerItem it = layer_item<MAXM>(lead_of(task), e_lane, same);
@@ -601,8 +647,8 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_down_sum_kernel(LayerArg
         L::template compute<MAXM, ActBlock>(region, delta + jl * L::kBytes, ab, M, V, D);
 #pragma unroll
       for (int m = 0; m < MAXM; ++m)
-        if (m < M) Vbuf[m * 64 + lane] = V[m];
-      if (L::kHasD) Dbuf[lane] = D;
+        if (m < M && lane < blocks) Vbuf[m * fold_set + to] = V[m];
+      if (L::kHasD && lane < blocks) Dbuf[to] = D;
       __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the stage has been read
       wave_sync();
       issue(task + W);
@@ -611,7 +657,7 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_down_sum_kernel(LayerArg
         if (fr >= nrows) continue;
         const int p = it.pair(fm);
         float acc[1];
-        fold_row<TYPE, 1>(nb, ad + p * nb, Vbuf + fm * 64 + fr * nb, 0, Dbuf + fr * nb, acc);
+        fold_row<TYPE, 1>(nb, ad + p * fold, Vbuf + fm * fold_set + fr * fold, 0, Dbuf + fr * fold, 0, acc);
         down[p * rows + n0 + fr] = acc[0];
       }
       wave_sync();  // the block values are read before the next set's are written
@@ -644,55 +690,49 @@ __global__ __launch_bounds__(256) void moe_topk_kernel(const void* __restrict__ 
               });
 }
 
-// Rows per wave, row waves and LDS for a matrix of rows of nb blocks; false when not one wave's rows fit.
+// Rows per wave, row waves and LDS for a matrix of rows of nb blocks, the most rows that the LDS holds at once (of 6
+// blocks of Q8_0, gate and up, seven waves of 6 rows, not four of 10); false when not one wave's rows fit.
 template <int TYPE, int MAXM, bool GATEUP>
 bool layer_shape(int nb, int& R, int& W, int& lds) {
-  R = 64 / nb;
-  const int region = layer_region_bytes<TYPE, MAXM, GATEUP>(R * nb);
   const int act = kLayerFixed + layer_act_bytes(MAXM, nb);
-  W = min(kLayerWaves - kLayerStagers, (kLayerLds - act) / region);
-  lds = act + W * region;
+  R = W = lds = 0;
+  if (act >= kLayerLds) return false;
+  for (int r = 64 / nb; r >= 1; --r) {
+    const int region = layer_region_bytes<TYPE, MAXM, GATEUP>(r, nb);
+    const int w = min(kLayerWaves - kLayerStagers, (kLayerLds - act) / region);
+    if (w * r > W * R) R = r, W = w, lds = act + w * region;
+  }
   return W >= 1;
 }
 
-template <int TYPE, int MAXM, bool GATEUP>
-int launch_layer(LayerArgs a, int grid, hipStream_t stream) {
-  int lds;
-  if (!layer_shape<TYPE, MAXM, GATEUP>(a.nb, a.R, a.W, lds)) return -1;
-  auto kern = moe_layer_kernel<TYPE, MAXM, GATEUP>;
-  allow_lds((const void*)kern, kLayerLds);
-  hipLaunchKernelGGL(kern, dim3(grid), dim3(64 * kLayerWaves), lds, stream, a);
-  return 0;
-}
-
 // The same of the second launch that adds up: `rows` output rows a workgroup, at least kSumWaves waves of them, and up
-// to kSumPairs pairs: a workgroup quantizes the activations of all of them. Both launches from start to end, adding up
-// and with the combine's launch: one token of 8 experts top 2 (4096 x 14336) 59.0 and 61.9 us, of 64 top 8 (2048 x
-// 1024) 23.6 and 27.8, of 5 top 1 (4096 x 4096) 20.6 and 26.6; 12 pairs (16 top 4, 2048 x 1536) 28.9 and 30.4; 24
-// pairs (40 top 8, 1536 x 512) 33.3 and 33.5, (32 top 3, 2560 x 768) 44.4 and 43.4; 32 and 64 pairs of 64 top 8 46.1
-// and 42.5, 66.4 and 55.2.
+// to kSumPairs pairs, all of whose activations a workgroup quantizes. Both launches from start to end, adding up and
+// with the combine's launch: one token of 8 experts top 2 (4096 x 14336) 56.3 and 58.0 us, of 64 top 8 (2048 x 1024)
+// 25.0 and 27.4, of 5 top 1 (4096 x 4096) 22.7 and 26.3; 12 pairs (16 top 4, 2048 x 1536) 30.8 both; 16 pairs (128 top
+// 8, 2048 x 768) 28.3 and 29.2; 24 pairs (40 top 8, 1536 x 512) 28.2 and 27.6, (32 top 3, 2560 x 768) 44.3 and 43.2;
+// 32 and 64 pairs of 64 top 8 45.8 and 42.8, 65.3 and 53.1.
 constexpr int kSumWaves = 8, kSumPairs = 16;
 template <int TYPE, int MAXM>
 bool layer_sum_shape(int nb, int pairs, int rows, int& R, int& W, int& lds) {
   R = min(64 / nb, rows);
-  const int region = layer_region_bytes<TYPE, MAXM, false>(R * nb);
+  const int region = layer_region_bytes<TYPE, MAXM, false>(R, nb);
   const int fixed = layer_sum_bytes(pairs, nb, rows);
   W = min(kLayerWaves - kLayerStagers, (kLayerLds - fixed) / region);
   lds = fixed + W * region;
   return pairs <= kSumPairs && fixed < kLayerLds && W >= kSumWaves;
 }
 
-// Pairs of an item: one for one token; for more, four, or two where four rows of activations take the LDS of the
-// waves' stages (down on 56-block rows, eight tokens: 143 us with four, 139 with two).
-constexpr int kLayerLongRow = 32;
-inline int layer_pairs(bool one, int nb) { return one ? 1 : nb > kLayerLongRow ? 2 : 4; }
+// Pairs of an item: one for one token, four for more. (Two for rows of more than 32 blocks, of which four rows of
+// activations take half the LDS: down of 4096 x 14336, eight tokens of 8 experts top 2, 115 us, with four 100; two
+// tokens 38 and 41.)
+inline int layer_pairs(bool one) { return one ? 1 : 4; }
 
 // f.template operator()<TYPE, MAXM>() of a type and a number of pairs; -1 for another type.
 template <class F>
 int with_layer_kernel(int type, int pairs, F f) {
   switch (type) {
 #define MXA_LAYER(t) \
-  case t: return pairs == 1 ? f.template operator()<t, 1>() : pairs == 2 ? f.template operator()<t, 2>() : f.template operator()<t, 4>();
+  case t: return pairs == 1 ? f.template operator()<t, 1>() : f.template operator()<t, 4>();
     MXA_LAYER(T_Q4_K)
     MXA_LAYER(T_Q6_K)
     MXA_LAYER(T_Q8_0)
@@ -701,24 +741,22 @@ int with_layer_kernel(int type, int pairs, F f) {
   }
 }
 
-template <bool GATEUP>
-struct LayerFits {
-  int nb;
-  template <int TYPE, int MAXM>
-  int operator()() const {
-    int R, W, lds;
-    return layer_shape<TYPE, MAXM, GATEUP>(nb, R, W, lds) ? 0 : -1;
-  }
-};
-
+// The first launch (GATEUP) or the second's item form; `dry`: whether it fits, no launch. -1 where it does not.
 template <bool GATEUP>
 struct LaunchLayer {
-  const LayerArgs& a;
+  LayerArgs a;
   int grid;
   hipStream_t stream;
+  bool dry;
   template <int TYPE, int MAXM>
-  int operator()() const {
-    return launch_layer<TYPE, MAXM, GATEUP>(a, grid, stream);
+  int operator()() {
+    int lds;
+    if (!layer_shape<TYPE, MAXM, GATEUP>(a.nb, a.R, a.W, lds)) return -1;
+    if (dry) return 0;
+    auto kern = moe_layer_kernel<TYPE, MAXM, GATEUP>;
+    allow_lds((const void*)kern, kLayerLds);
+    hipLaunchKernelGGL(kern, dim3(grid), dim3(64 * kLayerWaves), lds, stream, a);
+    return 0;
   }
 };
 
@@ -747,9 +785,11 @@ bool moe_layer_supported(int gate_type, int down_type, int n_experts, int top_k,
       n_embd < QK || ffn < QK || n_embd > 64 * QK || ffn > 64 * QK)
     return false;
   const bool one = n_tokens == 1;
-  const int kb = n_embd / QK, fb = ffn / QK;
-  return with_layer_kernel(gate_type, layer_pairs(one, kb), LayerFits<true>{kb}) == 0 &&
-         with_layer_kernel(down_type, layer_pairs(one, fb), LayerFits<false>{fb}) == 0;
+  LayerArgs a{};
+  a.nb = n_embd / QK;
+  if (with_layer_kernel(gate_type, layer_pairs(one), LaunchLayer<true>{a, 0, nullptr, true}) != 0) return false;
+  a.nb = ffn / QK;
+  return with_layer_kernel(down_type, layer_pairs(one), LaunchLayer<false>{a, 0, nullptr, true}) == 0;
 }
 
 size_t moe_layer_workspace(int n_tokens, int top_k, int n_embd, int ffn, bool bf16) {
@@ -764,25 +804,29 @@ int launch_moe_layer(int gate_type, int down_type, const uint8_t* gate, const ui
                      YOut out, void* ws, hipStream_t stream) {
   const int grid = cu_count();
   // a workgroup for every item, by their costs of 3 to 6
-  if (!moe_layer_supported(gate_type, down_type, n_experts, top_k, n_tokens, n_embd, ffn) || grid < 2 * n_tokens * top_k)
+  if (!moe_layer_supported(gate_type, down_type, n_experts, top_k, n_tokens, n_embd, ffn) ||
+      grid < 2 * n_tokens * top_k)
     return -1;
   const size_t pairs = (size_t)n_tokens * top_k;
   uint8_t* const act = (uint8_t*)ws;
   uint8_t* const rows = act + align256(pairs * ffn * (bf16 ? 2 : 4));
   LayerArgs a{gate, up, gate_stride, gate_row, x, ids, wts, act, logits, ffn, n_embd, n_embd / QK, 0, 0,
-              n_experts, top_k, n_tokens, logits_bf16 ? 1 : 0, norm_topk ? 1 : 0, bf16 ? 1 : 0, reciprocal ? 1 : 0, scale};
+              n_experts, top_k, n_tokens, logits_bf16 ? 1 : 0, norm_topk ? 1 : 0, bf16 ? 1 : 0, reciprocal ? 1 : 0,
+              scale};
   const bool one = n_tokens == 1;
-  if (with_layer_kernel(gate_type, layer_pairs(one, a.nb), LaunchLayer<true>{a, grid, stream}) != 0) return -1;
+  if (with_layer_kernel(gate_type, layer_pairs(one), LaunchLayer<true>{a, grid, stream, false}) != 0) return -1;
   a.w0 = down, a.w1 = nullptr, a.stride = down_stride, a.row_bytes = down_row, a.x = act, a.act = rows;
   a.n = n_embd, a.k = ffn, a.nb = ffn / QK;
-  if (with_layer_kernel(down_type, layer_pairs(one, a.nb), LaunchSum{a, out, grid, stream}) == 0) return 0;
-  if (with_layer_kernel(down_type, layer_pairs(one, a.nb), LaunchLayer<false>{a, grid, stream}) != 0) return -1;
-  return launch_moe_combine((const float*)rows, nullptr, ids, wts, n_tokens, top_k, n_embd, bf16 ? 1 : 0, 1, out, stream);
+  if (with_layer_kernel(down_type, layer_pairs(one), LaunchSum{a, out, grid, stream}) == 0) return 0;
+  if (with_layer_kernel(down_type, layer_pairs(one), LaunchLayer<false>{a, grid, stream, false}) != 0) return -1;
+  return launch_moe_combine((const float*)rows, nullptr, ids, wts, n_tokens, top_k, n_embd, bf16 ? 1 : 0, 1, out,
+                            stream);
 }
 
 int launch_moe_topk(const void* logits, bool bf16, int n_tokens, int n_experts, int top_k, bool norm_topk, float scale,
                     int32_t* ids, float* wts, hipStream_t stream) {
-  if (n_tokens < 1 || n_experts < 1 || n_experts > kMoeRouteMaxExperts || top_k < 1 || top_k > min(n_experts, 64)) return -1;
+  if (n_tokens < 1 || n_experts < 1 || n_experts > kMoeRouteMaxExperts || top_k < 1 || top_k > min(n_experts, 64))
+    return -1;
   hipLaunchKernelGGL(moe_topk_kernel, dim3((n_tokens + 3) / 4), dim3(256), 0, stream, logits, bf16 ? 1 : 0, n_tokens,
                      n_experts, top_k, norm_topk ? 1 : 0, scale, ids, wts);
   return 0;

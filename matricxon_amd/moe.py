@@ -123,7 +123,8 @@ class HipPackedMoEExperts(nn.Module):
         gives the same bits.
 
         Up to eight tokens (and 64 pairs) of Q4_K, Q6_K or Q8_0 experts, gate and up of one type, with a SiLU: one
-        library call, two launches over the weights and the sum (`mxa_moe_layer`). Otherwise the routing in one launch, then the grouped projections.
+        library call (`mxa_moe_layer`) of two launches, three where more than 16 pairs are added up. Otherwise the
+        routing in one launch, then the grouped projections.
 
         `q8k_scale` "reciprocal" takes the codes of the activations' blocks as rint(v * (127 * (1 / amax))), which is
         what torch evaluates for `127.0 / amax`, for layers that were tuned or are checked against such an emulation;
