@@ -23,8 +23,8 @@
 // What bounds it, MI355X, kernel alone with weights that no cache holds: 8 experts top 2 of 4096 x 14336 (Q4_K, Q6_K
 // down), one token, gate and up 28 us for 132 MB (4.7 TB/s; a read of as many bytes 21), of which 3 us before the
 // first copy and 3 after the last; down 28.5 us for 96 MB (3.4 TB/s), the LDS holding 11 rows of 56 blocks, which
-// wait and compute in turn. Eight tokens: 99 and 100 us, 4.8 and 3.5 TB/s: each further pair of an expert adds to
-// the part of a wave's turn in which its stage is not in flight. 64 experts top 8 of 2048 x 1024, one token: 11.7
+// wait and compute in turn. Eight tokens: 95 and 86 us, 5.0 and 4.0 TB/s: each further pair of an expert takes LDS from
+// the rows and adds to the part of a wave's turn in which its stage is not in flight. 64 experts top 8 of 2048 x 1024, one token: 11.7
 // and 11.5 us, latency from end to end (logits, routing, activations, weights, block arithmetic).
 //
 // The sum needs every pair's rows in one place. Up to 16 pairs the second launch's workgroups take rows, each through
@@ -324,19 +324,28 @@ __device__ __forceinline__ void fold_row(int nb, const float* xd, const float* v
 }
 
 template <int TYPE>
-constexpr int layer_stage_bytes(int blocks) {  // Q6_K rows start on any even byte
+__host__ __device__ constexpr int layer_stage_bytes(int blocks) {  // Q6_K rows start on any even byte
   return (blocks * Lpb<TYPE>::kBytes + (TYPE == T_Q6_K ? 15 : 0) + 1023) / 1024 * 1024;
 }
-template <int TYPE, int MAXM, bool GATEUP>
-constexpr int layer_region_bytes(int R, int nb) {
+// A wave's LDS for R rows and M activation rows: its stages and block values.
+template <int TYPE, bool GATEUP>
+__host__ __device__ constexpr int layer_region_bytes(int M, int R, int nb) {
   constexpr int kMats = GATEUP ? 2 : 1;
-  return kMats * (layer_stage_bytes<TYPE>(R * nb) +
-                  R * layer_fold_row(nb) * 4 * (MAXM + (Lpb<TYPE>::kHasD ? 1 : 0)));
+  return kMats * (layer_stage_bytes<TYPE>(R * nb) + R * layer_fold_row(nb) * 4 * (M + (Lpb<TYPE>::kHasD ? 1 : 0)));
 }
 // Activations of `rows` rows in LDS: q (272 bytes a block), bsums, d; and the routing.
-constexpr int layer_row_act(int nb) { return nb * (kActStride + 32) + 4 * layer_fold_row(nb); }
-constexpr int layer_act_bytes(int rows, int nb) { return (rows * layer_row_act(nb) + 15) / 16 * 16; }
+__host__ __device__ constexpr int layer_row_act(int nb) { return nb * (kActStride + 32) + 4 * layer_fold_row(nb); }
+__host__ __device__ constexpr int layer_act_bytes(int rows, int nb) {
+  return (rows * layer_row_act(nb) + 15) / 16 * 16;
+}
 constexpr int kLayerFixed = 4 * kLayerMaxPairs;
+// Waves with rows of an item of M pairs, 0 or less where not one's fit. Fewer pairs leave LDS to more of them (with
+// as many waves for any item, eight tokens of 8 experts top 2, 4096 x 14336, took 99 and 100 us, not 95 and 86).
+template <int TYPE, bool GATEUP>
+__host__ __device__ constexpr int layer_waves(int M, int R, int nb) {
+  const int w = (kLayerLds - kLayerFixed - layer_act_bytes(M, nb)) / layer_region_bytes<TYPE, GATEUP>(M, R, nb);
+  return w < kLayerWaves - kLayerStagers ? w : kLayerWaves - kLayerStagers;
+}
 
 template <int TYPE, int MAXM, bool GATEUP>
 __global__ __launch_bounds__(64 * kLayerWaves) void moe_layer_kernel(LayerArgs a) {
@@ -346,26 +355,23 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_layer_kernel(LayerArgs a
   extern __shared__ __align__(16) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 63, wg = blockIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = blockDim.x >> 6;
-  const int pairs = a.n_tokens * a.top_k, W = a.W, nb = a.nb;
+  const int pairs = a.n_tokens * a.top_k, nb = a.nb, R = a.R;
   int* const sid = (int*)smem;  // the pairs' experts
   uint8_t* const acts = smem + kLayerFixed;
   int8_t* const aq = (int8_t*)acts;  // row m, block b at (m nb + b) 272
-  int16_t* const abs_ = (int16_t*)(acts + MAXM * nb * kActStride);
-  float* const ad = (float*)(acts + MAXM * nb * (kActStride + 32));
-  const bool rows_wave = wave < W;
 
   constexpr int kBufs = kLayerBufs;
-  const int step = 4 * (waves - W), p16 = lane & 15, g0 = 4 * (wave - W) + (lane >> 4);
   uint4 raw[kBufs][4] = {};
-  const auto part_of = [&](int g, int total, long long row, int b, int d_at) __attribute__((always_inline)) {
-    return ActPart{g < total, row * a.k + b * QK + 16 * p16, aq + (size_t)g * kActStride, abs_ + 16 * g, ad + d_at};
-  };
+  const int p16 = lane & 15;
   constexpr bool kOneToken = GATEUP && MAXM == 1;  // its row is known before its experts are
-  const auto token_block = [&](int i) __attribute__((always_inline)) {
-    const int g = g0 + step * i;
-    return part_of(g, nb, 0, g, g);
-  };
-  if (kOneToken && !rows_wave) fetch_acts(a, 0, token_block, raw);
+  if constexpr (kOneToken) {
+    const int W = layer_waves<TYPE, GATEUP>(1, R, nb);
+    const auto token_block = [&](int i) __attribute__((always_inline)) {
+      const int g = 4 * (wave - W) + (lane >> 4) + 4 * (waves - W) * i;
+      return ActPart{g < nb, (long long)g * QK + 16 * p16, nullptr, nullptr, nullptr};
+    };
+    if (wave >= W) fetch_acts(a, 0, token_block, raw);
+  }
 
   // the pairs' experts
   int e_lane = -1;
@@ -414,16 +420,18 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_layer_kernel(LayerArgs a
     part = wg - __builtin_amdgcn_readlane(from, lead);
   }
   const LayerItem it = layer_item<MAXM>(lead, e_lane, same);
-  const int M = it.M;
+  const int M = it.M, W = layer_waves<TYPE, GATEUP>(M, R, nb);
+  const bool rows_wave = wave < W;
+  int16_t* const abs_ = (int16_t*)(acts + M * nb * kActStride);
+  float* const ad = (float*)(acts + M * nb * (kActStride + 32));
 
-  const int R = a.R, sets = (a.n + R - 1) / R;
+  const int sets = (a.n + R - 1) / R;
   const int lo = part * sets / wpi, hi = (part + 1) * sets / wpi;  // below 2^8 * 2^14
   const int blocks = R * nb, stage = layer_stage_bytes<TYPE>(blocks);
-  uint8_t* const region =
-      acts + layer_act_bytes(MAXM, nb) + (size_t)wave * layer_region_bytes<TYPE, MAXM, GATEUP>(R, nb);
+  uint8_t* const region = acts + layer_act_bytes(M, nb) + (size_t)wave * layer_region_bytes<TYPE, GATEUP>(M, R, nb);
   const int fold = layer_fold_row(nb), fold_set = R * fold;
   float* const Vbuf = (float*)(region + kMats * stage);  // [matrix][activation row][row][fold]
-  float* const Dbuf = Vbuf + kMats * MAXM * fold_set;    // [matrix][row][fold]
+  float* const Dbuf = Vbuf + kMats * M * fold_set;       // [matrix][row][fold]
   const uintptr_t base0 = (uintptr_t)a.w0 + (uintptr_t)((long long)it.expert * a.stride);
   const uintptr_t base1 = (uintptr_t)a.w1 + (uintptr_t)((long long)it.expert * a.stride);
   // The packed bytes of set s's rows of matrix t into its stage, and the copies that takes (none past the last set).
@@ -434,10 +442,11 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_layer_kernel(LayerArgs a
                      (uint32_t)min(R, a.n - n0) * (uint32_t)a.row_bytes, lds_addr(region) + (uint32_t)(t * stage));
   };
 
-  const int total = M * nb;
+  const int total = M * nb, step = 4 * (waves - W), g0 = 4 * (wave - W) + (lane >> 4);
   const auto item_block = [&](int i) __attribute__((always_inline)) {  // of the item's rows
     const int g = g0 + step * i, m = MAXM == 1 ? 0 : g / nb, p = MAXM == 1 ? lead : it.pair(m);
-    return part_of(g, total, GATEUP ? p / a.top_k : p, g - m * nb, m * fold + g - m * nb);
+    return ActPart{g < total, (long long)(GATEUP ? p / a.top_k : p) * a.k + (g - m * nb) * QK + 16 * p16,
+                   aq + (size_t)g * kActStride, abs_ + 16 * g, ad + m * fold + g - m * nb};
   };
   int s = lo + wave, behind = 0;  // copies issued behind those of the stage that is waited for next
   if (rows_wave) {
@@ -491,9 +500,11 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_layer_kernel(LayerArgs a
           L::template compute<1, ActRegs>(region + t * stage, delta + jl * L::kBytes, &areg, 1, V, D);
         else
           L::template compute<MAXM, ActBlock>(region + t * stage, delta + jl * L::kBytes, ab, M, V, D);
+        uint32_t v_at = (uint32_t)(t * M * fold_set + to);
+        if constexpr (MAXM > 1) asm volatile("" : "+v"(v_at));  // counted up, not MAXM kept across the sets: they spill
 #pragma unroll
-        for (int m = 0; m < MAXM; ++m)
-          if (m < M && lane < blocks) Vbuf[(t * MAXM + m) * fold_set + to] = V[m];
+        for (int m = 0; m < MAXM; ++m, v_at += (uint32_t)fold_set)
+          if (m < M && lane < blocks) Vbuf[v_at] = V[m];
         if (L::kHasD && lane < blocks) Dbuf[t * fold_set + to] = D;
         __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0): the stage has been read
         wave_sync();
@@ -504,7 +515,7 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_layer_kernel(LayerArgs a
         const int fr = f % R, fm = f / R;
         if (fr >= nrows) continue;
         float acc[kMats];
-        fold_row<TYPE, kMats>(nb, ad + fm * fold, Vbuf + fm * fold_set + fr * fold, MAXM * fold_set, Dbuf + fr * fold,
+        fold_row<TYPE, kMats>(nb, ad + fm * fold, Vbuf + fm * fold_set + fr * fold, M * fold_set, Dbuf + fr * fold,
                               fold_set, acc);
         const int p = MAXM == 1 ? lead : it.pair(fm);
         const long long at = (long long)p * a.n + n0 + fr;
@@ -562,7 +573,7 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_down_sum_kernel(LayerArg
   const int sets = (nr + R - 1) / R, tasks = items * sets;
   const int blocks = R * nb, stage = layer_stage_bytes<TYPE>(blocks);
   uint8_t* const region =
-      acts + layer_sum_bytes(pairs, nb, rows) - kSumFixed + (size_t)wave * layer_region_bytes<TYPE, MAXM, false>(R, nb);
+      acts + layer_sum_bytes(pairs, nb, rows) - kSumFixed + (size_t)wave * layer_region_bytes<TYPE, false>(MAXM, R, nb);
   const int fold = layer_fold_row(nb), fold_set = R * fold;
   float* const Vbuf = (float*)(region + stage);  // [activation row][row][fold]
   float* const Dbuf = Vbuf + MAXM * fold_set;
@@ -690,22 +701,19 @@ __global__ __launch_bounds__(256) void moe_topk_kernel(const void* __restrict__ 
               });
 }
 
-// Rows per wave, row waves and LDS for a matrix of rows of nb blocks, the most rows that the LDS holds at once (of 6
-// blocks of Q8_0, gate and up, seven waves of 6 rows, not four of 10); false when not one wave's rows fit.
+// Rows per wave for a matrix of rows of nb blocks, the most rows that the LDS holds at once (of 6 blocks of Q8_0, gate
+// and up, seven waves of 6 rows, not four of 10); 0 where not one wave's rows fit.
 template <int TYPE, int MAXM, bool GATEUP>
-bool layer_shape(int nb, int& R, int& W, int& lds) {
-  const int act = kLayerFixed + layer_act_bytes(MAXM, nb);
-  R = W = lds = 0;
-  if (act >= kLayerLds) return false;
+int layer_rows(int nb) {
+  int R = 0, most = 0;
   for (int r = 64 / nb; r >= 1; --r) {
-    const int region = layer_region_bytes<TYPE, MAXM, GATEUP>(r, nb);
-    const int w = min(kLayerWaves - kLayerStagers, (kLayerLds - act) / region);
-    if (w * r > W * R) R = r, W = w, lds = act + w * region;
+    const int held = r * layer_waves<TYPE, GATEUP>(MAXM, r, nb);
+    if (held > most) R = r, most = held;
   }
-  return W >= 1;
+  return R;
 }
 
-// The same of the second launch that adds up: `rows` output rows a workgroup, at least kSumWaves waves of them, and up
+// The shape of the second launch that adds up: `rows` output rows a workgroup, at least kSumWaves waves of them, and up
 // to kSumPairs pairs, all of whose activations a workgroup quantizes. Both launches from start to end, adding up and
 // with the combine's launch: one token of 8 experts top 2 (4096 x 14336) 56.3 and 58.0 us, of 64 top 8 (2048 x 1024)
 // 25.0 and 27.4, of 5 top 1 (4096 x 4096) 22.7 and 26.3; 12 pairs (16 top 4, 2048 x 1536) 30.8 both; 16 pairs (128 top
@@ -715,16 +723,16 @@ constexpr int kSumWaves = 8, kSumPairs = 16;
 template <int TYPE, int MAXM>
 bool layer_sum_shape(int nb, int pairs, int rows, int& R, int& W, int& lds) {
   R = min(64 / nb, rows);
-  const int region = layer_region_bytes<TYPE, MAXM, false>(R, nb);
+  const int region = layer_region_bytes<TYPE, false>(MAXM, R, nb);
   const int fixed = layer_sum_bytes(pairs, nb, rows);
   W = min(kLayerWaves - kLayerStagers, (kLayerLds - fixed) / region);
   lds = fixed + W * region;
   return pairs <= kSumPairs && fixed < kLayerLds && W >= kSumWaves;
 }
 
-// Pairs of an item: one for one token, four for more. (Two for rows of more than 32 blocks, of which four rows of
-// activations take half the LDS: down of 4096 x 14336, eight tokens of 8 experts top 2, 115 us, with four 100; two
-// tokens 38 and 41.)
+// Pairs of an item: one for one token, four for more. With two, experts of three and four pairs are read twice: eight
+// tokens of 8 experts top 2 (4096 x 14336) 234 us, with four 187; where experts rarely have more than two, two save
+// registers only (eight tokens of 32 top 3, 2560 x 768, 41 and 44; of 64 top 8, 2048 x 1024, 56 and 54).
 inline int layer_pairs(bool one) { return one ? 1 : 4; }
 
 // f.template operator()<TYPE, MAXM>() of a type and a number of pairs; -1 for another type.
@@ -750,12 +758,12 @@ struct LaunchLayer {
   bool dry;
   template <int TYPE, int MAXM>
   int operator()() {
-    int lds;
-    if (!layer_shape<TYPE, MAXM, GATEUP>(a.nb, a.R, a.W, lds)) return -1;
+    a.R = layer_rows<TYPE, MAXM, GATEUP>(a.nb);
+    if (a.R == 0) return -1;
     if (dry) return 0;
     auto kern = moe_layer_kernel<TYPE, MAXM, GATEUP>;
     allow_lds((const void*)kern, kLayerLds);
-    hipLaunchKernelGGL(kern, dim3(grid), dim3(64 * kLayerWaves), lds, stream, a);
+    hipLaunchKernelGGL(kern, dim3(grid), dim3(64 * kLayerWaves), kLayerLds, stream, a);
     return 0;
   }
 };
