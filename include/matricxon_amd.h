@@ -269,14 +269,17 @@ int mxa_moe_combine_masked(const float *down, const int32_t *rows, const int32_t
                            const float *weights, int n_tokens, int top_k, int n_embd, int round_bf16,
                            float *out, void *stream);
 
+/* Most tokens of one mxa_moe_topk, mxa_add_rms_norm_q8_k or mxa_rope: a grid holds below 2^32 threads. */
+#define MXA_MAX_TOKENS (1 << 24)
+
 /* Routing of MoE tokens from router logits (n_tokens, n_experts), float32 or bfloat16 (logits_bf16 != 0): ids
  * and weights (n_tokens, top_k), DEVICE int32 and float32. Slot i of a token is its i-th largest logit, ties to
  * the lowest id; its weight is exp(logit - max) over the sum of those of all experts (norm_topk 0) or of the
  * chosen ones (norm_topk 1), times scale. A logit of -inf is an expert that the token may not take: where
  * fewer than top_k are left the slots behind them get id -1 and weight 0 (all of them for a token with
  * none). NaN counts as the largest logit and makes its token's weights NaN. n_experts <= 256, top_k <= 64
- * and <= n_experts; else -1. The router's softmax and top-k before `QuantizedMoEExperts.forward`
- * (app/architectures/moe_experts.py:29-89). */
+ * and <= n_experts, n_tokens <= MXA_MAX_TOKENS; else -1. The router's softmax and top-k before
+ * `QuantizedMoEExperts.forward` (app/architectures/moe_experts.py:29-89). */
 int mxa_moe_topk(const void *logits, int logits_bf16, int n_tokens, int n_experts, int top_k,
                  int norm_topk, float scale, int32_t *ids, float *weights, void *stream);
 
@@ -286,17 +289,17 @@ int mxa_moe_topk(const void *logits, int logits_bf16, int n_tokens, int n_expert
 size_t mxa_moe_layer_workspace_bytes(int gate_type, int down_type, int n_experts, int top_k, int n_tokens,
                                      int n_embd, int ffn_len, int bf16);
 
-/* A whole mixture-of-experts layer of packed experts for a few tokens, in two launches (three past 16 pairs): the routing of
- * mxa_moe_topk, silu(gate_e x) * (up_e x) of each token's experts, down_e of that, and their weighted sum
- * in ascending expert id. x (n_tokens, n_embd) bfloat16 (bf16 != 0) or float32, 16-byte aligned; expert e at
- * gate and up + e * gate_stride (ffn_len rows) and down + e * down_stride (n_embd rows), 16-byte aligned
+/* A whole mixture-of-experts layer of packed experts for a few tokens, in two launches (three past 16 pairs):
+ * the routing of mxa_moe_topk, silu(gate_e x) * (up_e x) of each token's experts, down_e of that, and their
+ * weighted sum in ascending expert id. x (n_tokens, n_embd) bfloat16 (bf16 != 0) or float32, 16-byte aligned;
+ * expert e at gate and up + e * gate_stride (ffn_len rows) and down + e * down_stride (n_embd rows), 16-byte aligned
  * bases and strides; ids and weights (n_tokens, top_k) are written as mxa_moe_topk writes them; out (n_tokens,
  * n_embd) float32 or bfloat16 (out_bf16 != 0). The steps, roundings and bits are those of mxa_gemm_moe(_bf16)
  * for gate and up, mxa_silu_mul_q8_k(_bf16), mxa_gemm_moe for down and mxa_moe_combine_masked
  * (round_bf16 = bf16), then the cast to out's type; with reciprocal != 0 the codes of the Q8_K blocks are
  * rint(v * (127 * (1 / amax))) in place of rint(v * (127 / amax)), as an emulation in torch computes them
- * (its 127.0 / amax is that product), which differ where v * 127 / amax is next to a half. Replaces the per-expert loop of
- * `QuantizedMoEExperts.forward` (app/architectures/moe_experts.py:81-88) with its routing. */
+ * (its 127.0 / amax is that product), which differ where v * 127 / amax is next to a half. Replaces the
+ * per-expert loop of `QuantizedMoEExperts.forward` (app/architectures/moe_experts.py:81-88) with its routing. */
 int mxa_moe_layer(int gate_type, int down_type, const void *gate, const void *up, long long gate_stride,
                   const void *down, long long down_stride, int n_experts, const void *x, int bf16,
                   const void *logits, int logits_bf16, int top_k, int norm_topk, float scale, int n_tokens,
@@ -342,8 +345,8 @@ int mxa_silu_mul_q8_k(const float *gate, const float *up, long long ld, int n_to
  *   u = x, or with post_weight x * post_weight / sqrt(mean(x^2) + post_eps)
  *   hidden = r + scale * gate * u
  *   out = hidden * weight / sqrt(mean(hidden^2) + eps), of hidden as it was stored
- * over n_tokens rows of dim values (1 .. 32768), in float32, hidden and out each rounded once. x,
- * post_weight, gate, weight and out are bfloat16 (bf16 != 0) or float32, residual and hidden bfloat16
+ * over n_tokens rows (up to MXA_MAX_TOKENS) of dim values (1 .. 32768), in float32, hidden and out each
+ * rounded once. x, post_weight, gate, weight and out are bfloat16 (bf16 != 0) or float32, residual and hidden bfloat16
  * (residual_bf16 != 0, with bf16 only) or float32. Rows of x, residual and gate are ldx, ldr and ldg values
  * apart (0: one row for all); gate is NULL, or has a value for each column (gate_step 1) or one for a row
  * (gate_step 0); post_weight is NULL or dim values. hidden and out are contiguous and overlap no input.
@@ -365,11 +368,12 @@ int mxa_add_rms_norm_q8_k(const void *x, long long ldx, const void *residual, lo
  * position * turns[i] full turns (DEVICE float64, rotary_dim / 2: the angle per position / 2 pi), times
  * scale; the others are copied. The position of a token is positions[pos_batch * sequence + pos_token *
  * step], DEVICE int32 or int64. Values float32 or bfloat16 (bf16 != 0), each rounded once from float32. Any
- * position: the angle is reduced in float64. head_dim and rotary_dim even, head_dim <= MXA_ROPE_MAX_DIM.
+ * position: the angle is reduced in float64. head_dim and rotary_dim even, head_dim <= MXA_ROPE_MAX_DIM,
+ * n_tokens <= MXA_MAX_TOKENS.
  * The reference's CPU libraries fuse the same step (app/native/src/mx_fused_ops.c); its GPU layers run it
  * in torch operations. */
 #define MXA_ROPE_MAX_DIM 1024
-#define MXA_ROPE_MAX_HEADS 65536
+#define MXA_ROPE_MAX_HEADS 65536 /* of q, and of k */
 int mxa_rope(const void *q, const long long *q_strides, int q_heads, const void *k,
              const long long *k_strides, int k_heads, const void *positions, int positions_int64,
              long long pos_batch, long long pos_token, const double *turns, int n_tokens, int seq_len,

@@ -505,8 +505,8 @@ int mxa_moe_combine_masked(const float* down, const int32_t* rows, const int32_t
 
 int mxa_moe_topk(const void* logits, int logits_bf16, int n_tokens, int n_experts, int top_k, int norm_topk,
                  float scale, int32_t* ids, float* weights, void* stream) {
-  if (logits == nullptr || ids == nullptr || weights == nullptr || !aligned(logits, logits_bf16 ? 2 : 4) ||
-      !aligned(ids, 4) || !aligned(weights, 4))
+  if (logits == nullptr || ids == nullptr || weights == nullptr || n_tokens > MXA_MAX_TOKENS ||
+      !aligned(logits, logits_bf16 ? 2 : 4) || !aligned(ids, 4) || !aligned(weights, 4))
     return MXA_ERR_UNSUPPORTED;
   if (mxa::launch_moe_topk(logits, logits_bf16 != 0, n_tokens, n_experts, top_k, norm_topk != 0, scale, ids, weights,
                            (hipStream_t)stream) != 0)
@@ -523,21 +523,25 @@ size_t mxa_moe_layer_workspace_bytes(int gate_type, int down_type, int n_experts
 int mxa_moe_layer(int gate_type, int down_type, const void* gate, const void* up, long long gate_stride,
                   const void* down, long long down_stride, int n_experts, const void* x, int bf16, const void* logits,
                   int logits_bf16, int top_k, int norm_topk, float scale, int n_tokens, int n_embd, int ffn_len,
-                  int reciprocal, int32_t* ids, float* weights, void* out, int out_bf16, void* workspace, size_t workspace_bytes,
-                  void* stream) {
-  const size_t need = mxa_moe_layer_workspace_bytes(gate_type, down_type, n_experts, top_k, n_tokens, n_embd, ffn_len, bf16);
+                  int reciprocal, int32_t* ids, float* weights, void* out, int out_bf16, void* workspace,
+                  size_t workspace_bytes, void* stream) {
+  const size_t need =
+      mxa_moe_layer_workspace_bytes(gate_type, down_type, n_experts, top_k, n_tokens, n_embd, ffn_len, bf16);
   if (need == 0 || gate == nullptr || up == nullptr || down == nullptr || x == nullptr || logits == nullptr ||
       ids == nullptr || weights == nullptr || out == nullptr || !aligned(gate, 16) || !aligned(up, 16) ||
       !aligned(down, 16) || !aligned(x, 16) || !aligned(logits, logits_bf16 ? 2 : 4) || !aligned(ids, 4) ||
       !aligned(weights, 4) || !aligned(out, out_bf16 ? 2 : 4) || !aligned(workspace, 16))
     return MXA_ERR_UNSUPPORTED;
-  const long long gate_row = (long long)mxa_row_bytes(gate_type, n_embd), down_row = (long long)mxa_row_bytes(down_type, ffn_len);
-  if (gate_stride < gate_row * ffn_len || down_stride < down_row * n_embd || gate_stride % 16 != 0 || down_stride % 16 != 0)
+  const long long gate_row = (long long)mxa_row_bytes(gate_type, n_embd);
+  const long long down_row = (long long)mxa_row_bytes(down_type, ffn_len);
+  if (gate_stride < gate_row * ffn_len || down_stride < down_row * n_embd || gate_stride % 16 != 0 ||
+      down_stride % 16 != 0)
     return MXA_ERR_UNSUPPORTED;
   if (workspace == nullptr || workspace_bytes < need) return MXA_ERR_WORKSPACE;
   if (mxa::launch_moe_layer(gate_type, down_type, (const uint8_t*)gate, (const uint8_t*)up, gate_stride, gate_row,
                             (const uint8_t*)down, down_stride, down_row, n_experts, x, bf16 != 0, logits,
-                            logits_bf16 != 0, top_k, norm_topk != 0, scale, n_tokens, n_embd, ffn_len, reciprocal != 0, ids, weights,
+                            logits_bf16 != 0, top_k, norm_topk != 0, scale, n_tokens, n_embd, ffn_len,
+                            reciprocal != 0, ids, weights,
                             out_bf16 ? mxa::YOut::bf16(out) : mxa::YOut::f32((float*)out), workspace,
                             (hipStream_t)stream) != 0)
     return MXA_ERR_UNSUPPORTED;
@@ -631,7 +635,8 @@ int mxa_add_rms_norm_q8_k(const void* x, long long ldx, const void* residual, lo
                           void* workspace, size_t workspace_bytes, void* stream) {
   const uintptr_t xa = bf16 ? 2 : 4, ra = residual_bf16 ? 2 : 4;
   if (x == nullptr || residual == nullptr || weight == nullptr || hidden == nullptr || out == nullptr ||
-      n_tokens <= 0 || dim <= 0 || ldx < 0 || ldr < 0 || ldg < 0 || (gate_step != 0 && gate_step != 1) ||
+      n_tokens <= 0 || n_tokens > MXA_MAX_TOKENS || dim <= 0 || ldx < 0 || ldr < 0 || ldg < 0 ||
+      (gate_step != 0 && gate_step != 1) ||
       (residual_bf16 && !bf16) || !aligned(x, xa) || !aligned(weight, xa) || !aligned(post_weight, xa) ||
       !aligned(gate, xa) || !aligned(out, xa) || !aligned(residual, ra) || !aligned(hidden, ra) ||
       !aligned(workspace, 16))
@@ -656,11 +661,13 @@ int mxa_rope(const void* q, const long long* q_strides, int q_heads, const void*
   const uintptr_t ea = bf16 ? 2 : 4;
   if (q == nullptr || q_strides == nullptr || q_out == nullptr || positions == nullptr || turns == nullptr ||
       q_heads < 1 || k_heads < 0 || q_heads > MXA_ROPE_MAX_HEADS || k_heads > MXA_ROPE_MAX_HEADS ||
-      n_tokens < 1 || seq_len < 1 || head_dim < 2 || head_dim > MXA_ROPE_MAX_DIM || head_dim % 2 != 0 ||
+      n_tokens < 1 || n_tokens > MXA_MAX_TOKENS || seq_len < 1 || head_dim < 2 || head_dim > MXA_ROPE_MAX_DIM ||
+      head_dim % 2 != 0 ||
       rotary_dim < 2 || rotary_dim > head_dim || rotary_dim % 2 != 0 || !aligned(q, ea) || !aligned(q_out, ea) ||
       !aligned(positions, positions_int64 ? 8 : 4) || !aligned(turns, 8))
     return MXA_ERR_UNSUPPORTED;
-  if (k_heads > 0 && (k == nullptr || k_strides == nullptr || k_out == nullptr || !aligned(k, ea) || !aligned(k_out, ea)))
+  if (k_heads > 0 &&
+      (k == nullptr || k_strides == nullptr || k_out == nullptr || !aligned(k, ea) || !aligned(k_out, ea)))
     return MXA_ERR_UNSUPPORTED;
   if (mxa::launch_rope(q, q_strides, q_heads, k, k_strides, k_heads, positions, positions_int64 != 0, pos_batch,
                        pos_token, turns, n_tokens, seq_len, head_dim, rotary_dim, interleaved != 0, scale,

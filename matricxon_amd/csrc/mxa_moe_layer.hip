@@ -24,8 +24,8 @@
 // down), one token, gate and up 28 us for 132 MB (4.7 TB/s; a read of as many bytes 21), of which 3 us before the
 // first copy and 3 after the last; down 28.5 us for 96 MB (3.4 TB/s), the LDS holding 11 rows of 56 blocks, which
 // wait and compute in turn. Eight tokens: 95 and 86 us, 5.0 and 4.0 TB/s: each further pair of an expert takes LDS from
-// the rows and adds to the part of a wave's turn in which its stage is not in flight. 64 experts top 8 of 2048 x 1024, one token: 11.7
-// and 11.5 us, latency from end to end (logits, routing, activations, weights, block arithmetic).
+// the rows and adds to the part of a wave's turn in which its stage is not in flight. 64 experts top 8 of 2048 x
+// 1024, one token: 11.7 and 11.5 us, latency from end to end (logits, routing, activations, weights, block arithmetic).
 //
 // The sum needs every pair's rows in one place. Up to 16 pairs the second launch's workgroups take rows, each through
 // all items, and add up in LDS. For more they take items, and the combine is a launch of its own (4 to 5 us): adding up

@@ -180,7 +180,7 @@ void launch_rope_v(const RopeArgs& a, hipStream_t stream) {
   // of so many tokens would not survive in (700 tokens 6.3 and 6.0, 1500 10.2 and 8.4, 4096 17.3 and 15.5).
   const bool many = a.n_tokens > 512;
   const int TP = many ? min(8, (a.n_tokens + 1023) / 1024) : 1;
-  const int split = many ? 1 : (H + HP - 1) / HP;
+  const int split = many ? 1 : min(4096, (H + HP - 1) / HP);  // a grid's threads have to stay below 2^32
   auto kern = many ? rope_kernel<T, INTER, V, true> : rope_kernel<T, INTER, V, false>;
   hipLaunchKernelGGL(kern, dim3((a.n_tokens + TP - 1) / TP, split), dim3(kRopeThreads),
                      (size_t)TP * a.rot * sizeof(float), stream, a, TP, C, CR, HP);
@@ -202,7 +202,8 @@ int launch_rope(const void* q, const long long* q_strides, int q_heads, const vo
                 const double* turns, int n_tokens, int seq, int dim, int rot, bool interleaved, float mscale,
                 bool bf16, void* q_out, void* k_out, hipStream_t stream) {
   const RopeArgs a{{q, q_out, q_strides[0], q_strides[1], q_strides[2], q_heads},
-                   {k, k_out, k_heads ? k_strides[0] : 0, k_heads ? k_strides[1] : 0, k_heads ? k_strides[2] : 0, k_heads},
+                   {k, k_out, k_heads ? k_strides[0] : 0, k_heads ? k_strides[1] : 0, k_heads ? k_strides[2] : 0,
+                    k_heads},
                    pos, pos_batch, pos_tok, turns, pos64 ? 1 : 0, n_tokens, seq, dim, rot, mscale};
   if (bf16)
     interleaved ? launch_rope_t<uint16_t, true>(a, stream) : launch_rope_t<uint16_t, false>(a, stream);

@@ -51,6 +51,9 @@ class _Handoff:
         self._local = threading.local()
 
     def offer(self, out: torch.Tensor, workspace: torch.Tensor) -> None:
+        if out.is_inference():  # without a version, a later write to it would go unseen
+            self._local.slot = None
+            return
         self._local.slot = (out, out._version, workspace, out.device, _stream_of(out.device))
 
     def clear(self) -> None:
@@ -130,12 +133,13 @@ class HipFusedOps:
         256-value blocks). `gate` broadcasts to x: one value, one a channel, one a token, or all. The stream may
         be float32 beside a bfloat16 block; the weights and the gate have x's dtype, post_eps is eps unless given.
         Float32 steps; hidden and normed are each rounded once (rms_norm's bfloat16 steps round twice, as torch's
-        do). None for what it does not take: CPU tensors, other dtypes or shapes, rows of more than 32768 values."""
+        do). None for what it does not take: CPU tensors, other dtypes or shapes, rows of more than 32768 values,
+        more than 2^24 rows."""
         shape, dt, dev = x.shape, x.dtype, x.device
         k = shape[-1] if shape else 0
         if (dev.type != "cuda" or (dt is not torch.bfloat16 and dt is not torch.float32) or residual.shape != shape
                 or (residual.dtype is not dt and residual.dtype is not torch.float32) or residual.device != dev
-                or not 1 <= k <= HipGemm.NORM_MAX_VALUES or x.numel() == 0):
+                or not 1 <= k <= HipGemm.NORM_MAX_VALUES or not 0 < x.numel() <= k * HipGemm.MAX_TOKENS):
             return None
         for w in (weight,) if post_weight is None else (weight, post_weight):
             if w.dtype is not dt or w.shape != (k,) or w.device != dev:

@@ -439,6 +439,7 @@ class HipGemm:
         self._check(status, "mxa_rms_norm_q8_k_bf16", 15)
         return out, ws
 
+    MAX_TOKENS = 1 << 24  # rows of one add_rms_norm_q8k, tokens of one rope or moe_topk
     NORM_MAX_VALUES = 32768  # the longest row of add_rms_norm_q8k
 
     def add_rms_norm_q8k(self, residual: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, eps: float,
@@ -459,6 +460,8 @@ class HipGemm:
         if not 1 <= k <= self.NORM_MAX_VALUES or residual.shape != x.shape or residual.device != dev:
             raise ValueError(f"x and residual must be (..., K) on one device, K in 1..{self.NORM_MAX_VALUES}, got "
                              f"{tuple(x.shape)} and {tuple(residual.shape)}")
+        if x.numel() > k * self.MAX_TOKENS:
+            raise ValueError(f"x must have up to {self.MAX_TOKENS} rows, got {tuple(x.shape)}")
         for name, w in (("weight", weight), ("post_weight", post_weight)):
             if w is not None and (w.shape != (k,) or w.dtype != dt or w.device != dev):
                 raise ValueError(f"{name} must be ({k},) {dt} on {dev}")
@@ -501,8 +504,8 @@ class HipGemm:
             return hidden, out, ws
         status = self._lib.mxa_add_rms_norm_q8_k(
             x2.data_ptr(), ldx, r2.data_ptr(), ldr, post, float(eps if post_eps is None else post_eps), gate_ptr, ldg,
-            gstep, float(scale), weight.data_ptr(), float(eps), m, k, x.dtype is torch.bfloat16, residual.dtype is torch.bfloat16,
-            hidden.data_ptr(), out.data_ptr(), ws_ptr, ws_bytes, _stream(dev))
+            gstep, float(scale), weight.data_ptr(), float(eps), m, k, x.dtype is torch.bfloat16,
+            residual.dtype is torch.bfloat16, hidden.data_ptr(), out.data_ptr(), ws_ptr, ws_bytes, _stream(dev))
         if status != 0:
             self._check(status, "mxa_add_rms_norm_q8_k", 15)
         return hidden, out, ws
@@ -539,6 +542,8 @@ class HipGemm:
                 return self.rope(q, k, positions, turns, rotary_dim, interleaved, scale)
         seq = lead[-1]
         n_tokens = seq if nd == 3 else lead[0] * seq
+        if n_tokens > self.MAX_TOKENS:
+            raise ValueError(f"q must have up to {self.MAX_TOKENS} tokens, got {tuple(q.shape)}")
         ps = positions.stride()
         pos_batch = 0 if len(ps) == 1 or positions.shape[0] == 1 else ps[0]
         q, q_strides = _head_strides(q, nd)
@@ -759,7 +764,7 @@ class HipGemm:
         the lowest id, weights the softmax over all experts or (`norm_topk`) over the chosen ones, times `scale`. A
         logit of -inf is no expert: slots without one have id -1 and weight 0."""
         _require_device_tensor("logits", logits)
-        self._check_router(logits, logits.shape[0] if logits.dim() == 2 else 0, logits.shape[-1], top_k)
+        self._check_router(logits, *(logits.shape if logits.dim() == 2 else (0, 0)), top_k)
         dev, n_tokens = logits.device, logits.shape[0]
         logits = logits.detach().contiguous()
         ids = torch.empty((n_tokens, top_k), dtype=torch.int32, device=dev)
@@ -776,10 +781,10 @@ class HipGemm:
         return ids, weights
 
     def _check_router(self, logits: torch.Tensor, n_tokens: int, n_experts: int, top_k: int) -> None:
-        if logits.dim() != 2 or tuple(logits.shape) != (n_tokens, n_experts) or \
+        if logits.dim() != 2 or tuple(logits.shape) != (n_tokens, n_experts) or n_tokens > self.MAX_TOKENS or \
                 logits.dtype not in (torch.float32, torch.bfloat16):
-            raise ValueError(f"router logits must be float32 or bfloat16 ({n_tokens}, {n_experts}), got {logits.dtype} "
-                             f"{tuple(logits.shape)}")
+            raise ValueError(f"router logits must be float32 or bfloat16 ({n_tokens}, {n_experts}) of up to "
+                             f"{self.MAX_TOKENS} tokens, got {logits.dtype} {tuple(logits.shape)}")
         if not 1 <= top_k <= min(n_experts, self.MOE_MAX_TOP_K) or n_experts > self.MOE_ROUTE_MAX_EXPERTS:
             raise ValueError(f"top_k must be 1..min(n_experts, {self.MOE_MAX_TOP_K}) of up to "
                              f"{self.MOE_ROUTE_MAX_EXPERTS} experts, got {top_k} of {n_experts}")

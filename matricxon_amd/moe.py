@@ -94,7 +94,7 @@ class HipPackedMoEExperts(nn.Module):
                           self._gemm.row_bytes(int(t), k) % 16 == 0
                           for t, k in ((gate_type, n_embd), (up_type, n_embd), (down_type, ffn_len)))
         # what mxa_moe_layer takes besides its sizes; its workspace by (tokens, top_k), 0 where it declines
-        self._layer_ok = (gate_type == up_type and _is_silu(activation) and dtype in (torch.float32, torch.bfloat16)
+        self._layer_ok = (gate_type == up_type and dtype in (torch.float32, torch.bfloat16)
                           and all(w.is_contiguous() and w.data_ptr() % 16 == 0 and w.stride(0) % 16 == 0
                                   for w in (gate, up, down)))
         self._layer_bytes: dict[tuple[int, int], int] = {}
@@ -119,8 +119,8 @@ class HipPackedMoEExperts(nn.Module):
         int32, weights float32, the last two (n_tokens, top_k)). A token takes its top_k largest logits, ties to the
         lowest id, weighted by the softmax over all experts or (`norm_topk`) over the chosen ones, times `scale`. A
         logit of -inf masks its expert; a slot without an expert has id -1 and weight 0 and adds nothing, so that a
-        token of -inf alone (padding) gets a row of zeros, whatever x holds there. `forward` on those ids and weights
-        gives the same bits.
+        token of -inf alone (padding) gets a row of zeros, whatever x holds there. `forward` on those ids and weights,
+        where no id is -1, gives the same bits.
 
         Up to eight tokens (and 64 pairs) of Q4_K, Q6_K or Q8_0 experts, gate and up of one type, with a SiLU: one
         library call (`mxa_moe_layer`) of two launches, three where more than 16 pairs are added up. Otherwise the
@@ -167,7 +167,7 @@ class HipPackedMoEExperts(nn.Module):
                     ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor] | None:
         """`forward_logits` in one library call, or None where it does not take the layer."""
         n_tokens, dev = x.shape[0], x.device
-        if not 1 <= n_tokens <= _LAYER_MAX_TOKENS or not self._layer_ok:
+        if not 1 <= n_tokens <= _LAYER_MAX_TOKENS or not self._layer_ok or not _is_silu(self.activation):
             return None
         if _elsewhere(dev):
             with torch.cuda.device(dev):
@@ -194,9 +194,9 @@ class HipPackedMoEExperts(nn.Module):
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         status = lib.mxa_moe_layer(
             gt, dt, gate.data_ptr(), up.data_ptr(), gate.stride(0), down.data_ptr(), down.stride(0), self.num_experts,
-            xs.data_ptr(), bf16, logits.data_ptr(), logits.dtype is torch.bfloat16, top_k, bool(norm_topk), float(scale),
-            n_tokens, self.n_embd, self.ffn_len, reciprocal, ids.data_ptr(), weights.data_ptr(), out.data_ptr(), out_bf16,
-            ws.data_ptr(), ws_bytes, _stream(dev))
+            xs.data_ptr(), bf16, logits.data_ptr(), logits.dtype is torch.bfloat16, top_k, bool(norm_topk),
+            float(scale), n_tokens, self.n_embd, self.ffn_len, reciprocal, ids.data_ptr(), weights.data_ptr(),
+            out.data_ptr(), out_bf16, ws.data_ptr(), ws_bytes, _stream(dev))
         if status == -1:
             return None
         if status != 0:

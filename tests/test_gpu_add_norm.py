@@ -239,3 +239,32 @@ def test_refusals(gpu, ops) -> None:
         gpu.add_rms_norm_q8k(x, x, w, EPS, gate=w.bfloat16())
     hidden, out, _ = gpu.add_rms_norm_q8k(x[:0], x[:0], w, EPS)  # no rows: nothing to launch
     assert hidden.shape == out.shape == (0, 512)
+
+
+def test_the_most_rows(gpu, ops) -> None:
+    m = 1 << 24
+    g = torch.Generator(device="cuda").manual_seed(7)
+    x, r, w = rand(g, m, 1, dt=BF16), rand(g, m, 1, dt=BF16), 1 + rand(g, 1, dt=BF16)
+    check(ops.add_rms_norm(r, x, w, EPS), x, r, w, EPS)
+    more = torch.zeros(1, 1, device="cuda").expand(m + 1, 1)
+    assert ops.add_rms_norm(more, more, more[0], EPS) is None
+    with pytest.raises(ValueError, match="rows"):
+        gpu.add_rms_norm_q8k(more, more, more[0], EPS)
+
+
+def test_in_inference_mode(gpu, ops) -> None:
+    """Tensors without a version hand no blocks on: the projections behind quantize the values they are given."""
+    k = 512
+    owner = torch.nn.Module()
+    owner.p = DevicePackedLinear(torch.from_numpy(S.packed_weight(D.Q4_K, 256, k, seed=3)).cuda(), k, D.Q4_K)
+    g = torch.Generator(device="cuda").manual_seed(8)
+    x, r, w = rand(g, 4, k, dt=BF16), rand(g, 4, k, dt=BF16), 1 + rand(g, k, dt=BF16, scale=0.1)
+    want = ops.add_rms_norm(r, x, w, EPS)
+    y = project_shared(owner, ("p",), want[1])[0]
+    with torch.inference_mode():
+        got = ops.add_rms_norm(r, x, w, EPS)
+        assert HANDOFF.claim(got[1]) is None
+        assert torch.equal(project_shared(owner, ("p",), got[1])[0], y)
+        got[1].mul_(2)
+        twice = project_shared(owner, ("p",), got[1])[0]
+    assert torch.equal(got[0], want[0]) and torch.equal(twice, project_shared(owner, ("p",), 2 * want[1])[0])

@@ -356,3 +356,40 @@ def test_refusals(gpu) -> None:
                  (torch.zeros(1, 257, device="cuda"), 2), (torch.zeros(1, 40, device="cuda"), 17)):
         with pytest.raises(ValueError):
             gpu.moe_topk(b, k)
+
+
+def test_an_activation_set_later(gpu) -> None:
+    mod, _ = build_experts((D.Q4_K, D.Q4_K, D.Q6_K), 4, 512, 256, BF16, seed=16)
+    x = torch.from_numpy(S.activations(3, 512, seed=6)).cuda().bfloat16()
+    logits = router(3, 4, 9)
+    silu = mod.forward_logits(x, logits, 2)[0]
+    mod.activation = F.gelu
+    out, ids, wts = mod.forward_logits(x, logits, 2)
+    assert torch.equal(out, mod(x, wts, ids.long())) and not torch.equal(out, silu)
+    mod.activation = torch.nn.SiLU()
+    assert torch.equal(mod.forward_logits(x, logits, 2)[0], silu)
+
+
+def test_the_most_tokens(gpu) -> None:
+    n = 1 << 24
+    ids, wts = gpu.moe_topk(torch.zeros(n, 1, dtype=BF16, device="cuda"), 1, True, 0.5)
+    assert (ids == 0).all() and (wts == 0.5).all()
+    with pytest.raises(ValueError, match="tokens"):
+        gpu.moe_topk(torch.zeros(1, 2, device="cuda").expand(n + 1, 2), 1)
+    for bad in (torch.zeros((), device="cuda"), torch.zeros(4, device="cuda")):
+        with pytest.raises(ValueError, match="router logits"):
+            gpu.moe_topk(bad, 1)
+
+
+def test_many_tokens_half_of_them_padding(gpu) -> None:
+    """More tokens than one routing launch takes; a row of padding costs the others nothing."""
+    mod, _ = build_experts((D.Q8_0, D.Q8_0, D.Q8_0), 8, 256, 256, BF16, seed=17)
+    t = 32768 + 40
+    x = torch.from_numpy(S.activations(64, 256, seed=7)).cuda().bfloat16().repeat(t // 64 + 1, 1)[:t]
+    logits = router(64, 8, 10).repeat(t // 64 + 1, 1)[:t]
+    want, wids, _ = mod.forward_logits(x[:64], logits[:64], 2)
+    logits[1::2] = -INF
+    out, ids, _ = mod.forward_logits(x, logits, 2)
+    even = torch.arange(0, t, 2, device="cuda")
+    assert torch.equal(out[even], want[even % 64]) and torch.equal(ids[even], wids[even % 64])
+    assert (out[1::2] == 0).all() and (ids[1::2] == -1).all()

@@ -217,3 +217,25 @@ def test_refusals(gpu) -> None:
     q2, k2 = rot(q[:0], k[:0], pos[:0])  # no tokens
     assert q2.shape == (0, 4, 64) and k2.shape == (0, 2, 64)
     assert math.isclose(HipRotary(64, scaling=SCALINGS[3]).scale, 0.1 * math.log(16) + 1)
+
+
+def test_more_heads_than_workgroups_side_by_side(gpu) -> None:
+    g = torch.Generator(device="cuda").manual_seed(8)
+    rot = HipRotary(1022)
+    q, k, pos = rand(g, 2, 5000, 1022), rand(g, 2, 3, 1022), torch.tensor([7, 100000], device="cuda")
+    q2, k2 = rot(q, k, pos)
+    check(rot, q, q2, pos)
+    check(rot, k, k2, pos)
+
+
+def test_the_most_tokens(gpu) -> None:
+    n = 1 << 24
+    g = torch.Generator(device="cuda").manual_seed(9)
+    rot, q, pos = HipRotary(2), rand(g, n, 1, 2, dt=BF16), torch.arange(n, dtype=torch.int32, device="cuda")
+    got = rot(q, None, pos)[0]
+    for part in (slice(0, 500), slice(n // 2 - 7, n // 2 + 900), slice(n - 500, n)):
+        check(rot, q[part], got[part], pos[part])
+    assert got.isfinite().all()
+    more = torch.zeros(1, 1, 2, device="cuda").expand(n + 1, 1, 2)
+    with pytest.raises(ValueError, match="tokens"):
+        rot(more, None, torch.zeros(1, dtype=torch.int32, device="cuda").expand(n + 1))

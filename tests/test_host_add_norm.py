@@ -46,3 +46,12 @@ def test_broadcasts() -> None:
         assert not _broadcasts(torch.Size(shape), to), shape
         with pytest.raises(RuntimeError):
             torch.zeros(shape).expand(to) if shape != (1, 3, 5, 8) else torch.zeros(shape).expand(*to)
+
+
+def test_more_rows_than_a_grid_holds_are_refused() -> None:
+    from matricxon_amd import _lib
+
+    a = ctypes.c_void_p(0x10000)
+    for m in ((1 << 24) + 1, 2 ** 31 - 1):
+        assert _lib.load().mxa_add_rms_norm_q8_k(a, 1, a, 1, None, 1e-5, None, 0, 0, 1.0, a, 1e-5, m, 1, 1, 1, a, a, None,
+                                                 0, None) == -1

@@ -58,3 +58,9 @@ def test_argument_errors_return_status_without_launching() -> None:
 
     for bad in (dict(down=None), dict(ids=None), dict(w=None), dict(out=None), dict(t=0), dict(k=17), dict(n=0)):
         assert combine(**bad) == -1, bad
+
+
+def test_more_tokens_than_a_grid_holds_are_refused() -> None:
+    a = ctypes.c_void_p(0x10000)
+    for t in ((1 << 24) + 1, 2 ** 31 - 1):
+        assert load().mxa_moe_topk(a, 0, t, 8, 2, 1, 1.0, a, a, None) == -1

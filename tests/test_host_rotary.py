@@ -85,3 +85,11 @@ def test_argument_errors_return_status_without_launching() -> None:
                 dict(q_out=vp(0x10001)), dict(k_out=vp(0x10001)), dict(pos=vp(0x10004)), dict(pos64=0, pos=vp(0x10002)),
                 dict(turns=vp(0x10004))):
         assert call(**bad) == -1, bad
+
+
+def test_more_tokens_than_a_grid_holds_are_refused() -> None:
+    from matricxon_amd import _lib
+
+    a, st = ctypes.c_void_p(0x10000), (ctypes.c_longlong * 3)(0, 2, 2)
+    for n in ((1 << 24) + 1, 2 ** 31 - 1):
+        assert _lib.load().mxa_rope(a, st, 1, None, None, 0, a, 1, 0, 1, a, n, n, 2, 2, 0, 1.0, 1, a, None, None) == -1
