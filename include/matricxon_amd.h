@@ -250,6 +250,12 @@ int mxa_moe_route(const void *ids, int ids_int64, int n_tokens, int top_k, int n
                   int32_t *offsets, int32_t *pair_tok, int32_t *rows, int32_t *ids32,
                   void *stream);
 
+/* mxa_moe_route in which pairs of a negative id belong to no expert: they are placed behind all others, and
+ * offsets[n_experts] is the number of the others, so that a grouped launch leaves their rows alone. */
+int mxa_moe_route_masked(const void *ids, int ids_int64, int n_tokens, int top_k, int n_experts,
+                         int32_t *offsets, int32_t *pair_tok, int32_t *rows, int32_t *ids32,
+                         void *stream);
+
 /* Routing-weighted combine of MoE expert outputs, one launch: out (n_tokens, n_embd) fp32, row t =
  * the sum over token t's top_k slots k, in ascending expert id ids[t * top_k + k] (a DEVICE int32
  * array; equal ids in slot order), of down[r] * weights[t * top_k + k] with r = rows[t * top_k +

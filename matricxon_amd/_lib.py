@@ -30,6 +30,7 @@ EXPORTS = (
     "mxa_gemm_moe_pairs",
     "mxa_gemm_moe_pairs_bf16",
     "mxa_moe_route",
+    "mxa_moe_route_masked",
     "mxa_moe_combine",
     "mxa_moe_combine_masked",
     "mxa_moe_topk",
@@ -112,6 +113,8 @@ def load() -> ctypes.CDLL:
     lib.mxa_gemm_moe_pairs_bf16.restype = _i
     lib.mxa_moe_route.argtypes = [_vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]
     lib.mxa_moe_route.restype = _i
+    lib.mxa_moe_route_masked.argtypes = lib.mxa_moe_route.argtypes
+    lib.mxa_moe_route_masked.restype = _i
     lib.mxa_moe_combine.argtypes = [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp]
     lib.mxa_moe_combine.restype = _i
     lib.mxa_moe_combine_masked.argtypes = lib.mxa_moe_combine.argtypes

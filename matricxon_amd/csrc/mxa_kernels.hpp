@@ -253,7 +253,7 @@ constexpr int kMoeMaxTopK = 16;
 constexpr int kMoeRouteMaxExperts = 256;
 constexpr int kMoeRouteMaxPairs = 1 << 20;
 int launch_moe_route(const void* ids, bool ids64, int n_tokens, int top_k, int n_experts,
-                     int32_t* offsets, int32_t* pair_tok, int32_t* rows, int32_t* ids32,
+                     bool masked, int32_t* offsets, int32_t* pair_tok, int32_t* rows, int32_t* ids32,
                      hipStream_t stream);
 int launch_moe_combine(const float* down, const int32_t* rows, const int32_t* ids,
                        const float* weights, int n_tokens, int top_k, int n_embd, int bf16,

@@ -59,19 +59,25 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(
 // Bound: latency, of a step's ballots and counter and of the ids' loads (four steps requested at a time);
 // the runs need no barrier. Measured on MI355X, kernel alone, 4096 pairs of 64 experts: 7.8 us; a ballot
 // per distinct expert of a wave, in chunks of 1024 pairs between barriers, took 26.5.
+//
+// MASKED: pairs of a negative id belong to no expert and are placed behind all others, past offsets[n_experts], where
+// no projection reads or writes a row (4096 tokens of 64 experts top 8, 2048 x 1024, half of them padding: the layer
+// 691 us, with the padding clamped to expert 0 988; 589 for the other half alone).
 constexpr int kRouteWaves = 16;
+template <bool MASKED>
 __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(
     const void* __restrict__ ids, int ids64, int n_pairs, int top_k, int n_experts,
     int32_t* __restrict__ offsets, int32_t* __restrict__ pair_tok, int32_t* __restrict__ rows,
     int32_t* __restrict__ ids32) {
   __shared__ int cnt[kRouteWaves][kMoeRouteMaxExperts];
   __shared__ int part[kMoeRouteMaxExperts / 64];
+  __shared__ int none[kRouteWaves];  // a wave's pairs without an expert
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int bits = n_experts > 1 ? 32 - __builtin_clz(n_experts - 1) : 0;
   const int run = (n_pairs + 64 * kRouteWaves - 1) / (64 * kRouteWaves) * 64;
   const int begin = wave * run, end = min(begin + run, n_pairs);
   const uint64_t below = (1ull << lane) - 1ull;
-  // step(p, valid, v, e, m) for every 64 pairs of the run: m, the lanes of this lane's expert
+  // step(p, valid, live, v, e, m) for every 64 pairs of the run: m, the lanes of this lane's expert; live, it has one
   auto walk = [&](auto&& step) {
     for (int c0 = begin; c0 < end; c0 += 256) {
       long long v[4];
@@ -84,15 +90,15 @@ __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(
       for (int j = 0; j < 4; ++j) {
         if (c0 + 64 * j >= end) break;
         const int p = c0 + 64 * j + lane;
-        const bool valid = p < end;
+        const bool valid = p < end, live = valid && !(MASKED && v[j] < 0);
         const int e = v[j] < 0 ? 0 : v[j] >= n_experts ? n_experts - 1 : (int)v[j];
-        uint64_t m = __ballot(valid);
+        uint64_t m = __ballot(live);
         for (int b = 0; b < bits; ++b) {
           const bool one = (e >> b) & 1;
           const uint64_t ones = __ballot(one);
           m &= one ? ones : ~ones;
         }
-        step(p, valid, v[j], e, m);
+        step(p, valid, live, v[j], e, m);
         wave_sync();  // the next step reads the counters that this one wrote
       }
     }
@@ -100,11 +106,14 @@ __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(
 #pragma unroll
   for (int i = 0; i < kMoeRouteMaxExperts / 64; ++i) cnt[wave][64 * i + lane] = 0;
   wave_sync();
-  walk([&](int p, bool valid, long long v, int e, uint64_t m) {
+  int without = 0;
+  walk([&](int p, bool valid, bool live, long long v, int e, uint64_t m) {
+    if (MASKED) without += __popcll(__ballot(valid && !live));
     if (!valid) return;
-    if ((m & below) == 0) cnt[wave][e] += __popcll(m);
+    if (live && (m & below) == 0) cnt[wave][e] += __popcll(m);
     if (ids32 != nullptr) ids32[p] = (int32_t)v;  // torch's int64 -> int32 conversion
   });
+  if (MASKED && lane == 0) none[wave] = without;
   __syncthreads();
   // thread e: the waves' counts of expert e, prefixed; the experts' totals scanned over a wave, then waves
   int before[kRouteWaves], total = 0, incl = 0;
@@ -133,29 +142,46 @@ __global__ __launch_bounds__(64 * kRouteWaves) void moe_route_kernel(
 #pragma unroll
     for (int w = 0; w < kRouteWaves; ++w) cnt[w][tid] = before[w] + base;
   }
-  if (tid == 0) offsets[n_experts] = n_pairs;
+  int behind = n_pairs;  // the place of this wave's next pair without an expert
+  if (MASKED) {
+    int earlier = 0;
+    without = 0;
+    for (int w = 0; w < kRouteWaves; ++w) {
+      earlier += w < wave ? none[w] : 0;
+      without += none[w];
+    }
+    behind = n_pairs - without + earlier;
+  }
+  if (tid == 0) offsets[n_experts] = n_pairs - without;
   __syncthreads();
-  walk([&](int p, bool valid, long long, int e, uint64_t m) {
-    const int first = cnt[wave][e], place = first + __popcll(m & below);
+  walk([&](int p, bool valid, bool live, long long, int e, uint64_t m) {
+    const int first = cnt[wave][e];
+    int place = first + __popcll(m & below);
+    if (MASKED) {
+      const uint64_t d = __ballot(valid && !live);
+      if (!live) place = behind + __popcll(d & below);
+      behind += __popcll(d);
+    }
     if (valid) {
       rows[p] = place;
       pair_tok[place] = p / top_k;
     }
     wave_sync();  // every lane has read its counter
-    if (valid && (m & below) == 0) cnt[wave][e] = first + __popcll(m);
+    if (live && (m & below) == 0) cnt[wave][e] = first + __popcll(m);
   });
 }
 
 }  // namespace
 
 int launch_moe_route(const void* ids, bool ids64, int n_tokens, int top_k, int n_experts,
-                     int32_t* offsets, int32_t* pair_tok, int32_t* rows, int32_t* ids32,
+                     bool masked, int32_t* offsets, int32_t* pair_tok, int32_t* rows, int32_t* ids32,
                      hipStream_t stream) {
   if (ids == nullptr || offsets == nullptr || pair_tok == nullptr || rows == nullptr ||
       n_tokens < 1 || top_k < 1 || n_experts < 1 || n_experts > kMoeRouteMaxExperts ||
       (long long)n_tokens * top_k > kMoeRouteMaxPairs)
     return -1;
-  hipLaunchKernelGGL(moe_route_kernel, dim3(1), dim3(64 * kRouteWaves), 0, stream, ids,
+  auto kern = masked ? moe_route_kernel<true> : moe_route_kernel<false>;
+  hipLaunchKernelGGL(kern, dim3(1), dim3(64 * kRouteWaves), 0, stream, ids,
                      ids64 ? 1 : 0, n_tokens * top_k, top_k, n_experts, offsets, pair_tok, rows,
                      ids32);
   return 0;

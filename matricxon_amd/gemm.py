@@ -620,7 +620,7 @@ class HipGemm:
         """Grouped projection of packed MoE experts (`mxa_gemm_moe`), one launch for all of
         them: `experts` (n_experts, out_features, row_bytes) uint8 on the device; rows
         [offsets[e], offsets[e + 1]) of `x` (n_rows, in_features) go through expert e
-        (`offsets`: int32 on the device, n_experts + 1 ascending values from 0 to n_rows, so no
+        (`offsets`: int32 on the device, n_experts + 1 ascending values from 0, up to n_rows, so no
         host sync). x None: `workspace` already holds the Q8_K activations of the n_rows rows.
         Returns (n_rows, out_features) float32; each row equals `matmul` of that row alone bit
         for bit. `out_dtype` bfloat16 writes the result as bfloat16, each value the float32
@@ -724,7 +724,7 @@ class HipGemm:
     MOE_ROUTE_MAX_EXPERTS = 256
     MOE_ROUTE_MAX_PAIRS = 1 << 20
 
-    def moe_route(self, top_k_idx: torch.Tensor, num_experts: int
+    def moe_route(self, top_k_idx: torch.Tensor, num_experts: int, masked: bool = False
                   ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
         """The routing of MoE (token, slot) pairs in one launch (`mxa_moe_route`), no host sync:
         (offsets (num_experts + 1,), pair_tok (n_pairs,), rows (n_tokens, top_k), ids32 (n_tokens,
@@ -733,7 +733,9 @@ class HipGemm:
         [0, num_experts)), `rows[t, k]` is the place of pair (t, k) in that order, `offsets`
         delimits each expert's pairs and `ids32` is top_k_idx converted to int32. `top_k_idx`:
         (n_tokens, top_k) int32 or int64 on the device; num_experts <= MOE_ROUTE_MAX_EXPERTS and
-        n_tokens * top_k <= MOE_ROUTE_MAX_PAIRS (else ValueError)."""
+        n_tokens * top_k <= MOE_ROUTE_MAX_PAIRS (else ValueError). `masked`: pairs of a negative id
+        belong to no expert and come behind all others, past offsets[num_experts]
+        (`mxa_moe_route_masked`)."""
         _require_device_tensor("top_k_idx", top_k_idx)
         if top_k_idx.dim() != 2 or top_k_idx.dtype not in (torch.int32, torch.int64):
             raise ValueError("top_k_idx must be an int32 or int64 (n_tokens, top_k) tensor")
@@ -748,10 +750,11 @@ class HipGemm:
         pair_tok = torch.empty(n_tokens * top_k, dtype=torch.int32, device=device)
         rows = torch.empty((n_tokens, top_k), dtype=torch.int32, device=device)
         ids32 = torch.empty((n_tokens, top_k), dtype=torch.int32, device=device)
-        status = self._lib.mxa_moe_route(ids.data_ptr(), int(ids.dtype == torch.int64), n_tokens,
-                                         top_k, int(num_experts), offsets.data_ptr(),
-                                         pair_tok.data_ptr(), rows.data_ptr(), ids32.data_ptr(),
-                                         _stream(device))
+        route = self._lib.mxa_moe_route_masked if masked else self._lib.mxa_moe_route
+        status = route(ids.data_ptr(), int(ids.dtype == torch.int64), n_tokens,
+                       top_k, int(num_experts), offsets.data_ptr(),
+                       pair_tok.data_ptr(), rows.data_ptr(), ids32.data_ptr(),
+                       _stream(device))
         self._check(status, "mxa_moe_route", 0)
         return offsets, pair_tok, rows, ids32
 

@@ -215,7 +215,7 @@ class HipPackedMoEExperts(nn.Module):
                 top_k_idx.dtype in (torch.int32, torch.int64):
             # one launch: the sort, each pair's token and place, the ids as int32 for the combine
             order = None
-            offsets, pair_tok, rows, ids32 = g.moe_route(top_k_idx, self.num_experts)
+            offsets, pair_tok, rows, ids32 = g.moe_route(top_k_idx, self.num_experts, masked)
         else:
             order, offsets, pair_tok = route_pairs(top_k_idx, self.num_experts)
         # the reference casts x to the layer dtype before each matmul (device_packed.py:54)

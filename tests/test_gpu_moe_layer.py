@@ -393,3 +393,21 @@ def test_many_tokens_half_of_them_padding(gpu) -> None:
     even = torch.arange(0, t, 2, device="cuda")
     assert torch.equal(out[even], want[even % 64]) and torch.equal(ids[even], wids[even % 64])
     assert (out[1::2] == 0).all() and (ids[1::2] == -1).all()
+
+
+@pytest.mark.parametrize("t,e,k", [(1, 1, 1), (1, 8, 2), (7, 256, 16), (63, 3, 3), (300, 64, 8), (5000, 16, 4)])
+@pytest.mark.parametrize("share", [0.0, 0.3, 1.0])
+@pytest.mark.parametrize("dt", [torch.int32, torch.int64], ids=["int32", "int64"])
+def test_masked_routing(gpu, t, e, k, share, dt) -> None:
+    """Pairs in expert order, those without an expert behind them in their own order."""
+    g = torch.Generator().manual_seed(t + k)
+    ids = torch.randint(0, e, (t, k), generator=g)
+    ids[torch.rand(t, k, generator=g) < share] = -1
+    offsets, pair_tok, rows, ids32 = gpu.moe_route(ids.to(dt).cuda(), e, masked=True)
+    key = torch.where(ids < 0, e, ids).flatten()
+    order = torch.argsort(key, stable=True)
+    place = torch.empty_like(order)
+    place[order] = torch.arange(t * k)
+    assert torch.equal(offsets.cpu().long(), torch.tensor([int((key < i).sum()) for i in range(e + 1)]))
+    assert torch.equal(pair_tok.cpu().long(), order // k) and torch.equal(rows.cpu().long(), place.view(t, k))
+    assert torch.equal(ids32.cpu().long(), ids)

@@ -64,3 +64,14 @@ def test_more_tokens_than_a_grid_holds_are_refused() -> None:
     a = ctypes.c_void_p(0x10000)
     for t in ((1 << 24) + 1, 2 ** 31 - 1):
         assert load().mxa_moe_topk(a, 0, t, 8, 2, 1, 1.0, a, a, None) == -1
+
+
+def test_masked_routing_refuses_bad_arguments_without_launching() -> None:
+    lib, a = load(), ctypes.c_void_p(0x10000)
+
+    def call(ids=a, t=2, k=2, e=8, offsets=a, pair_tok=a, rows=a):
+        return lib.mxa_moe_route_masked(ids, 0, t, k, e, offsets, pair_tok, rows, None, None)
+
+    for bad in (dict(ids=None), dict(offsets=None), dict(pair_tok=None), dict(rows=None), dict(t=0), dict(k=0),
+                dict(e=0), dict(e=257), dict(t=1 << 18, k=5)):
+        assert call(**bad) == -1, bad
