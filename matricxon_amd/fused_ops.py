@@ -137,14 +137,15 @@ class HipFusedOps:
         more than 2^24 rows."""
         shape, dt, dev = x.shape, x.dtype, x.device
         k = shape[-1] if shape else 0
-        if (dev.type != "cuda" or (dt is not torch.bfloat16 and dt is not torch.float32) or residual.shape != shape
+        if (not x.is_cuda or (dt is not torch.bfloat16 and dt is not torch.float32) or residual.shape != shape
                 or (residual.dtype is not dt and residual.dtype is not torch.float32) or residual.device != dev
                 or not 1 <= k <= HipGemm.NORM_MAX_VALUES or not 0 < x.numel() <= k * HipGemm.MAX_TOKENS):
             return None
         for w in (weight,) if post_weight is None else (weight, post_weight):
             if w.dtype is not dt or w.shape != (k,) or w.device != dev:
                 return None
-        if gate is not None and (gate.dtype is not dt or gate.device != dev or not _broadcasts(gate.shape, shape)):
+        if gate is not None and (gate.dtype is not dt or gate.device != dev
+                                 or (gate.shape != (k,) and not _broadcasts(gate.shape, shape))):
             return None
         hidden, out, ws = self._gemm._add_rms_norm(residual, x, weight, eps, post_weight, post_eps, gate, scale, q8k)
         if ws is not None:

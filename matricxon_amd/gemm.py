@@ -36,10 +36,16 @@ def _stream(device: torch.device) -> int:
     return _RAW_STREAM(torch.cuda.current_device() if index is None else index)
 
 
+_CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_FLOATS = (torch.float32, torch.bfloat16)
+_INTS = (torch.int32, torch.int64)
+
+
 def _elsewhere(device: torch.device) -> bool:
     """Whether `device` is not the current one: a launch goes to the current device, whatever device its tensors and
     its stream belong to."""
-    return device.index is not None and device.index != torch._C._cuda_getDevice()
+    index = device.index
+    return index is not None and index != _CURRENT_DEVICE()
 
 
 def _al256(n: int) -> int:
@@ -90,12 +96,11 @@ _Strides3 = ctypes.c_longlong * 3
 
 
 def _head_strides(x: torch.Tensor, nd: int) -> tuple[torch.Tensor, ctypes.Array]:
-    """x (T, heads, dim) or (B, T, heads, dim) with adjacent values in a head (a copy where they are not), without its
-    history, and its strides of a sequence, a step and a head as the library takes them."""
-    x = x.detach()
+    """x (T, heads, dim) or (B, T, heads, dim) with adjacent values in a head (a copy where they are not), and its
+    strides of a sequence, a step and a head as the library takes them."""
     st = x.stride()
     if st[-1] != 1:
-        x = x.contiguous()
+        x = x.detach().contiguous()
         st = x.stride()
     return x, _Strides3(0, st[0], st[1]) if nd == 3 else _Strides3(st[0], st[1], st[2])
 
@@ -473,14 +478,20 @@ class HipGemm:
                       post_weight: torch.Tensor | None, post_eps: float | None, gate: torch.Tensor | None,
                       scale: float, want_q8k: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor | None]:
         """The library call of `add_rms_norm_q8k` on checked operands."""
-        dev = x.device
+        dev, k = x.device, x.shape[-1]
         if _elsewhere(dev):
             with torch.cuda.device(dev):
                 return self._add_rms_norm(residual, x, weight, eps, post_weight, post_eps, gate, scale, want_q8k)
-        k = x.shape[-1]
         m = x.numel() // k
-        x2, ldx = (x, k) if x.is_contiguous() else _rows_of(x, k)
-        r2, ldr = (residual, k) if residual.is_contiguous() else _rows_of(residual, k)
+        if x.is_contiguous():
+            x2, ldx, out = x, k, torch.empty_like(x)
+        else:
+            (x2, ldx), out = _rows_of(x, k), torch.empty_like(x, memory_format=torch.contiguous_format)
+        if residual.is_contiguous():
+            r2, ldr, hidden = residual, k, torch.empty_like(residual)
+        else:
+            r2, ldr = _rows_of(residual, k)
+            hidden = torch.empty_like(residual, memory_format=torch.contiguous_format)
         if not weight.is_contiguous():
             weight = weight.contiguous()
         post = 0
@@ -489,12 +500,17 @@ class HipGemm:
             post = post_weight.data_ptr()
         gate_ptr, ldg, gstep = 0, 0, 0
         if gate is not None:
-            gate = gate.expand(x.shape).reshape(-1, k)  # RuntimeError where it does not broadcast
-            if gate.stride(1) > 1 and k > 1:
-                gate = gate.contiguous()
-            gate_ptr, ldg, gstep = gate.data_ptr(), gate.stride(0), min(gate.stride(1), 1) if k > 1 else 0
-        out = torch.empty_like(x, memory_format=torch.contiguous_format)
-        hidden = torch.empty_like(residual, memory_format=torch.contiguous_format)
+            gs = gate.shape
+            if len(gs) == 1 and gs[0] == k and gate.is_contiguous():
+                gstep = 1
+            elif gs == x.shape and gate.is_contiguous():
+                ldg, gstep = k, 1
+            else:
+                gate = gate.expand(x.shape).reshape(-1, k)  # RuntimeError where it does not broadcast
+                if gate.stride(1) > 1 and k > 1:
+                    gate = gate.contiguous()
+                ldg, gstep = gate.stride(0), min(gate.stride(1), 1) if k > 1 else 0
+            gate_ptr = gate.data_ptr()
         ws, ws_ptr, ws_bytes = None, 0, 0
         if want_q8k and k % 256 == 0:
             ws_bytes = q8k_bytes(m, k)
@@ -518,46 +534,58 @@ class HipGemm:
         """Rotary positions of q and k in one launch (`mxa_rope`), `turns` (rotary_dim / 2) float64 on their device;
         `matricxon_amd.rotary.HipRotary` is the face of it."""
         _require_device_tensor("q", q)
-        dev, dt, nd, dim = q.device, q.dtype, q.dim(), q.shape[-1] if q.dim() else 0
-        if dt not in (torch.float32, torch.bfloat16) or nd not in (3, 4):
+        if turns.dtype != torch.float64 or turns.shape != (rotary_dim // 2,) or turns.device != q.device or \
+                not turns.is_contiguous():
+            raise ValueError(f"turns must be ({rotary_dim // 2},) float64, contiguous, on {q.device}")
+        return self._rope(q, k, positions, turns, rotary_dim, interleaved, scale)
+
+    def _rope(self, q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, turns: torch.Tensor,
+              rotary_dim: int, interleaved: bool, scale: float) -> tuple[torch.Tensor, torch.Tensor | None]:
+        """`rope` with a table of q's device."""
+        dev, dt, shape = q.device, q.dtype, q.shape
+        nd = len(shape)
+        if dt not in _FLOATS or nd not in (3, 4):
             raise ValueError(f"q must be float32 or bfloat16 (T, heads, head_dim) or (B, T, heads, head_dim), got {dt} "
-                             f"{tuple(q.shape)}")
-        if dim % 2 or not rotary_dim <= dim <= self.ROPE_MAX_DIM or not 1 <= q.shape[-2] <= self.ROPE_MAX_HEADS:
+                             f"{tuple(shape)}")
+        seq, heads, dim = shape[-3:]
+        if dim % 2 or not rotary_dim <= dim <= self.ROPE_MAX_DIM or not 1 <= heads <= self.ROPE_MAX_HEADS:
             raise ValueError(f"head_dim must be even, {rotary_dim}..{self.ROPE_MAX_DIM}, and 1..{self.ROPE_MAX_HEADS} "
-                             f"heads, got {tuple(q.shape)}")
-        if k is not None and (k.dtype != dt or k.device != dev or k.dim() != nd or k.shape[-1] != dim
-                              or k.shape[:-2] != q.shape[:-2] or not 1 <= k.shape[-2] <= self.ROPE_MAX_HEADS):
-            raise ValueError(f"k must be {dt} on {dev} and have q's shape but for the heads, got {k.dtype} "
-                             f"{tuple(k.shape)} on {k.device} for q {tuple(q.shape)}")
-        if turns.dtype != torch.float64 or turns.shape != (rotary_dim // 2,) or turns.device != dev:
-            raise ValueError(f"turns must be ({rotary_dim // 2},) float64 on {dev}")
-        if positions.dtype not in (torch.int32, torch.int64) or positions.device != dev:
+                             f"heads, got {tuple(shape)}")
+        k_heads = 0
+        if k is not None:
+            ks = k.shape
+            k_heads = ks[-2] if len(ks) == nd else 0
+            if (k.dtype is not dt or k.device != dev or not 1 <= k_heads <= self.ROPE_MAX_HEADS or ks[-1] != dim
+                    or ks[0] != shape[0] or ks[-3] != seq):
+                raise ValueError(f"k must be {dt} on {dev} and have q's shape but for the heads, got {k.dtype} "
+                                 f"{tuple(ks)} on {k.device} for q {tuple(shape)}")
+        if positions.dtype not in _INTS or positions.device != dev:
             raise ValueError(f"positions must be int32 or int64 on {dev}, got {positions.dtype} on {positions.device}")
-        lead = q.shape[:-2]
-        if positions.dim() == 0 or positions.shape[-1] != lead[-1] or (
-                positions.dim() != 1 and (positions.dim() != nd - 2 or positions.shape[0] not in (1, lead[0]))):
-            raise ValueError(f"positions must be {tuple(lead)} or {tuple(lead[-1:])}, got {tuple(positions.shape)}")
+        ps, pst = positions.shape, positions.stride()
+        if len(ps) == 1 and ps[0] == seq:
+            pos_batch = 0
+        elif len(ps) == 2 and nd == 4 and ps[1] == seq and ps[0] in (1, shape[0]):
+            pos_batch = 0 if ps[0] == 1 else pst[0]
+        else:
+            raise ValueError(f"positions must be {tuple(shape[:-2])} or {(seq,)}, got {tuple(ps)}")
+        n_tokens = seq if nd == 3 else shape[0] * seq
+        if n_tokens > self.MAX_TOKENS:
+            raise ValueError(f"q must have up to {self.MAX_TOKENS} tokens, got {tuple(shape)}")
         if _elsewhere(dev):
             with torch.cuda.device(dev):
-                return self.rope(q, k, positions, turns, rotary_dim, interleaved, scale)
-        seq = lead[-1]
-        n_tokens = seq if nd == 3 else lead[0] * seq
-        if n_tokens > self.MAX_TOKENS:
-            raise ValueError(f"q must have up to {self.MAX_TOKENS} tokens, got {tuple(q.shape)}")
-        ps = positions.stride()
-        pos_batch = 0 if len(ps) == 1 or positions.shape[0] == 1 else ps[0]
+                return self._rope(q, k, positions, turns, rotary_dim, interleaved, scale)
         q, q_strides = _head_strides(q, nd)
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        k_heads, k_ptr, k_strides, k_out, k_out_ptr = 0, 0, None, None, 0
+        k_ptr, k_strides, k_out, k_out_ptr = 0, None, None, 0
         if k is not None:
             k, k_strides = _head_strides(k, nd)
             k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
-            k_heads, k_ptr, k_out_ptr = k.shape[-2], k.data_ptr(), k_out.data_ptr()
+            k_ptr, k_out_ptr = k.data_ptr(), k_out.data_ptr()
         if n_tokens == 0:
             return q_out, k_out
         status = self._lib.mxa_rope(
-            q.data_ptr(), q_strides, q.shape[-2], k_ptr, k_strides, k_heads, positions.data_ptr(),
-            positions.dtype is torch.int64, pos_batch, ps[-1], turns.data_ptr(), n_tokens, seq, dim, rotary_dim,
+            q.data_ptr(), q_strides, heads, k_ptr, k_strides, k_heads, positions.data_ptr(),
+            positions.dtype is torch.int64, pos_batch, pst[-1], turns.data_ptr(), n_tokens, seq, dim, rotary_dim,
             interleaved, scale, dt is torch.bfloat16, q_out.data_ptr(), k_out_ptr, _stream(dev))
         if status != 0:
             self._check(status, "mxa_rope", 0)

@@ -113,6 +113,8 @@ class HipRotary:
         """Turns per position of each pair, on `device` (laid out at the first use of a device)."""
         table = self._turns.get(device)
         if table is None:
+            if device.type != "cuda":
+                raise ValueError(f"q and k must be tensors on a HIP device, got {device}")
             table = self._turns[device] = (self.frequencies / (2 * math.pi)).to(device)
         return table
 
@@ -122,11 +124,9 @@ class HipRotary:
         any strides with adjacent values in a head, as the columns of a q | k | v buffer; positions int32 or int64
         (T,), or (B, T) for a batch. Returns new contiguous tensors of those shapes and that dtype, float32 or
         bfloat16. Any position, negative ones turning back."""
-        return self._gemm.rope(q, k, positions, self._table(q.device) if q.device.type == "cuda" else None,
-                               self.rotary_dim, self.interleaved, self.scale)
+        return self._gemm._rope(q, k, positions, self._table(q.device), self.rotary_dim, self.interleaved, self.scale)
 
     def shift(self, k: torch.Tensor, delta: torch.Tensor) -> torch.Tensor:
         """Keys that were turned for their positions, turned on by `delta` positions (a tensor as `positions`;
         negative: back), as a cache needs whose start moves. The scaling's factor on the values is already in them."""
-        return self._gemm.rope(k, None, delta, self._table(k.device) if k.device.type == "cuda" else None,
-                               self.rotary_dim, self.interleaved, 1.0)[0]
+        return self._gemm._rope(k, None, delta, self._table(k.device), self.rotary_dim, self.interleaved, 1.0)[0]
