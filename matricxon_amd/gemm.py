@@ -500,11 +500,13 @@ class HipGemm:
             post = post_weight.data_ptr()
         gate_ptr, ldg, gstep = 0, 0, 0
         if gate is not None:
-            gs = gate.shape
-            if len(gs) == 1 and gs[0] == k and gate.is_contiguous():
+            gs, plain = gate.shape, gate.is_contiguous()
+            if plain and len(gs) == 1 and gs[0] == k:
                 gstep = 1
-            elif gs == x.shape and gate.is_contiguous():
+            elif plain and gs == x.shape:
                 ldg, gstep = k, 1
+            elif plain and len(gs) == x.dim() and gs[-1] == 1 and gs[:-1] == x.shape[:-1]:
+                ldg = 1
             else:
                 gate = gate.expand(x.shape).reshape(-1, k)  # RuntimeError where it does not broadcast
                 if gate.stride(1) > 1 and k > 1:
