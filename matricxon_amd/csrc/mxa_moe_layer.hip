@@ -22,15 +22,16 @@
 //
 // What bounds it, MI355X, kernel alone with weights that no cache holds: 8 experts top 2 of 4096 x 14336 (Q4_K, Q6_K
 // down), one token, gate and up 28 us for 132 MB (4.7 TB/s; a read of as many bytes 21), of which 3 us before the
-// first copy and 3 after the last; down 28.5 us for 96 MB (3.4 TB/s), the LDS holding 11 rows of 56 blocks, which
-// wait and compute in turn. Eight tokens: 95 and 86 us, 5.0 and 4.0 TB/s: each further pair of an expert takes LDS from
-// the rows and adds to the part of a wave's turn in which its stage is not in flight. 64 experts top 8 of 2048 x
-// 1024, one token: 11.7 and 11.5 us, latency from end to end (logits, routing, activations, weights, block arithmetic).
+// first copy and 3 after the last; down 26 us for 96 MB (3.7 TB/s): 3 us before the first copy, 9 before the two
+// activation rows are blocks, then the LDS holds 10 rows of 56 blocks, which wait and compute in turn. Eight tokens: 95
+// and 86 us, 5.0 and 4.0 TB/s: each further pair of an expert takes LDS from the rows and adds to the part of a wave's
+// turn in which its stage is not in flight. 64 experts top 8 of 2048 x 1024, one token: 12 and 9 us, latency from end
+// to end (logits, routing, activations, weights, block arithmetic).
 //
 // The sum needs every pair's rows in one place. Up to 16 pairs the second launch's workgroups take rows, each through
 // all items, and add up in LDS. For more they take items, and the combine is a launch of its own (4 to 5 us): adding up
 // by the last workgroup to finish a range of rows was slower, the fences that such a hand-over needs between XCDs cost
-// the weights' stream more (down 62.8 against 29.3 + 4.4 us, one token of 8 experts top 2, 4096 x 14336).
+// the weights' stream more (down 62.8 against then 29.3 + 4.4 us, one token of 8 experts top 2, 4096 x 14336).
 #include "mxa_kernels.hpp"
 #include "mxa_lpb.hpp"
 
@@ -561,12 +562,25 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_down_sum_kernel(LayerArg
   int16_t* const abs_ = (int16_t*)(acts + pairs * nb * kActStride);
   float* const ad = (float*)(acts + pairs * nb * (kActStride + 32));
   float* const down = (float*)(acts + layer_act_bytes(pairs, nb));  // (pairs, rows)
-  const int r0 = (int)blockIdx.x * rows, nr = min(rows, a.n - r0);
+  const int r0 = (int)blockIdx.x * rows, nr = min(rows, a.n - r0), fold = layer_fold_row(nb);
   if (nr <= 0) return;
 
   int e_lane = -1;
   float w_lane = 0.0f;
   if (lane < pairs) e_lane = a.ids[lane], w_lane = a.wts[lane];
+  // Every pair's row is requested before the pairs' experts are known, also a row of no expert, which nothing has
+  // written and nothing reads.
+  constexpr int kBufs = kLayerBufs;
+  const int step = 4 * (waves - W), p16 = lane & 15, g0 = 4 * (wave - W) + (lane >> 4), total = pairs * nb;
+  uint4 raw[kBufs][4] = {};
+  const auto block = [&](int i) __attribute__((always_inline)) {
+    const int g = g0 + step * i, p = g / nb;
+    return ActPart{g < total, (long long)p * a.k + (g - p * nb) * QK + 16 * p16, aq + (size_t)g * kActStride,
+                   abs_ + 16 * g, ad + p * fold + g - p * nb};
+  };
+  if (wave >= W) fetch_acts(a, 0, block, raw);
+  __builtin_amdgcn_sched_barrier(0);  // not sunk below the barrier
+  __builtin_amdgcn_s_barrier();       // the activations are requested
   uint64_t same, leaders;
   const int bits = a.n_experts > 1 ? 32 - __builtin_clz(a.n_experts - 1) : 0;
   const int items = count_items<MAXM>(e_lane, bits, same, leaders);
@@ -574,7 +588,7 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_down_sum_kernel(LayerArg
   const int blocks = R * nb, stage = layer_stage_bytes<TYPE>(blocks);
   uint8_t* const region =
       acts + layer_sum_bytes(pairs, nb, rows) - kSumFixed + (size_t)wave * layer_region_bytes<TYPE, false>(MAXM, R, nb);
-  const int fold = layer_fold_row(nb), fold_set = R * fold;
+  const int fold_set = R * fold;
   float* const Vbuf = (float*)(region + stage);  // [activation row][row][fold]
   float* const Dbuf = Vbuf + MAXM * fold_set;
   const auto lead_of = [&](int task) __attribute__((always_inline)) {
@@ -591,34 +605,23 @@ __global__ __launch_bounds__(64 * kLayerWaves) void moe_down_sum_kernel(LayerArg
 
   int task = wave;
   if (wave < W) {
-    __builtin_amdgcn_s_barrier();  // the activations are requested
     wait_vmcnt(0);  // as in moe_layer_kernel
     issue(task);
   } else {
-    // every pair's row, those without an expert (which nothing has written) left out
-    constexpr int kBufs = kLayerBufs;
-    const int step = 4 * (waves - W), p16 = lane & 15, g0 = 4 * (wave - W) + (lane >> 4), total = pairs * nb;
-    uint4 raw[kBufs][4] = {};
-    const auto block = [&](int i) __attribute__((always_inline)) {
-      const int g = g0 + step * i, p = min(g / nb, pairs - 1);
-      const int e = __shfl(e_lane, p);  // every lane: a lane reads what another one holds
-      return ActPart{g < total && e >= 0, (long long)p * a.k + (g - p * nb) * QK + 16 * p16,
-                     aq + (size_t)g * kActStride, abs_ + 16 * g, ad + p * fold + g - p * nb};
-    };
-    fetch_acts(a, 0, block, raw);
-    __builtin_amdgcn_sched_barrier(0);  // not sunk below the barrier
-    __builtin_amdgcn_s_barrier();
-    if (wave == W && lane < pairs) {  // the sum's order
+    if (wave == W) {  // the sum's order
       const int t = lane / a.top_k;
       int rank = 0, n = 0;
-      for (int i = t * a.top_k; i < (t + 1) * a.top_k; ++i) {
-        const int o = a.ids[i];
-        rank += o >= 0 && (o < e_lane || (o == e_lane && i < lane));
-        n += o >= 0;
+      for (int i = 0; i < pairs; ++i) {
+        const int o = __builtin_amdgcn_readlane(e_lane, i);
+        const bool counts = i / a.top_k == t && o >= 0;
+        rank += counts && (o < e_lane || (o == e_lane && i < lane));
+        n += counts;
       }
-      if (e_lane >= 0) place[t * a.top_k + rank] = lane;
-      live[t] = n;
-      swt[lane] = w_lane;
+      if (lane < pairs) {
+        if (e_lane >= 0) place[t * a.top_k + rank] = lane;
+        live[t] = n;
+        swt[lane] = w_lane;
+      }
     }
     const int per = a.xbf16 ? 2 * kBufs : kBufs;
     for (int i = 0;;) {
@@ -714,11 +717,12 @@ int layer_rows(int nb) {
 }
 
 // The shape of the second launch that adds up: `rows` output rows a workgroup, at least kSumWaves waves of them, and up
-// to kSumPairs pairs, all of whose activations a workgroup quantizes. Both launches from start to end, adding up and
-// with the combine's launch: one token of 8 experts top 2 (4096 x 14336) 56.3 and 58.0 us, of 64 top 8 (2048 x 1024)
-// 25.0 and 27.4, of 5 top 1 (4096 x 4096) 22.7 and 26.3; 12 pairs (16 top 4, 2048 x 1536) 30.8 both; 16 pairs (128 top
-// 8, 2048 x 768) 28.3 and 29.2; 24 pairs (40 top 8, 1536 x 512) 28.2 and 27.6, (32 top 3, 2560 x 768) 44.3 and 43.2;
-// 32 and 64 pairs of 64 top 8 45.8 and 42.8, 65.3 and 53.1.
+// to kSumPairs pairs, all of whose activations a workgroup quantizes. The second launch adding up, and by items with
+// the combine's launch: one token of 8 experts top 2 (4096 x 14336) 26 us and 25.8 + 4.6, of 64 top 8 (2048 x 1024)
+// 9.0 and 9.2 + 5.0, of 5 top 1 (4096 x 4096) 7.7 and 9.0 + 3; 12 pairs (16 top 4, 2048 x 1536) 10.9 and 9.4 + 3.9;
+// 16 pairs (128 top 8, 2048 x 768) 11.2 and 9.0 + 5.0; 24 pairs (40 top 8, 1536 x 512) 13.7 and 8.0 + 5.4, (32 top 3,
+// 2560 x 768) 18.4 and 12.8 + 4.0; 32 and 64 pairs of 64 top 8 24.0 and 15.8 + 4.7, 40.6 and 20.9 + 4.8. With six waves
+// (two tokens of 8 top 2, 4096 x 14336) 46.2 and 36.9 + 4.6.
 constexpr int kSumWaves = 8, kSumPairs = 16;
 template <int TYPE, int MAXM>
 bool layer_sum_shape(int nb, int pairs, int rows, int& R, int& W, int& lds) {
@@ -726,8 +730,10 @@ bool layer_sum_shape(int nb, int pairs, int rows, int& R, int& W, int& lds) {
   const int region = layer_region_bytes<TYPE, false>(MAXM, R, nb);
   const int fixed = layer_sum_bytes(pairs, nb, rows);
   W = min(kLayerWaves - kLayerStagers, (kLayerLds - fixed) / region);
+  if (pairs > kSumPairs || fixed >= kLayerLds || W < kSumWaves) return false;
+  W = min(W, pairs * ((rows + R - 1) / R));  // the others quantize
   lds = fixed + W * region;
-  return pairs <= kSumPairs && fixed < kLayerLds && W >= kSumWaves;
+  return true;
 }
 
 // Pairs of an item: one for one token, four for more. With two, experts of three and four pairs are read twice: eight

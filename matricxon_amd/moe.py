@@ -136,9 +136,9 @@ class HipPackedMoEExperts(nn.Module):
         reciprocal = q8k_scale == "reciprocal"
         g = self._gemm
         n_tokens = x.shape[0] if x.dim() == 2 else -1
-        if n_tokens < 0 or x.shape[1] != self.n_embd or x.device != self.gate_packed.device:
-            raise ValueError(f"x must be (n_tokens, {self.n_embd}) on {self.gate_packed.device}, got {tuple(x.shape)} "
-                             f"on {x.device}")
+        dev = self._buffers["gate_packed"].device
+        if n_tokens < 0 or x.shape[1] != self.n_embd or x.device != dev:
+            raise ValueError(f"x must be (n_tokens, {self.n_embd}) on {dev}, got {tuple(x.shape)} on {x.device}")
         g._check_router(logits, n_tokens, self.num_experts, top_k)
         if logits.device != x.device or self.dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"router logits on {x.device} and a float32 or bfloat16 layer, got {logits.device} and "
@@ -185,7 +185,8 @@ class HipPackedMoEExperts(nn.Module):
             xs = xs.clone(memory_format=torch.contiguous_format)
         if not logits.is_contiguous():
             logits = logits.contiguous()
-        gate, up, down = self.gate_packed, self.up_packed, self.down_packed
+        held = self._buffers  # as attributes they take a third of a microsecond each
+        gate, up, down = held["gate_packed"], held["up_packed"], held["down_packed"]
         out_bf16 = x.dtype is torch.bfloat16
         out = torch.empty_like(x, dtype=torch.bfloat16 if out_bf16 else torch.float32,
                                memory_format=torch.contiguous_format)
