@@ -249,7 +249,8 @@ int launch_moe_lpb(int type, const uint8_t* w, long long row_bytes, long long ex
 // rounded to bfloat16 first; masked != 0: slots of a negative id are left out. top_k <= kMoeMaxTopK; -1 otherwise.
 constexpr int kMoeMaxTopK = 16;
 // MoE routing (one workgroup, stable counting sort): up to kMoeRouteMaxExperts experts and
-// kMoeRouteMaxPairs (token, slot) pairs; -1 otherwise.
+// kMoeRouteMaxPairs (token, slot) pairs; -1 otherwise. masked: pairs of a negative id belong to no expert and come
+// behind all others.
 constexpr int kMoeRouteMaxExperts = 256;
 constexpr int kMoeRouteMaxPairs = 1 << 20;
 int launch_moe_route(const void* ids, bool ids64, int n_tokens, int top_k, int n_experts,
@@ -264,7 +265,7 @@ int launch_moe_combine(const float* down, const int32_t* rows, const int32_t* id
 int launch_moe_topk(const void* logits, bool bf16, int n_tokens, int n_experts, int top_k, bool norm_topk, float scale,
                     int32_t* ids, float* wts, hipStream_t stream);
 // A whole layer of packed experts for up to kMoeLayerMaxTokens tokens (mxa_moe_layer.hip), from router logits to the
-// weighted sum, in two launches; ws of moe_layer_workspace bytes. -1 where it does not apply.
+// weighted sum, in two launches (three past 16 pairs); ws of moe_layer_workspace bytes. -1 where it does not apply.
 constexpr int kMoeLayerMaxTokens = 8;
 bool moe_layer_supported(int gate_type, int down_type, int n_experts, int top_k, int n_tokens, int n_embd, int ffn);
 size_t moe_layer_workspace(int n_tokens, int top_k, int n_embd, int ffn, bool bf16);
