@@ -29,7 +29,7 @@
 // to end (logits, routing, activations, weights, block arithmetic).
 //
 // The sum needs every pair's rows in one place. Up to 16 pairs the second launch's workgroups take rows, each through
-// all items, and add up in LDS. For more they take items, and the combine is a launch of its own (4 to 5 us): adding up
+// all items, and add up in LDS. For more they take items, and the combine is a launch of its own (3 to 4 us): adding up
 // by the last workgroup to finish a range of rows was slower, the fences that such a hand-over needs between XCDs cost
 // the weights' stream more (down 62.8 against then 29.3 + 4.4 us, one token of 8 experts top 2, 4096 x 14336).
 #include "mxa_kernels.hpp"
@@ -718,11 +718,11 @@ int layer_rows(int nb) {
 
 // The shape of the second launch that adds up: `rows` output rows a workgroup, at least kSumWaves waves of them, and up
 // to kSumPairs pairs, all of whose activations a workgroup quantizes. The second launch adding up, and by items with
-// the combine's launch: one token of 8 experts top 2 (4096 x 14336) 26 us and 25.8 + 4.6, of 64 top 8 (2048 x 1024)
-// 9.0 and 9.2 + 5.0, of 5 top 1 (4096 x 4096) 7.7 and 9.0 + 3; 12 pairs (16 top 4, 2048 x 1536) 10.9 and 9.4 + 3.9;
-// 16 pairs (128 top 8, 2048 x 768) 11.2 and 9.0 + 5.0; 24 pairs (40 top 8, 1536 x 512) 13.7 and 8.0 + 5.4, (32 top 3,
-// 2560 x 768) 18.4 and 12.8 + 4.0; 32 and 64 pairs of 64 top 8 24.0 and 15.8 + 4.7, 40.6 and 20.9 + 4.8. With six waves
-// (two tokens of 8 top 2, 4096 x 14336) 46.2 and 36.9 + 4.6.
+// the combine's launch: one token of 8 experts top 2 (4096 x 14336) 26 us and 25.7 + 4.4, of 64 top 8 (2048 x 1024)
+// 9.0 and 9.0 + 3.5, of 5 top 1 (4096 x 4096) 7.6 and 8.2 + 2.5; 12 pairs (16 top 4, 2048 x 1536) 11.2 and 10.4 + 3.8;
+// 16 pairs (128 top 8, 2048 x 768) 11.3 and 9.3 + 3.8; 24 pairs (40 top 8, 1536 x 512) 13.3 and 7.4 + 3.5, (32 top 3,
+// 2560 x 768) 18.7 and 12.8 + 3.9; 32 and 64 pairs of 64 top 8 24.0 and 15.6 + 3.8, 40.4 and 21.1 + 3.9. With six waves
+// (two tokens of 8 top 2, 4096 x 14336) 45.5 and 35.8 + 4.5.
 constexpr int kSumWaves = 8, kSumPairs = 16;
 template <int TYPE, int MAXM>
 bool layer_sum_shape(int nb, int pairs, int rows, int& R, int& W, int& lds) {
