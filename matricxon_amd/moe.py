@@ -94,9 +94,13 @@ class HipPackedMoEExperts(nn.Module):
                           self._gemm.row_bytes(int(t), k) % 16 == 0
                           for t, k in ((gate_type, n_embd), (up_type, n_embd), (down_type, ffn_len)))
         # what mxa_moe_layer takes besides its sizes; its workspace by (tokens, top_k), 0 where it declines
+        shapes = [(self.num_experts, n, self._gemm.row_bytes(int(t), k))
+                  for n, t, k in ((ffn_len, gate_type, n_embd), (ffn_len, up_type, n_embd),
+                                  (n_embd, down_type, ffn_len))]
         self._layer_ok = (gate_type == up_type and dtype in (torch.float32, torch.bfloat16)
-                          and all(w.is_contiguous() and w.data_ptr() % 16 == 0 and w.stride(0) % 16 == 0
-                                  for w in (gate, up, down)))
+                          and all(tuple(w.shape) == shape and w.dtype == torch.uint8 and w.device == gate.device
+                                  and w.is_contiguous() and w.data_ptr() % 16 == 0 and w.stride(0) % 16 == 0
+                                  for w, shape in zip((gate, up, down), shapes)))
         self._layer_bytes: dict[tuple[int, int], int] = {}
         self.register_buffer("gate_packed", gate, persistent=False)
         self.register_buffer("up_packed", up, persistent=False)
@@ -137,8 +141,9 @@ class HipPackedMoEExperts(nn.Module):
         g = self._gemm
         n_tokens = x.shape[0] if x.dim() == 2 else -1
         dev = self._buffers["gate_packed"].device
-        if n_tokens < 0 or x.shape[1] != self.n_embd or x.device != dev:
-            raise ValueError(f"x must be (n_tokens, {self.n_embd}) on {dev}, got {tuple(x.shape)} on {x.device}")
+        if n_tokens < 0 or x.shape[1] != self.n_embd or x.device != dev or not x.is_cuda:
+            raise ValueError(f"x must be (n_tokens, {self.n_embd}) on the HIP device of the experts, {dev}, got "
+                             f"{tuple(x.shape)} on {x.device}")
         g._check_router(logits, n_tokens, self.num_experts, top_k)
         if logits.device != x.device or self.dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"router logits on {x.device} and a float32 or bfloat16 layer, got {logits.device} and "

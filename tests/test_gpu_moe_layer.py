@@ -411,3 +411,16 @@ def test_masked_routing(gpu, t, e, k, share, dt) -> None:
     assert torch.equal(offsets.cpu().long(), torch.tensor([int((key < i).sum()) for i in range(e + 1)]))
     assert torch.equal(pair_tok.cpu().long(), order // k) and torch.equal(rows.cpu().long(), place.view(t, k))
     assert torch.equal(ids32.cpu().long(), ids)
+
+
+@pytest.mark.parametrize("e,k,t", [(1, 1, 1), (1, 1, 3), (1, 1, 8), (2, 2, 8), (256, 16, 4), (200, 9, 7), (64, 16, 1)])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_one_expert_to_the_most(gpu, e, k, t, dtype) -> None:
+    """Every token's pairs in one item after another, and every pair an item of its own."""
+    mod, _ = build_experts((D.Q8_0, D.Q8_0, D.Q4_K), e, 256, 512, dtype, seed=18)
+    x = torch.from_numpy(S.activations(t, 256, seed=8)).cuda().to(dtype)
+    logits = router(t, e, 11)
+    out, ids, wts = mod.forward_logits(x, logits, k)
+    assert mod._layer_bytes[t, k] > 0
+    check_routing(logits, k, True, 1.0, ids, wts)
+    assert torch.equal(out, mod._grouped(x, wts, ids))

@@ -75,3 +75,36 @@ def test_masked_routing_refuses_bad_arguments_without_launching() -> None:
     for bad in (dict(ids=None), dict(offsets=None), dict(pair_tok=None), dict(rows=None), dict(t=0), dict(k=0),
                 dict(e=0), dict(e=257), dict(t=1 << 18, k=5)):
         assert call(**bad) == -1, bad
+
+
+def test_experts_moved_to_the_host_are_refused() -> None:
+    """What `module.cpu()` leaves: a layer whose host addresses may not reach a kernel."""
+    import pytest
+    import torch
+
+    from matricxon_amd.moe import HipPackedMoEExperts
+
+    mod = HipPackedMoEExperts.__new__(HipPackedMoEExperts)
+    torch.nn.Module.__init__(mod)
+    for name in ("gate_packed", "up_packed", "down_packed"):
+        mod.register_buffer(name, torch.zeros(4, 256, 144, dtype=torch.uint8))
+    mod.n_embd, mod.num_experts, mod.dtype, mod._gemm = 256, 4, torch.float32, None
+    with pytest.raises(ValueError, match="HIP device"):
+        mod.forward_logits(torch.zeros(2, 256), torch.zeros(2, 4), 2)
+
+
+def test_experts_of_other_shapes_do_not_reach_the_layer_call() -> None:
+    """up of fewer rows than gate, down of fewer experts' bytes, other dtypes: not what `mxa_moe_layer` assumes."""
+    import torch
+    import torch.nn.functional as F
+
+    from matricxon_amd.moe import HipPackedMoEExperts
+
+    def layer(gate=(4, 512, 144), up=(4, 512, 144), down=(4, 256, 288), dtype=torch.uint8):
+        w = [torch.zeros(s, dtype=dtype) for s in (gate, up, down)]
+        return HipPackedMoEExperts(*w, Q4_K, Q4_K, Q4_K, 256, 512, F.silu)
+
+    assert layer()._layer_ok
+    for bad in (dict(gate=(4, 256, 144)), dict(up=(4, 256, 144)), dict(up=(4, 512, 160)), dict(down=(4, 128, 288)),
+                dict(down=(4, 256, 144)), dict(dtype=torch.int8)):
+        assert not layer(**bad)._layer_ok, bad
