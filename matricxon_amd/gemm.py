@@ -507,6 +507,8 @@ class HipGemm:
                 ldg, gstep = k, 1
             elif plain and len(gs) == x.dim() and gs[-1] == 1 and gs[:-1] == x.shape[:-1]:
                 ldg = 1
+            elif len(gs) <= x.dim() and gate.numel() == 1:
+                pass  # one value for all
             else:
                 gate = gate.expand(x.shape).reshape(-1, k)  # RuntimeError where it does not broadcast
                 if gate.stride(1) > 1 and k > 1:
