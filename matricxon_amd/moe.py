@@ -138,16 +138,24 @@ class HipPackedMoEExperts(nn.Module):
         if q8k_scale not in ("divide", "reciprocal"):
             raise ValueError(f'q8k_scale must be "divide" or "reciprocal", got {q8k_scale!r}')
         reciprocal = q8k_scale == "reciprocal"
-        g = self._gemm
         n_tokens = x.shape[0] if x.dim() == 2 else -1
         dev = self._buffers["gate_packed"].device
         if n_tokens < 0 or x.shape[1] != self.n_embd or x.device != dev or not x.is_cuda:
             raise ValueError(f"x must be (n_tokens, {self.n_embd}) on the HIP device of the experts, {dev}, got "
                              f"{tuple(x.shape)} on {x.device}")
-        g._check_router(logits, n_tokens, self.num_experts, top_k)
+        self._gemm._check_router(logits, n_tokens, self.num_experts, top_k)
         if logits.device != x.device or self.dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"router logits on {x.device} and a float32 or bfloat16 layer, got {logits.device} and "
                              f"{self.dtype}")
+        if _elsewhere(dev):
+            with torch.cuda.device(dev):
+                return self._from_logits(x, logits, top_k, norm_topk, scale, reciprocal)
+        return self._from_logits(x, logits, top_k, norm_topk, scale, reciprocal)
+
+    def _from_logits(self, x: torch.Tensor, logits: torch.Tensor, top_k: int, norm_topk: bool, scale: float,
+                     reciprocal: bool) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """`forward_logits` of checked arguments, with the experts' device the current one."""
+        g, n_tokens = self._gemm, x.shape[0]
         res = self._few_tokens(x, logits, top_k, norm_topk, scale, reciprocal)
         if res is not None:
             return res
@@ -174,9 +182,6 @@ class HipPackedMoEExperts(nn.Module):
         n_tokens, dev = x.shape[0], x.device
         if not 1 <= n_tokens <= _LAYER_MAX_TOKENS or not self._layer_ok or not _is_silu(self.activation):
             return None
-        if _elsewhere(dev):
-            with torch.cuda.device(dev):
-                return self._few_tokens(x, logits, top_k, norm_topk, scale, reciprocal)
         lib, bf16 = self._gemm._lib, self.dtype == torch.bfloat16
         gt, _, dt = self.types
         ws_bytes = self._layer_bytes.get((n_tokens, top_k))

@@ -108,3 +108,55 @@ def test_experts_of_other_shapes_do_not_reach_the_layer_call() -> None:
     for bad in (dict(gate=(4, 256, 144)), dict(up=(4, 256, 144)), dict(up=(4, 512, 160)), dict(down=(4, 128, 288)),
                 dict(down=(4, 256, 144)), dict(dtype=torch.int8)):
         assert not layer(**bad)._layer_ok, bad
+
+
+def test_every_launch_goes_to_the_device_of_the_experts(monkeypatch) -> None:
+    """Experts on a device that is not the current one: the grouped launches, too, run with theirs as the current one."""
+    import contextlib
+
+    import pytest
+    import torch
+
+    from matricxon_amd import moe
+
+    current, seen = [0], []
+
+    @contextlib.contextmanager
+    def device(d):
+        kept, current[0] = current[0], d.index
+        try:
+            yield
+        finally:
+            current[0] = kept
+
+    class OnDevice1(torch.Tensor):  # host values that say they are on the second device
+        device, is_cuda = torch.device("cuda", 1), True
+
+    def there(*shape):
+        return torch.zeros(*shape).as_subclass(OnDevice1)
+
+    class Gemm:
+        @staticmethod
+        def _check_router(*_):
+            pass
+
+        @staticmethod
+        def moe_topk(logits, top_k, *_):
+            seen.append(current[0])
+            return there(len(logits), top_k), there(len(logits), top_k)
+
+    monkeypatch.setattr(moe, "_elsewhere", lambda d: d.index != current[0])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    mod = moe.HipPackedMoEExperts.__new__(moe.HipPackedMoEExperts)
+    torch.nn.Module.__init__(mod)
+    mod._buffers["gate_packed"] = there(4, 256, 144)
+    mod.n_embd, mod.num_experts, mod.dtype, mod._gemm = 256, 4, torch.float32, Gemm
+    mod._few_tokens = lambda *_: seen.append(current[0])
+    mod._grouped = lambda x, *_, **__: (seen.append(current[0]), x)[1]
+    for tokens in (3, 20):
+        out, _, _ = mod.forward_logits(there(tokens, 256), there(tokens, 4), 2)
+        assert out.shape == (tokens, 256) and seen == [1, 1, 1] and current == [0], seen
+        seen.clear()
+    with pytest.raises(ValueError, match="reciprocal"):
+        mod.forward_logits(there(20, 256), there(20, 4), 2, q8k_scale="reciprocal")
+    assert set(seen) == {1} and current == [0]
