@@ -275,8 +275,10 @@ int mxa_moe_combine_masked(const float *down, const int32_t *rows, const int32_t
                            const float *weights, int n_tokens, int top_k, int n_embd, int round_bf16,
                            float *out, void *stream);
 
-/* Most tokens of one mxa_moe_topk, mxa_add_rms_norm_q8_k or mxa_rope: a grid holds below 2^32 threads. */
+/* Most tokens of one mxa_moe_topk, mxa_add_rms_norm_q8_k or mxa_rope, and most values (n_tokens * dim) of one
+ * mxa_add_rms_norm_q8_k, whose rows take more threads the longer they are: a grid holds below 2^32 threads. */
 #define MXA_MAX_TOKENS (1 << 24)
+#define MXA_NORM_MAX_TOTAL (1LL << 35)
 
 /* Routing of MoE tokens from router logits (n_tokens, n_experts), float32 or bfloat16 (logits_bf16 != 0): ids
  * and weights (n_tokens, top_k), DEVICE int32 and float32. Slot i of a token is its i-th largest logit, ties to
@@ -351,9 +353,9 @@ int mxa_silu_mul_q8_k(const float *gate, const float *up, long long ld, int n_to
  *   u = x, or with post_weight x * post_weight / sqrt(mean(x^2) + post_eps)
  *   hidden = r + scale * gate * u
  *   out = hidden * weight / sqrt(mean(hidden^2) + eps), of hidden as it was stored
- * over n_tokens rows (up to MXA_MAX_TOKENS) of dim values (1 .. 32768), in float32, hidden and out each
- * rounded once. x, post_weight, gate, weight and out are bfloat16 (bf16 != 0) or float32, residual and hidden bfloat16
- * (residual_bf16 != 0, with bf16 only) or float32. Rows of x, residual and gate are ldx, ldr and ldg values
+ * over n_tokens rows (up to MXA_MAX_TOKENS, and MXA_NORM_MAX_TOTAL values) of dim values (1 .. 32768), in float32,
+ * hidden and out each rounded once. x, post_weight, gate, weight and out are bfloat16 (bf16 != 0) or float32,
+ * residual and hidden bfloat16 (residual_bf16 != 0, with bf16 only) or float32. Rows of x, residual and gate are ldx, ldr and ldg values
  * apart (0: one row for all); gate is NULL, or has a value for each column (gate_step 1) or one for a row
  * (gate_step 0); post_weight is NULL or dim values. hidden and out are contiguous and overlap no input.
  * workspace: NULL, or (dim a multiple of 256) written with the Q8_K blocks of out, mxa_quantize_q8_k's

@@ -644,6 +644,7 @@ int mxa_add_rms_norm_q8_k(const void* x, long long ldx, const void* residual, lo
   const uintptr_t xa = bf16 ? 2 : 4, ra = residual_bf16 ? 2 : 4;
   if (x == nullptr || residual == nullptr || weight == nullptr || hidden == nullptr || out == nullptr ||
       n_tokens <= 0 || n_tokens > MXA_MAX_TOKENS || dim <= 0 || ldx < 0 || ldr < 0 || ldg < 0 ||
+      (long long)n_tokens * dim > MXA_NORM_MAX_TOTAL ||
       (gate_step != 0 && gate_step != 1) ||
       (residual_bf16 && !bf16) || !aligned(x, xa) || !aligned(weight, xa) || !aligned(post_weight, xa) ||
       !aligned(gate, xa) || !aligned(out, xa) || !aligned(residual, ra) || !aligned(hidden, ra) ||

@@ -134,12 +134,13 @@ class HipFusedOps:
         be float32 beside a bfloat16 block; the weights and the gate have x's dtype, post_eps is eps unless given.
         Float32 steps; hidden and normed are each rounded once (rms_norm's bfloat16 steps round twice, as torch's
         do). None for what it does not take: CPU tensors, other dtypes or shapes, rows of more than 32768 values,
-        more than 2^24 rows."""
+        more than 2^24 rows or 2^35 values."""
         shape, dt, dev = x.shape, x.dtype, x.device
         k = shape[-1] if shape else 0
         if (not x.is_cuda or (dt is not torch.bfloat16 and dt is not torch.float32) or residual.shape != shape
                 or (residual.dtype is not dt and residual.dtype is not torch.float32) or residual.device != dev
-                or not 1 <= k <= HipGemm.NORM_MAX_VALUES or not 0 < x.numel() <= k * HipGemm.MAX_TOKENS):
+                or not 1 <= k <= HipGemm.NORM_MAX_VALUES
+                or not 0 < x.numel() <= min(k * HipGemm.MAX_TOKENS, HipGemm.NORM_MAX_TOTAL)):
             return None
         for w in (weight,) if post_weight is None else (weight, post_weight):
             if w.dtype is not dt or w.shape != (k,) or w.device != dev:

@@ -446,6 +446,7 @@ class HipGemm:
 
     MAX_TOKENS = 1 << 24  # rows of one add_rms_norm_q8k, tokens of one rope or moe_topk
     NORM_MAX_VALUES = 32768  # the longest row of add_rms_norm_q8k
+    NORM_MAX_TOTAL = 1 << 35  # and the values of all its rows
 
     def add_rms_norm_q8k(self, residual: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, eps: float,
                          post_weight: torch.Tensor | None = None, post_eps: float | None = None,
@@ -456,7 +457,7 @@ class HipGemm:
         residual's dtype, out = RMSNorm(hidden; weight, eps) in x's, and the workspace the Q8_K blocks of out
         (None where they are not wanted or the rows are not whole blocks). x and residual (..., K), of float32 or
         bfloat16 each, residual not narrower than x; weight and post_weight (K,) and gate, which broadcasts to x,
-        in x's dtype. K up to NORM_MAX_VALUES."""
+        in x's dtype. K up to NORM_MAX_VALUES, up to MAX_TOKENS rows and NORM_MAX_TOTAL values in all."""
         _require_device_tensor("x", x)
         dev, dt, k = x.device, x.dtype, x.shape[-1] if x.dim() else 0
         if dt not in (torch.float32, torch.bfloat16) or residual.dtype not in (torch.float32, dt):
@@ -465,8 +466,9 @@ class HipGemm:
         if not 1 <= k <= self.NORM_MAX_VALUES or residual.shape != x.shape or residual.device != dev:
             raise ValueError(f"x and residual must be (..., K) on one device, K in 1..{self.NORM_MAX_VALUES}, got "
                              f"{tuple(x.shape)} and {tuple(residual.shape)}")
-        if x.numel() > k * self.MAX_TOKENS:
-            raise ValueError(f"x must have up to {self.MAX_TOKENS} rows, got {tuple(x.shape)}")
+        if x.numel() > min(k * self.MAX_TOKENS, self.NORM_MAX_TOTAL):
+            raise ValueError(f"x must have up to {self.MAX_TOKENS} rows and {self.NORM_MAX_TOTAL} values, got "
+                             f"{tuple(x.shape)}")
         for name, w in (("weight", weight), ("post_weight", post_weight)):
             if w is not None and (w.shape != (k,) or w.dtype != dt or w.device != dev):
                 raise ValueError(f"{name} must be ({k},) {dt} on {dev}")

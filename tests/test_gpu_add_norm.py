@@ -268,3 +268,13 @@ def test_in_inference_mode(gpu, ops) -> None:
         got[1].mul_(2)
         twice = project_shared(owner, ("p",), got[1])[0]
     assert torch.equal(got[0], want[0]) and torch.equal(twice, project_shared(owner, ("p",), 2 * want[1])[0])
+
+
+def test_more_values_than_a_grid_holds(gpu, ops) -> None:
+    """Rows whose count alone is within the limit, their threads together not: refused before anything is allocated."""
+    one = torch.zeros(1, 32768, dtype=BF16, device="cuda")
+    for m, k in ((1 << 24, 4096), (1 << 23, 8192), ((1 << 20) + 1, 32768)):
+        x, w = one[:, :k].expand(m, k), one[0, :k]
+        assert ops.add_rms_norm(x, x, w, EPS) is None
+        with pytest.raises(ValueError, match="values"):
+            gpu.add_rms_norm_q8k(x, x, w, EPS)

@@ -55,3 +55,30 @@ def test_more_rows_than_a_grid_holds_are_refused() -> None:
     for m in ((1 << 24) + 1, 2 ** 31 - 1):
         assert _lib.load().mxa_add_rms_norm_q8_k(a, 1, a, 1, None, 1e-5, None, 0, 0, 1.0, a, 1e-5, m, 1, 1, 1, a, a, None,
                                                  0, None) == -1
+
+
+def test_more_values_than_a_grid_holds_are_refused() -> None:
+    """Rows of up to 1024 threads each, of counts that alone are within the limit; inputs of one row cost no memory."""
+    from matricxon_amd import _lib
+
+    a = ctypes.c_void_p(0x10000)
+    for m, k in ((1 << 24, 4096), (1 << 23, 8192), (1 << 22, 16384), (1 << 22, 32768), ((1 << 20) + 1, 32768),
+                 (1 << 24, 2049)):
+        for bf16 in (0, 1):
+            assert _lib.load().mxa_add_rms_norm_q8_k(a, 0, a, 0, None, 1e-5, None, 0, 0, 1.0, a, 1e-5, m, k, bf16, bf16, a,
+                                                     a, None, 0, None) == -1, (m, k)
+
+
+def test_every_grid_that_is_taken_is_below_2_to_the_32() -> None:
+    """The launch's threads at the most rows that each length may have: whole waves of eight values a lane, in one, two
+    or four vectors."""
+    total, rows = 1 << 35, 1 << 24
+    assert HipGemm.NORM_MAX_TOTAL == total and HipGemm.MAX_TOKENS == rows
+    for k in range(1, HipGemm.NORM_MAX_VALUES + 1):
+        vectors = (k + 7) // 8
+        for per_thread in (1, 2, 4):
+            threads = ((vectors + per_thread - 1) // per_thread + 63) // 64 * 64
+            many = min(rows, total // k)
+            if threads > 1024 or (per_thread == 1 and vectors >= 128):  # two at least where there are many rows
+                continue
+            assert (many + 3) * threads < 1 << 32, (k, per_thread)
