@@ -244,10 +244,17 @@ template <bool XB, bool RB, bool POST>
 void launch_norm(const NormArgs& a, const ActBuffers* q, hipStream_t stream) {
   const int nv = (a.k + 7) / 8;
   // Few rows: as many threads a row as there are vectors. Many rows: two vectors a thread, half the waves and
-  // reductions for the same bytes in flight, and h and n past the caches, which they would not survive in (bfloat16
-  // rows of 4096 with a norm on both sides, kernel alone: 4096 rows one vector a thread 37.1 us, two 35.8, two past
-  // the caches 29.9, four 45.8; 1024 rows 13.1 and 11.9 past the caches; 256 rows one vector 6.2 and 5.8).
+  // reductions (4096 bfloat16 rows of 4096 with a norm on both sides, kernel alone: one vector a thread 37.1 us, two
+  // 35.8, four 45.8).
   const bool many = a.rows > 512;
+  // h and n past the caches from 8 MB of them together. Times past the caches against plain stores, of this kernel
+  // alone and with the next add_rms_norm behind it, which reads h and n at once (every output in memory of its own, x
+  // just written or not): below 8 MB within 6%, both; both bfloat16 12 to 48 MB 4 to 29% less alone and from 19% less to
+  // 3% more together, 56 to 128 MB 3 to 15% less and -9 to +9%, above 0 to 10% and 1 to 8% less; one or both float32
+  // 12 to 28 MB 11 to 17% and 1 to 19% less, 32 to 128 MB -15 to +4% and -3 to +13%, above -5 to +1% and -4 to +4%. (A
+  // layer reads n at once or its blocks alone, h after the block. 1024 bfloat16 rows of 4096: 10.2 us plain and 8.5,
+  // with the next 18.4 and 16.1.)
+  const bool once = (long long)a.rows * a.k * ((RB ? 2 : 4) + (XB ? 2 : 4)) >= 8000000;
   const int fewest = (nv + kNormMaxThreads - 1) / kNormMaxThreads;
   const int want = many && nv >= 128 ? 2 : 1;
   const int p = max(fewest, want) <= 1 ? 1 : max(fewest, want) <= 2 ? 2 : 4;
@@ -257,7 +264,7 @@ void launch_norm(const NormArgs& a, const ActBuffers* q, hipStream_t stream) {
   int8_t* qq = q != nullptr ? q->q : nullptr;
   float* qd = q != nullptr ? q->d : nullptr;
   int16_t* qb = q != nullptr ? q->bsums : nullptr;
-  auto kern = many ? (p == 1 ? add_rms_norm_kernel<XB, RB, POST, 1, true>
+  auto kern = once ? (p == 1 ? add_rms_norm_kernel<XB, RB, POST, 1, true>
                       : p == 2 ? add_rms_norm_kernel<XB, RB, POST, 2, true>
                                : add_rms_norm_kernel<XB, RB, POST, 4, true>)
                    : (p == 1 ? add_rms_norm_kernel<XB, RB, POST, 1, false>

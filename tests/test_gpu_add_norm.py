@@ -278,3 +278,18 @@ def test_more_values_than_a_grid_holds(gpu, ops) -> None:
         assert ops.add_rms_norm(x, x, w, EPS) is None
         with pytest.raises(ValueError, match="values"):
             gpu.add_rms_norm_q8k(x, x, w, EPS)
+
+
+# outputs of 1 MB in many rows and of 5 to 180 MB in few and many: stored past the caches or not, one, two and four
+# vectors a thread, whole and not
+@pytest.mark.parametrize("dtypes", DTYPES, ids=["f32", "bf16", "bf16-f32"])
+@pytest.mark.parametrize("m,k", [(1030, 256), (300, 8192), (400, 3079), (100, 32768), (65, 32765), (5000, 513),
+                                 (5003, 4096), (2500, 4099), (600, 20000), (12000, 4096), (90000, 500)])
+def test_every_size_of_outputs(gpu, ops, m, k, dtypes) -> None:
+    dt, rt = dtypes
+    g = torch.Generator(device="cuda").manual_seed(m + k)
+    x, r = rand(g, m, k, dt=dt, scale=1.5), rand(g, m, k, dt=rt, scale=4)
+    w, wp = 1 + rand(g, k, dt=dt, scale=0.2), 1 + rand(g, k, dt=dt, scale=0.2)
+    _, normed = check(ops.add_rms_norm(r, x, w, EPS, post_weight=wp), x, r, w, EPS, wp)
+    if k % 256 == 0:
+        assert_blocks(gpu, HANDOFF.claim(normed), normed)
