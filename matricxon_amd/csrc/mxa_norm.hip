@@ -249,8 +249,8 @@ void launch_norm(const NormArgs& a, const ActBuffers* q, hipStream_t stream) {
   const bool many = a.rows > 512;
   // h and n past the caches from 8 MB of them together. Times past the caches against plain stores, of this kernel
   // alone and with the next add_rms_norm behind it, which reads h and n at once (every output in memory of its own, x
-  // just written or not): below 8 MB within 6%, both; both bfloat16 12 to 48 MB 4 to 29% less alone and from 19% less to
-  // 3% more together, 56 to 128 MB 3 to 15% less and -9 to +9%, above 0 to 10% and 1 to 8% less; one or both float32
+  // just written or not): below 8 MB within 8%, both; both bfloat16 12 to 48 MB 4 to 29% less alone and from 19% less
+  // to 3% more together, 56 to 128 MB 3 to 15% less and -9 to +9%, above 0 to 10% and 1 to 8% less; one or both float32
   // 12 to 28 MB 11 to 17% and 1 to 19% less, 32 to 128 MB -15 to +4% and -3 to +13%, above -5 to +1% and -4 to +4%. (A
   // layer reads n at once or its blocks alone, h after the block. 1024 bfloat16 rows of 4096: 10.2 us plain and 8.5,
   // with the next 18.4 and 16.1.)

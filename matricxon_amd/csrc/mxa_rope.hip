@@ -176,12 +176,24 @@ void launch_rope_v(const RopeArgs& a, hipStream_t stream) {
   // Up to 512 tokens the heads of one token over several workgroups, a row a thread (32 + 8 bfloat16 heads of 128,
   // kernel alone: 300 tokens 5.0 us, a workgroup a token 5.4; 700 tokens 7.0 and 6.3). More: a workgroup a token, or
   // as many tokens each as leave about a thousand workgroups, what the CUs hold at once (1500 tokens by one 11.2, by
-  // two 10.2, by four 11.6; 4096 by two 19.6, by four 17.3, by eight 19.6), stored past the caches, which the heads
-  // of so many tokens would not survive in (700 tokens 6.3 and 6.0, 1500 10.2 and 8.4, 4096 17.3 and 15.5).
+  // two 10.2, by four 11.6; 4096 by two 19.6, by four 17.3, by eight 19.6).
   const bool many = a.n_tokens > 512;
   const int TP = many ? min(8, (a.n_tokens + 1023) / 1024) : 1;
   const int split = many ? 1 : min(4096, (H + HP - 1) / HP);  // a grid's threads have to stay below 2^32
-  auto kern = many ? rope_kernel<T, INTER, V, true> : rope_kernel<T, INTER, V, false>;
+  // The outputs past the caches from 4 MB of them on, where every head turns whole, in 16-byte vectors. Times past the
+  // caches against plain stores, of this kernel alone and with a kernel behind it that reads what it wrote (every
+  // output in memory of its own, q and k just written or not): below 4 MB within 5%, both; bfloat16 4 to 12 MB 1 to
+  // 13% less alone and 0 to 13% less together, 16 to 48 MB 3 to 29% less and from 21% less to 8% more, 56 to 128 MB 2
+  // to 15% less and -10 to +7%, above 0 to 8% less and from 9% less to 1% more; float32 in halves much the same,
+  // interleaved from 20 MB on from 30% less to 1% more and -8 to +13%. Parts of a head, stored in pieces that are no
+  // whole lines, and vectors of less than 16 bytes gain less than they lose: from 29% less to 26% more alone, up to
+  // 38% more with the reader (bfloat16 32 of 80 values, 42 MB: 33.9 us plain and 35.1, with the reader 61.8 and 76.3;
+  // 20 of 80 127 and 117, 241 and 259).
+  auto kern = rope_kernel<T, INTER, V, false>;
+  if constexpr (V * sizeof(T) == 16) {
+    if (a.rot == a.dim && (long long)a.n_tokens * H * a.dim * (long long)sizeof(T) >= 4000000)
+      kern = rope_kernel<T, INTER, V, true>;
+  }
   hipLaunchKernelGGL(kern, dim3((a.n_tokens + TP - 1) / TP, split), dim3(kRopeThreads),
                      (size_t)TP * a.rot * sizeof(float), stream, a, TP, C, CR, HP);
 }

@@ -239,3 +239,39 @@ def test_the_most_tokens(gpu) -> None:
     more = torch.zeros(1, 1, 2, device="cuda").expand(n + 1, 1, 2)
     with pytest.raises(ValueError, match="tokens"):
         rot(more, None, torch.zeros(1, dtype=torch.int32, device="cuda").expand(n + 1))
+
+
+# whole vectors, vectors of four, two and one value, whole heads and parts of them
+WIDE = [(128, 128), (64, 64), (80, 32), (80, 20), (96, 24), (48, 44), (66, 2), (256, 64), (512, 512)]
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dim,rot_dim", WIDE)
+@pytest.mark.parametrize("t", [513, 1027, 2051])
+def test_many_tokens(gpu, dt, interleaved, dim, rot_dim, t) -> None:
+    """Token counts of every share of a workgroup, outputs of less than 4 MB and of more, in pieces of every width."""
+    g = torch.Generator(device="cuda").manual_seed(dim + t)
+    rot = HipRotary(dim, rotary_dim=rot_dim, interleaved=interleaved)
+    q, k = rand(g, t, 5, dim, dt=dt), rand(g, t, 2, dim, dt=dt)
+    pos = torch.randint(0, 100000, (t,), device="cuda", generator=g)
+    q2, k2 = rot(q, k, pos)
+    check(rot, q, q2, pos)
+    check(rot, k, k2, pos)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dim,rot_dim", [(64, 64), (80, 32), (96, 24)])
+@pytest.mark.parametrize("b,t", [(3, 401), (7, 333), (1031, 3), (2, 600)])
+def test_workgroups_across_sequences(gpu, dt, interleaved, dim, rot_dim, b, t) -> None:
+    """More than 512 tokens in sequences of odd lengths, a workgroup's tokens in two or more of them, with positions of
+    their own."""
+    g = torch.Generator(device="cuda").manual_seed(b * t)
+    rot = HipRotary(dim, rotary_dim=rot_dim, interleaved=interleaved)
+    q, k = rand(g, b, 9, t, dim, dt=dt).transpose(1, 2), rand(g, b, t + 1, 3, dim, dt=dt)[:, 1:]
+    pos = torch.randint(0, 100000, (b, t), device="cuda", generator=g)
+    for p in (pos, pos[:1].int(), pos[0]):
+        q2, k2 = rot(q, k, p)
+        check(rot, q, q2, p.expand(b, t))
+        check(rot, k, k2, p.expand(b, t))
