@@ -540,6 +540,8 @@ class HipGemm:
         """Rotary positions of q and k in one launch (`mxa_rope`), `turns` (rotary_dim / 2) float64 on their device;
         `matricxon_amd.rotary.HipRotary` is the face of it."""
         _require_device_tensor("q", q)
+        if rotary_dim < 2 or rotary_dim % 2:
+            raise ValueError(f"rotary_dim must be even and positive, got {rotary_dim}")
         if turns.dtype != torch.float64 or turns.shape != (rotary_dim // 2,) or turns.device != q.device or \
                 not turns.is_contiguous():
             raise ValueError(f"turns must be ({rotary_dim // 2},) float64, contiguous, on {q.device}")

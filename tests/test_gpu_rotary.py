@@ -275,3 +275,24 @@ def test_workgroups_across_sequences(gpu, dt, interleaved, dim, rot_dim, b, t) -
         q2, k2 = rot(q, k, p)
         check(rot, q, q2, p.expand(b, t))
         check(rot, k, k2, p.expand(b, t))
+
+
+def test_the_library_face(gpu) -> None:
+    """`HipGemm.rope` on a table of the caller's: `HipRotary`'s bits, and its refusals."""
+    g = torch.Generator(device="cuda").manual_seed(10)
+    rot = HipRotary(64, rotary_dim=32, interleaved=True, scaling=SCALINGS[3])
+    q, k, pos = rand(g, 9, 4, 64), rand(g, 9, 2, 64), torch.arange(9, device="cuda")
+    turns = (rot.frequencies / (2 * math.pi)).cuda()
+    for a, b in zip(gpu.rope(q, k, pos, turns, 32, True, rot.scale), rot(q, k, pos)):
+        assert torch.equal(a, b)
+    for bad in (turns.float(), turns[:15], turns.cpu(), torch.zeros(32, dtype=torch.float64, device="cuda")[::2]):
+        with pytest.raises(ValueError, match="turns"):
+            gpu.rope(q, k, pos, bad, 32, True, 1.0)
+    with pytest.raises(ValueError, match="HIP device"):
+        gpu.rope(q.cpu(), None, pos, turns, 32, True, 1.0)
+    wide = torch.zeros(33, dtype=torch.float64, device="cuda")
+    with pytest.raises(ValueError, match="head_dim"):
+        gpu.rope(q, k, pos, wide, 66, True, 1.0)
+    for rotary_dim in (0, 3):  # no pair, and half a pair
+        with pytest.raises(ValueError, match="rotary_dim"):
+            gpu.rope(q, k, pos, turns[: rotary_dim // 2], rotary_dim, True, 1.0)
