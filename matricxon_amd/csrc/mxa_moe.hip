@@ -7,9 +7,12 @@
 // rounded to float32. One thread per output element; the pair order is ranked once per workgroup, by a
 // wave whose lanes hold a slot each.
 //
-// Bound: latency for few tokens (slots, order, rows), memory for many. Four rows are requested before the first is
-// added: 4 tokens of top 8 (rows of 1536) 3.5 us, requested one by one 4.5; 4096 tokens of top 2 (4096) 56 and 68, of
-// top 8 (2048) 63 and 115 (4.8 TB/s).
+// Bound: latency for few tokens (slots, order, rows), memory for many. Up to four rows are requested before the first
+// is added: 4 tokens of top 8 (rows of 1536) 3.7 us, requested one by one 4.5; 4096 tokens of top 2 (4096) 66 and 83, of
+// top 8 (2048) 70 and 117 (4.3 TB/s). A last group of fewer requests no row twice: 1024 tokens of top 1 (4096) 13.9 and
+// 13.4, 4096 of them 45 and 47.
+#include <type_traits>
+
 #include "mxa_kernels.hpp"
 
 #pragma clang fp contract(off)
@@ -25,7 +28,6 @@ __device__ __forceinline__ float round_bf16(float f) {
   return __uint_as_float((u + 0x7FFFu + ((u >> 16) & 1u)) & 0xFFFF0000u);
 }
 
-constexpr int kCombineRows = 4;  // rows requested before the first is added
 __global__ __launch_bounds__(256) void moe_combine_kernel(
     const float* __restrict__ down, const int32_t* __restrict__ rows,
     const int32_t* __restrict__ ids, const float* __restrict__ wts, int top_k, int n_embd,
@@ -54,16 +56,21 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(
   }
   __syncthreads();
   if (j >= n_embd) return;
-  const int n = count;
+  const int n = __builtin_amdgcn_readfirstlane(count);
   float acc = 0.0f;
-  for (int i = 0; i < n; i += kCombineRows) {
-    float v[kCombineRows];
+  int i = 0;
+  const auto add = [&](auto rows_at_once) __attribute__((always_inline)) {
+    constexpr int kRows = decltype(rows_at_once)::value;
+    float v[kRows];
 #pragma unroll
-    for (int u = 0; u < kCombineRows; ++u) v[u] = down[(size_t)srow[min(i + u, n - 1)] * n_embd + j];
+    for (int u = 0; u < kRows; ++u) v[u] = down[(size_t)srow[i + u] * n_embd + j];
 #pragma unroll
-    for (int u = 0; u < kCombineRows; ++u)
-      if (i + u < n) acc = acc + (bf16 ? round_bf16(v[u]) : v[u]) * swt[i + u];
-  }
+    for (int u = 0; u < kRows; ++u) acc = acc + (bf16 ? round_bf16(v[u]) : v[u]) * swt[i + u];
+    i += kRows;
+  };
+  while (i + 4 <= n) add(std::integral_constant<int, 4>{});
+  if (i + 2 <= n) add(std::integral_constant<int, 2>{});
+  if (i < n) add(std::integral_constant<int, 1>{});
   out.put((size_t)t * n_embd + j, acc);
 }
 

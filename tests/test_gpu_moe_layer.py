@@ -424,3 +424,28 @@ def test_one_expert_to_the_most(gpu, e, k, t, dtype) -> None:
     assert mod._layer_bytes[t, k] > 0
     check_routing(logits, k, True, 1.0, ids, wts)
     assert torch.equal(out, mod._grouped(x, wts, ids))
+
+
+@pytest.mark.parametrize("k", range(1, 17))
+@pytest.mark.parametrize("masked", [False, True])
+def test_combine_of_every_count_of_slots(gpu, k, masked) -> None:
+    """1 to 16 slots a token and, masked, any number of them without an expert, whose rows and weights hold NaN: the sum
+    in ascending id, one product and one addition at a time."""
+    t, n = 40, 260
+    g = torch.Generator(device="cuda").manual_seed(k)
+    ids = torch.stack([torch.randperm(40, device="cuda", generator=g)[:k] for _ in range(t)]).int()
+    wts, down = torch.rand(t, k, device="cuda", generator=g), torch.randn(t * k, n, device="cuda", generator=g)
+    rows = torch.randperm(t * k, device="cuda", generator=g).int().view(t, k)
+    if masked:
+        off = torch.arange(k, device="cuda") >= torch.arange(t, device="cuda")[:, None] % (k + 1)
+        off = off.gather(1, torch.rand(t, k, device="cuda", generator=g).argsort(1))
+        ids[off], wts[off] = -1, float("nan")
+        down[rows[off].long()] = float("nan")
+    want = torch.zeros(t, n, device="cuda")
+    order = torch.where(ids < 0, 1000, ids).argsort(1)
+    for j in range(k):
+        slot = order[:, j : j + 1]
+        live = ids.gather(1, slot) >= 0
+        term = down[rows.gather(1, slot).flatten().long()].bfloat16().float() * wts.gather(1, slot)
+        want = torch.where(live, want + term, want)
+    assert torch.equal(gpu.moe_combine(down, ids, wts, rows, round_bf16=True, masked=masked), want)
