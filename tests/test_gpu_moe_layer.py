@@ -426,6 +426,37 @@ def test_one_expert_to_the_most(gpu, e, k, t, dtype) -> None:
     assert torch.equal(out, mod._grouped(x, wts, ids))
 
 
+@pytest.mark.parametrize("gt,dt,e,embd,ffn,k,t", [
+    (D.Q4_K, D.Q6_K, 8, 512, 768, 4, 8), (D.Q8_0, D.Q8_0, 8, 512, 512, 4, 8), (D.Q8_0, D.Q8_0, 4, 1024, 256, 2, 1),
+    (D.Q6_K, D.Q8_0, 16, 512, 512, 3, 7), (D.Q6_K, D.Q4_K, 3, 256, 14336, 2, 4), (D.Q8_0, D.Q6_K, 5, 256, 512, 2, 21),
+    (D.Q4_K, D.Q4_K, 12, 256, 512, 9, 9)])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_reciprocal_code_scales_of_every_form(gpu, gt, dt, e, embd, ffn, k, t, dtype) -> None:
+    """More than 16 pairs (down by items, summed by the combine), rows of down that leave the sum too few waves, more
+    tokens than a call takes, 8-bit experts and float32 layers, whose activations are read and rounded by other code: the
+    layer's own silu(gate) * up, through each expert's projections on blocks that torch computes."""
+    mod, per_expert = build_experts((gt, gt, dt), e, embd, ffn, dtype, seed=19)
+    x = torch.from_numpy(S.activations(t, embd, seed=9)).cuda().to(dtype)
+    x[:, :256] *= 3.90625 / x[:, :256].abs().amax(1, keepdim=True)  # blocks whose codes differ
+    logits = router(t, e, 12)
+    out, ids, wts = mod.forward_logits(x, logits, k, q8k_scale="reciprocal")
+    check_routing(logits, k, True, 1.0, ids, wts)
+
+    def through(linear, v, out_dtype):
+        y = torch.empty(len(v), linear.out_features, dtype=out_dtype, device="cuda")
+        return gpu.matmul_q8k(linear.ggml_type, linear.packed, torch_q8k(v), None, y, len(v), linear.out_features,
+                              linear.in_features)
+
+    want = torch.zeros(t, embd, device="cuda")
+    for row in range(t):
+        for slot in sorted(range(k), key=lambda j: int(ids[row, j])):
+            gate, up, down = per_expert[int(ids[row, slot])]
+            g, u = (through(m, x[row][None], dtype) for m in (gate, up))
+            act = F.silu(g) * u if dtype == BF16 else gpu.silu_mul_q8k(g, u)[0]
+            want[row] += through(down, act, dtype)[0].float() * wts[row, slot]
+    assert torch.equal(out, want.to(dtype))
+
+
 @pytest.mark.parametrize("k", range(1, 17))
 @pytest.mark.parametrize("masked", [False, True])
 def test_combine_of_every_count_of_slots(gpu, k, masked) -> None:
