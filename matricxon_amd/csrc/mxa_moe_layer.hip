@@ -25,8 +25,10 @@
 // first copy and 3 after the last; down 26 us for 96 MB (3.7 TB/s): 3 us before the first copy, 9 before the two
 // activation rows are blocks, then the LDS holds 10 rows of 56 blocks, which wait and compute in turn. Eight tokens: 95
 // and 86 us, 5.0 and 4.0 TB/s: each further pair of an expert takes LDS from the rows and adds to the part of a wave's
-// turn in which its stage is not in flight. 64 experts top 8 of 2048 x 1024, one token: 12 and 9 us, latency from end
-// to end (logits, routing, activations, weights, block arithmetic).
+// turn in which its stage is not in flight. 64 experts top 8 of 2048 x 1024, one token: 12 and 9 us for 19 and 14 MB,
+// latency (logits, routing, activations, weights) and, not timed apart, the arithmetic of few waves: rows a wave are
+// taken by what LDS holds (layer_rows), eight in the first launch, so that a workgroup's share is four sets for its
+// eight waves with rows, each of which computes gate, then up, then folds; of the second, half the lanes hold a block.
 //
 // The sum needs every pair's rows in one place. Up to 16 pairs the second launch's workgroups take rows, each through
 // all items, and add up in LDS. For more they take items, and the combine is a launch of its own (3 to 4 us): adding up
@@ -705,7 +707,8 @@ __global__ __launch_bounds__(256) void moe_topk_kernel(const void* __restrict__ 
 }
 
 // Rows per wave for a matrix of rows of nb blocks, the most rows that the LDS holds at once (of 6 blocks of Q8_0, gate
-// and up, seven waves of 6 rows, not four of 10); 0 where not one wave's rows fit.
+// and up, seven waves of 6 rows, not four of 10); 0 where not one wave's rows fit. Whatever a workgroup's share of
+// rows is: small experts leave waves without any (above).
 template <int TYPE, int MAXM, bool GATEUP>
 int layer_rows(int nb) {
   int R = 0, most = 0;

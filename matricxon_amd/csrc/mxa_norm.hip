@@ -15,9 +15,11 @@
 // short. Rows of up to 512 values take one wave each, four rows to a workgroup, with no barrier; longer
 // rows a workgroup.
 //
-// Bound: memory from some 1000 rows on (4096 x 4096 bfloat16 with both norms 29.9 us for the 134 MB of x, r, h and
-// n and the 19 MB of blocks: 5.1 TB/s, what a large copy reaches), below that the latency of the loads and the two
-// reductions (1 x 4096: 3.6 us).
+// Bound: memory from some 1000 rows on (4096 x 4096 bfloat16 with both norms 28.4 us a call among others for the 134 MB
+// of x, r, h and n and the 19 MB of blocks: 5.4 TB/s, a large copy's rate), below that the latency of loads one behind
+// another, and of the reductions (1 x 4096 3.8 us; 16 x 5120 with both norms and a gate 6.0). As compiled, a bfloat16
+// vector is waited for before the next array's, or the thread's second, is requested (it is widened in the branch that
+// loads it); post, gate and w are requested behind the reductions; and of a short last vector one value at a time.
 #include "mxa_kernels.hpp"
 
 #pragma clang fp contract(off)

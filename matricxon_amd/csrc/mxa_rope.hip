@@ -12,11 +12,14 @@
 // computed once for a (token, pair) and read from LDS by every head.
 //
 // A thread keeps one place of the heads (a vector of V pairs, or of V / 2 pairs interleaved) and walks over the
-// (token, head) rows of its workgroup, a batch of rows requested before the first is computed; the first batch is
-// requested before the angles.
+// (token, head) rows of its workgroup, a batch of rows loaded before the first is computed, the first batch before the
+// angles. As compiled, a row's loads wait for those of the row before it in the batch (its address is formed behind a
+// branch, in registers that those loads write), the table's load for the position's, and the outputs are flat stores
+// (their pointer is q's or k's), behind which the reads of the next row's cosines wait.
 //
-// Bound: memory from some 500 tokens on (4096 tokens of 32 + 8 bfloat16 heads of 128: 15.5 us for 84 MB, 5.4 TB/s, a
-// large copy's rate), below that latency: the positions and the table, then sine and cosine (one token 3.1 us).
+// Bound: memory from some thousand tokens on (4096 tokens of 32 + 8 bfloat16 heads of 128: 15.6 us for 84 MB, 5.4 TB/s,
+// a large copy's rate), below that latency, of the loads above one behind another and of sine and cosine (one token
+// 3.1 us; 777 tokens of 40 + 8 heads 6.5, whose 19 MB take 3.7 at a copy's rate).
 #include "mxa_kernels.hpp"
 
 #pragma clang fp contract(off)

@@ -124,7 +124,7 @@ class HipPackedMoEExperts(nn.Module):
         lowest id, weighted by the softmax over all experts or (`norm_topk`) over the chosen ones, times `scale`. A
         logit of -inf masks its expert; a slot without an expert has id -1 and weight 0 and adds nothing, so that a
         token of -inf alone (padding) gets a row of zeros, whatever x holds there. `forward` on those ids and weights,
-        where no id is -1, gives the same bits.
+        where no id is -1, gives the same bits (with the default `q8k_scale`).
 
         Up to eight tokens (and 64 pairs) of Q4_K, Q6_K or Q8_0 experts, gate and up of one type, with a SiLU: one
         library call (`mxa_moe_layer`) of two launches, three where more than 16 pairs are added up. Otherwise the
