@@ -63,7 +63,7 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: dict | N
             raise ValueError("llama3 scaling needs 0 < low_freq_factor < high_freq_factor")
         if kind == "yarn" and (base == 1 or not 0 < opt["beta_slow"] < opt["beta_fast"]):
             raise ValueError("yarn scaling needs 0 < beta_slow < beta_fast and a base other than 1")
-    i = torch.arange(d // 2, dtype=torch.float64)
+    i = torch.arange(d // 2, dtype=torch.float64, device="cpu")
     if kind == "ntk":
         base = base * opt["factor"] ** (d / (d - 2))
     f = float(base) ** (-2 * i / d)

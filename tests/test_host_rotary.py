@@ -93,3 +93,11 @@ def test_more_tokens_than_a_grid_holds_are_refused() -> None:
     a, st = ctypes.c_void_p(0x10000), (ctypes.c_longlong * 3)(0, 2, 2)
     for n in ((1 << 24) + 1, 2 ** 31 - 1):
         assert _lib.load().mxa_rope(a, st, 1, None, None, 0, a, 1, 0, 1, a, n, n, 2, 2, 0, 1.0, 1, a, None, None) == -1
+
+
+def test_the_table_is_made_on_the_host_under_any_default_device() -> None:
+    want, _ = rotary_frequencies(64, 1e4, {"type": "yarn", "factor": 8.0, "original_context": 4096})
+    with torch.device("meta"):  # as torch.set_default_device sets one
+        f, _ = rotary_frequencies(64, 1e4, {"type": "yarn", "factor": 8.0, "original_context": 4096})
+        g, _ = rotary_frequencies(8, 1e4, None, torch.ones(4, device="cpu"))
+    assert f.device.type == g.device.type == "cpu" and torch.equal(f, want)
