@@ -296,3 +296,17 @@ def test_the_library_face(gpu) -> None:
     for rotary_dim in (0, 3):  # no pair, and half a pair
         with pytest.raises(ValueError, match="rotary_dim"):
             gpu.rope(q, k, pos, turns[: rotary_dim // 2], rotary_dim, True, 1.0)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("t,hq,hk,dim", [(300, 60, 60, 128), (1, 9000, 9000, 128), (511, 40, 3, 256)])
+def test_few_tokens_of_many_heads(gpu, dt, interleaved, t, hq, hk, dim) -> None:
+    """Outputs of more than 4 MB whose heads are split over workgroups."""
+    g = torch.Generator(device="cuda").manual_seed(t)
+    rot = HipRotary(dim, interleaved=interleaved)
+    q, k = rand(g, t, hq, dim, dt=dt), rand(g, t, hk, dim, dt=dt)
+    pos = torch.randint(0, 100000, (t,), device="cuda", generator=g)
+    q2, k2 = rot(q, k, pos)
+    check(rot, q, q2, pos)
+    check(rot, k, k2, pos)
