@@ -355,11 +355,12 @@ int mxa_silu_mul_q8_k(const float *gate, const float *up, long long ld, int n_to
  *   out = hidden * weight / sqrt(mean(hidden^2) + eps), of hidden as it was stored
  * over n_tokens rows (up to MXA_MAX_TOKENS, and MXA_NORM_MAX_TOTAL values) of dim values (1 .. 32768), in float32,
  * hidden and out each rounded once. x, post_weight, gate, weight and out are bfloat16 (bf16 != 0) or float32,
- * residual and hidden bfloat16 (residual_bf16 != 0, with bf16 only) or float32. Rows of x, residual and gate are ldx, ldr and ldg values
- * apart (0: one row for all); gate is NULL, or has a value for each column (gate_step 1) or one for a row
- * (gate_step 0); post_weight is NULL or dim values. hidden and out are contiguous and overlap no input.
- * workspace: NULL, or (dim a multiple of 256) written with the Q8_K blocks of out, mxa_quantize_q8_k's
- * layout. Pointers need their elements' alignment, the workspace 16 bytes.
+ * residual and hidden bfloat16 (residual_bf16 != 0, with bf16 only) or float32. Rows of x, residual and gate are
+ * ldx, ldr and ldg values apart (0: one row for all); gate is NULL, or has a value for each column (gate_step 1)
+ * or one for a row (gate_step 0); post_weight is NULL or dim values. hidden and out are contiguous and overlap no
+ * input.
+ * workspace: NULL, or (dim a multiple of 256) written with the Q8_K blocks of out, mxa_quantize_q8_k's layout.
+ * Pointers need their elements' alignment, the workspace 16 bytes.
  * The steps around the block of the reference's decoder layers, whose norms are RMSNorm.forward
  * (app/architectures/layers.py:72-81), and the next projections' quantization. */
 int mxa_add_rms_norm_q8_k(const void *x, long long ldx, const void *residual, long long ldr,
