@@ -389,6 +389,79 @@ int mxa_rope(const void *q, const long long *q_strides, int q_heads, const void 
              int head_dim, int rotary_dim, int interleaved, float scale, int bf16, void *q_out,
              void *k_out, void *stream);
 
+/* mxa_rope with a norm of each head before it, in the same pass: y = turn(x * w / sqrt(mean(x^2) + eps)) over the
+ * head_dim values of a head, w = q_weight for q and k_weight for k (head_dim values in the type of q and k; NULL: that
+ * side is not normed). Each value is rounded once, at the end. The other arguments are mxa_rope's. */
+int mxa_norm_rope(const void *q, const long long *q_strides, int q_heads, const void *q_weight,
+                  const void *k, const long long *k_strides, int k_heads, const void *k_weight,
+                  float eps, const void *positions, int positions_int64, long long pos_batch,
+                  long long pos_token, const double *turns, int n_tokens, int seq_len, int head_dim,
+                  int rotary_dim, int interleaved, float scale, int bf16, void *q_out, void *k_out,
+                  void *stream);
+
+/* The paged cache of 4-bit keys and values. 32 neighbouring values of a token's head share a float16 scale
+ * s = (max - min) / 15 and minimum m; a value is held as s * code + m, its code the nearest of 0 .. 15. A NaN is held as 0
+ * and a value beyond +-65000 as that.
+ *
+ * `pages` (n_pages, kv_heads, page_size / 32, 1280 * W) bytes, W = head_dim / 32 rounded up, 16-byte aligned
+ * (mxa_kv4_page_bytes a page): blocks of 32 tokens of a head, each
+ *   0       key codes     (token 32, octet 4, group W, 4 bytes): byte y of octet c of a group holds its values
+ *                         8 c + 2 y (low bits) and 8 c + 2 y + 1
+ *   512 W   key scales    (token, group) of (s, m)
+ *   640 W   value codes   (pair of groups, quad 4, i 16, group of the pair, half 2, z 4): the byte of a group's values 2 i
+ *                         (low bits) and 2 i + 1 of token 16 half + 4 quad + z; a last odd group (quad, i, half, z)
+ *   1152 W  value scales  (group, quad of tokens 8): s of its tokens 0 2 1 3, then m
+ * Sequence b (of n_seq) has lengths[b] tokens, place p of it in page table[b * table_stride + p / page_size]; a place
+ * whose page number is outside [0, n_pages), and one at or behind table_width * page_size, is not cached: nothing is
+ * written for it, it reads as zeros and is not attended to. The call's rows are the last tokens of the sequences: rows
+ * [query_starts[b], query_starts[b + 1]) those of b (n_seq + 1 ascending values; rows outside all belong to none), or
+ * with query_starts NULL n_tokens / n_seq of each. table, lengths and query_starts are DEVICE int32.
+ * kv_heads <= 65535, page_size a multiple of 32 up to MXA_KV4_MAX_PAGE, head_dim a multiple of 8 up to MXA_KV4_MAX_DIM,
+ * table_width * page_size <= MXA_KV4_MAX_PLACES, n_seq <= MXA_KV4_MAX_SEQ, n_tokens <= MXA_MAX_TOKENS; else -1. */
+#define MXA_KV4_MAX_DIM 256
+#define MXA_KV4_MAX_PAGE 65536
+#define MXA_KV4_MAX_PLACES (1 << 30)
+#define MXA_KV4_MAX_SEQ 65535
+
+/* Bytes of one page; 0 for sizes that are not supported. Host-only. */
+size_t mxa_kv4_page_bytes(int kv_heads, int page_size, int head_dim);
+
+/* q and k normed and turned as by mxa_norm_rope (a NULL weight: not normed; rotary_dim 0: not turned), k so and v written
+ * to the cache, q to q_out (n_tokens, q_heads, head_dim; q_heads 0: none), in one launch. positions NULL: a token's
+ * place is its position. Rows of no sequence come back as zeros in q_out. q_heads is a multiple of kv_heads. Two
+ * sequences must not write the same page; strides and types as mxa_rope. */
+int mxa_kv4_append(const void *q, const long long *q_strides, int q_heads, const void *q_weight,
+                   const void *k, const long long *k_strides, const void *k_weight, const void *v,
+                   const long long *v_strides, float eps, const void *positions, int positions_int64,
+                   long long pos_batch, long long pos_token, const double *turns, int n_tokens,
+                   int seq_len, int rotary_dim, int interleaved, float scale, int bf16, void *pages,
+                   int n_pages, int kv_heads, int page_size, int head_dim, const int32_t *table,
+                   long long table_stride, int table_width, const int32_t *lengths,
+                   const int32_t *query_starts, int n_seq, void *q_out, void *stream);
+
+/* The keys and values that the call's rows are held as: (n_tokens, kv_heads, head_dim) each, float32 or bfloat16
+ * (bf16 != 0), rounded once; zeros for what is not cached and for rows of no sequence. */
+int mxa_kv4_read(const void *pages, int n_pages, int kv_heads, int page_size, int head_dim,
+                 const int32_t *table, long long table_stride, int table_width, const int32_t *lengths,
+                 const int32_t *query_starts, int n_seq, int n_tokens, int bf16, void *k_out,
+                 void *v_out, void *stream);
+
+/* Causal attention of the call's rows (bfloat16 q, strides as mxa_rope's) over the cache: out (n_tokens, q_heads,
+ * head_dim) bfloat16, contiguous, = sum p v / sum p with p = exp(scale * q . k) over the places up to the row's own, the
+ * last `window` of them if that is positive. Query head h reads key head h / (q_heads / kv_heads). A row that attends to
+ * nothing is zeros; rows of no sequence are left as they were. max_length: a bound on the lengths by which the work is
+ * shared out (a longer sequence is right, and slower). workspace: mxa_kv4_attend_workspace_bytes, 16-byte aligned
+ * (ragged: whether query_starts is given); it holds nothing between calls.
+ * Replaces the reference's decode attention (app/native/src/mx_attention.c) for GPU layers on a 4-bit cache. */
+size_t mxa_kv4_attend_workspace_bytes(int n_seq, int n_tokens, int ragged, int q_heads, int kv_heads,
+                                      int head_dim, int max_length, int window);
+int mxa_kv4_attend(const void *q, const long long *q_strides, int q_heads, int n_tokens, int seq_len,
+                   const void *pages, int n_pages, int kv_heads, int page_size, int head_dim,
+                   const int32_t *table, long long table_stride, int table_width,
+                   const int32_t *lengths, const int32_t *query_starts, int n_seq, int max_length,
+                   int window, float scale, void *out, void *workspace, size_t workspace_bytes,
+                   void *stream);
+
 /* Q8_K activation quantization of x (n_tokens, in_features) into the workspace layout
  * q int8 (n_tokens, K) | d fp32 (n_tokens, K/256) | bsums int16 (n_tokens, K/256, 16), each
  * part starting on a 256-byte boundary (see mxa_workspace_bytes).

@@ -43,6 +43,12 @@ EXPORTS = (
     "mxa_silu_mul_q8_k",
     "mxa_add_rms_norm_q8_k",
     "mxa_rope",
+    "mxa_norm_rope",
+    "mxa_kv4_page_bytes",
+    "mxa_kv4_append",
+    "mxa_kv4_read",
+    "mxa_kv4_attend_workspace_bytes",
+    "mxa_kv4_attend",
     "mxa_dequantize",
     "mxa_dequant_rows",
     "mxa_embed_rows",
@@ -158,6 +164,21 @@ def load() -> ctypes.CDLL:
     lib.mxa_rope.argtypes = [_vp, _vp, _i, _vp, _vp, _i, _vp, _i, _ll, _ll, _vp, _i, _i, _i, _i, _i, _f, _i, _vp, _vp,
                              _vp]
     lib.mxa_rope.restype = _i
+    lib.mxa_norm_rope.argtypes = [_vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _f, _vp, _i, _ll, _ll, _vp, _i, _i, _i, _i, _i, _f,
+                                  _i, _vp, _vp, _vp]
+    lib.mxa_norm_rope.restype = _i
+    lib.mxa_kv4_page_bytes.argtypes = [_i, _i, _i]
+    lib.mxa_kv4_page_bytes.restype = _sz
+    lib.mxa_kv4_append.argtypes = [_vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _vp, _f, _vp, _i, _ll, _ll, _vp, _i, _i, _i, _i,
+                                   _f, _i, _vp, _i, _i, _i, _i, _vp, _ll, _i, _vp, _vp, _i, _vp, _vp]
+    lib.mxa_kv4_append.restype = _i
+    lib.mxa_kv4_read.argtypes = [_vp, _i, _i, _i, _i, _vp, _ll, _i, _vp, _vp, _i, _i, _i, _vp, _vp, _vp]
+    lib.mxa_kv4_read.restype = _i
+    lib.mxa_kv4_attend_workspace_bytes.argtypes = [_i] * 8
+    lib.mxa_kv4_attend_workspace_bytes.restype = _sz
+    lib.mxa_kv4_attend.argtypes = [_vp, _vp, _i, _i, _i, _vp, _i, _i, _i, _i, _vp, _ll, _i, _vp, _vp, _i, _i, _i, _f, _vp,
+                                   _vp, _sz, _vp]
+    lib.mxa_kv4_attend.restype = _i
     lib.mxa_dequantize.argtypes = [_i, _vp, _ll, _vp, _vp]
     lib.mxa_dequantize.restype = _i
     lib.mxa_dequant_rows.argtypes = [_i, _vp, _ll, _vp, _i, _i, _vp, _vp]

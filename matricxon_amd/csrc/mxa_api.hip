@@ -4,6 +4,7 @@
 #include <string.h>
 
 #include "../../include/matricxon_amd.h"
+#include "mxa_attend.hpp"
 #include "mxa_kernels.hpp"
 
 namespace {
@@ -39,6 +40,28 @@ int block_bytes(int t) {
     case MXA_TYPE_IQ4_XS: return 136;
     default: return 0;
   }
+}
+
+bool aligned(const void* p, uintptr_t a);
+
+bool kv4_supported(int kv_heads, int page_size, int head_dim) {
+  return kv_heads >= 1 && kv_heads <= 65535 && page_size >= mxa::kKvBlock && page_size % mxa::kKvBlock == 0 &&
+         page_size <= MXA_KV4_MAX_PAGE && head_dim >= 8 && head_dim % 8 == 0 && head_dim <= MXA_KV4_MAX_DIM;
+}
+
+// The arguments of a call on the 4-bit cache; false where they do not fit together.
+bool kv4_pages(mxa::KvPages& kv, void* pages, int n_pages, int kv_heads, int page_size, int head_dim,
+               const int32_t* table, long long table_stride, int table_width, const int32_t* lengths,
+               const int32_t* query_starts, int n_seq, int n_tokens) {
+  if (!kv4_supported(kv_heads, page_size, head_dim) || pages == nullptr || table == nullptr || lengths == nullptr ||
+      n_pages < 1 || table_width < 1 || (long long)table_width * page_size > MXA_KV4_MAX_PLACES || n_seq < 1 ||
+      n_seq > MXA_KV4_MAX_SEQ || n_tokens < 1 || n_tokens > MXA_MAX_TOKENS || !aligned(pages, 16) ||
+      !aligned(table, 4) || !aligned(lengths, 4) || !aligned(query_starts, 4) ||
+      (query_starts == nullptr && n_tokens % n_seq != 0))
+    return false;
+  kv = mxa::KvPages{(uint8_t*)pages, table, lengths, query_starts, table_stride, n_pages, kv_heads, page_size,
+                    table_width, n_seq, n_tokens / n_seq};
+  return true;
 }
 
 bool needs_q8k(int t) { return t != MXA_TYPE_IQ4_XS; }
@@ -682,6 +705,107 @@ int mxa_rope(const void* q, const long long* q_strides, int q_heads, const void*
                        pos_token, turns, n_tokens, seq_len, head_dim, rotary_dim, interleaved != 0, scale,
                        bf16 != 0, q_out, k_out, (hipStream_t)stream) != 0)
     return MXA_ERR_UNSUPPORTED;
+  return check_launch();
+}
+
+int mxa_norm_rope(const void* q, const long long* q_strides, int q_heads, const void* q_weight, const void* k,
+                  const long long* k_strides, int k_heads, const void* k_weight, float eps, const void* positions,
+                  int positions_int64, long long pos_batch, long long pos_token, const double* turns, int n_tokens,
+                  int seq_len, int head_dim, int rotary_dim, int interleaved, float scale, int bf16, void* q_out,
+                  void* k_out, void* stream) {
+  const uintptr_t ea = bf16 ? 2 : 4;
+  if (q == nullptr || q_strides == nullptr || q_out == nullptr || positions == nullptr || turns == nullptr ||
+      q_heads < 1 || k_heads < 0 || q_heads > MXA_ROPE_MAX_HEADS || k_heads > MXA_ROPE_MAX_HEADS || n_tokens < 1 ||
+      n_tokens > MXA_MAX_TOKENS || seq_len < 1 || head_dim < 2 || head_dim > MXA_ROPE_MAX_DIM || head_dim % 2 != 0 ||
+      rotary_dim < 2 || rotary_dim > head_dim || rotary_dim % 2 != 0 || !aligned(q, ea) || !aligned(q_out, ea) ||
+      !aligned(q_weight, ea) || !aligned(positions, positions_int64 ? 8 : 4) || !aligned(turns, 8))
+    return MXA_ERR_UNSUPPORTED;
+  if (k_heads > 0 && (k == nullptr || k_strides == nullptr || k_out == nullptr || !aligned(k, ea) ||
+                      !aligned(k_out, ea) || !aligned(k_weight, ea)))
+    return MXA_ERR_UNSUPPORTED;
+  if (mxa::launch_heads(q, q_strides, q_heads, q_weight, k, k_strides, k_heads, k_weight, eps, positions,
+                        positions_int64 != 0, pos_batch, pos_token, turns, n_tokens, seq_len, head_dim, rotary_dim,
+                        interleaved != 0, scale, bf16 != 0, q_out, k_out, (hipStream_t)stream) != 0)
+    return MXA_ERR_UNSUPPORTED;
+  return check_launch();
+}
+
+size_t mxa_kv4_page_bytes(int kv_heads, int page_size, int head_dim) {
+  if (!kv4_supported(kv_heads, page_size, head_dim)) return 0;
+  return (size_t)kv_heads * (page_size / mxa::kKvBlock) * mxa::kv_block_bytes(mxa::kv_groups(head_dim));
+}
+
+int mxa_kv4_append(const void* q, const long long* q_strides, int q_heads, const void* q_weight, const void* k,
+                   const long long* k_strides, const void* k_weight, const void* v, const long long* v_strides,
+                   float eps, const void* positions, int positions_int64, long long pos_batch, long long pos_token,
+                   const double* turns, int n_tokens, int seq_len, int rotary_dim, int interleaved, float scale,
+                   int bf16, void* pages, int n_pages, int kv_heads, int page_size, int head_dim, const int32_t* table,
+                   long long table_stride, int table_width, const int32_t* lengths, const int32_t* query_starts,
+                   int n_seq, void* q_out, void* stream) {
+  const uintptr_t ea = bf16 ? 2 : 4;
+  mxa::KvPages kv;
+  if (!kv4_pages(kv, pages, n_pages, kv_heads, page_size, head_dim, table, table_stride, table_width, lengths,
+                 query_starts, n_seq, n_tokens))
+    return MXA_ERR_UNSUPPORTED;
+  if (k == nullptr || k_strides == nullptr || v == nullptr || v_strides == nullptr || !aligned(k, ea) ||
+      !aligned(v, ea) || !aligned(k_weight, ea) || q_heads < 0 || q_heads > MXA_ROPE_MAX_HEADS ||
+      q_heads % kv_heads != 0 || seq_len < 1 || rotary_dim < 0 || rotary_dim > head_dim || rotary_dim % 2 != 0 ||
+      (rotary_dim > 0 && turns == nullptr) || !aligned(turns, 8) || !aligned(positions, positions_int64 ? 8 : 4))
+    return MXA_ERR_UNSUPPORTED;
+  if (q_heads > 0 && (q == nullptr || q_strides == nullptr || q_out == nullptr || !aligned(q, ea) ||
+                      !aligned(q_out, ea) || !aligned(q_weight, ea)))
+    return MXA_ERR_UNSUPPORTED;
+  if (mxa::launch_kv4_append(q, q_strides, q_heads, q_weight, k, k_strides, k_weight, v, v_strides, eps, positions,
+                             positions_int64 != 0, pos_batch, pos_token, turns, n_tokens, seq_len, head_dim, rotary_dim,
+                             interleaved != 0, scale, bf16 != 0, kv, q_out, (hipStream_t)stream) != 0)
+    return MXA_ERR_UNSUPPORTED;
+  return check_launch();
+}
+
+int mxa_kv4_read(const void* pages, int n_pages, int kv_heads, int page_size, int head_dim, const int32_t* table,
+                 long long table_stride, int table_width, const int32_t* lengths, const int32_t* query_starts,
+                 int n_seq, int n_tokens, int bf16, void* k_out, void* v_out, void* stream) {
+  const uintptr_t ea = bf16 ? 2 : 4;
+  mxa::KvPages kv;
+  if (!kv4_pages(kv, (void*)pages, n_pages, kv_heads, page_size, head_dim, table, table_stride, table_width, lengths,
+                 query_starts, n_seq, n_tokens) ||
+      k_out == nullptr || v_out == nullptr || !aligned(k_out, ea) || !aligned(v_out, ea))
+    return MXA_ERR_UNSUPPORTED;
+  if (mxa::launch_kv4_read(kv, n_tokens, head_dim, bf16 != 0, k_out, v_out, (hipStream_t)stream) != 0)
+    return MXA_ERR_UNSUPPORTED;
+  return check_launch();
+}
+
+size_t mxa_kv4_attend_workspace_bytes(int n_seq, int n_tokens, int ragged, int q_heads, int kv_heads, int head_dim,
+                                      int max_length, int window) {
+  if (n_seq < 1 || n_tokens < 1 || (!ragged && n_tokens % n_seq != 0) || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads != 0 ||
+      head_dim < 8 || head_dim > mxa::kKvMaxDim || max_length < 1 || window < 0)
+    return 0;
+  return mxa::attend_workspace(n_seq, kv_heads, q_heads / kv_heads, ragged ? n_tokens : n_tokens / n_seq, max_length,
+                               window, head_dim);
+}
+
+int mxa_kv4_attend(const void* q, const long long* q_strides, int q_heads, int n_tokens, int seq_len,
+                   const void* pages, int n_pages, int kv_heads, int page_size, int head_dim, const int32_t* table,
+                   long long table_stride, int table_width, const int32_t* lengths, const int32_t* query_starts,
+                   int n_seq, int max_length, int window, float scale, void* out, void* workspace,
+                   size_t workspace_bytes, void* stream) {
+  mxa::AttendArgs a{};
+  if (!kv4_pages(a.kv, (void*)pages, n_pages, kv_heads, page_size, head_dim, table, table_stride, table_width, lengths,
+                 query_starts, n_seq, n_tokens) ||
+      q == nullptr || q_strides == nullptr || out == nullptr || !aligned(q, 2) || !aligned(out, 2) || q_heads < 1 ||
+      q_heads > MXA_ROPE_MAX_HEADS || q_heads % kv_heads != 0 || seq_len < 1 || max_length < 1 || window < 0)
+    return MXA_ERR_UNSUPPORTED;
+  const size_t need = mxa_kv4_attend_workspace_bytes(n_seq, n_tokens, query_starts != nullptr, q_heads, kv_heads, head_dim,
+                                                     max_length, window);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return MXA_ERR_WORKSPACE;
+  if (need > 0 && !aligned(workspace, 16)) return MXA_ERR_UNSUPPORTED;
+  a.q = (const uint16_t*)q;
+  a.q_batch = q_strides[0], a.q_tok = q_strides[1], a.q_head = q_strides[2];
+  a.out = (uint16_t*)out;
+  a.n_tokens = n_tokens, a.seq = seq_len, a.dim = head_dim, a.heads = q_heads, a.group = q_heads / kv_heads;
+  a.window = window < MXA_KV4_MAX_PLACES ? window : MXA_KV4_MAX_PLACES, a.scale = scale;
+  if (mxa::launch_attend(a, query_starts != nullptr ? n_tokens : n_tokens / n_seq, max_length, workspace, (hipStream_t)stream) != 0) return MXA_ERR_UNSUPPORTED;
   return check_launch();
 }
 

@@ -105,6 +105,16 @@ def _head_strides(x: torch.Tensor, nd: int) -> tuple[torch.Tensor, ctypes.Array]
     return x, _Strides3(0, st[0], st[1]) if nd == 3 else _Strides3(st[0], st[1], st[2])
 
 
+def _head_weight(name: str, w: torch.Tensor | None, dim: int, dt: torch.dtype, dev: torch.device
+                 ) -> torch.Tensor | None:
+    """The weight of a head's norm, contiguous (ValueError where it does not fit)."""
+    if w is None:
+        return None
+    if w.dtype is not dt or w.device != dev or w.shape != (dim,):
+        raise ValueError(f"{name} must be {dt} ({dim},) on {dev}, got {w.dtype} {tuple(w.shape)} on {w.device}")
+    return w if w.is_contiguous() else w.contiguous()
+
+
 def _weight_arrays(items: list[tuple[int, torch.Tensor, int]], outs: list[int]):
     """The types, weight addresses and output widths of a group as the library's host arrays."""
     n = len(items)
@@ -548,8 +558,9 @@ class HipGemm:
         return self._rope(q, k, positions, turns, rotary_dim, interleaved, scale)
 
     def _rope(self, q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, turns: torch.Tensor,
-              rotary_dim: int, interleaved: bool, scale: float) -> tuple[torch.Tensor, torch.Tensor | None]:
-        """`rope` with a table of q's device."""
+              rotary_dim: int, interleaved: bool, scale: float, norms: tuple | None = None
+              ) -> tuple[torch.Tensor, torch.Tensor | None]:
+        """`rope` with a table of q's device; norms: (q_weight, k_weight, eps) of `mxa_norm_rope`."""
         dev, dt, shape = q.device, q.dtype, q.shape
         nd = len(shape)
         if dt not in _FLOATS or nd not in (3, 4):
@@ -579,9 +590,15 @@ class HipGemm:
         n_tokens = seq if nd == 3 else shape[0] * seq
         if n_tokens > self.MAX_TOKENS:
             raise ValueError(f"q must have up to {self.MAX_TOKENS} tokens, got {tuple(shape)}")
+        if norms is not None:
+            qw, kw, eps = norms
+            if kw is not None and k is None:
+                raise ValueError("k_weight needs k")
+            qw, kw = _head_weight("q_weight", qw, dim, dt, dev), _head_weight("k_weight", kw, dim, dt, dev)
+            norms = qw, kw, eps
         if _elsewhere(dev):
             with torch.cuda.device(dev):
-                return self._rope(q, k, positions, turns, rotary_dim, interleaved, scale)
+                return self._rope(q, k, positions, turns, rotary_dim, interleaved, scale, norms)
         q, q_strides = _head_strides(q, nd)
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
         k_ptr, k_strides, k_out, k_out_ptr = 0, None, None, 0
@@ -590,6 +607,15 @@ class HipGemm:
             k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
             k_ptr, k_out_ptr = k.data_ptr(), k_out.data_ptr()
         if n_tokens == 0:
+            return q_out, k_out
+        if norms is not None:
+            status = self._lib.mxa_norm_rope(
+                q.data_ptr(), q_strides, heads, 0 if qw is None else qw.data_ptr(), k_ptr, k_strides, k_heads,
+                0 if kw is None else kw.data_ptr(), eps, positions.data_ptr(), positions.dtype is torch.int64, pos_batch,
+                pst[-1], turns.data_ptr(), n_tokens, seq, dim, rotary_dim, interleaved, scale, dt is torch.bfloat16,
+                q_out.data_ptr(), k_out_ptr, _stream(dev))
+            if status != 0:
+                self._check(status, "mxa_norm_rope", 0)
             return q_out, k_out
         status = self._lib.mxa_rope(
             q.data_ptr(), q_strides, heads, k_ptr, k_strides, k_heads, positions.data_ptr(),

@@ -118,12 +118,19 @@ class HipRotary:
             table = self._turns[device] = (self.frequencies / (2 * math.pi)).to(device)
         return table
 
-    def __call__(self, q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor
+    def __call__(self, q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor, *,
+                 q_weight: torch.Tensor | None = None, k_weight: torch.Tensor | None = None, eps: float = 1e-6
                  ) -> tuple[torch.Tensor, torch.Tensor | None]:
         """q (T, heads, head_dim) or (B, T, heads, head_dim) and k likewise, of its own number of heads (or None), of
         any strides with adjacent values in a head, as the columns of a q | k | v buffer; positions int32 or int64
         (T,), or (B, T) for a batch. Returns new contiguous tensors of those shapes and that dtype, float32 or
-        bfloat16. Any position, negative ones turning back."""
+        bfloat16. Any position, negative ones turning back.
+
+        With `q_weight` or `k_weight` ((head_dim,) of q's dtype) the heads of that side are normed first, in the same
+        pass: x * weight / sqrt(mean(x^2) + eps) over a head's values, rounded once behind the rotation."""
+        if q_weight is not None or k_weight is not None:
+            return self._gemm._rope(q, k, positions, self._table(q.device), self.rotary_dim, self.interleaved,
+                                    self.scale, (q_weight, k_weight, float(eps)))
         return self._gemm._rope(q, k, positions, self._table(q.device), self.rotary_dim, self.interleaved, self.scale)
 
     def shift(self, k: torch.Tensor, delta: torch.Tensor) -> torch.Tensor:
