@@ -12,6 +12,8 @@
 // so nothing but the row's maximum crosses lanes. Codes are widened in registers, code to float16 exactly (an or of its
 // bits into a float16's, less that float16), then s * code + m rounded once; q is brought by a power of two into float16's
 // range, exactly but for values below 2^-24 of its largest. Scores, maxima, sums and outputs are float32.
+#include <algorithm>
+
 #include "mxa_attend.hpp"
 #include "mxa_kernels.hpp"
 
@@ -22,25 +24,28 @@ namespace {
 
 constexpr int kAttendThreads = 256, kAttendWaves = kAttendThreads / 64;
 
-// W groups of 32 values a head. Workgroup (split, key head and row tile, sequence): `chunk` blocks of 32 tokens, which its
-// waves take in turn and join in LDS; more than one split: unnormalised outputs, maxima and sums into `part`.
+// W groups of 32 values a head. Workgroup (split, pair, sequence) takes a split's blocks of a pair, which its waves take in
+// turn; their parts are joined in LDS, and the parts of a pair of several splits go to the workspace.
 template <int W>
-__global__ __launch_bounds__(kAttendThreads) void attend_kernel(AttendArgs a) {
+__global__ __launch_bounds__(kAttendThreads, W <= 4 ? 3 : 2) void attend_kernel(AttendArgs a) {
+  constexpr int AHEAD = W <= 3 ? 3 : 2;  // blocks of a wave in registers, all but one of them on their way
   __shared__ __align__(16) uint32_t scales[kAttendWaves][64 * W];
   __shared__ float o_join[kAttendWaves][16][32 * W + 4];
   __shared__ float m_join[kAttendWaves][16], l_join[kAttendWaves][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
   const int split = blockIdx.x, h = blockIdx.y % a.kv.heads, rt = blockIdx.y / a.kv.heads, b = blockIdx.z;
-  RowTile tile;
-  if (!tile.find(a, b, rt)) return;
-  if (split > 0 && split >= tile.used) return;
-  const int begin = tile.first_block + split * tile.chunk, end = min(begin + tile.chunk, tile.end_block);
+  const Sequence seq(a, b);
+  if (rt >= seq.tiles || split >= seq.splits) return;
+  const int begin = split * seq.chunk, end = min(begin + seq.chunk, seq.blocks);
+  const int blocks_of_page = a.kv.page / kKvBlock;
+  const CodeBits bits;
+  uint32_t* const sc = scales[wave];
 
   const int row = rt * 16 + n;  // the lane's row
-  const bool live = row < tile.rows;
-  const int place = tile.place0 + (live ? row / a.group : 0);
-  const int limit = live ? min(place + 1, tile.length) : 0, low = a.window > 0 ? max(place + 1, 0) - a.window : 0;
+  const bool live = row < seq.rows;
+  const int place = seq.place0 + (live ? row / a.group : 0);
+  const int limit = live ? min(place + 1, seq.length) : 0, low = a.window > 0 ? max(place + 1, 0) - a.window : 0;
 
   // q, by a power of two
   half8 q[W];
@@ -48,7 +53,7 @@ __global__ __launch_bounds__(kAttendThreads) void attend_kernel(AttendArgs a) {
   {
     float qf[W][8];
     float top = 0.0f;
-    const uint16_t* const src = a.q_row(tile.first + (live ? row / a.group : 0), h * a.group + (live ? row % a.group : 0));
+    const uint16_t* const src = a.q_row(seq.first + (live ? row / a.group : 0), h * a.group + (live ? row % a.group : 0));
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       const bool here = live && 32 * w + 8 * g < a.dim;
@@ -71,53 +76,94 @@ __global__ __launch_bounds__(kAttendThreads) void attend_kernel(AttendArgs a) {
   f32x4 o[2 * W];
 #pragma unroll
   for (int i = 0; i < 2 * W; ++i) o[i] = f32x4{0, 0, 0, 0};
-  float m = -INFINITY, l = 0.0f;
-  uint32_t* const sc = scales[wave];
-  const int blocks = a.kv.page / kKvBlock;
+  float m = -INFINITY, l = 0.0f;  // the row's reference (its maximum, or up to kSlack below) and the lane's sum
+  // places that every row of the tile attends to, but for rows that there are not
+  const int last_row = min(rt * 16 + 15, seq.rows - 1);
+  const int inside_lo = a.window > 0 ? max(seq.place0 + last_row / a.group + 1, 0) - a.window : 0;
+  const int inside_hi = min(seq.place0 + rt * 16 / a.group + 1, seq.length);
 
-  for (int u = begin + wave; u < end; u += kAttendWaves) {
-    const long long block = kv_block(a.kv, b, u * kKvBlock);
-    if (block < 0) continue;
-    const uint8_t* const blk = a.kv.pages + (block + (long long)h * blocks) * kv_block_bytes(W);
-    uint32_t kc[2][W], vc[W][2];
-    load_block<W>(blk, lane, kc, vc, sc);
-    if ((u + 1) * kKvBlock > tile.length) clear_tail<W>(sc, lane, tile.length - u * kKvBlock);
+  // The wave's blocks are begin + wave, + 4, ..; lane i finds where the i-th of 64 of them lies, so that no block's
+  // address waits for the page table.
+  long long where = -1;
+  int looked = 64;
+  BlockPart<W> part[AHEAD];
+  bool has[AHEAD];
+  const auto request = [&](BlockPart<W>& p, bool& there, int u) {
+    if (looked == 64) {
+      looked = 0;
+      const int mine = u + lane * kAttendWaves;
+      const long long block = mine < end ? kv_block(a.kv, b, (seq.first_block + mine) * kKvBlock) : -1;
+      where = block < 0 ? -1 : (block + (long long)h * blocks_of_page) * kv_block_bytes(W);
+    }
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)where, looked);
+    const uint32_t hi = __builtin_amdgcn_readlane((int)(where >> 32), looked);
+    ++looked;
+    there = (int)hi >= 0;
+    if (there) p.load(a.kv.pages + ((uint64_t)hi << 32 | lo), lane);
+  };
+  const auto compute = [&](const BlockPart<W>& p_, int u) {
+    const int first = (seq.first_block + u) * kKvBlock;
+    p_.share(sc, lane);
+    const bool inside = first >= inside_lo && first + kKvBlock <= inside_hi;
+    if (first + kKvBlock > seq.length) clear_tail<W>(sc, lane, seq.length - first);
     float s[8];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       f32x4 acc = f32x4{0, 0, 0, 0};
 #pragma unroll
       for (int w = 0; w < W; ++w)
-        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen8(kc[i][w], sc[(i * 16 + n) * W + w]), q[w], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen8(bits, p_.kc[i][w], sc[(i * 16 + n) * W + w]), q[w], acc, 0, 0, 0);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int t = u * kKvBlock + i * 16 + g * 4 + j;
-        s[i * 4 + j] = t < limit && t >= low ? acc[j] * back : -INFINITY;
+      for (int j = 0; j < 4; ++j) s[i * 4 + j] = acc[j] * back;
+    }
+    if (!inside) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int t = first + j / 4 * 16 + g * 4 + j % 4;
+        if (t >= limit || t < low) s[j] = -INFINITY;
       }
     }
-    float top = s[0];
+    float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+    if (__any(top > m + kSlack)) {  // the row's first places among them: its reference is -inf
+      top = fmaxf(top, __shfl_xor(top, 16));
+      top = fmaxf(top, __shfl_xor(top, 32));
+      const float m2 = fmaxf(m, top);
+      const float alpha = m2 == -INFINITY ? 1.0f : exp2_(m - m2);
+      m = m2;
+      l *= alpha;
 #pragma unroll
-    for (int j = 1; j < 8; ++j) top = fmaxf(top, s[j]);
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
-    const float m2 = fmaxf(m, top), ref = m2 == -INFINITY ? 0.0f : m2;
-    const float alpha = exp2_(m - ref);
-    m = m2;
+      for (int i = 0; i < 2 * W; ++i) o[i] *= alpha;
+    }
+    const float ref = (m == -INFINITY ? 0.0f : m) - kProbShift;
     float p[8], sum = 0.0f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      p[j] = exp2_(s[j] - ref + kProbShift);
+      p[j] = exp2_(s[j] - ref);
       sum += p[j];
     }
-    l = l * alpha + sum;
+    l += sum;
     const half8 ph = prob_order(p);
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       half8 v0, v1;
-      value_operands(vc[w], *(const u32x4*)(sc + 32 * W + (w * 8 + g) * 4), *(const u32x4*)(sc + 32 * W + (w * 8 + 4 + g) * 4),
-                     v0, v1);
-      o[2 * w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph, o[2 * w] * alpha, 0, 0, 0);
-      o[2 * w + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph, o[2 * w + 1] * alpha, 0, 0, 0);
+      value_operands(bits, p_.vc[w], *(const u32x4*)(sc + 32 * W + (w * 8 + g) * 4),
+                     *(const u32x4*)(sc + 32 * W + (w * 8 + 4 + g) * 4), v0, v1);
+      o[2 * w] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph, o[2 * w], 0, 0, 0);
+      o[2 * w + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph, o[2 * w + 1], 0, 0, 0);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  };
+  int u = begin + wave;
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (u + i * kAttendWaves < end) request(part[i], has[i], u + i * kAttendWaves);
+  while (u < end) {
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      if (u >= end) break;
+      if (has[i]) compute(part[i], u);
+      if (u + AHEAD * kAttendWaves < end) request(part[i], has[i], u + AHEAD * kAttendWaves);
+      u += kAttendWaves;
     }
   }
   l += __shfl_xor(l, 16);
@@ -136,103 +182,118 @@ __global__ __launch_bounds__(kAttendThreads) void attend_kernel(AttendArgs a) {
     l_join[wave][n] = l;
   }
   __syncthreads();
-  const int rows = min(16, tile.rows - rt * 16);
   const int r = threadIdx.x >> 4, piece = threadIdx.x & 15;  // sixteen threads a row
-  if (r >= rows) return;
-  float top = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < kAttendWaves; ++i) top = fmaxf(top, m_join[i][r]);
-  const float ref = top == -INFINITY ? 0.0f : top;
-  float f[kAttendWaves], total = 0.0f;
-#pragma unroll
-  for (int i = 0; i < kAttendWaves; ++i) {
-    f[i] = exp2_(m_join[i][r] - ref);
-    total += f[i] * l_join[i][r];
-  }
-  const bool alone = tile.used <= 1;
-  const float norm = alone ? (total > 0.0f || total != total ? 1.0f / total : 0.0f) : 1.0f;
-  const AttendPart part = a.part_of(b, h, rt, split, W);
-  uint16_t* const dst = a.out_row(tile.first + (rt * 16 + r) / a.group, h * a.group + (rt * 16 + r) % a.group);
-  if (!alone && piece == 0) {
-    part.ml[r] = top;
-    part.ml[16 + r] = total;
-  }
-  for (int d = piece; d < a.dim; d += 16) {
-    float v = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kAttendWaves; ++i) v += f[i] * o_join[i][r][d];
-    if (alone)
-      dst[d] = bf16_rne(v * norm);
-    else
-      part.o[r * 32 * W + d] = v;
-  }
-}
-
-// The splits' parts joined; rows of one split are written already.
-__global__ __launch_bounds__(kAttendThreads) void attend_join_kernel(AttendArgs a, int W) {
-  __shared__ float f[16][kAttendMaxSplits];
-  __shared__ float norm[16];
-  const int h = blockIdx.y % a.kv.heads, rt = blockIdx.y / a.kv.heads, b = blockIdx.z;
-  RowTile tile;
-  if (!tile.find(a, b, rt)) return;
-  const int used = tile.used;
-  if (used <= 1) return;
-  const int rows = min(16, tile.rows - rt * 16);
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (int r = wave; r < rows; r += kAttendWaves) {
+  if (r < min(16, seq.rows - rt * 16)) {
     float top = -INFINITY;
-    for (int s = lane; s < used; s += 64) top = fmaxf(top, a.part_of(b, h, rt, s, W).ml[r]);
-    for (int i = 1; i < 64; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
+#pragma unroll
+    for (int i = 0; i < kAttendWaves; ++i) top = fmaxf(top, m_join[i][r]);
     const float ref = top == -INFINITY ? 0.0f : top;
-    float total = 0.0f;
-    for (int s = lane; s < used; s += 64) {
-      const AttendPart p = a.part_of(b, h, rt, s, W);
-      const float e = exp2_(p.ml[r] - ref);
-      f[r][s] = e;
-      total += e * p.ml[16 + r];
+    float f[kAttendWaves], total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kAttendWaves; ++i) {
+      f[i] = exp2_(m_join[i][r] - ref);
+      total += f[i] * l_join[i][r];
     }
-    for (int i = 1; i < 64; i *= 2) total += __shfl_xor(total, i);
-    if (lane == 0) norm[r] = total > 0.0f || total != total ? 1.0f / total : 0.0f;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < rows * a.dim; i += kAttendThreads) {
-    const int r = i / a.dim, d = i - r * a.dim;
-    float v = 0.0f;
-    for (int s = 0; s < used; ++s) v += f[r][s] * a.part_of(b, h, rt, s, W).o[r * 32 * W + d];
-    a.out_row(tile.first + (rt * 16 + r) / a.group, h * a.group + (rt * 16 + r) % a.group)[d] = bf16_rne(v * norm[r]);
+    const bool whole = seq.splits == 1;
+    const float norm = total > 0.0f || total != total ? 1.0f / total : 0.0f;
+    const AttendPart to = a.part_of(b, blockIdx.y, split, W);
+    uint16_t* const dst = a.out_row(seq.first + (rt * 16 + r) / a.group, h * a.group + (rt * 16 + r) % a.group);
+    if (!whole && piece == 0) {
+      to.ml[r] = top;
+      to.ml[16 + r] = total;
+    }
+    for (int d = piece; d < a.dim; d += 16) {
+      float v = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kAttendWaves; ++i) v += f[i] * o_join[i][r][d];
+      if (whole)
+        dst[d] = bf16_rne(v * norm);
+      else
+        to.o[r * 32 * W + d] = v;
+    }
   }
 }
 
-// Row tiles, splits and blocks a split for up to `most` rows a key head and max_length tokens.
+// The parts of each pair of several splits, joined: a workgroup takes a row of a pair, its threads parts and vectors of
+// four values.
+__global__ __launch_bounds__(kAttendThreads) void attend_join_kernel(AttendArgs a, int W) {
+  __shared__ float f[kAttendMaxSplits];
+  __shared__ f32x4 sums[kAttendThreads];
+  __shared__ float wave_max[kAttendWaves], wave_sum[kAttendWaves];
+  const int b = blockIdx.z, r = blockIdx.x, pair = blockIdx.y, tid = threadIdx.x;
+  const int h = pair % a.kv.heads, rt = pair / a.kv.heads;
+  const Sequence seq(a, b);
+  const int parts = seq.splits;
+  if (rt * 16 + r >= seq.rows || parts == 1) return;
+  float top = -INFINITY, total = 0.0f;
+  for (int i = tid; i < parts; i += kAttendThreads) top = fmaxf(top, a.part_of(b, pair, i, W).ml[r]);
+  for (int i = 1; i < 64; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
+  if ((tid & 63) == 0) wave_max[tid >> 6] = top;
+  __syncthreads();
+  for (int i = 0; i < kAttendWaves; ++i) top = fmaxf(top, wave_max[i]);
+  const float ref = top == -INFINITY ? 0.0f : top;
+  for (int i = tid; i < parts; i += kAttendThreads) {
+    const AttendPart p = a.part_of(b, pair, i, W);
+    f[i] = exp2_(p.ml[r] - ref);
+    total += f[i] * p.ml[16 + r];
+  }
+  for (int i = 1; i < 64; i *= 2) total += __shfl_xor(total, i);
+  if ((tid & 63) == 0) wave_sum[tid >> 6] = total;
+  __syncthreads();
+  const int vectors = a.dim / 4, side = kAttendThreads / vectors, mine = tid / vectors, at = tid - mine * vectors;
+  f32x4 v{0, 0, 0, 0};
+  if (mine < side) {
+#pragma unroll 4
+    for (int i = mine; i < parts; i += side) v += f[i] * *(const f32x4*)(a.part_of(b, pair, i, W).o + r * 32 * W + 4 * at);
+  }
+  sums[tid] = v;
+  __syncthreads();
+  if (tid >= vectors) return;
+  total = 0.0f;
+  for (int i = 0; i < kAttendWaves; ++i) total += wave_sum[i];
+  for (int i = 1; i < side; ++i) v += sums[i * vectors + tid];
+  const float norm = total > 0.0f || total != total ? 1.0f / total : 0.0f;
+  uint16_t* const dst = a.out_row(seq.first + (rt * 16 + r) / a.group, h * a.group + (rt * 16 + r) % a.group);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) dst[4 * tid + j] = bf16_rne(v[j] * norm);
+}
+
+// (std::min and std::max here: on the host, HIP's own of that name take ints.)
+// How the blocks of up to `most` tokens of each sequence are shared out.
 struct Plan {
-  int tiles, splits, chunk;
+  long long pairs;  // of a sequence
+  int splits, chunk;
 };
-Plan plan_of(int n_seq, int kv_heads, int group, int most, int max_length, int window) {
+Plan plan_of(int n_seq, int kv_heads, int group, int most, int max_length, int window, int dim) {
   Plan p;
-  p.tiles = (int)(((long long)most * group + 15) / 16);
-  const int reach = window > 0 ? (int)min((long long)max_length, (long long)window + most) : max_length;
-  const int blocks = reach / kKvBlock + 2;
-  const long long groups = (long long)n_seq * kv_heads * p.tiles;
-  const long long want = max(1LL, min((long long)kAttendMaxSplits, 1024 / groups));
-  p.chunk = max(kAttendWaves, (int)((blocks + want - 1) / want));
-  p.splits = min(kAttendMaxSplits, (blocks + p.chunk - 1) / p.chunk);
+  p.pairs = (((long long)most * group + 15) / 16) * kv_heads;
+  const long long slots = 256 * (kv_groups(dim) <= 4 ? 3 : 2);  // workgroups that the CUs hold at once
+  const long long reach = window > 0 ? std::min<long long>(max_length, (long long)window + most) : max_length;
+  const long long blocks = reach / kKvBlock + 2;
+  // one sequence: what the CUs hold at once; several, whose lengths are not known: four times that, in parts small enough
+  // to even out
+  const long long want = std::max<long long>(1, (n_seq > 1 ? 4 * slots : slots) / (p.pairs * n_seq));
+  p.chunk = (int)std::max<long long>(kAttendWaves, (blocks + want - 1) / want);
+  p.splits = (int)std::min<long long>(kAttendMaxSplits, (blocks + p.chunk - 1) / p.chunk);
   return p;
 }
 
 }  // namespace
 
 size_t attend_workspace(int n_seq, int kv_heads, int group, int most, int max_length, int window, int dim) {
-  const Plan p = plan_of(n_seq, kv_heads, group, most, max_length, window);
+  const Plan p = plan_of(n_seq, kv_heads, group, most, max_length, window, dim);
   if (p.splits <= 1) return 0;
-  return (size_t)n_seq * kv_heads * p.tiles * p.splits * part_floats(kv_groups(dim)) * sizeof(float);
+  return (size_t)n_seq * p.pairs * p.splits * part_floats(kv_groups(dim)) * sizeof(float);
 }
 
 int launch_attend(AttendArgs a, int most, int max_length, void* workspace, hipStream_t stream) {
-  const Plan p = plan_of(a.kv.n_seq, a.kv.heads, a.group, most, max_length, a.window);
-  if ((long long)a.kv.heads * p.tiles > 65535 || a.kv.n_seq > 65535) return -1;
-  a.tiles = p.tiles, a.splits = p.splits, a.chunk = p.chunk, a.part = (float*)workspace;
-  const dim3 grid(p.splits, a.kv.heads * p.tiles, a.kv.n_seq);
-  switch (kv_groups(a.dim)) {
+  const Plan p = plan_of(a.kv.n_seq, a.kv.heads, a.group, most, max_length, a.window, a.dim);
+  if (p.pairs > 65535) return -1;
+  const int W = kv_groups(a.dim);
+  a.most_rows = 0x7fffffff;
+  a.pairs = (int)p.pairs, a.splits = p.splits, a.chunk = p.chunk, a.part = (float*)workspace;
+  const dim3 grid(p.splits, a.pairs, a.kv.n_seq);
+  switch (W) {
 #define MXA_CASE(W) \
   case W: hipLaunchKernelGGL(attend_kernel<W>, grid, dim3(kAttendThreads), 0, stream, a); break;
     MXA_CASE(1) MXA_CASE(2) MXA_CASE(3) MXA_CASE(4) MXA_CASE(5) MXA_CASE(6) MXA_CASE(7) MXA_CASE(8)
@@ -240,8 +301,8 @@ int launch_attend(AttendArgs a, int most, int max_length, void* workspace, hipSt
     default: return -1;
   }
   if (p.splits > 1)
-    hipLaunchKernelGGL(attend_join_kernel, dim3(1, a.kv.heads * p.tiles, a.kv.n_seq), dim3(kAttendThreads), 0, stream, a,
-                       kv_groups(a.dim));
+    hipLaunchKernelGGL(attend_join_kernel, dim3((unsigned)std::min<long long>((long long)most * a.group, 16), a.pairs, a.kv.n_seq),
+                       dim3(kAttendThreads), 0, stream, a, W);
   return 0;
 }
 

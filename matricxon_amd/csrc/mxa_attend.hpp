@@ -5,10 +5,12 @@
 
 namespace mxa {
 
-constexpr int kAttendMaxSplits = 256;
 constexpr float kLog2e = 1.4426950408889634f;
 // exp(s - max) is held times 2^8, so that a probability keeps its bits in float16 down to 2^-22 of the largest.
 constexpr float kProbShift = 8.0f;
+// A row's reference is its maximum so far, or up to this (log2) below: its sums are rescaled only where a score passes it
+// by more. A probability then is at most 2^15, within float16.
+constexpr float kSlack = 7.0f;
 
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -19,9 +21,12 @@ typedef uint16_t u16x8 __attribute__((ext_vector_type(8), aligned(2)));
 
 __device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
 
+constexpr int kAttendMaxSplits = 768;
+
+// A split's part of a pair's rows, unnormalised.
 struct AttendPart {
   float* o;   // 16 rows of 32 W values
-  float* ml;  // 16 maxima (of log2 p), 16 sums
+  float* ml;  // 16 references of log2 p, 16 sums
 };
 
 inline size_t part_floats(int w) { return 16 * 32 * (size_t)w + 32; }
@@ -33,7 +38,8 @@ struct AttendArgs {
   long long q_batch, q_tok, q_head;  // strides in elements
   KvPages kv;
   int n_tokens, seq, dim, heads, group, window;  // token t is step t % seq of q's batch entry t / seq
-  int tiles, splits, chunk;
+  int most_rows;  // sequences of more rows a key head are left out
+  int pairs, splits, chunk;  // of the grid: pairs and splits of a sequence, blocks of a split at least
   float scale;
 
   __device__ __forceinline__ const uint16_t* q_row(int t, int h) const {
@@ -41,35 +47,36 @@ struct AttendArgs {
     return q + (long long)b * q_batch + (long long)(t - b * seq) * q_tok + (long long)h * q_head;
   }
   __device__ __forceinline__ uint16_t* out_row(int t, int h) const { return out + ((long long)t * heads + h) * dim; }
-  __device__ __forceinline__ AttendPart part_of(int b, int h, int rt, int split, int w) const {
-    float* const p = part + ((((long long)b * tiles + rt) * kv.heads + h) * splits + split) * (16 * 32 * w + 32);
+  __device__ __forceinline__ AttendPart part_of(int b, int pair, int split, int w) const {
+    float* const p = part + (((long long)b * pairs + pair) * splits + split) * (16 * 32 * w + 32);
     return AttendPart{p, p + 16 * 32 * w};
   }
 };
 
-// Sixteen neighbouring rows (token i and query head of the group: row i * group + head) of a sequence and a key head.
-struct RowTile {
-  int first, rows;    // the sequence's first row of the call, its rows of one key head
-  int length, place0; // its tokens, the place of the first of this tile's call
-  int lo, hi;         // the places that any row of the tile attends to
-  int first_block, end_block, chunk, used;  // their blocks, a split's, the splits that have any
-  __host__ __device__ inline bool find(const AttendArgs& a, int b, int rt) {
-    int count;
+// What the call has of a sequence. Its rows of one key head (token i and query head of the group: row i * group + head)
+// go in tiles of 16; a (key head, tile) is a pair, and a pair has `blocks` blocks of places, one at least.
+struct Sequence {
+  int first, count;    // rows of the call
+  int rows, tiles;     // of one key head; tiles 0: none, or more than `most_rows`
+  int length, place0;  // its tokens, the place of its first row
+  int first_block, blocks;
+  int chunk, splits;  // blocks of a split, splits that have any
+  __host__ __device__ inline Sequence(const AttendArgs& a, int b) {
     kv_rows_of(a.kv, b, a.n_tokens, first, count);
-    rows = count * a.group;
-    if (rt * 16 >= rows) return false;
+    const long long all = (long long)count * a.group;
+    rows = all <= a.most_rows ? (int)all : 0;
+    tiles = (rows + 15) / 16;
     const int known = kv_length(a.kv, b);
     place0 = known - count;
-    length = min(max(known, 0), a.kv.width * a.kv.page);
-    const int t0 = rt * 16 / a.group, t1 = min((rt * 16 + 15) / a.group, count - 1);
-    hi = min(max(place0 + t1 + 1, 0), length);
-    lo = a.window > 0 ? min(max(max(place0 + t0 + 1, 0) - a.window, 0), hi) : 0;
+    length = known < 0 ? 0 : known < a.kv.width * a.kv.page ? known : a.kv.width * a.kv.page;
+    int lo = a.window > 0 ? (place0 + 1 > 0 ? place0 + 1 : 0) - a.window : 0;
+    lo = lo < 0 ? 0 : lo > length ? length : lo;
     first_block = lo / kKvBlock;
-    const int blocks = (hi + kKvBlock - 1) / kKvBlock - first_block;
-    chunk = max(a.chunk, (blocks + a.splits - 1) / a.splits);  // larger where lengths pass what the host was told
-    used = (blocks + chunk - 1) / chunk;
-    end_block = first_block + blocks;
-    return true;
+    blocks = (length + kKvBlock - 1) / kKvBlock - first_block;
+    if (blocks < 1) blocks = 1;
+    const int least = (blocks + a.splits - 1) / a.splits;  // more where a length passes what the host was told
+    chunk = a.chunk > least ? a.chunk : least;
+    splits = (blocks + chunk - 1) / chunk;
   }
 };
 
@@ -93,13 +100,21 @@ __device__ __forceinline__ half8 key_order(const float (&v)[8], int e) {
 
 // The float16 pairs of a word's codes, nibbles 0 and 4, 1 and 5, 2 and 6, 3 and 7: 1024 + c is 0x6400 | c, and 64 + c is
 // 0x5400 | c << 4.
-__device__ __forceinline__ void codes8(uint32_t w, half2v (&c)[4]) {
+struct CodeBits {
+  uint32_t low, high, k1024, k64;
+  __device__ __forceinline__ CodeBits() : low(0x000F000Fu), high(0x00F000F0u), k1024(0x64006400u), k64(0x54005400u) {
+    // in registers, masks scalar and the others not: an and and an or then are one instruction, which takes no constant
+    // and one scalar register
+    asm("" : "+s"(low), "+s"(high), "+v"(k1024), "+v"(k64));
+  }
+};
+__device__ __forceinline__ void codes8(const CodeBits& b, uint32_t w, half2v (&c)[4]) {
   const half2v k1024{(_Float16)-1024.0f, (_Float16)-1024.0f}, k64{(_Float16)-64.0f, (_Float16)-64.0f};
   const uint32_t x = w >> 8;
-  c[0] = __builtin_bit_cast(half2v, (w & 0x000F000Fu) | 0x64006400u) + k1024;
-  c[1] = __builtin_bit_cast(half2v, (w & 0x00F000F0u) | 0x54005400u) + k64;
-  c[2] = __builtin_bit_cast(half2v, (x & 0x000F000Fu) | 0x64006400u) + k1024;
-  c[3] = __builtin_bit_cast(half2v, (x & 0x00F000F0u) | 0x54005400u) + k64;
+  c[0] = __builtin_bit_cast(half2v, (w & b.low) | b.k1024) + k1024;
+  c[1] = __builtin_bit_cast(half2v, (w & b.high) | b.k64) + k64;
+  c[2] = __builtin_bit_cast(half2v, (x & b.low) | b.k1024) + k1024;
+  c[3] = __builtin_bit_cast(half2v, (x & b.high) | b.k64) + k64;
 }
 
 // A word as two float16. (By value: a bit cast of a vector's element itself reads element 0.)
@@ -109,9 +124,9 @@ __device__ __forceinline__ half2v half2_of(uint32_t w) { return __builtin_bit_ca
 __device__ __forceinline__ half2v fma2(half2v c, half2v s, half2v m) { return __builtin_elementwise_fma(c, s, m); }
 
 // Eight keys' or one key's eight values from a word of codes and (s, m).
-__device__ __forceinline__ half8 widen8(uint32_t w, uint32_t sm) {
+__device__ __forceinline__ half8 widen8(const CodeBits& b, uint32_t w, uint32_t sm) {
   half2v c[4];
-  codes8(w, c);
+  codes8(b, w, c);
   const half2v p = half2_of(sm), s{p[0], p[0]}, m{p[1], p[1]};
   half8 h;
 #pragma unroll
@@ -123,11 +138,12 @@ __device__ __forceinline__ half8 widen8(uint32_t w, uint32_t sm) {
 }
 
 // Two neighbouring values of eight tokens (four and four, words w and their scales) as operands: v0 the even value.
-__device__ __forceinline__ void value_operands(const uint32_t (&w)[2], u32x4 sa, u32x4 sb, half8& v0, half8& v1) {
+__device__ __forceinline__ void value_operands(const CodeBits& bits, const uint32_t (&w)[2], u32x4 sa, u32x4 sb, half8& v0,
+                                               half8& v1) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     half2v c[4];
-    codes8(w[i], c);
+    codes8(bits, w[i], c);
     const u32x4 q = i ? sb : sa;
     const half2v s02 = half2_of(q[0]), s13 = half2_of(q[1]), m02 = half2_of(q[2]), m13 = half2_of(q[3]);
     const half2v a = fma2(c[0], s02, m02), d = fma2(c[1], s02, m02), b = fma2(c[2], s13, m13), e = fma2(c[3], s13, m13);
@@ -147,24 +163,31 @@ __device__ __forceinline__ half8 prob_order(const float (&p)[8]) {
   return h;
 }
 
-// A lane's codes of a block, and the block's scales into the wave's 64 W words of LDS: keys' (token, group), then values'.
+// A lane's part of a block as it is loaded: its codes, and W of the block's 64 W words of scales.
 template <int W>
-__device__ __forceinline__ void load_block(const uint8_t* blk, int lane, uint32_t (&kc)[2][W], uint32_t (&vc)[W][2],
-                                           uint32_t* sc) {
-  const int n = lane & 15, g = lane >> 4;
-  const uint32_t* const from = (const uint32_t*)(blk + (lane < 32 ? kv_key_scales(W) : kv_value_scales(W)));
+struct BlockPart {
+  uint32_t kc[2][W], vc[W][2], sc[W];
+  __device__ __forceinline__ void load(const uint8_t* blk, int lane) {
+    const int n = lane & 15, g = lane >> 4;
+    const uint32_t* const from = (const uint32_t*)(blk + (lane < 32 ? kv_key_scales(W) : kv_value_scales(W)));
 #pragma unroll
-  for (int j = 0; j < W; ++j) sc[lane * W + j] = from[(lane & 31) * W + j];
+    for (int j = 0; j < W; ++j) sc[j] = from[(lane & 31) * W + j];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int w = 0; w < W; ++w) kc[i][w] = *(const uint32_t*)(blk + (i * 16 + n) * 16 * W + g * 4 * W + w * 4);
+      for (int w = 0; w < W; ++w) kc[i][w] = *(const uint32_t*)(blk + (i * 16 + n) * 16 * W + g * 4 * W + w * 4);
 #pragma unroll
-  for (int w = 0; w < W; ++w)
+    for (int w = 0; w < W; ++w)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) vc[w][i] = *(const uint32_t*)(blk + kv_value_codes(W) + kv_value_word(W, w, g, n, i));
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-}
+      for (int i = 0; i < 2; ++i) vc[w][i] = *(const uint32_t*)(blk + kv_value_codes(W) + kv_value_word(W, w, g, n, i));
+  }
+  // The scales into the wave's 64 W words of LDS: keys' (token, group), then values'.
+  __device__ __forceinline__ void share(uint32_t* lds, int lane) const {
+#pragma unroll
+    for (int j = 0; j < W; ++j) lds[lane * W + j] = sc[j];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+};
 
 // Scales of places behind the sequence's end (`have` tokens of the block are its own) become 0: what a page holds there,
 // another sequence's or none, may be no number, and 0 times that is none either.

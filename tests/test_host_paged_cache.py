@@ -95,7 +95,11 @@ def test_workspace_bytes(lib) -> None:
                 (3, 3, 0, 4, 2, 64, 0, 0), (3, 3, 0, 4, 2, 64, 64, -1)):
         assert lib.mxa_kv4_attend_workspace_bytes(*bad) == 0, bad
     assert lib.mxa_kv4_attend_workspace_bytes(3, 3, 0, 4, 2, 64, 64, 0) == 0  # a workgroup takes all of 64 places
-    # a window bounds what is shared out
+    # a window bounds what is shared out, whatever its size
+    for n in (1, 174):
+        want = lib.mxa_kv4_attend_workspace_bytes(7, 7 * n, 0, 10, 2, 64, 640, 0)
+        for window in (1 << 30, (1 << 31) - 175, (1 << 31) - 1):
+            assert lib.mxa_kv4_attend_workspace_bytes(7, 7 * n, 0, 10, 2, 64, 640, window) == want > 0
     assert lib.mxa_kv4_attend_workspace_bytes(1, 1, 0, 4, 2, 64, 1 << 20, 64) == 0
 
 
