@@ -781,8 +781,7 @@ size_t mxa_kv4_attend_workspace_bytes(int n_seq, int n_tokens, int ragged, int q
   if (n_seq < 1 || n_tokens < 1 || (!ragged && n_tokens % n_seq != 0) || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads != 0 ||
       head_dim < 8 || head_dim > mxa::kKvMaxDim || max_length < 1 || window < 0)
     return 0;
-  return mxa::attend_workspace(n_seq, kv_heads, q_heads / kv_heads, ragged ? n_tokens : n_tokens / n_seq, max_length,
-                               window, head_dim);
+  return mxa::attend_workspace(n_seq, n_tokens, ragged != 0, kv_heads, q_heads / kv_heads, max_length, window, head_dim);
 }
 
 int mxa_kv4_attend(const void* q, const long long* q_strides, int q_heads, int n_tokens, int seq_len,
@@ -805,7 +804,7 @@ int mxa_kv4_attend(const void* q, const long long* q_strides, int q_heads, int n
   a.out = (uint16_t*)out;
   a.n_tokens = n_tokens, a.seq = seq_len, a.dim = head_dim, a.heads = q_heads, a.group = q_heads / kv_heads;
   a.window = window < MXA_KV4_MAX_PLACES ? window : MXA_KV4_MAX_PLACES, a.scale = scale;
-  if (mxa::launch_attend(a, query_starts != nullptr ? n_tokens : n_tokens / n_seq, max_length, workspace, (hipStream_t)stream) != 0) return MXA_ERR_UNSUPPORTED;
+  if (mxa::launch_attend(a, max_length, workspace, (hipStream_t)stream) != 0) return MXA_ERR_UNSUPPORTED;
   return check_launch();
 }
 

@@ -259,50 +259,87 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join_kernel(AttendArgs 
 }
 
 // (std::min and std::max here: on the host, HIP's own of that name take ints.)
-// How the blocks of up to `most` tokens of each sequence are shared out.
+// How the places of up to `most` tokens of each sequence are shared out. Sequences of up to kFewRows rows a key head go in
+// tiles of 16 rows (attend_kernel), others in those of attend_tile_kernel; a call without query_starts has one kind.
+constexpr int kFewRows = 64;
 struct Plan {
-  long long pairs;  // of a sequence
-  int splits, chunk;
+  bool few, many;     // the kinds that there may be
+  long long pairs[2]; // (tile of 16 rows, key head) of a sequence
+  int splits[2], chunk[2];
+  long long tiles;    // of the call, for many rows
 };
-Plan plan_of(int n_seq, int kv_heads, int group, int most, int max_length, int window, int dim) {
-  Plan p;
-  p.pairs = (((long long)most * group + 15) / 16) * kv_heads;
-  const long long slots = 256 * (kv_groups(dim) <= 4 ? 3 : 2);  // workgroups that the CUs hold at once
-  const long long reach = window > 0 ? std::min<long long>(max_length, (long long)window + most) : max_length;
+
+void share_out(long long blocks, long long workgroups, long long slots, int least, int& splits, int& chunk) {
+  const long long want = std::max<long long>(1, slots / workgroups);
+  chunk = (int)std::max<long long>(least, (blocks + want - 1) / want);
+  splits = (int)std::min<long long>(kAttendMaxSplits, (blocks + chunk - 1) / chunk);
+}
+
+Plan plan_of(int n_seq, int n_tokens, bool ragged, int kv_heads, int group, int max_length, int window, int dim) {
+  Plan p{};
+  const long long most = (long long)(ragged ? n_tokens : n_tokens / n_seq) * group;
+  p.few = ragged || most <= kFewRows;
+  p.many = most > kFewRows;
+  const long long reach = window > 0 ? std::min<long long>(max_length, (long long)window + most / group) : max_length;
   const long long blocks = reach / kKvBlock + 2;
-  // one sequence: what the CUs hold at once; several, whose lengths are not known: four times that, in parts small enough
-  // to even out
-  const long long want = std::max<long long>(1, (n_seq > 1 ? 4 * slots : slots) / (p.pairs * n_seq));
-  p.chunk = (int)std::max<long long>(kAttendWaves, (blocks + want - 1) / want);
-  p.splits = (int)std::min<long long>(kAttendMaxSplits, (blocks + p.chunk - 1) / p.chunk);
+  const bool narrow = kv_groups(dim) <= 4;
+  if (p.few) {
+    p.pairs[0] = (std::min<long long>(most, kFewRows) + 15) / 16 * kv_heads;
+    const long long slots = 256 * (narrow ? 3 : 2);  // workgroups that the CUs hold at once
+    // one sequence: what the CUs hold at once; several, whose lengths are not known: four times that, in parts small
+    // enough to even out
+    share_out(blocks, p.pairs[0] * n_seq, n_seq > 1 ? 4 * slots : slots, 4, p.splits[0], p.chunk[0]);
+  }
+  if (p.many) {
+    p.pairs[1] = (most + 15) / 16 * kv_heads;
+    const int rows = attend_tile_rows(dim);
+    p.tiles = ragged ? most / rows + std::min<long long>(n_seq, most / (kFewRows + 1)) : (most + rows - 1) / rows * n_seq;
+    share_out(blocks, p.tiles * kv_heads, 256, 8, p.splits[1], p.chunk[1]);
+    // the workspace has room for as many rows of each sequence as any may have: not split where that is large
+    if ((long long)n_seq * p.pairs[1] * p.splits[1] * part_floats(kv_groups(dim)) > 16 << 20) p.splits[1] = 1;
+    if (p.splits[1] == 1) p.chunk[1] = 1 << 26;
+  }
   return p;
+}
+
+size_t part_bytes(const Plan& p, int kind, int n_seq, int dim) {
+  return p.splits[kind] <= 1 ? 0 : (size_t)n_seq * p.pairs[kind] * p.splits[kind] * part_floats(kv_groups(dim)) * sizeof(float);
+}
+
+template <int W>
+void launch_few(const AttendArgs& a, hipStream_t stream) {
+  hipLaunchKernelGGL(attend_kernel<W>, dim3(a.splits, a.pairs, a.kv.n_seq), dim3(kAttendThreads), 0, stream, a);
 }
 
 }  // namespace
 
-size_t attend_workspace(int n_seq, int kv_heads, int group, int most, int max_length, int window, int dim) {
-  const Plan p = plan_of(n_seq, kv_heads, group, most, max_length, window, dim);
-  if (p.splits <= 1) return 0;
-  return (size_t)n_seq * p.pairs * p.splits * part_floats(kv_groups(dim)) * sizeof(float);
+size_t attend_workspace(int n_seq, int n_tokens, bool ragged, int kv_heads, int group, int max_length, int window, int dim) {
+  const Plan p = plan_of(n_seq, n_tokens, ragged, kv_heads, group, max_length, window, dim);
+  return part_bytes(p, 0, n_seq, dim) + part_bytes(p, 1, n_seq, dim);
 }
 
-int launch_attend(AttendArgs a, int most, int max_length, void* workspace, hipStream_t stream) {
-  const Plan p = plan_of(a.kv.n_seq, a.kv.heads, a.group, most, max_length, a.window, a.dim);
-  if (p.pairs > 65535) return -1;
+int launch_attend(AttendArgs a, int max_length, void* workspace, hipStream_t stream) {
+  const Plan p = plan_of(a.kv.n_seq, a.n_tokens, a.kv.starts != nullptr, a.kv.heads, a.group, max_length, a.window, a.dim);
+  if (p.pairs[0] > 65535 || (p.splits[1] > 1 && p.pairs[1] > 65535) || p.tiles * a.kv.heads >= 1 << 23) return -1;
   const int W = kv_groups(a.dim);
-  a.most_rows = 0x7fffffff;
-  a.pairs = (int)p.pairs, a.splits = p.splits, a.chunk = p.chunk, a.part = (float*)workspace;
-  const dim3 grid(p.splits, a.pairs, a.kv.n_seq);
-  switch (W) {
+  for (int kind = 0; kind < 2; ++kind) {
+    if (!(kind ? p.many : p.few)) continue;
+    a.least_rows = kind ? kFewRows + 1 : 1, a.most_rows = kind ? 0x7fffffff : kFewRows;
+    a.pairs = (int)p.pairs[kind], a.splits = p.splits[kind], a.chunk = p.chunk[kind];
+    a.part = (float*)((char*)workspace + (kind ? part_bytes(p, 0, a.kv.n_seq, a.dim) : 0));
+    if (kind == 1) {
+      launch_attend_tile(a, p.tiles, stream);
+    } else {
+      switch (W) {
 #define MXA_CASE(W) \
-  case W: hipLaunchKernelGGL(attend_kernel<W>, grid, dim3(kAttendThreads), 0, stream, a); break;
-    MXA_CASE(1) MXA_CASE(2) MXA_CASE(3) MXA_CASE(4) MXA_CASE(5) MXA_CASE(6) MXA_CASE(7) MXA_CASE(8)
+  case W: launch_few<W>(a, stream); break;
+        MXA_CASE(1) MXA_CASE(2) MXA_CASE(3) MXA_CASE(4) MXA_CASE(5) MXA_CASE(6) MXA_CASE(7) MXA_CASE(8)
 #undef MXA_CASE
-    default: return -1;
+      }
+    }
+    if (a.splits > 1)
+      hipLaunchKernelGGL(attend_join_kernel, dim3(16, a.pairs, a.kv.n_seq), dim3(kAttendThreads), 0, stream, a, W);
   }
-  if (p.splits > 1)
-    hipLaunchKernelGGL(attend_join_kernel, dim3((unsigned)std::min<long long>((long long)most * a.group, 16), a.pairs, a.kv.n_seq),
-                       dim3(kAttendThreads), 0, stream, a, W);
   return 0;
 }
 

@@ -38,7 +38,7 @@ struct AttendArgs {
   long long q_batch, q_tok, q_head;  // strides in elements
   KvPages kv;
   int n_tokens, seq, dim, heads, group, window;  // token t is step t % seq of q's batch entry t / seq
-  int most_rows;  // sequences of more rows a key head are left out
+  int least_rows, most_rows;  // sequences of fewer or more rows a key head are left out
   int pairs, splits, chunk;  // of the grid: pairs and splits of a sequence, blocks of a split at least
   float scale;
 
@@ -57,14 +57,14 @@ struct AttendArgs {
 // go in tiles of 16; a (key head, tile) is a pair, and a pair has `blocks` blocks of places, one at least.
 struct Sequence {
   int first, count;    // rows of the call
-  int rows, tiles;     // of one key head; tiles 0: none, or more than `most_rows`
+  int rows, tiles;     // of one key head; 0: none, or another kernel's
   int length, place0;  // its tokens, the place of its first row
   int first_block, blocks;
   int chunk, splits;  // blocks of a split, splits that have any
   __host__ __device__ inline Sequence(const AttendArgs& a, int b) {
     kv_rows_of(a.kv, b, a.n_tokens, first, count);
     const long long all = (long long)count * a.group;
-    rows = all <= a.most_rows ? (int)all : 0;
+    rows = all >= a.least_rows && all <= a.most_rows ? (int)all : 0;
     tiles = (rows + 15) / 16;
     const int known = kv_length(a.kv, b);
     place0 = known - count;
@@ -79,6 +79,31 @@ struct Sequence {
     splits = (blocks + chunk - 1) / chunk;
   }
 };
+
+// The sequence and the tile (of `rows` rows a key head, the last first: those attend to most) that tile `flat` of the call
+// is; false behind the last. Lanes look at 64 sequences at a time.
+__device__ __forceinline__ bool find_tile(const AttendArgs& a, int flat, int rows, int& b, int& tile) {
+  const int lane = threadIdx.x & 63;
+  for (int base = 0; base < a.kv.n_seq; base += 64) {
+    int tiles = 0;
+    if (base + lane < a.kv.n_seq) tiles = (Sequence(a, base + lane).rows + rows - 1) / rows;
+    int run = tiles;
+#pragma unroll
+    for (int i = 1; i < 64; i *= 2) {
+      const int other = __shfl_up(run, i);
+      if (lane >= i) run += other;
+    }
+    const unsigned long long past = __ballot(run > flat);
+    if (past != 0) {
+      const int at = __builtin_ctzll(past);
+      b = base + at;
+      tile = __builtin_amdgcn_readlane(run, at) - 1 - flat;
+      return true;
+    }
+    flat -= __builtin_amdgcn_readlane(run, 63);
+  }
+  return false;
+}
 
 // The power of two that a row of q is divided by: its largest value then lies in [2^10, 2^11).
 __device__ __forceinline__ int row_exponent(float top) {
@@ -137,18 +162,28 @@ __device__ __forceinline__ half8 widen8(const CodeBits& b, uint32_t w, uint32_t 
   return h;
 }
 
+typedef _Float16 half4v __attribute__((ext_vector_type(4)));
+
+// Two neighbouring values of four tokens, in the order 0 2 1 3, from a word and its scales: v0 the even value.
+template <class H4>
+__device__ __forceinline__ void value4(const CodeBits& bits, uint32_t w, u32x4 sm, H4& v0, H4& v1) {
+  half2v c[4];
+  codes8(bits, w, c);
+  const half2v s02 = half2_of(sm[0]), s13 = half2_of(sm[1]), m02 = half2_of(sm[2]), m13 = half2_of(sm[3]);
+  const half2v a = fma2(c[0], s02, m02), d = fma2(c[1], s02, m02), b = fma2(c[2], s13, m13), e = fma2(c[3], s13, m13);
+  v0[0] = a[0], v0[1] = a[1], v0[2] = b[0], v0[3] = b[1];
+  v1[0] = d[0], v1[1] = d[1], v1[2] = e[0], v1[3] = e[1];
+}
+
 // Two neighbouring values of eight tokens (four and four, words w and their scales) as operands: v0 the even value.
 __device__ __forceinline__ void value_operands(const CodeBits& bits, const uint32_t (&w)[2], u32x4 sa, u32x4 sb, half8& v0,
                                                half8& v1) {
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    half2v c[4];
-    codes8(bits, w[i], c);
-    const u32x4 q = i ? sb : sa;
-    const half2v s02 = half2_of(q[0]), s13 = half2_of(q[1]), m02 = half2_of(q[2]), m13 = half2_of(q[3]);
-    const half2v a = fma2(c[0], s02, m02), d = fma2(c[1], s02, m02), b = fma2(c[2], s13, m13), e = fma2(c[3], s13, m13);
-    v0[4 * i] = a[0], v0[4 * i + 1] = a[1], v0[4 * i + 2] = b[0], v0[4 * i + 3] = b[1];
-    v1[4 * i] = d[0], v1[4 * i + 1] = d[1], v1[4 * i + 2] = e[0], v1[4 * i + 3] = e[1];
+    half4v a, b;
+    value4(bits, w[i], i ? sb : sa, a, b);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v0[4 * i + j] = a[j], v1[4 * i + j] = b[j];
   }
 }
 
@@ -204,8 +239,9 @@ __device__ __forceinline__ void clear_tail(uint32_t* sc, int lane, int have) {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
-// Bytes of workspace for up to `most` tokens of a sequence and max_length places.
-size_t attend_workspace(int n_seq, int kv_heads, int group, int most, int max_length, int window, int dim);
-int launch_attend(AttendArgs a, int most, int max_length, void* workspace, hipStream_t stream);
+size_t attend_workspace(int n_seq, int n_tokens, bool ragged, int kv_heads, int group, int max_length, int window, int dim);
+int attend_tile_rows(int dim);  // of a workgroup of the form for many rows
+void launch_attend_tile(const AttendArgs& a, long long tiles, hipStream_t stream);
+int launch_attend(AttendArgs a, int max_length, void* workspace, hipStream_t stream);
 
 }  // namespace mxa
