@@ -11,6 +11,8 @@ constexpr float kProbShift = 8.0f;
 // A row's reference is its maximum so far, or up to this (log2) below: its sums are rescaled only where a score passes it
 // by more. A probability then is at most 2^15, within float16.
 constexpr float kSlack = 7.0f;
+constexpr float kProbMost = 32768.0f;
+constexpr float kLowest = -3e38f;  // the reference of a row that has seen no place
 
 typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));

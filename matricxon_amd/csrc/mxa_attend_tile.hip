@@ -93,14 +93,17 @@ __global__ __launch_bounds__(TileShape<W>::threads, W <= 4 ? 2 : 1) void attend_
       for (int j = 0; j < 8; ++j) v[j] = bf16_to_float(raw[k][j]);
       q[k] = key_order(v, -e);
     }
-    back = ldexpf(a.scale * kLog2e, e);
+    if (a.scale < 0.0f)  // its sign goes to q: the largest product is the largest score
+#pragma unroll
+      for (int k = 0; k < 2 * W; ++k) q[k] = -q[k];
+    back = fmaxf(ldexpf(fabsf(a.scale) * kLog2e, e), 1e-37f);  // not 0, with which a place left out would be no number
   }
   f32x16 o[W];
 #pragma unroll
   for (int i = 0; i < W; ++i)
 #pragma unroll
     for (int j = 0; j < 16; ++j) o[i][j] = 0.0f;
-  float m = -INFINITY, l = 0.0f;
+  float m = kLowest, l = 0.0f;
   const int wave_last = min(row0 + wave * 32 + 31, seq.rows - 1);
   const int inside_lo = a.window > 0 ? max(seq.place0 + wave_last / a.group + 1, 0) - a.window : 0;
   const int inside_hi = min(seq.place0 + (row0 + wave * 32) / a.group + 1, seq.length);
@@ -109,8 +112,8 @@ __global__ __launch_bounds__(TileShape<W>::threads, W <= 4 ? 2 : 1) void attend_
   const int blocks_of_page = a.kv.page / kKvBlock;
   long long where = -1;
   int looked = begin - 64;  // the block that lane 0 has
-  const auto block_at = [&](int u) -> const uint8_t* {  // nullptr: no page, or behind the end
-    if (u >= end) return nullptr;
+  const auto block_at = [&](int u) -> long long {  // -1: no page, or behind the last
+    if (u >= end) return -1;
     if (u >= looked + 64) {
       looked = u;
       const long long block = u + lane < end ? kv_block(a.kv, b, (u + lane) * kKvBlock) : -1;
@@ -118,59 +121,55 @@ __global__ __launch_bounds__(TileShape<W>::threads, W <= 4 ? 2 : 1) void attend_
     }
     const uint32_t w0 = __builtin_amdgcn_readlane((int)(uint32_t)where, u - looked);
     const uint32_t w1 = __builtin_amdgcn_readlane((int)(where >> 32), u - looked);
-    return (int)w1 < 0 ? nullptr : a.kv.pages + ((uint64_t)w1 << 32 | w0);
+    return (long long)((uint64_t)w1 << 32 | w0);
   };
-  const uint8_t* at[2];
+  int next0 = 0, next1 = 0;  // places of the requested tile's blocks that are the sequence's
   Staged<W> st;
   const bool key_wave = wave < S::key_waves;
   // key wave w: block w / (waves / 4) of the tile; with 8 waves two to a block, an octet a lane, else two octets a lane
-  const int key_block = wave * 4 / S::waves, key_octet = S::waves == 8 ? (wave & 1) * 2 + g : 2 * g;
+  const int key_block = (wave * 4 / S::waves) & 1, key_octet = S::waves == 8 ? (wave & 1) * 2 + g : 2 * g;
   const auto request = [&](int u) {
-    at[0] = block_at(u);
-    at[1] = block_at(u + 1);
+    const long long w0 = block_at(u), w1 = block_at(u + 1);
+    // no page: any block, none of whose places count
+    const uint8_t *const at0 = a.kv.pages + max(w0, 0LL), *const at1 = a.kv.pages + max(w1, 0LL);
+    next0 = w0 < 0 ? 0 : min(seq.length - u * kKvBlock, kKvBlock);
+    next1 = w1 < 0 ? 0 : min(seq.length - (u + 1) * kKvBlock, kKvBlock);
     if (key_wave) {
-      const uint8_t* const blk = at[key_block & 1];
-      if (blk != nullptr) {
+      const uint8_t* const blk = key_block ? at1 : at0;
 #pragma unroll
-        for (int c = 0; c < S::octets; ++c)
+      for (int c = 0; c < S::octets; ++c)
 #pragma unroll
-          for (int w = 0; w < W; ++w)
-            st.key.codes[c][w] = *(const uint32_t*)(blk + n * 16 * W + (key_octet + c) * 4 * W + w * 4);
+        for (int w = 0; w < W; ++w)
+          st.key.codes[c][w] = *(const uint32_t*)(blk + n * 16 * W + (key_octet + c) * 4 * W + w * 4);
 #pragma unroll
-        for (int w = 0; w < W; ++w) st.key.scales[w] = *(const uint32_t*)(blk + kv_key_scales(W) + (n * W + w) * 4);
-      }
+      for (int w = 0; w < W; ++w) st.key.scales[w] = *(const uint32_t*)(blk + kv_key_scales(W) + (n * W + w) * 4);
     } else {
 #pragma unroll
       for (int t = 0; t < S::items; ++t) {
         const int item = (wave - S::key_waves) + t * (S::waves - S::key_waves);
         if (item >= 2 * S::pairs) break;
-        const uint8_t* const blk = at[item & 1];
+        const uint8_t* const blk = item & 1 ? at1 : at0;
         const int pair = item >> 1, i = lane & 15, quad = lane >> 4;
-        if (blk != nullptr) {
-          const bool two = 2 * pair + 1 < W;
+        const bool two = 2 * pair + 1 < W;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {  // (group of the pair, half)
-            if (k >= 2 && !two) break;
-            const int group = 2 * pair + (k >> 1);
-            st.value.codes[t][k] = *(const uint32_t*)(blk + kv_value_codes(W) + kv_value_word(W, group, quad, i, k & 1));
-            st.value.scales[t][k] =
-                *(const u32x4*)(blk + kv_value_scales(W) + (group * 8 + (k & 1) * 4 + quad) * 16);
-          }
+        for (int k = 0; k < 4; ++k) {  // (group of the pair, half)
+          if (k >= 2 && !two) break;
+          const int group = 2 * pair + (k >> 1);
+          st.value.codes[t][k] = *(const uint32_t*)(blk + kv_value_codes(W) + kv_value_word(W, group, quad, i, k & 1));
+          st.value.scales[t][k] = *(const u32x4*)(blk + kv_value_scales(W) + (group * 8 + (k & 1) * 4 + quad) * 16);
         }
       }
     }
   };
-  const auto widen = [&](int u, half8* to) {
+  const auto widen = [&](half8* to) {
     if (key_wave) {
-      const bool there = at[key_block & 1] != nullptr;
 #pragma unroll
       for (int c = 0; c < S::octets; ++c)
 #pragma unroll
         for (int w = 0; w < W; ++w) {
           const int octet = key_octet + c;
-          half8 v{};
-          if (there) v = widen8(bits, st.key.codes[c][w], st.key.scales[w]);
-          to[((key_block & 1) * 2 * W + 2 * w + (octet >> 1)) * 64 + (octet & 1) * 32 + n] = v;
+          to[(key_block * 2 * W + 2 * w + (octet >> 1)) * 64 + (octet & 1) * 32 + n] =
+              widen8(bits, st.key.codes[c][w], st.key.scales[w]);
         }
     } else {
       half4* const vt = (half4*)(to + S::frags * 64);
@@ -179,22 +178,23 @@ __global__ __launch_bounds__(TileShape<W>::threads, W <= 4 ? 2 : 1) void attend_
         const int item = (wave - S::key_waves) + t * (S::waves - S::key_waves);
         if (item >= 2 * S::pairs) break;
         const int blk = item & 1, pair = item >> 1, i = lane & 15, quad = lane >> 4;
-        const bool there = at[blk] != nullptr, two = 2 * pair + 1 < W;
-        const int have = seq.length - (u + blk) * kKvBlock;
+        const bool two = 2 * pair + 1 < W;
+        const int have = blk ? next1 : next0;
+        if (have < kKvBlock) {  // behind the sequence's end, or no page: whatever is there, 0
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int first = (k & 1) * 16 + quad * 4;
+            const uint32_t keep02 = (first < have ? 0xFFFFu : 0u) | (first + 2 < have ? 0xFFFF0000u : 0u);
+            const uint32_t keep13 = (first + 1 < have ? 0xFFFFu : 0u) | (first + 3 < have ? 0xFFFF0000u : 0u);
+            u32x4& sm = st.value.scales[t][k];
+            sm[0] &= keep02, sm[1] &= keep13, sm[2] &= keep02, sm[3] &= keep13;
+          }
+        }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           if (k >= 2 && !two) break;
-          half4 v0{}, v1{};
-          if (there) {
-            u32x4 sm = st.value.scales[t][k];
-            const int first = (k & 1) * 16 + quad * 4;
-            if (have < kKvBlock) {  // behind the sequence's end: whatever is there, 0
-              const uint32_t keep02 = (first < have ? 0xFFFFu : 0u) | (first + 2 < have ? 0xFFFF0000u : 0u);
-              const uint32_t keep13 = (first + 1 < have ? 0xFFFFu : 0u) | (first + 3 < have ? 0xFFFF0000u : 0u);
-              sm[0] &= keep02, sm[1] &= keep13, sm[2] &= keep02, sm[3] &= keep13;
-            }
-            value4(bits, st.value.codes[t][k], sm, v0, v1);
-          }
+          half4 v0, v1;
+          value4(bits, st.value.codes[t][k], st.value.scales[t][k], v0, v1);
           half4* const p = vt + ((((blk * 2 + (k & 1)) * W + 2 * pair + (k >> 1)) * 64 + (quad & 1) * 32 + 2 * i) * 2 + (quad >> 1));
           p[0] = v0;
           p[2] = v1;
@@ -203,12 +203,12 @@ __global__ __launch_bounds__(TileShape<W>::threads, W <= 4 ? 2 : 1) void attend_
     }
   };
 
-  bool there[2] = {false, false};
   int turn = 0;  // the half of LDS that holds the present tile
+  int have0 = 0, have1 = 0;
   if (begin < end) {
     request(begin);
-    widen(begin, lds);
-    there[0] = at[0] != nullptr, there[1] = at[1] != nullptr;
+    widen(lds);
+    have0 = next0, have1 = next1;
   }
   __syncthreads();
   for (int u = begin; u < end; u += 2) {
@@ -218,55 +218,59 @@ __global__ __launch_bounds__(TileShape<W>::threads, W <= 4 ? 2 : 1) void attend_
     if (more) request(u + 2);
     f32x16 s[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int j = 0; j < 16; ++j) s[i][j] = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 2 * W; ++k)
+    for (int k = 0; k < 2 * W; ++k)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
         s[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kt[(i * 2 * W + k) * 64 + lane], q[k], s[i], 0, 0, 0);
-    }
     const int first = u * kKvBlock;
-    const bool inside = there[0] && there[1] && first >= inside_lo && first + kTilePlaces <= inside_hi;
-    float top = -INFINITY;
-    if (inside) {
+    const bool inside = have0 == kKvBlock && have1 == kKvBlock && first >= inside_lo && first + kTilePlaces <= inside_hi;
+    if (!inside) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          s[i][j] *= back;
-          top = fmaxf(top, s[i][j]);
-        }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int t = first + i * kKvBlock + j / 4 * 8 + g * 4 + j % 4;
-          s[i][j] = there[i] && t < limit && t >= low ? s[i][j] * back : -INFINITY;
-          top = fmaxf(top, s[i][j]);
+          const int t = j / 4 * 8 + g * 4 + j % 4, at = first + i * kKvBlock + t;
+          if (t >= (i ? have1 : have0) || at >= limit || at < low) s[i][j] = -INFINITY;
         }
     }
-    if (__any(top > m + kSlack)) {
+    // p against the row's reference so far: a sum within float16's range says that every p is. A row's first places, whose
+    // reference is the lowest of all, sum to +inf.
+    half8 p[4];
+    float sum = 0.0f;
+    const auto probabilities = [&]() {
+      const float ref = kProbShift - m;
+      sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float e[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          e[j] = exp2_(fmaf(s[i >> 1][(i & 1) * 8 + j], back, ref));
+          sum += e[j];
+        }
+        p[i] = prob_order(e);
+      }
+    };
+    probabilities();
+    if (__any(!(sum <= kProbMost))) {
+      float top = s[0][0];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) top = fmaxf(top, s[i][j]);
       top = fmaxf(top, __shfl_xor(top, 32));
-      const float m2 = fmaxf(m, top);
-      const float alpha = m2 == -INFINITY ? 1.0f : exp2_(m - m2);
+      const float m2 = fmaxf(m, top * back), alpha = exp2_(m - m2);
       m = m2;
       l *= alpha;
 #pragma unroll
       for (int i = 0; i < W; ++i) o[i] *= alpha;
+      probabilities();
     }
-    const float ref = (m == -INFINITY ? 0.0f : m) - kProbShift;
-    half8 p[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float e[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        e[j] = exp2_(s[i >> 1][(i & 1) * 8 + j] - ref);
-        l += e[j];
-      }
-      p[i] = prob_order(e);
-    }
+    l += sum;
 #pragma unroll
     for (int k = 0; k < 4; ++k)
 #pragma unroll
@@ -274,8 +278,8 @@ __global__ __launch_bounds__(TileShape<W>::threads, W <= 4 ? 2 : 1) void attend_
         o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vt[(k * W + i) * 64 + lane], p[k], o[i], 0, 0, 0);
     if (more) {
       turn ^= 1;
-      widen(u + 2, lds + turn * 2 * S::frags * 64);
-      there[0] = at[0] != nullptr, there[1] = at[1] != nullptr;
+      widen(lds + turn * 2 * S::frags * 64);
+      have0 = next0, have1 = next1;
     }
     __syncthreads();
   }
