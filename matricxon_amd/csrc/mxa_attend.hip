@@ -266,6 +266,7 @@ struct Plan {
   bool few, many;     // the kinds that there may be
   long long pairs[2]; // (tile of 16 rows, key head) of a sequence
   int splits[2], chunk[2];
+  int rows;           // of a workgroup, for many rows
   long long tiles;    // of the call, for many rows
 };
 
@@ -292,9 +293,12 @@ Plan plan_of(int n_seq, int n_tokens, bool ragged, int kv_heads, int group, int 
   }
   if (p.many) {
     p.pairs[1] = (most + 15) / 16 * kv_heads;
-    const int rows = attend_tile_rows(dim);
-    p.tiles = ragged ? most / rows + std::min<long long>(n_seq, most / (kFewRows + 1)) : (most + rows - 1) / rows * n_seq;
-    share_out(blocks, p.tiles * kv_heads, 256, 8, p.splits[1], p.chunk[1]);
+    for (p.rows = narrow ? 256 : 128;; p.rows = 128) {
+      p.tiles = ragged ? most / p.rows + std::min<long long>(n_seq, most / (kFewRows + 1))
+                       : (most + p.rows - 1) / p.rows * n_seq;
+      if (p.rows == 128 || p.tiles * kv_heads >= 256) break;  // 256 rows only where they fill the CUs
+    }
+    share_out(blocks, p.tiles * kv_heads, narrow ? 512 : 256, 8, p.splits[1], p.chunk[1]);
     // the workspace has room for as many rows of each sequence as any may have: not split where that is large
     if ((long long)n_seq * p.pairs[1] * p.splits[1] * part_floats(kv_groups(dim)) > 16 << 20) p.splits[1] = 1;
     if (p.splits[1] == 1) p.chunk[1] = 1 << 26;
@@ -328,7 +332,7 @@ int launch_attend(AttendArgs a, int max_length, void* workspace, hipStream_t str
     a.pairs = (int)p.pairs[kind], a.splits = p.splits[kind], a.chunk = p.chunk[kind];
     a.part = (float*)((char*)workspace + (kind ? part_bytes(p, 0, a.kv.n_seq, a.dim) : 0));
     if (kind == 1) {
-      launch_attend_tile(a, p.tiles, stream);
+      launch_attend_tile(a, p.rows, p.tiles, stream);
     } else {
       switch (W) {
 #define MXA_CASE(W) \

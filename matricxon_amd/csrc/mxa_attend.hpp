@@ -242,8 +242,8 @@ __device__ __forceinline__ void clear_tail(uint32_t* sc, int lane, int have) {
 }
 
 size_t attend_workspace(int n_seq, int n_tokens, bool ragged, int kv_heads, int group, int max_length, int window, int dim);
-int attend_tile_rows(int dim);  // of a workgroup of the form for many rows
-void launch_attend_tile(const AttendArgs& a, long long tiles, hipStream_t stream);
+// The form for many rows, of 256 (heads of up to 128 values) or 128 rows of a key head a workgroup.
+void launch_attend_tile(const AttendArgs& a, int rows, long long tiles, hipStream_t stream);
 int launch_attend(AttendArgs a, int max_length, void* workspace, hipStream_t stream);
 
 }  // namespace mxa

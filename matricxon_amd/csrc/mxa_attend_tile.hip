@@ -1,11 +1,12 @@
 // Causal attention over the 4-bit cache for many rows (mxa_attend.hip has the mathematics and the form for few rows): a
-// workgroup takes 32 rows a wave of one key head, and widens each tile of 64 places once for all of them, into LDS in the
-// order of the matrix instructions' operands:
+// workgroup takes 32 rows a wave of one key head, and widens each tile of 64 (or 32) places once for all of them, into LDS
+// in the order of the matrix instructions' operands:
 //
 //   scores^T = K q^T    32 keys by 32 rows, 16 of a head's values an instruction
 //   o^T     += V^T p^T  32 of a head's values by 32 rows, 16 places an instruction; p as the scores come out
 //
-// The codes of the next tile are requested before a tile is computed, and widened into the other half of LDS behind it.
+// A tile's packed bytes are copied into a ring of LDS slots by copies that no wave waits for until they are widened, some
+// tiles later.
 #include "mxa_attend.hpp"
 #include "mxa_kernels.hpp"
 
@@ -17,44 +18,43 @@ namespace {
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 
-constexpr int kTilePlaces = 2 * kKvBlock;
+constexpr int kAhead = 6;  // operands read from LDS ahead of the instruction that takes them
 
-template <int W>
+// A barrier that waits for LDS alone: copies stay on their way.
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+// W groups a head, NW waves.
+template <int W, int NW>
 struct TileShape {
-  static constexpr int waves = W <= 4 ? 8 : 4;  // two to a SIMD where their registers allow
-  static constexpr int threads = 64 * waves, rows = 32 * waves;
-  static constexpr int key_waves = waves / 2;   // widen keys; the others widen values
-  static constexpr int octets = 8 / waves * 1;  // of a token's four, that a lane of a key wave has: 1 or 2
-  static constexpr int pairs = (W + 1) / 2;     // pairs of groups
-  static constexpr int items = (2 * pairs + waves / 2 - 1) / (waves / 2);  // (block, pair) that a value wave has at most
-  static constexpr int frags = 4 * W;           // operands of 1 KB: keys' of a tile, and as many of values
+  static constexpr int threads = 64 * NW, rows = 32 * NW;
+  static constexpr int blocks = NW / 4;                 // of a tile
+  static constexpr int value_waves = NW / 2;            // widen values; those before them keys
+  static constexpr int pairs = (W + 1) / 2;             // pairs of groups
+  static constexpr int items = (blocks * pairs + value_waves - 1) / value_waves;  // (block, pair) of a value wave at most
+  static constexpr int frags = 2 * W * blocks;          // operands of 1 KB: a tile's keys, and as many of its values
+  static constexpr int raw = blocks * 1280 * W;         // bytes of a tile in the cache
+  static constexpr int copies = (320 * W + 1023) / 1024;  // of a wave, a tile: a quarter of a block
+  static constexpr int ring = 4;                        // tiles in LDS as they are in the cache
+  static constexpr size_t lds = 4 * (size_t)frags * 1024 + (size_t)ring * raw;
 };
 
-// A thread's codes and scales of the next tile, as loaded.
-template <int W>
-struct Staged {
-  using S = TileShape<W>;
-  union {
-    struct {
-      uint32_t codes[S::octets][W], scales[W];
-    } key;
-    struct {
-      uint32_t codes[S::items][4];
-      u32x4 scales[S::items][4];
-    } value;
-  };
-};
-
-template <int W>
-__global__ __launch_bounds__(TileShape<W>::threads, W <= 4 ? 2 : 1) void attend_tile_kernel(AttendArgs a) {
-  using S = TileShape<W>;
+template <int W, int NW>
+__global__ __launch_bounds__(64 * NW, W <= 4 ? 2 : 1) void attend_tile_kernel(AttendArgs a) {
+  using S = TileShape<W, NW>;
+  constexpr int B = S::blocks;
   extern __shared__ __align__(16) unsigned char smem[];
   half8* const lds = (half8*)smem;  // [half of LDS][keys' operands, values' operands][lane]
+  unsigned char* const raw = smem + 4 * S::frags * 1024;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 31, g = lane >> 5;
   const int h = blockIdx.x % a.kv.heads, split = blockIdx.y;
   int b, tile;
   if (!find_tile(a, blockIdx.x / a.kv.heads, S::rows, b, tile)) return;
+  b = __builtin_amdgcn_readfirstlane(b), tile = __builtin_amdgcn_readfirstlane(tile);
   const Sequence seq(a, b);
   if (split >= seq.splits) return;
   const int row0 = tile * S::rows, row = row0 + wave * 32 + n;
@@ -123,79 +123,70 @@ __global__ __launch_bounds__(TileShape<W>::threads, W <= 4 ? 2 : 1) void attend_
     const uint32_t w1 = __builtin_amdgcn_readlane((int)(where >> 32), u - looked);
     return (long long)((uint64_t)w1 << 32 | w0);
   };
-  int next0 = 0, next1 = 0;  // places of the requested tile's blocks that are the sequence's
-  Staged<W> st;
-  const bool key_wave = wave < S::key_waves;
-  // key wave w: block w / (waves / 4) of the tile; with 8 waves two to a block, an octet a lane, else two octets a lane
-  const int key_block = (wave * 4 / S::waves) & 1, key_octet = S::waves == 8 ? (wave & 1) * 2 + g : 2 * g;
-  const auto request = [&](int u) {
-    const long long w0 = block_at(u), w1 = block_at(u + 1);
-    // no page: any block, none of whose places count
-    const uint8_t *const at0 = a.kv.pages + max(w0, 0LL), *const at1 = a.kv.pages + max(w1, 0LL);
-    next0 = w0 < 0 ? 0 : min(seq.length - u * kKvBlock, kKvBlock);
-    next1 = w1 < 0 ? 0 : min(seq.length - (u + 1) * kKvBlock, kKvBlock);
+  // Tile t (blocks begin + B t ..) into slot t % ring: every wave copies a quarter of a block, also of tiles behind the
+  // last, whose bytes are the pool's first, so that the copies on their way are always as many.
+  uint32_t there = 0;  // bit b of pair t of the last tiles requested: block b has a page
+  int asked = 0, slot = 0;
+  const auto request = [&]() {
+    const int u = begin + B * asked;
+    const long long w0 = block_at(u), w1 = B > 1 ? block_at(u + 1) : -1;
+    there = there << 2 | (w0 >= 0 ? 1u : 0u) | (w1 >= 0 ? 2u : 0u);
+    const long long mine = B > 1 && wave >= 4 ? w1 : w0;
+    const uint64_t offset = mine < 0 ? 0 : (uint64_t)mine;
+    const uint8_t* const from =
+        a.kv.pages + ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(offset >> 32)) << 32 |
+                      (uint32_t)__builtin_amdgcn_readfirstlane((int)offset)) + (wave & 3) * 320 * W;
+    const uint32_t to = lds_addr(raw) + slot * S::raw + wave * 320 * W;
+#pragma unroll
+    for (int c = 0; c < S::copies; ++c)
+      if (1024 * c + lane * 16 < 320 * W) copy16_to_lds_s(from, 1024 * c + lane * 16, to + 1024 * c);
+    ++asked;
+    slot = slot + 1 == S::ring ? 0 : slot + 1;
+  };
+  // The places of block u, of the tile `back` requests before the last, that are the sequence's.
+  const auto places = [&](int u, int block, int back) {
+    return there >> (2 * back + block) & 1 ? max(min(seq.length - u * kKvBlock, kKvBlock), 0) : 0;
+  };
+  const bool key_wave = wave < NW - S::value_waves;
+  const int key_block = B > 1 ? wave >> 1 & 1 : 0, key_octet = (wave & 1) * 2 + g;
+  const auto widen = [&](int t, int from, int back, half8* to) {  // tile t, in slot `from`
+    const unsigned char* const tile_raw = raw + from * S::raw;
     if (key_wave) {
-      const uint8_t* const blk = key_block ? at1 : at0;
+      const unsigned char* const blk = tile_raw + key_block * 1280 * W;
+      uint32_t codes[W], sm[W];
 #pragma unroll
-      for (int c = 0; c < S::octets; ++c)
+      for (int w = 0; w < W; ++w) {
+        codes[w] = *(const uint32_t*)(blk + n * 16 * W + key_octet * 4 * W + w * 4);
+        sm[w] = *(const uint32_t*)(blk + kv_key_scales(W) + (n * W + w) * 4);
+      }
 #pragma unroll
-        for (int w = 0; w < W; ++w)
-          st.key.codes[c][w] = *(const uint32_t*)(blk + n * 16 * W + (key_octet + c) * 4 * W + w * 4);
-#pragma unroll
-      for (int w = 0; w < W; ++w) st.key.scales[w] = *(const uint32_t*)(blk + kv_key_scales(W) + (n * W + w) * 4);
+      for (int w = 0; w < W; ++w)
+        to[(key_block * 2 * W + 2 * w + (key_octet >> 1)) * 64 + (key_octet & 1) * 32 + n] = widen8(bits, codes[w], sm[w]);
     } else {
+      half4* const vt = (half4*)(to + S::frags * 64);
 #pragma unroll
-      for (int t = 0; t < S::items; ++t) {
-        const int item = (wave - S::key_waves) + t * (S::waves - S::key_waves);
-        if (item >= 2 * S::pairs) break;
-        const uint8_t* const blk = item & 1 ? at1 : at0;
-        const int pair = item >> 1, i = lane & 15, quad = lane >> 4;
+      for (int j = 0; j < S::items; ++j) {
+        const int item = wave - (NW - S::value_waves) + j * S::value_waves;
+        if (item >= B * S::pairs) break;
+        const int blk = item % B, pair = item / B, i = lane & 15, quad = lane >> 4;
+        const unsigned char* const from_blk = tile_raw + blk * 1280 * W;
         const bool two = 2 * pair + 1 < W;
+        const int have = places(begin + B * t + blk, blk, back);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {  // (group of the pair, half)
           if (k >= 2 && !two) break;
           const int group = 2 * pair + (k >> 1);
-          st.value.codes[t][k] = *(const uint32_t*)(blk + kv_value_codes(W) + kv_value_word(W, group, quad, i, k & 1));
-          st.value.scales[t][k] = *(const u32x4*)(blk + kv_value_scales(W) + (group * 8 + (k & 1) * 4 + quad) * 16);
-        }
-      }
-    }
-  };
-  const auto widen = [&](half8* to) {
-    if (key_wave) {
-#pragma unroll
-      for (int c = 0; c < S::octets; ++c)
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-          const int octet = key_octet + c;
-          to[(key_block * 2 * W + 2 * w + (octet >> 1)) * 64 + (octet & 1) * 32 + n] =
-              widen8(bits, st.key.codes[c][w], st.key.scales[w]);
-        }
-    } else {
-      half4* const vt = (half4*)(to + S::frags * 64);
-#pragma unroll
-      for (int t = 0; t < S::items; ++t) {
-        const int item = (wave - S::key_waves) + t * (S::waves - S::key_waves);
-        if (item >= 2 * S::pairs) break;
-        const int blk = item & 1, pair = item >> 1, i = lane & 15, quad = lane >> 4;
-        const bool two = 2 * pair + 1 < W;
-        const int have = blk ? next1 : next0;
-        if (have < kKvBlock) {  // behind the sequence's end, or no page: whatever is there, 0
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
+          const uint32_t codes = *(const uint32_t*)(from_blk + kv_value_codes(W) + kv_value_word(W, group, quad, i, k & 1));
+          u32x4 sm = *(const u32x4*)(from_blk + kv_value_scales(W) + (group * 8 + (k & 1) * 4 + quad) * 16);
+          if (have < kKvBlock) {  // behind the sequence's end, or no page: whatever is there, 0
             const int first = (k & 1) * 16 + quad * 4;
             const uint32_t keep02 = (first < have ? 0xFFFFu : 0u) | (first + 2 < have ? 0xFFFF0000u : 0u);
             const uint32_t keep13 = (first + 1 < have ? 0xFFFFu : 0u) | (first + 3 < have ? 0xFFFF0000u : 0u);
-            u32x4& sm = st.value.scales[t][k];
             sm[0] &= keep02, sm[1] &= keep13, sm[2] &= keep02, sm[3] &= keep13;
           }
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (k >= 2 && !two) break;
           half4 v0, v1;
-          value4(bits, st.value.codes[t][k], st.value.scales[t][k], v0, v1);
-          half4* const p = vt + ((((blk * 2 + (k & 1)) * W + 2 * pair + (k >> 1)) * 64 + (quad & 1) * 32 + 2 * i) * 2 + (quad >> 1));
+          value4(bits, codes, sm, v0, v1);
+          half4* const p = vt + ((((blk * 2 + (k & 1)) * W + group) * 64 + (quad & 1) * 32 + 2 * i) * 2 + (quad >> 1));
           p[0] = v0;
           p[2] = v1;
         }
@@ -203,85 +194,115 @@ __global__ __launch_bounds__(TileShape<W>::threads, W <= 4 ? 2 : 1) void attend_
     }
   };
 
-  int turn = 0;  // the half of LDS that holds the present tile
-  int have0 = 0, have1 = 0;
-  if (begin < end) {
-    request(begin);
-    widen(lds);
-    have0 = next0, have1 = next1;
-  }
-  __syncthreads();
-  for (int u = begin; u < end; u += 2) {
-    const half8* const kt = lds + turn * 2 * S::frags * 64;
-    const half8* const vt = kt + S::frags * 64;
-    const bool more = u + 2 < end;
-    if (more) request(u + 2);
-    f32x16 s[2];
+  const int tiles = begin < end ? (end - begin + B - 1) / B : 0;
+  half8 p[2 * B];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < 2 * B; ++i) p[i] = half8{};
+  const auto add_values = [&](const half8* vt) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) s[i][j] = 0.0f;
-#pragma unroll
-    for (int k = 0; k < 2 * W; ++k)
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        s[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kt[(i * 2 * W + k) * 64 + lane], q[k], s[i], 0, 0, 0);
-    const int first = u * kKvBlock;
-    const bool inside = have0 == kKvBlock && have1 == kKvBlock && first >= inside_lo && first + kTilePlaces <= inside_hi;
-    if (!inside) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          const int t = j / 4 * 8 + g * 4 + j % 4, at = first + i * kKvBlock + t;
-          if (t >= (i ? have1 : have0) || at >= limit || at < low) s[i][j] = -INFINITY;
-        }
-    }
-    // p against the row's reference so far: a sum within float16's range says that every p is. A row's first places, whose
-    // reference is the lowest of all, sum to +inf.
-    half8 p[4];
-    float sum = 0.0f;
-    const auto probabilities = [&]() {
-      const float ref = kProbShift - m;
-      sum = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float e[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          e[j] = exp2_(fmaf(s[i >> 1][(i & 1) * 8 + j], back, ref));
-          sum += e[j];
-        }
-        p[i] = prob_order(e);
-      }
-    };
-    probabilities();
-    if (__any(!(sum <= kProbMost))) {
-      float top = s[0][0];
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) top = fmaxf(top, s[i][j]);
-      top = fmaxf(top, __shfl_xor(top, 32));
-      const float m2 = fmaxf(m, top * back), alpha = exp2_(m - m2);
-      m = m2;
-      l *= alpha;
-#pragma unroll
-      for (int i = 0; i < W; ++i) o[i] *= alpha;
-      probabilities();
-    }
-    l += sum;
-#pragma unroll
-    for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < 2 * B; ++k)
 #pragma unroll
       for (int i = 0; i < W; ++i)
         o[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vt[(k * W + i) * 64 + lane], p[k], o[i], 0, 0, 0);
-    if (more) {
-      turn ^= 1;
-      widen(lds + turn * 2 * S::frags * 64);
-      have0 = next0, have1 = next1;
+  };
+  // A tile is two steps, with a barrier behind each: the matrix instructions of the last tile's values and of this one's
+  // scores, then the exponentials and the widening of the next tile. Where two waves share a SIMD, the value waves are a
+  // step behind the key waves, so that one has the matrix unit while the other has the vector unit. (Values of tile t + 1
+  // are written where those of t - 1 were, which both have read by then; keys of t + 1 while the value waves read those of
+  // t.) A wave's copies of tile t + 1 have landed by the barrier before the key waves widen it: ring - 2 later tiles are on
+  // their way then.
+  const bool behind = NW == 8 && !key_wave;
+  if (tiles > 0) {
+    for (int i = 0; i < S::ring; ++i) request();
+    for (int i = threadIdx.x; i < S::frags * 64; i += S::threads) lds[3 * S::frags * 64 + i] = half8{};
+    wait_vmcnt((S::ring - 1) * S::copies);
+    lds_barrier();
+    widen(0, 0, S::ring - 1, lds);
+    if (behind) wait_vmcnt((S::ring - 2) * S::copies);
+    lds_barrier();
+    if (behind) lds_barrier();
+    int turn = 0;  // the half of LDS that holds the present tile
+    for (int t = 0; t < tiles; ++t) {
+      const int u = begin + B * t;
+      const half8* const kt = lds + turn * 2 * S::frags * 64;
+      add_values(lds + ((turn ^ 1) * 2 + 1) * S::frags * 64);  // of the first tile: zeros
+      f32x16 s[B];
+#pragma unroll
+      for (int i = 0; i < B; ++i)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[i][j] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < 2 * W; ++k)
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+          s[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kt[(i * 2 * W + k) * 64 + lane], q[k], s[i], 0, 0, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, kAhead, 0);
+#pragma unroll
+      for (int i = 0; i < 4 * W * B - kAhead; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+      if (!behind) wait_vmcnt((S::ring - 2) * S::copies);
+      lds_barrier();
+
+      const int first = u * kKvBlock;
+      const int have0 = places(u, 0, S::ring - 1), have1 = B > 1 ? places(u + 1, 1, S::ring - 1) : 0;
+      const bool inside = have0 == kKvBlock && (B == 1 || have1 == kKvBlock) && first >= inside_lo &&
+                          first + B * kKvBlock <= inside_hi;
+      if (!inside) {
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int at = j / 4 * 8 + g * 4 + j % 4, place_ = first + i * kKvBlock + at;
+            if (at >= (i ? have1 : have0) || place_ >= limit || place_ < low) s[i][j] = -INFINITY;
+          }
+      }
+      // p against the row's reference so far: a sum within float16's range says that every p is. A row's first places,
+      // whose reference is the lowest of all, sum to +inf.
+      float sum = 0.0f;
+      const auto probabilities = [&]() {
+        const float ref = kProbShift - m;
+        sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2 * B; ++i) {
+          float e[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            e[j] = exp2_(fmaf(s[i >> 1][(i & 1) * 8 + j], back, ref));
+            sum += e[j];
+          }
+          p[i] = prob_order(e);
+        }
+      };
+      probabilities();
+      if (__any(!(sum <= kProbMost))) {
+        float top = s[0][0];
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) top = fmaxf(top, s[i][j]);
+        top = fmaxf(top, __shfl_xor(top, 32));
+        const float m2 = fmaxf(m, top * back), alpha = exp2_(m - m2);
+        m = m2;
+        l *= alpha;
+#pragma unroll
+        for (int i = 0; i < W; ++i) o[i] *= alpha;
+        probabilities();
+      }
+      l += sum;
+      if (t + 1 < tiles) {
+        turn ^= 1;
+        widen(t + 1, (t + 1) % S::ring, S::ring - 2, lds + turn * 2 * S::frags * 64);
+      }
+      request();
+      if (behind) wait_vmcnt((S::ring - 2) * S::copies);
+      lds_barrier();
     }
-    __syncthreads();
+    add_values(lds + (turn * 2 + 1) * S::frags * 64);
+    if (NW == 8 && key_wave) lds_barrier();
+    wait_vmcnt(0);  // no copy outlives the workgroup's LDS
   }
   l += __shfl_xor(l, 32);
   if (!live) return;
@@ -319,26 +340,28 @@ __global__ __launch_bounds__(TileShape<W>::threads, W <= 4 ? 2 : 1) void attend_
   }
 }
 
-template <int W>
+template <int W, int NW>
 void launch_w(const AttendArgs& a, long long tiles, hipStream_t stream) {
-  using S = TileShape<W>;
-  constexpr size_t lds = 4 * (size_t)S::frags * 1024;
+  using S = TileShape<W, NW>;
   static const hipError_t once =
-      hipFuncSetAttribute((const void*)attend_tile_kernel<W>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+      hipFuncSetAttribute((const void*)attend_tile_kernel<W, NW>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)S::lds);
   (void)once;
-  hipLaunchKernelGGL(attend_tile_kernel<W>, dim3((unsigned)(tiles * a.kv.heads), a.splits), dim3(S::threads), lds,
+  hipLaunchKernelGGL((attend_tile_kernel<W, NW>), dim3((unsigned)(tiles * a.kv.heads), a.splits), dim3(S::threads), S::lds,
                      stream, a);
 }
 
 }  // namespace
 
-int attend_tile_rows(int dim) { return kv_groups(dim) <= 4 ? TileShape<4>::rows : TileShape<8>::rows; }
-
-void launch_attend_tile(const AttendArgs& a, long long tiles, hipStream_t stream) {
+void launch_attend_tile(const AttendArgs& a, int rows, long long tiles, hipStream_t stream) {
+  const bool wide = rows == TileShape<1, 8>::rows;
   switch (kv_groups(a.dim)) {
 #define MXA_CASE(W) \
-  case W: launch_w<W>(a, tiles, stream); break;
-    MXA_CASE(1) MXA_CASE(2) MXA_CASE(3) MXA_CASE(4) MXA_CASE(5) MXA_CASE(6) MXA_CASE(7) MXA_CASE(8)
+  case W: wide ? launch_w<W, 8>(a, tiles, stream) : launch_w<W, 4>(a, tiles, stream); break;
+    MXA_CASE(1) MXA_CASE(2) MXA_CASE(3) MXA_CASE(4)
+#undef MXA_CASE
+#define MXA_CASE(W) \
+  case W: launch_w<W, 4>(a, tiles, stream); break;
+    MXA_CASE(5) MXA_CASE(6) MXA_CASE(7) MXA_CASE(8)
 #undef MXA_CASE
   }
 }
