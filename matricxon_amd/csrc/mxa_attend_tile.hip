@@ -42,6 +42,21 @@ struct TileShape {
   static constexpr size_t lds = 4 * (size_t)frags * 1024 + (size_t)ring * raw;
 };
 
+// A thread's share of a tile, as it is in the cache.
+template <int W, int NW>
+struct Packed {
+  using S = TileShape<W, NW>;
+  union {
+    struct {
+      uint32_t codes[W], scales[W];
+    } key;
+    struct {
+      uint32_t codes[S::items][4];
+      u32x4 scales[S::items][4];
+    } value;
+  };
+};
+
 template <int W, int NW>
 __global__ __launch_bounds__(64 * NW, W <= 4 ? 2 : 1) void attend_tile_kernel(AttendArgs a) {
   using S = TileShape<W, NW>;
@@ -111,37 +126,38 @@ __global__ __launch_bounds__(64 * NW, W <= 4 ? 2 : 1) void attend_tile_kernel(At
   // Lane i knows where the i-th of 64 blocks lies; every wave looks up the same.
   const int blocks_of_page = a.kv.page / kKvBlock;
   long long where = -1;
-  int looked = begin - 64;  // the block that lane 0 has
-  const auto block_at = [&](int u) -> long long {  // -1: no page, or behind the last
-    if (u >= end) return -1;
-    if (u >= looked + 64) {
-      looked = u;
-      const long long block = u + lane < end ? kv_block(a.kv, b, (u + lane) * kKvBlock) : -1;
-      where = block < 0 ? -1 : (block + (long long)h * blocks_of_page) * kv_block_bytes(W);
-    }
-    const uint32_t w0 = __builtin_amdgcn_readlane((int)(uint32_t)where, u - looked);
-    const uint32_t w1 = __builtin_amdgcn_readlane((int)(where >> 32), u - looked);
-    return (long long)((uint64_t)w1 << 32 | w0);
+  int looked = begin - 64;  // the block that lane 0 has (a multiple of 2 from begin: a tile's blocks are in one look)
+  const auto look_up = [&](int u) {
+    looked = u;
+    const long long block = u + lane < end ? kv_block(a.kv, b, (u + lane) * kKvBlock) : -1;
+    where = block < 0 ? -1 : (block + (long long)h * blocks_of_page) * kv_block_bytes(W);
   };
   // Tile t (blocks begin + B t ..) into slot t % ring: every wave copies a quarter of a block, also of tiles behind the
   // last, whose bytes are the pool's first, so that the copies on their way are always as many.
   uint32_t there = 0;  // bit b of pair t of the last tiles requested: block b has a page
-  int asked = 0, slot = 0;
+  int asked = begin, slot = 0;  // the first block of the next tile, and its slot
   const auto request = [&]() {
-    const int u = begin + B * asked;
-    const long long w0 = block_at(u), w1 = B > 1 ? block_at(u + 1) : -1;
-    there = there << 2 | (w0 >= 0 ? 1u : 0u) | (w1 >= 0 ? 2u : 0u);
-    const long long mine = B > 1 && wave >= 4 ? w1 : w0;
-    const uint64_t offset = mine < 0 ? 0 : (uint64_t)mine;
-    const uint8_t* const from =
-        a.kv.pages + ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(offset >> 32)) << 32 |
-                      (uint32_t)__builtin_amdgcn_readfirstlane((int)offset)) + (wave & 3) * 320 * W;
+    uint32_t lo[B], hi[B];
+    there <<= 2;
+#pragma unroll
+    for (int i = 0; i < B; ++i) {
+      lo[i] = __builtin_amdgcn_readlane((int)(uint32_t)where, (asked + i - looked) & 63);
+      hi[i] = __builtin_amdgcn_readlane((int)(where >> 32), (asked + i - looked) & 63);
+      there |= (hi[i] >> 31 ^ 1) << i;
+    }
+    const bool second = B > 1 && wave >= 4;
+    uint32_t l = second ? lo[B - 1] : lo[0], u = second ? hi[B - 1] : hi[0];
+    if (u >> 31) l = u = 0;
+    const uint8_t* const from = a.kv.pages + ((uint64_t)u << 32 | l) + (wave & 3) * 320 * W;
     const uint32_t to = lds_addr(raw) + slot * S::raw + wave * 320 * W;
 #pragma unroll
     for (int c = 0; c < S::copies; ++c)
       if (1024 * c + lane * 16 < 320 * W) copy16_to_lds_s(from, 1024 * c + lane * 16, to + 1024 * c);
-    ++asked;
+    asked += B;
     slot = slot + 1 == S::ring ? 0 : slot + 1;
+  };
+  const auto prepare = [&]() {  // for the next request
+    if (asked >= looked + 64) look_up(asked);
   };
   // The places of block u, of the tile `back` requests before the last, that are the sequence's.
   const auto places = [&](int u, int block, int back) {
@@ -149,19 +165,39 @@ __global__ __launch_bounds__(64 * NW, W <= 4 ? 2 : 1) void attend_tile_kernel(At
   };
   const bool key_wave = wave < NW - S::value_waves;
   const int key_block = B > 1 ? wave >> 1 & 1 : 0, key_octet = (wave & 1) * 2 + g;
-  const auto widen = [&](int t, int from, int back, half8* to) {  // tile t, in slot `from`
+  Packed<W, NW> packed;
+  const auto unpack = [&](int from) {  // a thread's share of the tile in slot `from`
     const unsigned char* const tile_raw = raw + from * S::raw;
     if (key_wave) {
       const unsigned char* const blk = tile_raw + key_block * 1280 * W;
-      uint32_t codes[W], sm[W];
 #pragma unroll
       for (int w = 0; w < W; ++w) {
-        codes[w] = *(const uint32_t*)(blk + n * 16 * W + key_octet * 4 * W + w * 4);
-        sm[w] = *(const uint32_t*)(blk + kv_key_scales(W) + (n * W + w) * 4);
+        packed.key.codes[w] = *(const uint32_t*)(blk + n * 16 * W + key_octet * 4 * W + w * 4);
+        packed.key.scales[w] = *(const uint32_t*)(blk + kv_key_scales(W) + (n * W + w) * 4);
       }
+    } else {
+#pragma unroll
+      for (int j = 0; j < S::items; ++j) {
+        const int item = wave - (NW - S::value_waves) + j * S::value_waves;
+        if (item >= B * S::pairs) break;
+        const int pair = item / B, i = lane & 15, quad = lane >> 4;
+        const unsigned char* const blk = tile_raw + item % B * 1280 * W;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {  // (group of the pair, half)
+          if (k >= 2 && 2 * pair + 1 >= W) break;
+          const int group = 2 * pair + (k >> 1);
+          packed.value.codes[j][k] = *(const uint32_t*)(blk + kv_value_codes(W) + kv_value_word(W, group, quad, i, k & 1));
+          packed.value.scales[j][k] = *(const u32x4*)(blk + kv_value_scales(W) + (group * 8 + (k & 1) * 4 + quad) * 16);
+        }
+      }
+    }
+  };
+  const auto widen = [&](int u, int back, half8* to) {  // it, of first block u, into the operands
+    if (key_wave) {
 #pragma unroll
       for (int w = 0; w < W; ++w)
-        to[(key_block * 2 * W + 2 * w + (key_octet >> 1)) * 64 + (key_octet & 1) * 32 + n] = widen8(bits, codes[w], sm[w]);
+        to[(key_block * 2 * W + 2 * w + (key_octet >> 1)) * 64 + (key_octet & 1) * 32 + n] =
+            widen8(bits, packed.key.codes[w], packed.key.scales[w]);
     } else {
       half4* const vt = (half4*)(to + S::frags * 64);
 #pragma unroll
@@ -169,24 +205,24 @@ __global__ __launch_bounds__(64 * NW, W <= 4 ? 2 : 1) void attend_tile_kernel(At
         const int item = wave - (NW - S::value_waves) + j * S::value_waves;
         if (item >= B * S::pairs) break;
         const int blk = item % B, pair = item / B, i = lane & 15, quad = lane >> 4;
-        const unsigned char* const from_blk = tile_raw + blk * 1280 * W;
-        const bool two = 2 * pair + 1 < W;
-        const int have = places(begin + B * t + blk, blk, back);
+        const int have = places(u + blk, blk, back);
+        if (have < kKvBlock) {  // behind the sequence's end, or no page: whatever is there, 0
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {  // (group of the pair, half)
-          if (k >= 2 && !two) break;
-          const int group = 2 * pair + (k >> 1);
-          const uint32_t codes = *(const uint32_t*)(from_blk + kv_value_codes(W) + kv_value_word(W, group, quad, i, k & 1));
-          u32x4 sm = *(const u32x4*)(from_blk + kv_value_scales(W) + (group * 8 + (k & 1) * 4 + quad) * 16);
-          if (have < kKvBlock) {  // behind the sequence's end, or no page: whatever is there, 0
+          for (int k = 0; k < 4; ++k) {
             const int first = (k & 1) * 16 + quad * 4;
             const uint32_t keep02 = (first < have ? 0xFFFFu : 0u) | (first + 2 < have ? 0xFFFF0000u : 0u);
             const uint32_t keep13 = (first + 1 < have ? 0xFFFFu : 0u) | (first + 3 < have ? 0xFFFF0000u : 0u);
+            u32x4& sm = packed.value.scales[j][k];
             sm[0] &= keep02, sm[1] &= keep13, sm[2] &= keep02, sm[3] &= keep13;
           }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (k >= 2 && 2 * pair + 1 >= W) break;
           half4 v0, v1;
-          value4(bits, codes, sm, v0, v1);
-          half4* const p = vt + ((((blk * 2 + (k & 1)) * W + group) * 64 + (quad & 1) * 32 + 2 * i) * 2 + (quad >> 1));
+          value4(bits, packed.value.codes[j][k], packed.value.scales[j][k], v0, v1);
+          half4* const p =
+              vt + ((((blk * 2 + (k & 1)) * W + 2 * pair + (k >> 1)) * 64 + (quad & 1) * 32 + 2 * i) * 2 + (quad >> 1));
           p[0] = v0;
           p[2] = v1;
         }
@@ -209,22 +245,29 @@ __global__ __launch_bounds__(64 * NW, W <= 4 ? 2 : 1) void attend_tile_kernel(At
   // scores, then the exponentials and the widening of the next tile. Where two waves share a SIMD, the value waves are a
   // step behind the key waves, so that one has the matrix unit while the other has the vector unit. (Values of tile t + 1
   // are written where those of t - 1 were, which both have read by then; keys of t + 1 while the value waves read those of
-  // t.) A wave's copies of tile t + 1 have landed by the barrier before the key waves widen it: ring - 2 later tiles are on
-  // their way then.
+  // t.) A tile is requested ring - 1 tiles before it is computed, in the first step, when both have unpacked the slot's last.
+  // A wave's copies of tile t + 1 have landed by the barrier before the key waves unpack it: ring - 2 later tiles are on
+  // their way then, of the value waves' one less.
   const bool behind = NW == 8 && !key_wave;
   if (tiles > 0) {
-    for (int i = 0; i < S::ring; ++i) request();
+    for (int i = 0; i < S::ring - 1; ++i) {
+      prepare();
+      request();
+    }
+    prepare();
     for (int i = threadIdx.x; i < S::frags * 64; i += S::threads) lds[3 * S::frags * 64 + i] = half8{};
-    wait_vmcnt((S::ring - 1) * S::copies);
+    wait_vmcnt((S::ring - 2) * S::copies);
     lds_barrier();
-    widen(0, 0, S::ring - 1, lds);
-    if (behind) wait_vmcnt((S::ring - 2) * S::copies);
+    unpack(0);
+    widen(begin, S::ring - 2, lds);
+    if (behind) wait_vmcnt((S::ring - 3) * S::copies);
     lds_barrier();
     if (behind) lds_barrier();
     int turn = 0;  // the half of LDS that holds the present tile
     for (int t = 0; t < tiles; ++t) {
       const int u = begin + B * t;
       const half8* const kt = lds + turn * 2 * S::frags * 64;
+      request();
       add_values(lds + ((turn ^ 1) * 2 + 1) * S::frags * 64);  // of the first tile: zeros
       f32x16 s[B];
 #pragma unroll
@@ -245,6 +288,8 @@ __global__ __launch_bounds__(64 * NW, W <= 4 ? 2 : 1) void attend_tile_kernel(At
       __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
       if (!behind) wait_vmcnt((S::ring - 2) * S::copies);
       lds_barrier();
+      const int next = t + 1 & S::ring - 1;
+      if (t + 1 < tiles) unpack(next);
 
       const int first = u * kKvBlock;
       const int have0 = places(u, 0, S::ring - 1), have1 = B > 1 ? places(u + 1, 1, S::ring - 1) : 0;
@@ -294,10 +339,10 @@ __global__ __launch_bounds__(64 * NW, W <= 4 ? 2 : 1) void attend_tile_kernel(At
       l += sum;
       if (t + 1 < tiles) {
         turn ^= 1;
-        widen(t + 1, (t + 1) % S::ring, S::ring - 2, lds + turn * 2 * S::frags * 64);
+        widen(u + B, S::ring - 2, lds + turn * 2 * S::frags * 64);
       }
-      request();
-      if (behind) wait_vmcnt((S::ring - 2) * S::copies);
+      prepare();
+      if (behind) wait_vmcnt((S::ring - 3) * S::copies);
       lds_barrier();
     }
     add_values(lds + (turn * 2 + 1) * S::frags * 64);
