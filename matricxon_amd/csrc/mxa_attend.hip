@@ -35,7 +35,7 @@ __global__ __launch_bounds__(kAttendThreads, W <= 4 ? 3 : 2) void attend_kernel(
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
   const int split = blockIdx.x, h = blockIdx.y % a.kv.heads, rt = blockIdx.y / a.kv.heads, b = blockIdx.z;
-  const Sequence seq(a, b);
+  const Sequence seq = Sequence(a, b).uniform();
   if (rt >= seq.tiles || split >= seq.splits) return;
   const int begin = split * seq.chunk, end = min(begin + seq.chunk, seq.blocks);
   const int blocks_of_page = a.kv.page / kKvBlock;
@@ -258,10 +258,35 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join_kernel(AttendArgs 
   for (int j = 0; j < 4; ++j) dst[4 * tid + j] = bf16_rne(v[j] * norm);
 }
 
+// The same for few parts: a workgroup takes the 16 rows of a pair, sixteen threads each.
+__global__ __launch_bounds__(kAttendThreads) void attend_join_rows_kernel(AttendArgs a, int W) {
+  const int b = blockIdx.y, pair = blockIdx.x, r = threadIdx.x >> 4, piece = threadIdx.x & 15;
+  const int h = pair % a.kv.heads, rt = pair / a.kv.heads;
+  const Sequence seq(a, b);
+  if (rt * 16 + r >= seq.rows) return;
+  float top = -INFINITY, total = 0.0f;
+  for (int i = 0; i < a.splits; ++i) top = fmaxf(top, a.part_of(b, pair, i, W).ml[r]);
+  for (int i = 0; i < a.splits; ++i) {
+    const AttendPart p = a.part_of(b, pair, i, W);
+    total += exp2_(p.ml[r] - top) * p.ml[16 + r];
+  }
+  const float norm = total > 0.0f || total != total ? 1.0f / total : 0.0f;
+  uint16_t* const dst = a.out_row(seq.first + (rt * 16 + r) / a.group, h * a.group + (rt * 16 + r) % a.group);
+  for (int d = 4 * piece; d < a.dim; d += 64) {
+    f32x4 v{0, 0, 0, 0};
+    for (int i = 0; i < a.splits; ++i) {
+      const AttendPart p = a.part_of(b, pair, i, W);
+      v += exp2_(p.ml[r] - top) * *(const f32x4*)(p.o + r * 32 * W + d);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) dst[d + j] = bf16_rne(v[j] * norm);
+  }
+}
+
 // (std::min and std::max here: on the host, HIP's own of that name take ints.)
 // How the places of up to `most` tokens of each sequence are shared out. Sequences of up to kFewRows rows a key head go in
 // tiles of 16 rows (attend_kernel), others in those of attend_tile_kernel; a call without query_starts has one kind.
-constexpr int kFewRows = 64;
+constexpr int kFewRows = 64, kTileSplits = 16;
 struct Plan {
   bool few, many;     // the kinds that there may be
   long long pairs[2]; // (tile of 16 rows, key head) of a sequence
@@ -293,15 +318,20 @@ Plan plan_of(int n_seq, int n_tokens, bool ragged, int kv_heads, int group, int 
   }
   if (p.many) {
     p.pairs[1] = (most + 15) / 16 * kv_heads;
-    for (p.rows = narrow ? 256 : 128;; p.rows = 128) {
-      p.tiles = ragged ? most / p.rows + std::min<long long>(n_seq, most / (kFewRows + 1))
-                       : (most + p.rows - 1) / p.rows * n_seq;
-      if (p.rows == 128 || p.tiles * kv_heads >= 256) break;  // 256 rows only where they fill the CUs
+    p.rows = narrow && most > 128 ? 256 : 128;
+    p.tiles = ragged ? most / p.rows + std::min<long long>(n_seq, most / (kFewRows + 1)) : (most + p.rows - 1) / p.rows * n_seq;
+    const long long span = window > 0 ? std::min<long long>(max_length, window + p.rows / group) / kKvBlock + 2 : blocks;
+    const long long groups = p.tiles * kv_heads, slots = narrow && p.rows == 128 ? 512 : 256;
+    // Parts of a tile's places, by what they cost: as many rounds of the CUs as the workgroups take, each a part's blocks
+    // and some 10 blocks' time to begin and end, and the join
+    double least = 0;
+    for (int n = 1; n <= kTileSplits && (n == 1 || span / n >= 8); ++n) {
+      const double cost = (double)((groups * n + slots - 1) / slots) * ((double)span / n + 10) + (n > 1 ? 8 : 0);
+      if (n == 1 || cost < 0.95 * least) least = cost, p.splits[1] = n;
     }
-    share_out(blocks, p.tiles * kv_heads, narrow ? 512 : 256, 8, p.splits[1], p.chunk[1]);
     // the workspace has room for as many rows of each sequence as any may have: not split where that is large
     if ((long long)n_seq * p.pairs[1] * p.splits[1] * part_floats(kv_groups(dim)) > 16 << 20) p.splits[1] = 1;
-    if (p.splits[1] == 1) p.chunk[1] = 1 << 26;
+    p.chunk[1] = 0;
   }
   return p;
 }
@@ -341,7 +371,9 @@ int launch_attend(AttendArgs a, int max_length, void* workspace, hipStream_t str
 #undef MXA_CASE
       }
     }
-    if (a.splits > 1)
+    if (a.splits > 1 && kind == 1)
+      hipLaunchKernelGGL(attend_join_rows_kernel, dim3(a.pairs, a.kv.n_seq), dim3(kAttendThreads), 0, stream, a, W);
+    else if (a.splits > 1)
       hipLaunchKernelGGL(attend_join_kernel, dim3(16, a.pairs, a.kv.n_seq), dim3(kAttendThreads), 0, stream, a, W);
   }
   return 0;

@@ -41,7 +41,8 @@ struct AttendArgs {
   KvPages kv;
   int n_tokens, seq, dim, heads, group, window;  // token t is step t % seq of q's batch entry t / seq
   int least_rows, most_rows;  // sequences of fewer or more rows a key head are left out
-  int pairs, splits, chunk;  // of the grid: pairs and splits of a sequence, blocks of a split at least
+  int pairs, splits, chunk;  // of the grid: pairs and splits of a sequence, blocks of a split at least (0: each tile in
+                             // `splits` even parts)
   float scale;
 
   __device__ __forceinline__ const uint16_t* q_row(int t, int h) const {
@@ -63,6 +64,16 @@ struct Sequence {
   int length, place0;  // its tokens, the place of its first row
   int first_block, blocks;
   int chunk, splits;  // blocks of a split, splits that have any
+  // The same in scalar registers, where b is one for all lanes.
+  __device__ __forceinline__ Sequence uniform() const {
+    Sequence s = *this;
+    s.first = __builtin_amdgcn_readfirstlane(first), s.count = __builtin_amdgcn_readfirstlane(count);
+    s.rows = __builtin_amdgcn_readfirstlane(rows), s.tiles = __builtin_amdgcn_readfirstlane(tiles);
+    s.length = __builtin_amdgcn_readfirstlane(length), s.place0 = __builtin_amdgcn_readfirstlane(place0);
+    s.first_block = __builtin_amdgcn_readfirstlane(first_block), s.blocks = __builtin_amdgcn_readfirstlane(blocks);
+    s.chunk = __builtin_amdgcn_readfirstlane(chunk), s.splits = __builtin_amdgcn_readfirstlane(splits);
+    return s;
+  }
   __host__ __device__ inline Sequence(const AttendArgs& a, int b) {
     kv_rows_of(a.kv, b, a.n_tokens, first, count);
     const long long all = (long long)count * a.group;
@@ -78,7 +89,7 @@ struct Sequence {
     if (blocks < 1) blocks = 1;
     const int least = (blocks + a.splits - 1) / a.splits;  // more where a length passes what the host was told
     chunk = a.chunk > least ? a.chunk : least;
-    splits = (blocks + chunk - 1) / chunk;
+    splits = a.chunk > 0 ? (blocks + chunk - 1) / chunk : a.splits;
   }
 };
 

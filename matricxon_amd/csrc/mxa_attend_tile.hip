@@ -70,8 +70,7 @@ __global__ __launch_bounds__(64 * NW, W <= 4 ? 2 : 1) void attend_tile_kernel(At
   int b, tile;
   if (!find_tile(a, blockIdx.x / a.kv.heads, S::rows, b, tile)) return;
   b = __builtin_amdgcn_readfirstlane(b), tile = __builtin_amdgcn_readfirstlane(tile);
-  const Sequence seq(a, b);
-  if (split >= seq.splits) return;
+  const Sequence seq = Sequence(a, b).uniform();
   const int row0 = tile * S::rows, row = row0 + wave * 32 + n;
   const bool live = row < seq.rows;
   const int place = seq.place0 + (live ? row / a.group : 0);
@@ -80,9 +79,9 @@ __global__ __launch_bounds__(64 * NW, W <= 4 ? 2 : 1) void attend_tile_kernel(At
   const int last = min(row0 + S::rows, seq.rows) - 1;
   const int hi = min(max(seq.place0 + last / a.group + 1, 0), seq.length);
   const int lo = a.window > 0 ? max(max(seq.place0 + row0 / a.group + 1, 0) - a.window, 0) : 0;
-  const int begin = max(seq.first_block + split * seq.chunk, lo / kKvBlock);
-  const int end = min(min(seq.first_block + min((split + 1) * seq.chunk, seq.blocks), (hi + kKvBlock - 1) / kKvBlock),
-                      a.kv.width * (a.kv.page / kKvBlock));
+  const int first_block = lo / kKvBlock, blocks = max((hi + kKvBlock - 1) / kKvBlock - first_block, 0);
+  const int part_blocks = ((blocks + a.splits - 1) / a.splits + B - 1) / B * B;
+  const int begin = first_block + min(split * part_blocks, blocks), end = first_block + min((split + 1) * part_blocks, blocks);
   const CodeBits bits;
 
   // q, by a power of two
@@ -351,7 +350,7 @@ __global__ __launch_bounds__(64 * NW, W <= 4 ? 2 : 1) void attend_tile_kernel(At
   }
   l += __shfl_xor(l, 32);
   if (!live) return;
-  if (seq.splits == 1) {
+  if (a.splits == 1) {
     const float norm = l > 0.0f || l != l ? 1.0f / l : 0.0f;
     uint16_t* const dst = a.out_row(seq.first + row / a.group, h * a.group + row % a.group);
 #pragma unroll
