@@ -20,7 +20,7 @@
 namespace mxa {
 namespace {
 
-constexpr int kHeadThreads = 256, kHeadBatch = 4;
+constexpr int kHeadThreads = 256, kHeadBatch = 3;
 
 struct HeadSide {
   const void* x;
@@ -136,7 +136,62 @@ __global__ __launch_bounds__(kHeadThreads) void heads_kernel(HeadArgs a, int TP,
     return (const T*)s.x + (long long)b * s.batch + (long long)(t - b * a.seq) * s.tok + (long long)h * s.head;
   };
 
+  const int per = kHeadThreads / L, c = tid % L;
+  const int CR = FAST ? (INTER ? a.rot / V : half / V) : 0, C = FAST ? CR + (a.dim - a.rot) / V : 0;
+  const bool turned = c < CR;
+  const int at = turned ? c * V : a.rot + (c - CR) * V;  // the lane's vector in a head, and its partner's at half + at
+  const bool paired = !INTER && turned;
+
+  struct Row {
+    bool live, isq;
+    int t, h, hh;
+  };
+  const auto row_of = [&](int r) {
+    Row w;
+    w.live = r < rows;
+    w.t = w.live ? r / H : 0;
+    w.hh = w.live ? r - w.t * H : 0;
+    w.isq = w.hh < nq;
+    w.h = w.isq ? q0 + w.hh : k0 + w.hh - nq;
+    return w;
+  };
+  // The rows of a batch, and a quad's values, are requested before what depends on the page table and the positions.
+  Piece x[kHeadBatch], y[kHeadBatch];
+  const auto load_rows = [&](int base) {
+#pragma unroll
+    for (int j = 0; j < kHeadBatch; ++j) {
+      const Row w = row_of(base + j * per + tid / L);
+      if (w.live && c < C) {
+        const T* const src = from(w.isq ? a.q : a.k, tok0 + w.t, w.h) + at;
+        x[j].v = *(const Vv*)src;
+        if (paired) y[j].v = *(const Vv*)(src + half);
+      }
+    }
+  };
+  // Four tokens' values of a head's group go to sixteen lanes: lane % 4 the octet, lane / 4 % 4 the token.
+  const int vlanes = 16 * W * nk, quads = (nt + 3) / 4;  // of four tokens
+  struct Place {
+    bool live, here;
+    int qd, h, gg, t, o;
+  };
+  const auto value_of = [&](int item) {
+    Place v;
+    v.live = item < quads * vlanes;
+    v.qd = v.live ? item / vlanes : 0;
+    const int in = v.live ? item - v.qd * vlanes : 0;
+    v.h = in / (16 * W);
+    v.gg = in / 16 % W;
+    v.t = v.qd * 4 + (in >> 2 & 3);
+    v.o = 4 * v.gg + (in & 3);
+    v.here = v.live && v.t < nt && v.o * 8 < a.dim;
+    return v;
+  };
+  typedef typename Vec<T, 8>::type V8;
+  V8 first_values{};
+  if constexpr (FAST) load_rows(0);
   if constexpr (CACHE) {
+    const Place v = value_of(tid);
+    if (v.here) first_values = *(const V8*)(from(a.v, tok0 + v.t, k0 + v.h) + v.o * 8);
     for (int t = tid; t < nt; t += kHeadThreads) {
       int place;
       const int b = kv_place(a.kv, tok0 + t, a.n_tokens, place);
@@ -152,8 +207,8 @@ __global__ __launch_bounds__(kHeadThreads) void heads_kernel(HeadArgs a, int TP,
     if (CACHE && a.pos == nullptr) {
       p = (double)spots[t].place;
     } else {
-      const long long at = b * a.pos_batch + (tt - b * a.seq) * a.pos_tok;
-      p = a.pos64 ? (double)((const long long*)a.pos)[at] : (double)((const int32_t*)a.pos)[at];
+      const long long from_ = b * a.pos_batch + (tt - b * a.seq) * a.pos_tok;
+      p = a.pos64 ? (double)((const long long*)a.pos)[from_] : (double)((const int32_t*)a.pos)[from_];
     }
     const double turns = p * a.turns[i - t * half];
     float s, co;
@@ -163,202 +218,173 @@ __global__ __launch_bounds__(kHeadThreads) void heads_kernel(HeadArgs a, int TP,
   }
   __syncthreads();
 
-  const int per = kHeadThreads / L, c = tid % L;
-  const int CR = FAST ? (INTER ? a.rot / V : half / V) : 0, C = FAST ? CR + (a.dim - a.rot) / V : 0;
-  for (int base = 0; base < rows; base += per) {  // the same count for every thread: lanes exchange sums
-    const int r = base + tid / L;
-    const bool live = r < rows;
-    const int t = live ? r / H : 0, hh = live ? r - t * H : 0;
-    const bool isq = hh < nq;
-    const HeadSide& s = isq ? a.q : a.k;
-    const int h = isq ? q0 + hh : k0 + hh - nq;
-    const T* const src = from(s, tok0 + t, h);
-    T* const dst = (T*)s.out + ((long long)(tok0 + t) * s.heads + h) * a.dim;
-    float* const key = CACHE && !isq ? keys + (t * HK + hh - nq) * 32 * W : nullptr;
-    const T* const w = (const T*)s.w;
-    const bool none = CACHE && spots[t].seq < 0;  // its q comes back as zeros
+  const bool normed = a.q.w != nullptr || a.k.w != nullptr;
+  for (int base = 0; base < rows; base += kHeadBatch * per) {  // the same count for every thread: lanes exchange sums
     if constexpr (FAST) {
-      Piece x, y;
-      float xf[V], yf[V];
-      const bool mine = live && c < C, turned = c < CR;
-      const int at = turned ? c * V : a.rot + (c - CR) * V;
-      float ss = 0.0f;
+      if (base > 0) load_rows(base);
+    }
 #pragma unroll
-      for (int i = 0; i < V; ++i) xf[i] = yf[i] = 0.0f;
-      if (mine) {
-        x.v = *(const Vv*)(src + at);
-        if (!INTER && turned) y.v = *(const Vv*)(src + half + at);
+    for (int j = 0; j < kHeadBatch; ++j) {
+      if (base + j * per >= rows) break;
+      const Row r = row_of(base + j * per + tid / L);
+      const HeadSide& s = r.isq ? a.q : a.k;
+      T* const dst = (T*)s.out + ((long long)(tok0 + r.t) * s.heads + r.h) * a.dim;
+      float* const key = CACHE && !r.isq ? keys + (r.t * HK + r.hh - nq) * 32 * W : nullptr;
+      const T* const w = (const T*)s.w;
+      const bool none = CACHE && spots[r.t].seq < 0;  // its q comes back as zeros
+      if constexpr (FAST) {
+        const bool mine = r.live && c < C;
+        float xf[V], yf[V];
+        float ss = 0.0f;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          xf[i] = widen(x.e[i]);
-          yf[i] = !INTER && turned ? widen(y.e[i]) : 0.0f;
+          xf[i] = mine ? widen(x[j].e[i]) : 0.0f;
+          yf[i] = mine && paired ? widen(y[j].e[i]) : 0.0f;
           ss += xf[i] * xf[i] + yf[i] * yf[i];
         }
-      }
-      if (a.q.w != nullptr || a.k.w != nullptr) ss = lanes_sum(ss, L);
-      if (mine) {
-        if (w != nullptr) {
-          const float rn = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
-          Piece wx, wy;
-          wx.v = *(const Vv*)(w + at);
-          if (!INTER && turned) wy.v = *(const Vv*)(w + half + at);
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            xf[i] = xf[i] * rn * widen(wx.e[i]);
-            if (!INTER && turned) yf[i] = yf[i] * rn * widen(wy.e[i]);
-          }
-        }
-        if (turned) {
-          if constexpr (INTER) {
-#pragma unroll
-            for (int i = 0; i < V / 2; ++i) {
-              const float co = cs[t * half + c * (V / 2) + i], si = sn[t * half + c * (V / 2) + i];
-              const float u = xf[2 * i], v = xf[2 * i + 1];
-              xf[2 * i] = fmaf(u, co, -(v * si));
-              xf[2 * i + 1] = fmaf(u, si, v * co);
-            }
-          } else {
+        if (normed) ss = lanes_sum(ss, L);
+        if (mine) {
+          if (w != nullptr) {
+            const float rn = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
+            Piece wx, wy;
+            wx.v = *(const Vv*)(w + at);
+            if (paired) wy.v = *(const Vv*)(w + half + at);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-              const float co = cs[t * half + c * V + i], si = sn[t * half + c * V + i];
-              const float u = xf[i], v = yf[i];
-              xf[i] = fmaf(u, co, -(v * si));
-              yf[i] = fmaf(u, si, v * co);
+              xf[i] = xf[i] * rn * widen(wx.e[i]);
+              if (paired) yf[i] = yf[i] * rn * widen(wy.e[i]);
             }
           }
-        }
-        if (key != nullptr) {
+          if (turned) {
+            const float* const co = cs + r.t * half + (INTER ? c * (V / 2) : c * V);
+            const float* const si = sn + r.t * half + (INTER ? c * (V / 2) : c * V);
+            if constexpr (INTER) {
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            key[at + i] = xf[i];
-            if (!INTER && turned) key[half + at + i] = yf[i];
-          }
-        } else {
+              for (int i = 0; i < V / 2; ++i) {
+                const float u = xf[2 * i], v = xf[2 * i + 1];
+                xf[2 * i] = fmaf(u, co[i], -(v * si[i]));
+                xf[2 * i + 1] = fmaf(u, si[i], v * co[i]);
+              }
+            } else {
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            x.e[i] = narrow<T>(none ? 0.0f : xf[i]);
-            y.e[i] = narrow<T>(none ? 0.0f : yf[i]);
+              for (int i = 0; i < V; ++i) {
+                const float u = xf[i], v = yf[i];
+                xf[i] = fmaf(u, co[i], -(v * si[i]));
+                yf[i] = fmaf(u, si[i], v * co[i]);
+              }
+            }
           }
-          *(Vv*)(dst + at) = x.v;
-          if (!INTER && turned) *(Vv*)(dst + half + at) = y.v;
+          if (key != nullptr) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              key[at + i] = xf[i];
+              if (paired) key[half + at + i] = yf[i];
+            }
+          } else {
+            Piece ox, oy;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              ox.e[i] = narrow<T>(none ? 0.0f : xf[i]);
+              oy.e[i] = narrow<T>(none ? 0.0f : yf[i]);
+            }
+            *(Vv*)(dst + at) = ox.v;
+            if (paired) *(Vv*)(dst + half + at) = oy.v;
+          }
         }
-      }
-    } else {
-      float ss = 0.0f;
-      if (live && w != nullptr)
-        for (int i = c; i < a.dim; i += L) {
+      } else {
+        const T* const src = from(s, tok0 + r.t, r.h);
+        float ss = 0.0f;
+        if (r.live && w != nullptr)
+          for (int i = c; i < a.dim; i += L) {
+            const float v = widen(src[i]);
+            ss += v * v;
+          }
+        if (normed) ss = lanes_sum(ss, L);
+        const float rn = w != nullptr ? 1.0f / sqrtf(ss / (float)a.dim + a.eps) : 1.0f;
+        const auto get = [&](int i) {
           const float v = widen(src[i]);
-          ss += v * v;
+          return w != nullptr ? v * rn * widen(w[i]) : v;
+        };
+        const auto put = [&](int i, float v) {
+          if (key != nullptr)
+            key[i] = v;
+          else
+            dst[i] = narrow<T>(none ? 0.0f : v);
+        };
+        if (r.live) {
+          for (int i = c; i < half; i += L) {
+            const int iu = INTER ? 2 * i : i, iv = INTER ? 2 * i + 1 : half + i;
+            const float co = cs[r.t * half + i], si = sn[r.t * half + i], u = get(iu), v = get(iv);
+            put(iu, fmaf(u, co, -(v * si)));
+            put(iv, fmaf(u, si, v * co));
+          }
+          for (int i = a.rot + c; i < a.dim; i += L) put(i, get(i));
         }
-      if (a.q.w != nullptr || a.k.w != nullptr) ss = lanes_sum(ss, L);
-      const float rn = w != nullptr ? 1.0f / sqrtf(ss / (float)a.dim + a.eps) : 1.0f;
-      const auto get = [&](int i) {
-        const float v = widen(src[i]);
-        return w != nullptr ? v * rn * widen(w[i]) : v;
-      };
-      const auto put = [&](int i, float v) {
-        if (key != nullptr)
-          key[i] = v;
-        else
-          dst[i] = narrow<T>(none ? 0.0f : v);
-      };
-      if (live) {
-        for (int i = c; i < half; i += L) {
-          const int iu = INTER ? 2 * i : i, iv = INTER ? 2 * i + 1 : half + i;
-          const float co = cs[t * half + i], si = sn[t * half + i], u = get(iu), v = get(iv);
-          put(iu, fmaf(u, co, -(v * si)));
-          put(iv, fmaf(u, si, v * co));
-        }
-        for (int i = a.rot + c; i < a.dim; i += L) put(i, get(i));
       }
     }
   }
 
   if constexpr (CACHE) {
-    __syncthreads();
     const int O = 4 * W, blocks = a.kv.page / kKvBlock;
     const long long bytes = kv_block_bytes(W);
+    for (int base = 0; base < quads * vlanes; base += kHeadThreads) {  // whole rows of sixteen lanes
+      const Place p = value_of(base + tid);
+      V8 v = first_values;
+      if (base > 0 && p.here) v = *(const V8*)(from(a.v, tok0 + p.t, k0 + p.h) + p.o * 8);
+      float f[8];
+      int code[8];
+      uint16_t sb, mb;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = p.here ? widen(v[j]) : 0.0f;
+      quantize8(f, p.here, code, sb, mb);
+      const int z = tid >> 2 & 3, t = min(p.t, nt - 1);
+      const Spot spot = spots[t];
+      const bool cached = p.live && p.t < nt && spot.block >= 0;
+      uint8_t* const blk = a.kv.pages + (spot.block + (long long)(k0 + p.h) * blocks) * bytes;
+      const int tok = spot.place & (kKvBlock - 1), oct = p.o & 3;
+      // four neighbouring tokens of one block: whole words, of which lane z stores the z-th
+      const Spot head = spots[min(p.qd * 4, nt - 1)];
+      const bool in_row = cached && spot.block == head.block && spot.place == head.place + z && head.place % 4 == 0;
+      const bool whole = (__ballot(in_row) >> (tid & 48) & 0xFFFF) == 0xFFFF;
+      uint32_t word = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        uint32_t w = (uint32_t)(code[2 * j] | code[2 * j + 1] << 4);
+        if (!whole && cached)
+          blk[kv_value_codes(W) + kv_value_word(W, p.gg, tok >> 2 & 3, oct * 4 + j, tok >> 4) + (tok & 3)] = (uint8_t)w;
+        w <<= 8 * z;
+        w |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0x128, 0xF, 0xF, false);  // row_ror:8, then 4: over z
+        w |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0x124, 0xF, 0xF, false);
+        if (j == z) word = w;
+      }
+      if (whole)
+        *(uint32_t*)(blk + kv_value_codes(W) + kv_value_word(W, p.gg, tok >> 2 & 3, oct * 4 + z, tok >> 4)) = word;
+      if (cached && oct == 0) {
+        uint16_t* const to = (uint16_t*)(blk + kv_value_scales(W) + (p.gg * 8 + (tok >> 2)) * 16) + ((tok & 1) * 2 + (tok >> 1 & 1));
+        to[0] = sb;
+        to[4] = mb;
+      }
+    }
+    __syncthreads();
     for (int base = 0; base < nt * nk * O; base += kHeadThreads) {  // quads of lanes share a group: O is whole quads
       const int item = base + tid;
       const bool live = item < nt * nk * O;
       const int row = live ? item / O : 0, o = live ? item - row * O : 0, t = row / nk, h = row - t * nk;
       const bool here = live && o * 8 < a.dim;
-      float x[8];
+      float f[8];
       int code[8];
       uint16_t sb, mb;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = here ? keys[(t * HK + h) * 32 * W + o * 8 + j] : 0.0f;
-      quantize8(x, here, code, sb, mb);
+      for (int j = 0; j < 8; ++j) f[j] = here ? keys[(t * HK + h) * 32 * W + o * 8 + j] : 0.0f;
+      quantize8(f, here, code, sb, mb);
       if (!live || spots[t].block < 0) continue;
       uint32_t word = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) word |= (uint32_t)code[j] << (4 * j);
       uint8_t* const blk = a.kv.pages + (spots[t].block + (long long)(k0 + h) * blocks) * bytes;
-      const int tok = spots[t].place % kKvBlock;
+      const int tok = spots[t].place & (kKvBlock - 1);
       *(uint32_t*)(blk + tok * 16 * W + (o % 4) * 4 * W + (o / 4) * 4) = word;
       if (o % 4 == 0) *(uint32_t*)(blk + kv_key_scales(W) + (tok * W + o / 4) * 4) = sb | (uint32_t)mb << 16;
-    }
-    const int quads = (nt + 3) / 4;
-    for (int base = 0; base < quads * nk * O; base += kHeadThreads) {
-      const int item = base + tid;
-      const bool live = item < quads * nk * O;
-      const int row = live ? item / O : 0, o = live ? item - row * O : 0, qd = row / nk, h = row - qd * nk;
-      const bool here = live && o * 8 < a.dim;
-      uint32_t words[4] = {0, 0, 0, 0};
-      uint16_t sb[4], mb[4];
-#pragma unroll
-      for (int z = 0; z < 4; ++z) {
-        const int t = qd * 4 + z;
-        const bool has = here && t < nt;
-        float x[8];
-        int code[8];
-        const T* const src = from(a.v, tok0 + min(t, nt - 1), k0 + h) + o * 8;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = has ? widen(src[j]) : 0.0f;
-        quantize8(x, has, code, sb[z], mb[z]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) words[j] |= (uint32_t)(code[2 * j] | code[2 * j + 1] << 4) << (8 * z);
-      }
-      if (!live) continue;
-      const Spot first = spots[qd * 4];
-      bool whole = qd * 4 + 3 < nt && first.block >= 0 && first.place % 4 == 0;
-#pragma unroll
-      for (int z = 1; z < 4; ++z)
-        whole = whole && spots[min(qd * 4 + z, nt - 1)].block == first.block &&
-                spots[min(qd * 4 + z, nt - 1)].place == first.place + z;
-      const auto at = [&](long long block) { return a.kv.pages + (block + (long long)(k0 + h) * blocks) * bytes; };
-      const int gg = o / 4;
-      if (whole) {
-        uint8_t* const blk = at(first.block);
-        const int tok = first.place % kKvBlock;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          *(uint32_t*)(blk + kv_value_codes(W) + kv_value_word(W, gg, tok / 4 % 4, o % 4 * 4 + j, tok / 16)) = words[j];
-        if (o % 4 == 0) {
-          uint32_t* const to = (uint32_t*)(blk + kv_value_scales(W) + (gg * 8 + tok / 4) * 16);
-          to[0] = sb[0] | (uint32_t)sb[2] << 16;
-          to[1] = sb[1] | (uint32_t)sb[3] << 16;
-          to[2] = mb[0] | (uint32_t)mb[2] << 16;
-          to[3] = mb[1] | (uint32_t)mb[3] << 16;
-        }
-      } else {
-#pragma unroll
-        for (int z = 0; z < 4; ++z) {
-          const int t = qd * 4 + z;
-          if (t >= nt || spots[t].block < 0) continue;
-          uint8_t* const blk = at(spots[t].block);
-          const int tok = spots[t].place % kKvBlock;
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            blk[kv_value_codes(W) + kv_value_word(W, gg, tok / 4 % 4, o % 4 * 4 + j, tok / 16) + tok % 4] =
-                (uint8_t)(words[j] >> (8 * z));
-          if (o % 4 == 0) {
-            uint16_t* const to = (uint16_t*)(blk + kv_value_scales(W) + (gg * 8 + tok / 4) * 16) + (tok % 2 * 2 + tok / 2 % 2);
-            to[0] = sb[z];
-            to[4] = mb[z];
-          }
-        }
-      }
     }
   }
 }
@@ -379,7 +405,7 @@ void launch_heads_t(const HeadArgs& a, hipStream_t stream) {
     TP = a.n_tokens > 512 ? 4 : 1;
     const int G = qh / kh;
     const int room = max(1, 8192 / (TP * 32 * W));  // keys that 32 KB hold
-    HK = min(min(kh, room), max(1, 2 * per / (TP * (G + 1))));
+    HK = min(min(kh, room), max(1, 64 / (TP == 1 ? 4 : 4 * W)));  // a lane an octet of the values of four tokens
     HQ = HK * G;
     split = (kh + HK - 1) / HK;
   } else {
