@@ -39,6 +39,7 @@ class HipPagedCache:
     MAX_PAGE = 65536
     MAX_PLACES = 1 << 30  # width of a table times page_size
     MAX_SEQUENCES = 65535
+    MAX_ROWS = 1 << 28  # tokens times heads of attend's q
 
     def __init__(self, n_pages: int, page_size: int, kv_heads: int, head_dim: int, *,
                  device: torch.device | str = "cuda", pages: torch.Tensor | None = None) -> None:
@@ -49,7 +50,7 @@ class HipPagedCache:
         page_bytes = self._lib.mxa_kv4_page_bytes(self.kv_heads, self.page_size, self.head_dim)
         if page_bytes == 0 or not 1 <= self.n_pages < 1 << 31:
             raise ValueError(f"a cache needs pages, a page_size that is a multiple of {self.BLOCK} up to {self.MAX_PAGE}, "
-                             f"1..65535 heads and a head_dim that is a multiple of 8 up to 256, got {n_pages} pages of "
+                             f"1..4096 heads and a head_dim that is a multiple of 8 up to 256, got {n_pages} pages of "
                              f"{page_size} tokens, {kv_heads} heads of {head_dim}")
         blocks = self.page_size // self.BLOCK
         shape = (self.n_pages, self.kv_heads, blocks, page_bytes // (self.kv_heads * blocks))
@@ -186,6 +187,8 @@ class HipPagedCache:
         if q.dtype is not _BF16:
             raise ValueError(f"q must be bfloat16, got {q.dtype}")
         heads = self._query_heads(q)
+        if n * heads > self.MAX_ROWS:
+            raise ValueError(f"q must have up to {self.MAX_ROWS} tokens times heads, got {tuple(q.shape)}")
         where = self._where(table, lengths, query_starts, n, q.shape[0] if nd == 4 else None)
         places = table.shape[1] * self.page_size
         most = places if max_length is None else min(max(int(max_length), 1), places)

@@ -45,7 +45,7 @@ int block_bytes(int t) {
 bool aligned(const void* p, uintptr_t a);
 
 bool kv4_supported(int kv_heads, int page_size, int head_dim) {
-  return kv_heads >= 1 && kv_heads <= 65535 && page_size >= mxa::kKvBlock && page_size % mxa::kKvBlock == 0 &&
+  return kv_heads >= 1 && kv_heads <= MXA_KV4_MAX_HEADS && page_size >= mxa::kKvBlock && page_size % mxa::kKvBlock == 0 &&
          page_size <= MXA_KV4_MAX_PAGE && head_dim >= 8 && head_dim % 8 == 0 && head_dim <= MXA_KV4_MAX_DIM;
 }
 
@@ -779,7 +779,7 @@ int mxa_kv4_read(const void* pages, int n_pages, int kv_heads, int page_size, in
 size_t mxa_kv4_attend_workspace_bytes(int n_seq, int n_tokens, int ragged, int q_heads, int kv_heads, int head_dim,
                                       int max_length, int window) {
   if (n_seq < 1 || n_tokens < 1 || (!ragged && n_tokens % n_seq != 0) || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads != 0 ||
-      head_dim < 8 || head_dim > mxa::kKvMaxDim || max_length < 1 || window < 0)
+      (long long)n_tokens * q_heads > MXA_KV4_MAX_ROWS || head_dim < 8 || head_dim > mxa::kKvMaxDim || max_length < 1 || window < 0)
     return 0;
   return mxa::attend_workspace(n_seq, n_tokens, ragged != 0, kv_heads, q_heads / kv_heads, max_length, window, head_dim);
 }
@@ -793,18 +793,17 @@ int mxa_kv4_attend(const void* q, const long long* q_strides, int q_heads, int n
   if (!kv4_pages(a.kv, (void*)pages, n_pages, kv_heads, page_size, head_dim, table, table_stride, table_width, lengths,
                  query_starts, n_seq, n_tokens) ||
       q == nullptr || q_strides == nullptr || out == nullptr || !aligned(q, 2) || !aligned(out, 2) || q_heads < 1 ||
-      q_heads > MXA_ROPE_MAX_HEADS || q_heads % kv_heads != 0 || seq_len < 1 || max_length < 1 || window < 0)
+      q_heads > MXA_ROPE_MAX_HEADS || q_heads % kv_heads != 0 || (long long)n_tokens * q_heads > MXA_KV4_MAX_ROWS || seq_len < 1 ||
+      max_length < 1 || window < 0)
     return MXA_ERR_UNSUPPORTED;
-  const size_t need = mxa_kv4_attend_workspace_bytes(n_seq, n_tokens, query_starts != nullptr, q_heads, kv_heads, head_dim,
-                                                     max_length, window);
-  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return MXA_ERR_WORKSPACE;
-  if (need > 0 && !aligned(workspace, 16)) return MXA_ERR_UNSUPPORTED;
+  if (!aligned(workspace, 16)) return MXA_ERR_UNSUPPORTED;
   a.q = (const uint16_t*)q;
   a.q_batch = q_strides[0], a.q_tok = q_strides[1], a.q_head = q_strides[2];
   a.out = (uint16_t*)out;
   a.n_tokens = n_tokens, a.seq = seq_len, a.dim = head_dim, a.heads = q_heads, a.group = q_heads / kv_heads;
   a.window = window < MXA_KV4_MAX_PLACES ? window : MXA_KV4_MAX_PLACES, a.scale = scale;
-  if (mxa::launch_attend(a, max_length, workspace, (hipStream_t)stream) != 0) return MXA_ERR_UNSUPPORTED;
+  const int status = mxa::launch_attend(a, max_length, workspace, workspace_bytes, (hipStream_t)stream);
+  if (status != 0) return status == mxa::kAttendWorkspace ? MXA_ERR_WORKSPACE : MXA_ERR_UNSUPPORTED;
   return check_launch();
 }
 

@@ -12,6 +12,8 @@
 // so nothing but the row's maximum crosses lanes. Codes are widened in registers, code to float16 exactly (an or of its
 // bits into a float16's, less that float16), then s * code + m rounded once; q is brought by a power of two into float16's
 // range, exactly but for values below 2^-24 of its largest. Scores, maxima, sums and outputs are float32.
+#include <limits.h>
+
 #include <algorithm>
 
 #include "mxa_attend.hpp"
@@ -46,6 +48,30 @@ __global__ __launch_bounds__(kAttendThreads, W <= 4 ? 3 : 2) void attend_kernel(
   const bool live = row < seq.rows;
   const int place = seq.place0 + (live ? row / a.group : 0);
   const int limit = live ? min(place + 1, seq.length) : 0, low = a.window > 0 ? max(place + 1, 0) - a.window : 0;
+
+  // The wave's blocks are begin + wave, + 4, ..; lane i finds where the i-th of 64 of them lies, so that no block's
+  // address waits for the page table.
+  long long where = -1;
+  int looked = 64;
+  BlockPart<W> part[AHEAD];
+  bool has[AHEAD];
+  const auto request = [&](BlockPart<W>& p, bool& there, int u) {
+    if (looked == 64) {
+      looked = 0;
+      const int mine = u + lane * kAttendWaves;
+      const long long block = mine < end ? kv_block(a.kv, b, (seq.first_block + mine) * kKvBlock) : -1;
+      where = block < 0 ? -1 : (block + (long long)h * blocks_of_page) * kv_block_bytes(W);
+    }
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)where, looked);
+    const uint32_t hi = __builtin_amdgcn_readlane((int)(where >> 32), looked);
+    ++looked;
+    there = (int)hi >= 0;
+    if (there) p.load(a.kv.pages + ((uint64_t)hi << 32 | lo), lane);
+  };
+  int u = begin + wave;
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (u + i * kAttendWaves < end) request(part[i], has[i], u + i * kAttendWaves);
 
   // q, by a power of two
   half8 q[W];
@@ -82,25 +108,6 @@ __global__ __launch_bounds__(kAttendThreads, W <= 4 ? 3 : 2) void attend_kernel(
   const int inside_lo = a.window > 0 ? max(seq.place0 + last_row / a.group + 1, 0) - a.window : 0;
   const int inside_hi = min(seq.place0 + rt * 16 / a.group + 1, seq.length);
 
-  // The wave's blocks are begin + wave, + 4, ..; lane i finds where the i-th of 64 of them lies, so that no block's
-  // address waits for the page table.
-  long long where = -1;
-  int looked = 64;
-  BlockPart<W> part[AHEAD];
-  bool has[AHEAD];
-  const auto request = [&](BlockPart<W>& p, bool& there, int u) {
-    if (looked == 64) {
-      looked = 0;
-      const int mine = u + lane * kAttendWaves;
-      const long long block = mine < end ? kv_block(a.kv, b, (seq.first_block + mine) * kKvBlock) : -1;
-      where = block < 0 ? -1 : (block + (long long)h * blocks_of_page) * kv_block_bytes(W);
-    }
-    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)where, looked);
-    const uint32_t hi = __builtin_amdgcn_readlane((int)(where >> 32), looked);
-    ++looked;
-    there = (int)hi >= 0;
-    if (there) p.load(a.kv.pages + ((uint64_t)hi << 32 | lo), lane);
-  };
   const auto compute = [&](const BlockPart<W>& p_, int u) {
     const int first = (seq.first_block + u) * kKvBlock;
     p_.share(sc, lane);
@@ -153,10 +160,6 @@ __global__ __launch_bounds__(kAttendThreads, W <= 4 ? 3 : 2) void attend_kernel(
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   };
-  int u = begin + wave;
-#pragma unroll
-  for (int i = 0; i < AHEAD; ++i)
-    if (u + i * kAttendWaves < end) request(part[i], has[i], u + i * kAttendWaves);
   while (u < end) {
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
@@ -262,31 +265,37 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join_kernel(AttendArgs 
 __global__ __launch_bounds__(kAttendThreads) void attend_join_rows_kernel(AttendArgs a, int W) {
   const int b = blockIdx.y, pair = blockIdx.x, r = threadIdx.x >> 4, piece = threadIdx.x & 15;
   const int h = pair % a.kv.heads, rt = pair / a.kv.heads;
-  const Sequence seq(a, b);
-  if (rt * 16 + r >= seq.rows) return;
+  const Sequence seq = Sequence(a, b).uniform();
+  const int parts = seq.splits;
+  if (rt * 16 + r >= seq.rows || parts == 1) return;
+  const AttendPart first = a.part_of(b, pair, 0, W);
+  const size_t step = 16 * 32 * W + 32;
   float top = -INFINITY, total = 0.0f;
-  for (int i = 0; i < a.splits; ++i) top = fmaxf(top, a.part_of(b, pair, i, W).ml[r]);
-  for (int i = 0; i < a.splits; ++i) {
-    const AttendPart p = a.part_of(b, pair, i, W);
-    total += exp2_(p.ml[r] - top) * p.ml[16 + r];
+#pragma unroll 4
+  for (int i = 0; i < parts; ++i) top = fmaxf(top, first.ml[i * step + r]);
+  const float ref = top == -INFINITY ? 0.0f : top;
+  f32x4 v[4]{};
+#pragma unroll 2
+  for (int i = 0; i < parts; ++i) {
+    const float f = exp2_(first.ml[i * step + r] - ref);
+    total += f * first.ml[i * step + 16 + r];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (4 * piece + 64 * j < a.dim) v[j] += f * *(const f32x4*)(first.o + i * step + r * 32 * W + 4 * piece + 64 * j);
   }
   const float norm = total > 0.0f || total != total ? 1.0f / total : 0.0f;
   uint16_t* const dst = a.out_row(seq.first + (rt * 16 + r) / a.group, h * a.group + (rt * 16 + r) % a.group);
-  for (int d = 4 * piece; d < a.dim; d += 64) {
-    f32x4 v{0, 0, 0, 0};
-    for (int i = 0; i < a.splits; ++i) {
-      const AttendPart p = a.part_of(b, pair, i, W);
-      v += exp2_(p.ml[r] - top) * *(const f32x4*)(p.o + r * 32 * W + d);
-    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) dst[d + j] = bf16_rne(v[j] * norm);
-  }
+  for (int j = 0; j < 4; ++j)
+    if (4 * piece + 64 * j < a.dim)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) dst[4 * piece + 64 * j + i] = bf16_rne(v[j][i] * norm);
 }
 
 // (std::min and std::max here: on the host, HIP's own of that name take ints.)
 // How the places of up to `most` tokens of each sequence are shared out. Sequences of up to kFewRows rows a key head go in
 // tiles of 16 rows (attend_kernel), others in those of attend_tile_kernel; a call without query_starts has one kind.
-constexpr int kFewRows = 64, kTileSplits = 16;
+constexpr int kFewRows = 64, kTileSplits = 16, kFewParts = 16;
 struct Plan {
   bool few, many;     // the kinds that there may be
   long long pairs[2]; // (tile of 16 rows, key head) of a sequence
@@ -295,18 +304,20 @@ struct Plan {
   long long tiles;    // of the call, for many rows
 };
 
-void share_out(long long blocks, long long workgroups, long long slots, int least, int& splits, int& chunk) {
+void share_out(long long blocks, long long workgroups, long long slots, int least, int most, int& splits, int& chunk) {
   const long long want = std::max<long long>(1, slots / workgroups);
-  chunk = (int)std::max<long long>(least, (blocks + want - 1) / want);
-  splits = (int)std::min<long long>(kAttendMaxSplits, (blocks + chunk - 1) / chunk);
+  chunk = (int)std::max<long long>(least, std::min<long long>(most, (blocks + want - 1) / want));
+  chunk = (int)std::max<long long>(chunk, (blocks + kAttendMaxSplits - 1) / kAttendMaxSplits);
+  splits = (int)((blocks + chunk - 1) / chunk);
+  chunk = (int)((blocks + splits - 1) / splits);
 }
 
-Plan plan_of(int n_seq, int n_tokens, bool ragged, int kv_heads, int group, int max_length, int window, int dim) {
+Plan plan_of(int n_seq, int n_tokens, bool ragged, int kv_heads, int group, int max_length, long long window, int dim) {
   Plan p{};
   const long long most = (long long)(ragged ? n_tokens : n_tokens / n_seq) * group;
   p.few = ragged || most <= kFewRows;
   p.many = most > kFewRows;
-  const long long reach = window > 0 ? std::min<long long>(max_length, (long long)window + most / group) : max_length;
+  const long long reach = window > 0 ? std::min<long long>(max_length, window + most / group) : max_length;
   const long long blocks = reach / kKvBlock + 2;
   const bool narrow = kv_groups(dim) <= 4;
   if (p.few) {
@@ -314,7 +325,7 @@ Plan plan_of(int n_seq, int n_tokens, bool ragged, int kv_heads, int group, int 
     const long long slots = 256 * (narrow ? 3 : 2);  // workgroups that the CUs hold at once
     // one sequence: what the CUs hold at once; several, whose lengths are not known: four times that, in parts small
     // enough to even out
-    share_out(blocks, p.pairs[0] * n_seq, n_seq > 1 ? 4 * slots : slots, 4, p.splits[0], p.chunk[0]);
+    share_out(blocks, p.pairs[0] * n_seq, slots, 8, n_seq > 1 ? 128 : INT_MAX, p.splits[0], p.chunk[0]);
   }
   if (p.many) {
     p.pairs[1] = (most + 15) / 16 * kv_heads;
@@ -339,6 +350,7 @@ Plan plan_of(int n_seq, int n_tokens, bool ragged, int kv_heads, int group, int 
 size_t part_bytes(const Plan& p, int kind, int n_seq, int dim) {
   return p.splits[kind] <= 1 ? 0 : (size_t)n_seq * p.pairs[kind] * p.splits[kind] * part_floats(kv_groups(dim)) * sizeof(float);
 }
+size_t parts_bytes(const Plan& p, int n_seq, int dim) { return part_bytes(p, 0, n_seq, dim) + part_bytes(p, 1, n_seq, dim); }
 
 template <int W>
 void launch_few(const AttendArgs& a, hipStream_t stream) {
@@ -349,12 +361,14 @@ void launch_few(const AttendArgs& a, hipStream_t stream) {
 
 size_t attend_workspace(int n_seq, int n_tokens, bool ragged, int kv_heads, int group, int max_length, int window, int dim) {
   const Plan p = plan_of(n_seq, n_tokens, ragged, kv_heads, group, max_length, window, dim);
-  return part_bytes(p, 0, n_seq, dim) + part_bytes(p, 1, n_seq, dim);
+  return parts_bytes(p, n_seq, dim);
 }
 
-int launch_attend(AttendArgs a, int max_length, void* workspace, hipStream_t stream) {
+int launch_attend(AttendArgs a, int max_length, void* workspace, size_t workspace_bytes, hipStream_t stream) {
   const Plan p = plan_of(a.kv.n_seq, a.n_tokens, a.kv.starts != nullptr, a.kv.heads, a.group, max_length, a.window, a.dim);
-  if (p.pairs[0] > 65535 || (p.splits[1] > 1 && p.pairs[1] > 65535) || p.tiles * a.kv.heads >= 1 << 23) return -1;
+  if (p.pairs[0] > 65535 || (p.splits[1] > 1 && p.pairs[1] > 65535) || p.tiles * a.kv.heads >= 1 << 23) return kAttendUnsupported;
+  const size_t need = parts_bytes(p, a.kv.n_seq, a.dim);  // of the plan that is launched
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return kAttendWorkspace;
   const int W = kv_groups(a.dim);
   for (int kind = 0; kind < 2; ++kind) {
     if (!(kind ? p.many : p.few)) continue;
@@ -371,7 +385,7 @@ int launch_attend(AttendArgs a, int max_length, void* workspace, hipStream_t str
 #undef MXA_CASE
       }
     }
-    if (a.splits > 1 && kind == 1)
+    if (a.splits > 1 && a.splits <= kFewParts)
       hipLaunchKernelGGL(attend_join_rows_kernel, dim3(a.pairs, a.kv.n_seq), dim3(kAttendThreads), 0, stream, a, W);
     else if (a.splits > 1)
       hipLaunchKernelGGL(attend_join_kernel, dim3(16, a.pairs, a.kv.n_seq), dim3(kAttendThreads), 0, stream, a, W);

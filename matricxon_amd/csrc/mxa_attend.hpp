@@ -255,6 +255,7 @@ __device__ __forceinline__ void clear_tail(uint32_t* sc, int lane, int have) {
 size_t attend_workspace(int n_seq, int n_tokens, bool ragged, int kv_heads, int group, int max_length, int window, int dim);
 // The form for many rows, of 256 (heads of up to 128 values) or 128 rows of a key head a workgroup.
 void launch_attend_tile(const AttendArgs& a, int rows, long long tiles, hipStream_t stream);
-int launch_attend(AttendArgs a, int max_length, void* workspace, hipStream_t stream);
+constexpr int kAttendUnsupported = -1, kAttendWorkspace = -2;
+int launch_attend(AttendArgs a, int max_length, void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 }  // namespace mxa

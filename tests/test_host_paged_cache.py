@@ -19,7 +19,7 @@ def lib():
 def test_page_bytes(lib) -> None:
     assert lib.mxa_kv4_page_bytes(8, 64, 128) == 8 * 2 * 5120  # 5 bits a value of keys and of values
     assert lib.mxa_kv4_page_bytes(1, 32, 8) == 1280 and lib.mxa_kv4_page_bytes(3, 96, 40) == 3 * 3 * 2560
-    for bad in ((0, 64, 128), (65536, 64, 128), (8, 0, 128), (8, 48, 128), (8, 1 << 17, 128), (8, 64, 0), (8, 64, 12),
+    for bad in ((0, 64, 128), (4097, 64, 128), (8, 0, 128), (8, 48, 128), (8, 1 << 17, 128), (8, 64, 0), (8, 64, 12),
                 (8, 64, 264), (-1, 64, 128), (8, -32, 128)):
         assert lib.mxa_kv4_page_bytes(*bad) == 0, bad
 
@@ -40,7 +40,7 @@ def test_norm_rope_refuses_without_launching(lib) -> None:
 
 
 PLACES = dict(pages=A, n_pages=4, heads=2, page=32, dim=64, table=A, width=2, lengths=A, starts=None, n_seq=3)
-BAD_PLACES = (dict(pages=None), dict(pages=VP(0x10008)), dict(n_pages=0), dict(heads=0), dict(heads=65536), dict(page=16),
+BAD_PLACES = (dict(pages=None), dict(pages=VP(0x10008)), dict(n_pages=0), dict(heads=0), dict(heads=4097), dict(page=16),
               dict(page=40), dict(page=1 << 17), dict(dim=0), dict(dim=60), dict(dim=264), dict(table=None),
               dict(table=VP(0x10002)), dict(width=0), dict(width=(1 << 25) + 1), dict(lengths=None),
               dict(lengths=VP(0x10002)), dict(starts=VP(0x10002)), dict(n_seq=0), dict(n_seq=65536), dict(n=0), dict(n=4),
@@ -81,7 +81,7 @@ def test_attend_refuses_without_launching(lib) -> None:
                                   None)
 
     for bad in (*BAD_PLACES, dict(q=None), dict(qs=None), dict(out=None), dict(q=ODD), dict(out=ODD), dict(hq=0), dict(hq=3),
-                dict(hq=65538), dict(seq=0), dict(most=0), dict(window=-1)):
+                dict(hq=65538), dict(seq=0), dict(most=0), dict(window=-1), dict(n=1 << 24, hq=18, n_seq=1, seq=1 << 24)):
         assert call(**bad) == -1, bad
     long = dict(width=1 << 12, most=1 << 17)  # shared out over workgroups, which needs a workspace
     need = lib.mxa_kv4_attend_workspace_bytes(3, 3, 0, 4, 2, 64, 1 << 17, 0)
@@ -101,6 +101,15 @@ def test_workspace_bytes(lib) -> None:
         for window in (1 << 30, (1 << 31) - 175, (1 << 31) - 1):
             assert lib.mxa_kv4_attend_workspace_bytes(7, 7 * n, 0, 10, 2, 64, 640, window) == want > 0
     assert lib.mxa_kv4_attend_workspace_bytes(1, 1, 0, 4, 2, 64, 1 << 20, 64) == 0
+
+
+@pytest.mark.parametrize("max_length", [64, 640, 768, 20000, 1 << 30])
+@pytest.mark.parametrize("shape", [(7, 174, 1, 10, 2, 64), (1, 512, 0, 32, 8, 128), (3, 3, 0, 4, 2, 256), (4, 515, 1, 40, 8, 64)])
+def test_windows_past_every_length_change_no_workspace(lib, shape, max_length) -> None:
+    """What a launch needs is computed with the window cut to the most places there are; the query's numbers are the same."""
+    want = lib.mxa_kv4_attend_workspace_bytes(*shape, max_length, 0)
+    for window in (1 << 30, (1 << 31) - 512, (1 << 31) - 175, (1 << 31) - 1):
+        assert lib.mxa_kv4_attend_workspace_bytes(*shape, max_length, window) == want
 
 
 def test_a_cache_lies_on_a_device() -> None:
