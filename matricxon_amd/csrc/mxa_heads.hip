@@ -83,32 +83,63 @@ __device__ __forceinline__ float quad_max(float v) {
 }
 
 // The codes of eight values of a group that the four lanes of a quad hold between them (`here`: whether this lane has
-// any), and the group's scale and minimum, which come back as bits of float16. A NaN is held as 0 and an infinity as
-// the largest: a cached value is always finite.
-__device__ __forceinline__ void quantize8(float (&x)[8], bool here, int (&code)[8], uint16_t& s_bits, uint16_t& m_bits) {
+// any), two to a byte's value, and the group's scale and minimum, which come back as bits of float16. A NaN is held as 0
+// and an infinity as the largest: a cached value is always finite.
+//
+// Quotients by s share its reciprocal, brought to the last bit by a Newton step; a product with it is put right by its
+// residual, which is exact (Markstein's division).
+__device__ __forceinline__ void quantize8(float (&x)[8], bool here, float (&bytes)[4], uint16_t& s_bits, uint16_t& m_bits) {
   float lo = INFINITY, hi = -INFINITY;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    x[j] = x[j] == x[j] ? fminf(fmaxf(x[j], -kKvHeld), kKvHeld) : 0.0f;
-    if (here) {
-      lo = fminf(lo, x[j]);
-      hi = fmaxf(hi, x[j]);
-    }
+    x[j] = __builtin_amdgcn_fmed3f(x[j] == x[j] ? x[j] : 0.0f, -kKvHeld, kKvHeld);
+    lo = fminf(lo, x[j]);
+    hi = fmaxf(hi, x[j]);
   }
-  lo = quad_min(lo);
-  hi = quad_max(hi);
+  lo = quad_min(here ? lo : INFINITY);
+  hi = quad_max(here ? hi : -INFINITY);
   const _Float16 mh = (_Float16)lo, sh = (_Float16)((hi - lo) / 15.0f);
   const float m = (float)mh, s = (float)sh;
+  float y = __builtin_amdgcn_rcpf(s);
+  y = fmaf(fmaf(-s, y, 1.0f), y, y);
+  if (!here || !(s > 0.0f)) y = 0.0f;
+  float c[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) code[j] = here && s > 0.0f ? (int)fminf(fmaxf(rintf((x[j] - m) / s), 0.0f), 15.0f) : 0;
+  for (int j = 0; j < 8; ++j) {
+    const float d = x[j] - m, q = d * y;
+    c[j] = here ? __builtin_amdgcn_fmed3f(rintf(fmaf(fmaf(-q, s, d), y, q)), 0.0f, 15.0f) : 0.0f;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) bytes[j] = fmaf(c[2 * j + 1], 16.0f, c[2 * j]);
   s_bits = __builtin_bit_cast(uint16_t, sh);
   m_bits = __builtin_bit_cast(uint16_t, mh);
 }
 
-struct Spot {       // of one token of the workgroup
-  long long block;  // of its first head, or -1: it is not cached
-  int place, seq;   // seq -1: a row of no sequence
+struct Spot {      // of one token of the workgroup
+  long long at;    // byte offset of its block of the first head in the pages, or -1: it is not cached
+  int place, seq;  // seq -1: a row of no sequence
 };
+
+// Whole vectors' products: a multiplication of 32 bits costs four of 24.
+__device__ __forceinline__ int mul24(int a, int b) { return __mul24(a, b); }
+__device__ __forceinline__ long long mul64(int a, long long b) { return (long long)((uint64_t)(uint32_t)a * (uint64_t)b); }
+
+template <class T, int V>
+__device__ __forceinline__ typename Vec<T, V>::type narrow_all(const float (&v)[V]) {
+  typename Vec<T, V>::type r;
+#pragma unroll
+  for (int i = 0; i < V; i += 2) {
+    if constexpr (sizeof(T) == 2) {
+      typedef float f2 __attribute__((ext_vector_type(2)));
+      typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+      const uint32_t w = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){v[i], v[i + 1]}, b2));
+      r[i] = (uint16_t)w, r[i + 1] = (uint16_t)(w >> 16);
+    } else {
+      r[i] = v[i], r[i + 1] = v[i + 1];
+    }
+  }
+  return r;
+}
 
 // T the element type; FAST: vectors of V values. A workgroup takes TP tokens and, from grid.y, HQ heads of q and HK of k.
 template <class T, bool INTER, bool FAST, bool CACHE>
@@ -131,9 +162,10 @@ __global__ __launch_bounds__(kHeadThreads) void heads_kernel(HeadArgs a, int TP,
   const int k0 = (int)blockIdx.y * HK, nk = max(0, min(HK, a.k.heads - k0));
   const int H = nq + nk, rows = nt * H;
   const bool one = a.seq >= a.n_tokens;
-  const auto from = [&](const HeadSide& s, int t, int h) {
-    const int b = one ? 0 : t / a.seq;
-    return (const T*)s.x + (long long)b * s.batch + (long long)(t - b * a.seq) * s.tok + (long long)h * s.head;
+  const auto from = [&](const HeadSide& s, int t, int h) {  // t: of the workgroup
+    if (one) return (const T*)s.x + tok0 * s.tok + mul64(t, s.tok) + mul64(h, s.head);
+    const int b = (tok0 + t) / a.seq;
+    return (const T*)s.x + mul64(b, s.batch) + mul64(tok0 + t - b * a.seq, s.tok) + mul64(h, s.head);
   };
 
   const int per = kHeadThreads / L, c = tid % L;
@@ -142,62 +174,83 @@ __global__ __launch_bounds__(kHeadThreads) void heads_kernel(HeadArgs a, int TP,
   const int at = turned ? c * V : a.rot + (c - CR) * V;  // the lane's vector in a head, and its partner's at half + at
   const bool paired = !INTER && turned;
 
+  // A thread's rows, `per` apart: (token, head of the workgroup's), stepped on without a division each.
   struct Row {
+    int t, hh, h;
     bool live, isq;
-    int t, h, hh;
   };
-  const auto row_of = [&](int r) {
+  const int step_t = per / max(H, 1), step_h = per - step_t * max(H, 1);
+  const auto row_at = [&](int t, int hh) {
     Row w;
-    w.live = r < rows;
-    w.t = w.live ? r / H : 0;
-    w.hh = w.live ? r - w.t * H : 0;
+    w.live = t < nt;
+    w.t = w.live ? t : 0;
+    w.hh = w.live ? hh : 0;
     w.isq = w.hh < nq;
     w.h = w.isq ? q0 + w.hh : k0 + w.hh - nq;
     return w;
   };
+  const auto step = [&](int& t, int& hh) {
+    t += step_t, hh += step_h;
+    if (hh >= H) hh -= H, ++t;
+  };
+  int now_t = tid / L / max(H, 1), now_h = tid / L - now_t * H;
   // The rows of a batch, and a quad's values, are requested before what depends on the page table and the positions.
   Piece x[kHeadBatch], y[kHeadBatch];
-  const auto load_rows = [&](int base) {
+  const auto load_rows = [&] {
+    int t = now_t, hh = now_h;
 #pragma unroll
     for (int j = 0; j < kHeadBatch; ++j) {
-      const Row w = row_of(base + j * per + tid / L);
+      const Row w = row_at(t, hh);
       if (w.live && c < C) {
-        const T* const src = from(w.isq ? a.q : a.k, tok0 + w.t, w.h) + at;
+        const T* const src = from(w.isq ? a.q : a.k, w.t, w.h) + at;
         x[j].v = *(const Vv*)src;
         if (paired) y[j].v = *(const Vv*)(src + half);
       }
+      step(t, hh);
     }
   };
-  // Four tokens' values of a head's group go to sixteen lanes: lane % 4 the octet, lane / 4 % 4 the token.
-  const int vlanes = 16 * W * nk, quads = (nt + 3) / 4;  // of four tokens
+  // The workgroup's four tokens' values of a head's group go to sixteen lanes: lane % 4 the octet, lane / 4 % 4 the token.
+  const int vlanes = 16 * W * nk, over_w = 65536 / W + 1;  // x * over_w >> 16 is x / W, for x up to some thousands
   struct Place {
     bool live, here;
-    int qd, h, gg, t, o;
+    int h, gg, t, o;
   };
   const auto value_of = [&](int item) {
     Place v;
-    v.live = item < quads * vlanes;
-    v.qd = v.live ? item / vlanes : 0;
-    const int in = v.live ? item - v.qd * vlanes : 0;
-    v.h = in / (16 * W);
-    v.gg = in / 16 % W;
-    v.t = v.qd * 4 + (in >> 2 & 3);
+    v.live = item < vlanes;
+    const int in = v.live ? item : 0;
+    v.h = mul24(in >> 4, over_w) >> 16;
+    v.gg = (in >> 4) - mul24(v.h, W);
+    v.t = in >> 2 & 3;
     v.o = 4 * v.gg + (in & 3);
     v.here = v.live && v.t < nt && v.o * 8 < a.dim;
     return v;
   };
   typedef typename Vec<T, 8>::type V8;
   V8 first_values{};
-  if constexpr (FAST) load_rows(0);
+  Piece qw, qw2, kw, kw2;  // a lane's norm weights are the same for all of its rows
+  if constexpr (FAST) {
+    load_rows();
+    if (c < C && a.q.w != nullptr) {
+      qw.v = *(const Vv*)((const T*)a.q.w + at);
+      if (paired) qw2.v = *(const Vv*)((const T*)a.q.w + half + at);
+    }
+    if (c < C && a.k.w != nullptr) {
+      kw.v = *(const Vv*)((const T*)a.k.w + at);
+      if (paired) kw2.v = *(const Vv*)((const T*)a.k.w + half + at);
+    }
+  }
+  const double first_turn = tid < nt * half ? a.turns[tid % half] : 0.0;
   if constexpr (CACHE) {
     const Place v = value_of(tid);
-    if (v.here) first_values = *(const V8*)(from(a.v, tok0 + v.t, k0 + v.h) + v.o * 8);
+    if (v.here) first_values = *(const V8*)(from(a.v, v.t, k0 + v.h) + v.o * 8);
     for (int t = tid; t < nt; t += kHeadThreads) {
       int place;
       const int b = kv_place(a.kv, tok0 + t, a.n_tokens, place);
       spots[t].place = place;
       spots[t].seq = b;
-      spots[t].block = b < 0 ? -1 : kv_block(a.kv, b, place);
+      const long long block = b < 0 ? -1 : kv_block(a.kv, b, place);
+      spots[t].at = block < 0 ? -1 : block * kv_block_bytes(W);
     }
     __syncthreads();
   }
@@ -210,7 +263,7 @@ __global__ __launch_bounds__(kHeadThreads) void heads_kernel(HeadArgs a, int TP,
       const long long from_ = b * a.pos_batch + (tt - b * a.seq) * a.pos_tok;
       p = a.pos64 ? (double)((const long long*)a.pos)[from_] : (double)((const int32_t*)a.pos)[from_];
     }
-    const double turns = p * a.turns[i - t * half];
+    const double turns = p * (i == tid ? first_turn : a.turns[i - t * half]);
     float s, co;
     sincospif(2.0f * (float)(turns - rint(turns)), &s, &co);
     cs[i] = a.mscale * co;
@@ -221,14 +274,15 @@ __global__ __launch_bounds__(kHeadThreads) void heads_kernel(HeadArgs a, int TP,
   const bool normed = a.q.w != nullptr || a.k.w != nullptr;
   for (int base = 0; base < rows; base += kHeadBatch * per) {  // the same count for every thread: lanes exchange sums
     if constexpr (FAST) {
-      if (base > 0) load_rows(base);
+      if (base > 0) load_rows();
     }
 #pragma unroll
     for (int j = 0; j < kHeadBatch; ++j) {
       if (base + j * per >= rows) break;
-      const Row r = row_of(base + j * per + tid / L);
+      const Row r = row_at(now_t, now_h);
+      step(now_t, now_h);
       const HeadSide& s = r.isq ? a.q : a.k;
-      T* const dst = (T*)s.out + ((long long)(tok0 + r.t) * s.heads + r.h) * a.dim;
+      T* const dst = (T*)s.out + (long long)tok0 * s.heads * a.dim + mul24(mul24(r.t, s.heads) + r.h, a.dim);
       float* const key = CACHE && !r.isq ? keys + (r.t * HK + r.hh - nq) * 32 * W : nullptr;
       const T* const w = (const T*)s.w;
       const bool none = CACHE && spots[r.t].seq < 0;  // its q comes back as zeros
@@ -246,9 +300,7 @@ __global__ __launch_bounds__(kHeadThreads) void heads_kernel(HeadArgs a, int TP,
         if (mine) {
           if (w != nullptr) {
             const float rn = 1.0f / sqrtf(ss / (float)a.dim + a.eps);
-            Piece wx, wy;
-            wx.v = *(const Vv*)(w + at);
-            if (paired) wy.v = *(const Vv*)(w + half + at);
+            const Piece wx = r.isq ? qw : kw, wy = r.isq ? qw2 : kw2;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
               xf[i] = xf[i] * rn * widen(wx.e[i]);
@@ -281,18 +333,12 @@ __global__ __launch_bounds__(kHeadThreads) void heads_kernel(HeadArgs a, int TP,
               if (paired) key[half + at + i] = yf[i];
             }
           } else {
-            Piece ox, oy;
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-              ox.e[i] = narrow<T>(none ? 0.0f : xf[i]);
-              oy.e[i] = narrow<T>(none ? 0.0f : yf[i]);
-            }
-            *(Vv*)(dst + at) = ox.v;
-            if (paired) *(Vv*)(dst + half + at) = oy.v;
+            *(Vv*)(dst + at) = none ? Vv{} : narrow_all<T, V>(xf);
+            if (paired) *(Vv*)(dst + half + at) = none ? Vv{} : narrow_all<T, V>(yf);
           }
         }
       } else {
-        const T* const src = from(s, tok0 + r.t, r.h);
+        const T* const src = from(s, r.t, r.h);
         float ss = 0.0f;
         if (r.live && w != nullptr)
           for (int i = c; i < a.dim; i += L) {
@@ -325,34 +371,33 @@ __global__ __launch_bounds__(kHeadThreads) void heads_kernel(HeadArgs a, int TP,
   }
 
   if constexpr (CACHE) {
-    const int O = 4 * W, blocks = a.kv.page / kKvBlock;
-    const long long bytes = kv_block_bytes(W);
-    for (int base = 0; base < quads * vlanes; base += kHeadThreads) {  // whole rows of sixteen lanes
+    const int O = 4 * W;
+    const uint32_t head_bytes = (uint32_t)(a.kv.page / kKvBlock * kv_block_bytes(W));
+    for (int base = 0; base < vlanes; base += kHeadThreads) {  // whole rows of sixteen lanes
       const Place p = value_of(base + tid);
       V8 v = first_values;
-      if (base > 0 && p.here) v = *(const V8*)(from(a.v, tok0 + p.t, k0 + p.h) + p.o * 8);
+      if (base > 0 && p.here) v = *(const V8*)(from(a.v, p.t, k0 + p.h) + p.o * 8);
       float f[8];
-      int code[8];
+      float codes[4];
       uint16_t sb, mb;
 #pragma unroll
       for (int j = 0; j < 8; ++j) f[j] = p.here ? widen(v[j]) : 0.0f;
-      quantize8(f, p.here, code, sb, mb);
+      quantize8(f, p.here, codes, sb, mb);
       const int z = tid >> 2 & 3, t = min(p.t, nt - 1);
       const Spot spot = spots[t];
-      const bool cached = p.live && p.t < nt && spot.block >= 0;
-      uint8_t* const blk = a.kv.pages + (spot.block + (long long)(k0 + p.h) * blocks) * bytes;
+      const bool cached = p.live && p.t < nt && spot.at >= 0;
+      uint8_t* const blk = a.kv.pages + spot.at + (uint64_t)(uint32_t)(k0 + p.h) * head_bytes;
       const int tok = spot.place & (kKvBlock - 1), oct = p.o & 3;
       // four neighbouring tokens of one block: whole words, of which lane z stores the z-th
-      const Spot head = spots[min(p.qd * 4, nt - 1)];
-      const bool in_row = cached && spot.block == head.block && spot.place == head.place + z && head.place % 4 == 0;
+      const Spot head = spots[0];
+      const bool in_row = cached && spot.at == head.at && spot.place == head.place + z && head.place % 4 == 0;
       const bool whole = (__ballot(in_row) >> (tid & 48) & 0xFFFF) == 0xFFFF;
       uint32_t word = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        uint32_t w = (uint32_t)(code[2 * j] | code[2 * j + 1] << 4);
         if (!whole && cached)
-          blk[kv_value_codes(W) + kv_value_word(W, p.gg, tok >> 2 & 3, oct * 4 + j, tok >> 4) + (tok & 3)] = (uint8_t)w;
-        w <<= 8 * z;
+          blk[kv_value_codes(W) + kv_value_word(W, p.gg, tok >> 2 & 3, oct * 4 + j, tok >> 4) + (tok & 3)] = (uint8_t)codes[j];
+        uint32_t w = __builtin_amdgcn_cvt_pk_u8_f32(codes[j], z, 0);
         w |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0x128, 0xF, 0xF, false);  // row_ror:8, then 4: over z
         w |= (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, 0x124, 0xF, 0xF, false);
         if (j == z) word = w;
@@ -369,19 +414,20 @@ __global__ __launch_bounds__(kHeadThreads) void heads_kernel(HeadArgs a, int TP,
     for (int base = 0; base < nt * nk * O; base += kHeadThreads) {  // quads of lanes share a group: O is whole quads
       const int item = base + tid;
       const bool live = item < nt * nk * O;
-      const int row = live ? item / O : 0, o = live ? item - row * O : 0, t = row / nk, h = row - t * nk;
+      const int rw = live ? item >> 2 : 0, row = mul24(rw, over_w) >> 16, o = live ? item - mul24(row, O) : 0;
+      const int t = (row >= nk) + (row >= 2 * nk) + (row >= 3 * nk), h = row - mul24(t, nk);
       const bool here = live && o * 8 < a.dim;
       float f[8];
-      int code[8];
+      float codes[4];
       uint16_t sb, mb;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = here ? keys[(t * HK + h) * 32 * W + o * 8 + j] : 0.0f;
-      quantize8(f, here, code, sb, mb);
-      if (!live || spots[t].block < 0) continue;
+      for (int j = 0; j < 8; ++j) f[j] = here ? keys[mul24(mul24(t, HK) + h, 32 * W) + o * 8 + j] : 0.0f;
+      quantize8(f, here, codes, sb, mb);
+      if (!live || spots[t].at < 0) continue;
       uint32_t word = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) word |= (uint32_t)code[j] << (4 * j);
-      uint8_t* const blk = a.kv.pages + (spots[t].block + (long long)(k0 + h) * blocks) * bytes;
+      for (int j = 0; j < 4; ++j) word = __builtin_amdgcn_cvt_pk_u8_f32(codes[j], j, word);
+      uint8_t* const blk = a.kv.pages + spots[t].at + (uint64_t)(uint32_t)(k0 + h) * head_bytes;
       const int tok = spots[t].place & (kKvBlock - 1);
       *(uint32_t*)(blk + tok * 16 * W + (o % 4) * 4 * W + (o / 4) * 4) = word;
       if (o % 4 == 0) *(uint32_t*)(blk + kv_key_scales(W) + (tok * W + o / 4) * 4) = sb | (uint32_t)mb << 16;
@@ -402,10 +448,10 @@ void launch_heads_t(const HeadArgs& a, hipStream_t stream) {
   const int kh = a.k.heads, qh = a.q.heads, H = qh + kh;
   int TP, HQ, HK, split;
   if (CACHE) {
-    TP = a.n_tokens > 512 ? 4 : 1;
+    TP = a.n_tokens > 256 ? 4 : 1;
     const int G = qh / kh;
     const int room = max(1, 8192 / (TP * 32 * W));  // keys that 32 KB hold
-    HK = min(min(kh, room), max(1, 64 / (TP == 1 ? 4 : 4 * W)));  // a lane an octet of the values of four tokens
+    HK = min(min(kh, room), TP == 1 ? 4 : max(1, (a.n_tokens >= 4096 ? 32 : 16) / W));  // a lane an octet of the values of four tokens
     HQ = HK * G;
     split = (kh + HK - 1) / HK;
   } else {
