@@ -39,11 +39,6 @@ struct HeadArgs {
   KvPages kv;
 };
 
-template <class T, int V>
-struct Vec {
-  typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T))));
-};
-
 template <class T>
 __device__ __forceinline__ float widen(T v) {
   if constexpr (sizeof(T) == 2)
@@ -115,31 +110,9 @@ __device__ __forceinline__ void quantize8(float (&x)[8], bool here, float (&byte
   m_bits = __builtin_bit_cast(uint16_t, mh);
 }
 
-struct Spot {      // of one token of the workgroup
-  long long at;    // byte offset of its block of the first head in the pages, or -1: it is not cached
-  int place, seq;  // seq -1: a row of no sequence
-};
-
 // Whole vectors' products: a multiplication of 32 bits costs four of 24.
 __device__ __forceinline__ int mul24(int a, int b) { return __mul24(a, b); }
 __device__ __forceinline__ long long mul64(int a, long long b) { return (long long)((uint64_t)(uint32_t)a * (uint64_t)b); }
-
-template <class T, int V>
-__device__ __forceinline__ typename Vec<T, V>::type narrow_all(const float (&v)[V]) {
-  typename Vec<T, V>::type r;
-#pragma unroll
-  for (int i = 0; i < V; i += 2) {
-    if constexpr (sizeof(T) == 2) {
-      typedef float f2 __attribute__((ext_vector_type(2)));
-      typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-      const uint32_t w = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){v[i], v[i + 1]}, b2));
-      r[i] = (uint16_t)w, r[i + 1] = (uint16_t)(w >> 16);
-    } else {
-      r[i] = v[i], r[i + 1] = v[i + 1];
-    }
-  }
-  return r;
-}
 
 // T the element type; FAST: vectors of V values. A workgroup takes TP tokens and, from grid.y, HQ heads of q and HK of k.
 template <class T, bool INTER, bool FAST, bool CACHE>
@@ -244,14 +217,7 @@ __global__ __launch_bounds__(kHeadThreads) void heads_kernel(HeadArgs a, int TP,
   if constexpr (CACHE) {
     const Place v = value_of(tid);
     if (v.here) first_values = *(const V8*)(from(a.v, v.t, k0 + v.h) + v.o * 8);
-    for (int t = tid; t < nt; t += kHeadThreads) {
-      int place;
-      const int b = kv_place(a.kv, tok0 + t, a.n_tokens, place);
-      spots[t].place = place;
-      spots[t].seq = b;
-      const long long block = b < 0 ? -1 : kv_block(a.kv, b, place);
-      spots[t].at = block < 0 ? -1 : block * kv_block_bytes(W);
-    }
+    for (int t = tid; t < nt; t += kHeadThreads) spots[t] = kv_spot(a.kv, tok0 + t, a.n_tokens, W);
     __syncthreads();
   }
   for (int i = tid; i < nt * half; i += kHeadThreads) {

@@ -98,6 +98,41 @@ __host__ __device__ inline int kv_place(const KvPages& p, int t, int n_tokens, i
   return b;
 }
 
+struct Spot {      // of one token of a workgroup
+  long long at;    // byte offset of its block of the first head in the pages, or -1: it has none
+  int place, seq;  // seq -1: a row of no sequence
+};
+__device__ __forceinline__ Spot kv_spot(const KvPages& p, int t, int n_tokens, int W) {
+  Spot s;
+  s.seq = kv_place(p, t, n_tokens, s.place);
+  const long long block = s.seq < 0 ? -1 : kv_block(p, s.seq, s.place);
+  s.at = block < 0 ? -1 : block * kv_block_bytes(W);
+  return s;
+}
+
+// V adjacent values, and their rounding.
+template <class T, int V>
+struct Vec {
+  typedef T type __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+};
+
+template <class T, int V>
+__device__ __forceinline__ typename Vec<T, V>::type narrow_all(const float (&v)[V]) {
+  typename Vec<T, V>::type r;
+#pragma unroll
+  for (int i = 0; i < V; i += 2) {
+    if constexpr (sizeof(T) == 2) {
+      typedef float f2 __attribute__((ext_vector_type(2)));
+      typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+      const uint32_t w = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){v[i], v[i + 1]}, b2));
+      r[i] = (uint16_t)w, r[i + 1] = (uint16_t)(w >> 16);
+    } else {
+      r[i] = v[i], r[i + 1] = v[i + 1];
+    }
+  }
+  return r;
+}
+
 // Heads normed and turned, with a cache or without (mxa_heads.hip); cached values read back (mxa_kv4.hip).
 int launch_heads(const void* q, const long long* q_strides, int q_heads, const void* q_weight, const void* k,
                  const long long* k_strides, int k_heads, const void* k_weight, float eps, const void* pos, bool pos64,
