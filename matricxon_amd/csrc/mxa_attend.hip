@@ -9,7 +9,8 @@
 //   o^T     += V^T p^T   the lane's own p, rounded to float16, is the second operand as it stands: the layout of the value
 //                        codes has the tokens in the order in which the scores come out
 //
-// so nothing but the row's maximum crosses lanes. Codes are widened in registers, code to float16 exactly (an or of its
+// so nothing but the row's maximum crosses lanes. HBM bounds it: 64 replies at 16384 places each, 8 key heads of 128 values,
+// read 1.34 GB in 257 us (5.2 TB/s), one at 131072 168 MB in 44 us with its join. Codes are widened in registers, code to float16 exactly (an or of its
 // bits into a float16's, less that float16), then s * code + m rounded once; q is brought by a power of two into float16's
 // range, exactly but for values below 2^-24 of its largest. Scores, maxima, sums and outputs are float32.
 #include <limits.h>
@@ -27,7 +28,9 @@ namespace {
 constexpr int kAttendThreads = 256, kAttendWaves = kAttendThreads / 64;
 
 // W groups of 32 values a head. Workgroup (split, pair, sequence) takes a split's blocks of a pair, which its waves take in
-// turn; their parts are joined in LDS, and the parts of a pair of several splits go to the workspace.
+// turn; their parts are joined in LDS, and the parts of a pair of several splits go to the workspace. No LDS holds the
+// codes: a lane's are adjacent and go to its registers, the next blocks' while the present one is computed, as many as leave
+// room for three workgroups a CU (two of heads above 128 values).
 template <int W>
 __global__ __launch_bounds__(kAttendThreads, W <= 4 ? 3 : 2) void attend_kernel(AttendArgs a) {
   constexpr int AHEAD = W <= 3 ? 3 : 2;  // blocks of a wave in registers, all but one of them on their way
@@ -261,7 +264,8 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join_kernel(AttendArgs 
   for (int j = 0; j < 4; ++j) dst[4 * tid + j] = bf16_rne(v[j] * norm);
 }
 
-// The same for few parts: a workgroup takes the 16 rows of a pair, sixteen threads each.
+// The same for few parts (16 and fewer): a workgroup takes the 16 rows of a pair, sixteen threads each. 64 replies of 6
+// parts: 6 us, and 17 with a workgroup a row; one reply of 96 parts the other way round.
 __global__ __launch_bounds__(kAttendThreads) void attend_join_rows_kernel(AttendArgs a, int W) {
   const int b = blockIdx.y, pair = blockIdx.x, r = threadIdx.x >> 4, piece = threadIdx.x & 15;
   const int h = pair % a.kv.heads, rt = pair / a.kv.heads;
@@ -293,17 +297,9 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join_rows_kernel(Attend
 }
 
 // (std::min and std::max here: on the host, HIP's own of that name take ints.)
-// How the places of up to `most` tokens of each sequence are shared out. Sequences of up to kFewRows rows a key head go in
-// tiles of 16 rows (attend_kernel), others in those of attend_tile_kernel; a call without query_starts has one kind.
-constexpr int kFewRows = 64, kTileSplits = 16, kFewParts = 16;
-struct Plan {
-  bool few, many;     // the kinds that there may be
-  long long pairs[2]; // (tile of 16 rows, key head) of a sequence
-  int splits[2], chunk[2];
-  int rows;           // of a workgroup, for many rows
-  long long tiles;    // of the call, for many rows
-};
-
+// Shares of `least` to `most` blocks for the workgroups that the CUs hold at once. At least two blocks a wave: 1000 places
+// of one reply 13.8 us in shares of 4 blocks, 11.8 of 8, 12.2 of 16. At most 128 blocks where several sequences end at
+// places that the host does not know: 64 replies of up to 16384 places 188 us without, 149 us with that bound, 160 of 96.
 void share_out(long long blocks, long long workgroups, long long slots, int least, int most, int& splits, int& chunk) {
   const long long want = std::max<long long>(1, slots / workgroups);
   chunk = (int)std::max<long long>(least, std::min<long long>(most, (blocks + want - 1) / want));
@@ -311,6 +307,20 @@ void share_out(long long blocks, long long workgroups, long long slots, int leas
   splits = (int)((blocks + chunk - 1) / chunk);
   chunk = (int)((blocks + splits - 1) / splits);
 }
+
+// How the places of up to `most` tokens of each sequence are shared out. Sequences of up to kFewRows rows a key head go in
+// tiles of 16 rows (attend_kernel), others in those of attend_tile_kernel, which widens a
+// place once for all of them; a call without query_starts has one kind. 16 sequences of
+// 2048 places take, of 64 rows a key head, 32 us in tiles of 16 and 41 in the others; of 96 rows 39 and 43; of 128 rows 51
+// and 45, and of every length up to that 36 and 43.
+constexpr int kFewRows = 128, kTileSplits = 16, kFewParts = 16, kLeastBlocks = 8, kMostBlocks = 128;
+struct Plan {
+  bool few, many;     // the kinds that there may be
+  long long pairs[2]; // (tile of 16 rows, key head) of a sequence
+  int splits[2], chunk[2];
+  int rows;           // of a workgroup, for many rows
+  long long tiles;    // of the call, for many rows
+};
 
 Plan plan_of(int n_seq, int n_tokens, bool ragged, int kv_heads, int group, int max_length, long long window, int dim) {
   Plan p{};
@@ -323,15 +333,20 @@ Plan plan_of(int n_seq, int n_tokens, bool ragged, int kv_heads, int group, int 
   if (p.few) {
     p.pairs[0] = (std::min<long long>(most, kFewRows) + 15) / 16 * kv_heads;
     const long long slots = 256 * (narrow ? 3 : 2);  // workgroups that the CUs hold at once
-    // one sequence: what the CUs hold at once; several, whose lengths are not known: four times that, in parts small
-    // enough to even out
-    share_out(blocks, p.pairs[0] * n_seq, slots, 8, n_seq > 1 ? 128 : INT_MAX, p.splits[0], p.chunk[0]);
+    share_out(blocks, p.pairs[0] * n_seq, slots, kLeastBlocks, n_seq > 1 ? kMostBlocks : INT_MAX, p.splits[0], p.chunk[0]);
   }
   if (p.many) {
     p.pairs[1] = (most + 15) / 16 * kv_heads;
-    p.rows = narrow && most > 128 ? 256 : 128;
+    // Workgroups of 256 rows widen a place once for all; where they are too few for the CUs and their places few as well,
+    // two of 128 rows hide each other's waits: 128 tokens x 32 heads of 128, window 1024: 27.9 and 22.3 us; without, over
+    // 8192 places, 52.7 and 57.2.
+    const auto span_of = [&](int rows) {
+      return window > 0 ? std::min<long long>(max_length, (long long)window + rows / group) / kKvBlock + 2 : blocks;
+    };
+    const bool fill = (most + 255) / 256 * kv_heads * (ragged ? 1 : n_seq) >= 256;
+    p.rows = narrow && most > 128 && (fill || span_of(256) > 48) ? 256 : 128;
     p.tiles = ragged ? most / p.rows + std::min<long long>(n_seq, most / (kFewRows + 1)) : (most + p.rows - 1) / p.rows * n_seq;
-    const long long span = window > 0 ? std::min<long long>(max_length, window + p.rows / group) / kKvBlock + 2 : blocks;
+    const long long span = span_of(p.rows);
     const long long groups = p.tiles * kv_heads, slots = narrow && p.rows == 128 ? 512 : 256;
     // Parts of a tile's places, by what they cost: as many rounds of the CUs as the workgroups take, each a part's blocks
     // and some 10 blocks' time to begin and end, and the join

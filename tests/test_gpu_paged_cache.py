@@ -549,3 +549,115 @@ def test_refusals(gpu) -> None:
     assert attend(q=q[:0]).shape == (0, 4, 64) and append(q=q[:0], k=k[:0], v=k[:0]).shape == (0, 4, 64)
     assert cache.read(0, table, lengths)[0].shape == (0, 2, 64)
     assert attend(q=q[:0], table=table[:0], lengths=lengths[:0]).numel() == 0
+
+
+# ---- many rows of a key head: tiles of 128 and 256 rows, whose places may be shared out
+@pytest.mark.parametrize("dim", [8, 32, 64, 96, 128, 160, 200, 256])
+@pytest.mark.parametrize("group, n", [(1, 65), (1, 129), (4, 33), (5, 70), (16, 40)])
+@pytest.mark.parametrize("length", [0, 2500])
+def test_many_rows(gpu, dim, group, n, length) -> None:
+    """At the beginning of a sequence and behind some thousand places; ends inside a block, a page and a tile."""
+    g = torch.Generator(device="cuda").manual_seed(dim + group + n + length)
+    lengths = [n + length, n, n + length // 2 + 7]
+    cache, table = filled(g, 3, lengths, 2, dim, 96)
+    q = rand(g, 3 * n, 2 * group, dim, dt=BF16)
+    check_attention(cache, q, cache.attend(q, table, i32(lengths)), table, lengths, [n] * 3)
+
+
+@pytest.mark.parametrize("window", [1, 31, 64, 700])
+@pytest.mark.parametrize("dim, n", [(64, 40), (128, 300), (192, 70)])
+def test_many_rows_in_a_window(gpu, dim, n, window) -> None:
+    g = torch.Generator(device="cuda").manual_seed(window + n)
+    lengths = [1500, n]
+    cache, table = filled(g, 2, lengths, 1, dim, 64)
+    q = rand(g, 2 * n, 4, dim, dt=BF16)
+    for most in (None, 100):
+        got = cache.attend(q, table, i32(lengths), window=window, max_length=most)
+        check_attention(cache, q, got, table, lengths, [n, n], window=window)
+
+
+@pytest.mark.parametrize("n", [40, 300])
+def test_many_rows_with_steep_scores(gpu, n) -> None:
+    """As test_steep_and_flat_scores; places whose scores rise, fall, and are alike."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    lengths = [700]
+    cache, table = filled(g, 1, lengths, 1, 64, 64, scale=4.0)
+    q = rand(g, n, 4, 64) * torch.logspace(-6, 1.3, 4 * n, device="cuda").view(n, 4, 1)
+    q[3] = 0
+    for scale in (None, -0.25, 0.0, 1.0):
+        got = cache.attend(q.bfloat16(), table, i32(lengths), scale=scale)
+        check_attention(cache, q.bfloat16(), got, table, lengths, [n], scale=scale)
+    big = (q * 1e30).bfloat16()
+    check_attention(cache, big, cache.attend(big, table, i32(lengths), scale=1e-30), table, lengths, [n], scale=1e-30)
+    ramp = torch.linspace(-20, 20, 700, device="cuda")[:, None, None] + 0.1 * rand(g, 700, 1, 64)
+    for sign in (1, -1):
+        cache.append(None, (sign * ramp).contiguous(), rand(g, 700, 1, 64), table, i32(lengths))
+        q = rand(g, n, 4, 64, dt=BF16).abs()
+        check_attention(cache, q, cache.attend(q, table, i32(lengths)), table, lengths, [n])
+
+
+def test_many_rows_that_attend_to_nothing(gpu) -> None:
+    """Lengths of 0, below 0 and shorter than the rows; pages that are none before, in and behind what is attended to."""
+    g = torch.Generator(device="cuda").manual_seed(21)
+    cache, table = filled(g, 5, [512] * 5, 2, 64, 32)
+    table[3, :4], table[3, 9], table[4] = -1, cache.n_pages, -5
+    lengths, n = [0, -7, 30, 512, 512], 70
+    q = rand(g, 5 * n, 4, 64, dt=BF16)
+    for window in (0, 40):
+        got = cache.attend(q, table, i32(lengths), window=window)
+        assert (got[: 2 * n + 40] == 0).all() and (got[4 * n :] == 0).all() and got.isfinite().all()
+        check_attention(cache, q[3 * n : 4 * n], got[3 * n : 4 * n], table[3:4], [512], [n], window=window)
+        check_attention(cache, q[2 * n + 40 : 3 * n], got[2 * n + 40 : 3 * n], table[2:3], [30], [30], window=window)
+
+
+@pytest.mark.parametrize("n", [70, 300])
+def test_many_rows_and_not_a_number(gpu, n) -> None:
+    """In q it stays in its row; in later tokens, and in what lies behind the end, it reaches nobody before."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    cache, table = filled(g, 1, [900], 1, 64, 32)
+    q = rand(g, n, 4, 64, dt=BF16)
+    clean = cache.attend(q, table, i32([900]))
+    dirty = q.clone()
+    dirty[1, 2, 7], dirty[n - 1, 0, 0] = math.nan, math.inf
+    got = cache.attend(dirty, table, i32([900]))
+    others = torch.ones(n, 4, dtype=torch.bool, device="cuda")
+    others[1, 2] = others[n - 1, 0] = False
+    assert got[1, 2].isnan().all()
+    check_attention(cache, q, torch.where(others[..., None], got, clean), table, [900], [n])
+    k, v = rand(g, n, 1, 64, dt=BF16), rand(g, n, 1, 64, dt=BF16)
+    cache.append(None, k, v, table, i32([900]))
+    clean = cache.attend(q, table, i32([900]))
+    k[n // 2 :], v[n // 2 :] = math.nan, math.inf
+    cache.append(None, k, v, table, i32([900]))
+    got = cache.attend(q, table, i32([900]))
+    assert same(got[: n // 2], clean[: n // 2]) and got.isfinite().all()
+
+
+def test_many_rows_captured(gpu) -> None:
+    """Chunks and replies in one captured call, which moves on with lengths and starts; two graphs in turn."""
+    g = torch.Generator(device="cuda").manual_seed(23)
+    lengths, counts = [900, 640, 33], [100, 1, 33]
+    cache, table = filled(g, 3, [1000, 700, 300], 2, 128, 64)
+    q, out = rand(g, 160, 8, 128, dt=BF16), torch.full((160, 8, 128), 7.0, dtype=BF16, device="cuda")
+    length, starts = i32(lengths), starts_of(counts)
+    graphs = []
+    for _ in range(2):
+        cache.attend(q, table, length, starts, out=out)
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            cache.attend(q, table, length, starts, out=out)
+    for i in range(4):
+        lengths = [lengths[0] + 20, lengths[1] + 11, lengths[2] + 60]
+        counts = [counts[0] - 20, 1 + 25 * i, counts[2] + 3]
+        length.copy_(i32(lengths))
+        starts.copy_(starts_of(counts))
+        q.copy_(rand(g, 160, 8, 128, dt=BF16))
+        out.fill_(7.0)
+        graphs[i % 2].replay()
+        got = out.clone()
+        t = sum(counts)
+        assert (got[t:] == 7.0).all()  # rows of no sequence: as they were
+        check_attention(cache, q[:t], got[:t], table, lengths, counts)
+        out.fill_(7.0)
+        assert same(cache.attend(q, table, length, starts, out=out), got)
