@@ -264,41 +264,52 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join_kernel(AttendArgs 
   for (int j = 0; j < 4; ++j) dst[4 * tid + j] = bf16_rne(v[j] * norm);
 }
 
-// The same for few parts (16 and fewer): a workgroup takes the 16 rows of a pair, sixteen threads each. 64 replies of 6
-// parts: 6 us, and 17 with a workgroup a row; one reply of 96 parts the other way round.
+// The same for few parts (16 and fewer): a workgroup takes the rows of a pair, its threads vectors of four values, whose
+// parts are requested eight at a time. 64 replies of up to 6 parts: 5 us,
+// 11 with sixteen threads a row and parts in turn, 17 with a workgroup a row; one reply of 96 parts takes 5 with that.
 __global__ __launch_bounds__(kAttendThreads) void attend_join_rows_kernel(AttendArgs a, int W) {
-  const int b = blockIdx.y, pair = blockIdx.x, r = threadIdx.x >> 4, piece = threadIdx.x & 15;
+  constexpr int U = 8;
+  const int b = blockIdx.y, pair = blockIdx.x;
   const int h = pair % a.kv.heads, rt = pair / a.kv.heads;
   const Sequence seq = Sequence(a, b).uniform();
-  const int parts = seq.splits;
-  if (rt * 16 + r >= seq.rows || parts == 1) return;
+  const int parts = seq.splits, rows = min(16, seq.rows - rt * 16), vectors = a.dim / 4;
+  if (parts == 1) return;
   const AttendPart first = a.part_of(b, pair, 0, W);
   const size_t step = 16 * 32 * W + 32;
-  float top = -INFINITY, total = 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < parts; ++i) top = fmaxf(top, first.ml[i * step + r]);
-  const float ref = top == -INFINITY ? 0.0f : top;
-  f32x4 v[4]{};
-#pragma unroll 2
-  for (int i = 0; i < parts; ++i) {
-    const float f = exp2_(first.ml[i * step + r] - ref);
-    total += f * first.ml[i * step + 16 + r];
+  for (int item = threadIdx.x; item < rows * vectors; item += kAttendThreads) {
+    const int r = item / vectors, at = item - r * vectors;
+    float top = -INFINITY, total = 0.0f;
+    f32x4 v{0, 0, 0, 0};
+    for (int base = 0; base < parts; base += U) {
+      float m[U], l[U], most = top;
+      f32x4 o[U];
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (4 * piece + 64 * j < a.dim) v[j] += f * *(const f32x4*)(first.o + i * step + r * 32 * W + 4 * piece + 64 * j);
+      for (int i = 0; i < U; ++i) {
+        const size_t from = step * min(base + i, parts - 1);  // behind the last, its own again, and left out
+        m[i] = first.ml[from + r], l[i] = first.ml[from + 16 + r];
+        o[i] = *(const f32x4*)(first.o + from + r * 32 * W + 4 * at);
+        most = fmaxf(most, m[i]);
+      }
+      const float ref = most == -INFINITY ? 0.0f : most, alpha = exp2_(top - ref);
+      total *= alpha, v *= alpha;
+#pragma unroll
+      for (int i = 0; i < U; ++i) {
+        const float f = base + i < parts ? exp2_(m[i] - ref) : 0.0f;
+        total += f * l[i];
+        v += f * o[i];
+      }
+      top = most;
+    }
+    const float norm = total > 0.0f || total != total ? 1.0f / total : 0.0f;
+    uint16_t* const dst = a.out_row(seq.first + (rt * 16 + r) / a.group, h * a.group + (rt * 16 + r) % a.group) + 4 * at;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) dst[j] = bf16_rne(v[j] * norm);
   }
-  const float norm = total > 0.0f || total != total ? 1.0f / total : 0.0f;
-  uint16_t* const dst = a.out_row(seq.first + (rt * 16 + r) / a.group, h * a.group + (rt * 16 + r) % a.group);
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (4 * piece + 64 * j < a.dim)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) dst[4 * piece + 64 * j + i] = bf16_rne(v[j][i] * norm);
 }
 
 // (std::min and std::max here: on the host, HIP's own of that name take ints.)
 // Shares of `least` to `most` blocks for the workgroups that the CUs hold at once. At least two blocks a wave: 1000 places
-// of one reply 13.8 us in shares of 4 blocks, 11.8 of 8, 12.2 of 16. At most 128 blocks where several sequences end at
+// of one reply took 13.8 us in shares of 4 blocks, 11.8 of 8, 12.2 of 16 (9.5 since their join is faster). At most 128 blocks where several sequences end at
 // places that the host does not know: 64 replies of up to 16384 places 188 us without, 149 us with that bound, 160 of 96.
 void share_out(long long blocks, long long workgroups, long long slots, int least, int most, int& splits, int& chunk) {
   const long long want = std::max<long long>(1, slots / workgroups);
@@ -309,10 +320,10 @@ void share_out(long long blocks, long long workgroups, long long slots, int leas
 }
 
 // How the places of up to `most` tokens of each sequence are shared out. Sequences of up to kFewRows rows a key head go in
-// tiles of 16 rows (attend_kernel), others in those of attend_tile_kernel, which widens a
-// place once for all of them; a call without query_starts has one kind. 16 sequences of
-// 2048 places take, of 64 rows a key head, 32 us in tiles of 16 and 41 in the others; of 96 rows 39 and 43; of 128 rows 51
-// and 45, and of every length up to that 36 and 43.
+// tiles of 16 rows (attend_kernel), others in those of attend_tile_kernel, which widens a place once for
+// all of them; a call without query_starts has one kind. 16 sequences of 2048 places take, of 64 rows a key head, 32 us in
+// tiles of 16 and 41 in the others; of 96 rows 39 and 43; of 128 rows 51 and 45, and with lengths of all sizes up to 2048
+// 36 and 43.
 constexpr int kFewRows = 128, kTileSplits = 16, kFewParts = 16, kLeastBlocks = 8, kMostBlocks = 128;
 struct Plan {
   bool few, many;     // the kinds that there may be
