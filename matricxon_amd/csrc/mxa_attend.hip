@@ -202,7 +202,7 @@ __global__ __launch_bounds__(kAttendThreads, W <= 4 ? 3 : 2) void attend_kernel(
     }
     const bool whole = seq.splits == 1;
     const float norm = total > 0.0f || total != total ? 1.0f / total : 0.0f;
-    const AttendPart to = a.part_of(b, blockIdx.y, split, W);
+    const AttendPart to = a.part_of(b, seq.first, rt, h, split, W);
     uint16_t* const dst = a.out_row(seq.first + (rt * 16 + r) / a.group, h * a.group + (rt * 16 + r) % a.group);
     if (!whole && piece == 0) {
       to.ml[r] = top;
@@ -232,14 +232,15 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join_kernel(AttendArgs 
   const int parts = seq.splits;
   if (rt * 16 + r >= seq.rows || parts == 1) return;
   float top = -INFINITY, total = 0.0f;
-  for (int i = tid; i < parts; i += kAttendThreads) top = fmaxf(top, a.part_of(b, pair, i, W).ml[r]);
+  const auto part = [&](int i) { return a.part_of(b, seq.first, rt, h, i, W); };
+  for (int i = tid; i < parts; i += kAttendThreads) top = fmaxf(top, part(i).ml[r]);
   for (int i = 1; i < 64; i *= 2) top = fmaxf(top, __shfl_xor(top, i));
   if ((tid & 63) == 0) wave_max[tid >> 6] = top;
   __syncthreads();
   for (int i = 0; i < kAttendWaves; ++i) top = fmaxf(top, wave_max[i]);
   const float ref = top == -INFINITY ? 0.0f : top;
   for (int i = tid; i < parts; i += kAttendThreads) {
-    const AttendPart p = a.part_of(b, pair, i, W);
+    const AttendPart p = part(i);
     f[i] = exp2_(p.ml[r] - ref);
     total += f[i] * p.ml[16 + r];
   }
@@ -250,7 +251,7 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join_kernel(AttendArgs 
   f32x4 v{0, 0, 0, 0};
   if (mine < side) {
 #pragma unroll 4
-    for (int i = mine; i < parts; i += side) v += f[i] * *(const f32x4*)(a.part_of(b, pair, i, W).o + r * 32 * W + 4 * at);
+    for (int i = mine; i < parts; i += side) v += f[i] * *(const f32x4*)(part(i).o + r * 32 * W + 4 * at);
   }
   sums[tid] = v;
   __syncthreads();
@@ -274,7 +275,7 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join_rows_kernel(Attend
   const Sequence seq = Sequence(a, b).uniform();
   const int parts = seq.splits, rows = min(16, seq.rows - rt * 16), vectors = a.dim / 4;
   if (parts == 1) return;
-  const AttendPart first = a.part_of(b, pair, 0, W);
+  const AttendPart first = a.part_of(b, seq.first, rt, h, 0, W);
   const size_t step = 16 * 32 * W + 32;
   for (int item = threadIdx.x; item < rows * vectors; item += kAttendThreads) {
     const int r = item / vectors, at = item - r * vectors;
@@ -309,12 +310,15 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join_rows_kernel(Attend
 
 // (std::min and std::max here: on the host, HIP's own of that name take ints.)
 // Shares of `least` to `most` blocks for the workgroups that the CUs hold at once. At least two blocks a wave: 1000 places
-// of one reply took 13.8 us in shares of 4 blocks, 11.8 of 8, 12.2 of 16 (9.5 since their join is faster). At most 128 blocks where several sequences end at
-// places that the host does not know: 64 replies of up to 16384 places 188 us without, 149 us with that bound, 160 of 96.
-void share_out(long long blocks, long long workgroups, long long slots, int least, int most, int& splits, int& chunk) {
+// of one reply took 13.8 us in shares of 4 blocks, 11.8 of 8, 12.2 of 16 (9.5 since their join is faster). At most 128
+// blocks where several sequences end at places that the host does not know: 64 replies of up to 16384 places 188 us without,
+// 149 us with that bound, 160 of 96. More of them where the parts would not fit into kMostFloats.
+void share_out(long long blocks, long long workgroups, long long slots, int least, int most, int most_splits, int& splits,
+               int& chunk) {
   const long long want = std::max<long long>(1, slots / workgroups);
   chunk = (int)std::max<long long>(least, std::min<long long>(most, (blocks + want - 1) / want));
-  chunk = (int)std::max<long long>(chunk, (blocks + kAttendMaxSplits - 1) / kAttendMaxSplits);
+  most_splits = std::min<int>(most_splits, kAttendMaxSplits);
+  chunk = (int)std::max<long long>(chunk, (blocks + most_splits - 1) / most_splits);
   splits = (int)((blocks + chunk - 1) / chunk);
   chunk = (int)((blocks + splits - 1) / splits);
 }
@@ -325,12 +329,14 @@ void share_out(long long blocks, long long workgroups, long long slots, int leas
 // tiles of 16 and 41 in the others; of 96 rows 39 and 43; of 128 rows 51 and 45, and with lengths of all sizes up to 2048
 // 36 and 43.
 constexpr int kFewRows = 128, kTileSplits = 16, kFewParts = 16, kLeastBlocks = 8, kMostBlocks = 128;
+constexpr long long kMostFloats = 64 << 20;  // of a workspace
 struct Plan {
   bool few, many;     // the kinds that there may be
   long long pairs[2]; // (tile of 16 rows, key head) of a sequence
   int splits[2], chunk[2];
   int rows;           // of a workgroup, for many rows
   long long tiles;    // of the call, for many rows
+  long long floats;   // of all tiles' parts, one each
 };
 
 Plan plan_of(int n_seq, int n_tokens, bool ragged, int kv_heads, int group, int max_length, long long window, int dim) {
@@ -341,10 +347,12 @@ Plan plan_of(int n_seq, int n_tokens, bool ragged, int kv_heads, int group, int 
   const long long reach = window > 0 ? std::min<long long>(max_length, window + most / group) : max_length;
   const long long blocks = reach / kKvBlock + 2;
   const bool narrow = kv_groups(dim) <= 4;
+  p.floats = ((long long)n_tokens * group / 16 + n_seq) * kv_heads * (long long)part_floats(kv_groups(dim));
   if (p.few) {
     p.pairs[0] = (std::min<long long>(most, kFewRows) + 15) / 16 * kv_heads;
     const long long slots = 256 * (narrow ? 3 : 2);  // workgroups that the CUs hold at once
-    share_out(blocks, p.pairs[0] * n_seq, slots, kLeastBlocks, n_seq > 1 ? kMostBlocks : INT_MAX, p.splits[0], p.chunk[0]);
+    share_out(blocks, p.pairs[0] * n_seq, slots, kLeastBlocks, n_seq > 1 ? kMostBlocks : INT_MAX,
+              (int)std::max<long long>(1, kMostFloats / p.floats), p.splits[0], p.chunk[0]);
   }
   if (p.many) {
     p.pairs[1] = (most + 15) / 16 * kv_heads;
@@ -366,17 +374,16 @@ Plan plan_of(int n_seq, int n_tokens, bool ragged, int kv_heads, int group, int 
       const double cost = (double)((groups * n + slots - 1) / slots) * ((double)span / n + 10) + (n > 1 ? 8 : 0);
       if (n == 1 || cost < 0.95 * least) least = cost, p.splits[1] = n;
     }
-    // the workspace has room for as many rows of each sequence as any may have: not split where that is large
-    if ((long long)n_seq * p.pairs[1] * p.splits[1] * part_floats(kv_groups(dim)) > 16 << 20) p.splits[1] = 1;
+    if (p.floats * p.splits[1] > kMostFloats) p.splits[1] = 1;
     p.chunk[1] = 0;
   }
   return p;
 }
 
-size_t part_bytes(const Plan& p, int kind, int n_seq, int dim) {
-  return p.splits[kind] <= 1 ? 0 : (size_t)n_seq * p.pairs[kind] * p.splits[kind] * part_floats(kv_groups(dim)) * sizeof(float);
+size_t part_bytes(const Plan& p, int kind) {
+  return p.splits[kind] <= 1 ? 0 : (size_t)(p.floats * p.splits[kind]) * sizeof(float);
 }
-size_t parts_bytes(const Plan& p, int n_seq, int dim) { return part_bytes(p, 0, n_seq, dim) + part_bytes(p, 1, n_seq, dim); }
+size_t parts_bytes(const Plan& p) { return part_bytes(p, 0) + part_bytes(p, 1); }
 
 template <int W>
 void launch_few(const AttendArgs& a, hipStream_t stream) {
@@ -387,20 +394,20 @@ void launch_few(const AttendArgs& a, hipStream_t stream) {
 
 size_t attend_workspace(int n_seq, int n_tokens, bool ragged, int kv_heads, int group, int max_length, int window, int dim) {
   const Plan p = plan_of(n_seq, n_tokens, ragged, kv_heads, group, max_length, window, dim);
-  return parts_bytes(p, n_seq, dim);
+  return parts_bytes(p);
 }
 
 int launch_attend(AttendArgs a, int max_length, void* workspace, size_t workspace_bytes, hipStream_t stream) {
   const Plan p = plan_of(a.kv.n_seq, a.n_tokens, a.kv.starts != nullptr, a.kv.heads, a.group, max_length, a.window, a.dim);
   if (p.pairs[0] > 65535 || (p.splits[1] > 1 && p.pairs[1] > 65535) || p.tiles * a.kv.heads >= 1 << 23) return kAttendUnsupported;
-  const size_t need = parts_bytes(p, a.kv.n_seq, a.dim);  // of the plan that is launched
+  const size_t need = parts_bytes(p);  // of the plan that is launched
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return kAttendWorkspace;
   const int W = kv_groups(a.dim);
   for (int kind = 0; kind < 2; ++kind) {
     if (!(kind ? p.many : p.few)) continue;
     a.least_rows = kind ? kFewRows + 1 : 1, a.most_rows = kind ? 0x7fffffff : kFewRows;
     a.pairs = (int)p.pairs[kind], a.splits = p.splits[kind], a.chunk = p.chunk[kind];
-    a.part = (float*)((char*)workspace + (kind ? part_bytes(p, 0, a.kv.n_seq, a.dim) : 0));
+    a.part = (float*)((char*)workspace + (kind ? part_bytes(p, 0) : 0));
     if (kind == 1) {
       launch_attend_tile(a, p.rows, p.tiles, stream);
     } else {

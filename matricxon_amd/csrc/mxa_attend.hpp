@@ -50,8 +50,11 @@ struct AttendArgs {
     return q + (long long)b * q_batch + (long long)(t - b * seq) * q_tok + (long long)h * q_head;
   }
   __device__ __forceinline__ uint16_t* out_row(int t, int h) const { return out + ((long long)t * heads + h) * dim; }
-  __device__ __forceinline__ AttendPart part_of(int b, int pair, int split, int w) const {
-    float* const p = part + (((long long)b * pairs + pair) * splits + split) * (16 * 32 * w + 32);
+  // Of tile rt of sequence b, whose rows begin at `first`: as each sequence has one tile of 16 rows more than its rows' share
+  // of the call's at most, the tiles of those before it are first * group / 16 + b and fewer.
+  __device__ __forceinline__ AttendPart part_of(int b, int first, int rt, int h, int split, int w) const {
+    const long long tile = (long long)first * group / 16 + b + rt;
+    float* const p = part + ((tile * kv.heads + h) * splits + split) * (16 * 32 * w + 32);
     return AttendPart{p, p + 16 * 32 * w};
   }
 };

@@ -370,7 +370,7 @@ __global__ __launch_bounds__(64 * NW, W <= 4 ? 2 : 1) void attend_tile_kernel(At
         }
       }
   } else {
-    const AttendPart part = a.part_of(b, row / 16 * a.kv.heads + h, split, W);
+    const AttendPart part = a.part_of(b, seq.first, row / 16, h, split, W);
     if (g == 0) {
       part.ml[row % 16] = m;
       part.ml[16 + row % 16] = l;

@@ -112,6 +112,14 @@ def test_windows_past_every_length_change_no_workspace(lib, shape, max_length) -
         assert lib.mxa_kv4_attend_workspace_bytes(*shape, max_length, window) == want
 
 
+def test_workspace_stays_small(lib) -> None:
+    """Many sequences, rows that differ, long tables: the parts share 256 MiB, and are as many as the rows need."""
+    for shape in ((64, 575, 1, 32, 8, 128), (64, 64, 0, 32, 8, 128), (1000, 1000, 0, 64, 8, 256), (65535, 65535, 1, 32, 8, 128),
+                  (4, 8000, 1, 32, 8, 128)):
+        for most in (4096, 1 << 20, 1 << 30):
+            assert lib.mxa_kv4_attend_workspace_bytes(*shape, most, 0) <= 2 * (1 << 28), (shape, most)
+
+
 def test_a_cache_lies_on_a_device() -> None:
     from matricxon_amd.attention import HipPagedCache
 
