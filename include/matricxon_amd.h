@@ -416,14 +416,15 @@ int mxa_norm_rope(const void *q, const long long *q_strides, int q_heads, const 
  * written for it, it reads as zeros and is not attended to. The call's rows are the last tokens of the sequences: rows
  * [query_starts[b], query_starts[b + 1]) those of b (n_seq + 1 ascending values; rows outside all belong to none), or
  * with query_starts NULL n_tokens / n_seq of each. table, lengths and query_starts are DEVICE int32.
- * kv_heads <= MXA_KV4_MAX_HEADS, page_size a multiple of 32 up to MXA_KV4_MAX_PAGE, head_dim a multiple of 8 up to MXA_KV4_MAX_DIM,
- * table_width * page_size <= MXA_KV4_MAX_PLACES, n_seq <= MXA_KV4_MAX_SEQ, n_tokens <= MXA_MAX_TOKENS; else -1. */
+ * kv_heads <= MXA_KV4_MAX_HEADS, page_size a multiple of 32 up to MXA_KV4_MAX_PAGE, head_dim a multiple of 8 up to
+ * MXA_KV4_MAX_DIM, table_width * page_size <= MXA_KV4_MAX_PLACES, n_seq <= MXA_KV4_MAX_SEQ, n_tokens <= MXA_MAX_TOKENS,
+ * of mxa_kv4_attend n_tokens * q_heads <= MXA_KV4_MAX_ROWS; else -1. */
 #define MXA_KV4_MAX_HEADS 4096
 #define MXA_KV4_MAX_DIM 256
 #define MXA_KV4_MAX_PAGE 65536
 #define MXA_KV4_MAX_PLACES (1 << 30)
 #define MXA_KV4_MAX_SEQ 65535
-#define MXA_KV4_MAX_ROWS (1 << 28) /* n_tokens * q_heads of mxa_kv4_attend */
+#define MXA_KV4_MAX_ROWS (1 << 28)
 
 /* Bytes of one page; 0 for sizes that are not supported. Host-only. */
 size_t mxa_kv4_page_bytes(int kv_heads, int page_size, int head_dim);

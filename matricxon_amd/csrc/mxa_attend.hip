@@ -10,9 +10,10 @@
 //                        codes has the tokens in the order in which the scores come out
 //
 // so nothing but the row's maximum crosses lanes. HBM bounds it: 64 replies at 16384 places each, 8 key heads of 128 values,
-// read 1.34 GB in 257 us (5.2 TB/s), one at 131072 168 MB in 44 us with its join. Codes are widened in registers, code to float16 exactly (an or of its
-// bits into a float16's, less that float16), then s * code + m rounded once; q is brought by a power of two into float16's
-// range, exactly but for values below 2^-24 of its largest. Scores, maxima, sums and outputs are float32.
+// read 1.34 GB in 257 us (5.2 TB/s), one at 131072 168 MB in 42 us with its join. Codes are widened in registers, code to
+// float16 exactly (an or of its bits into a float16's, less that float16), then s * code + m rounded once; q is brought by a
+// power of two into float16's range, exactly but for values below 2^-24 of its largest. Scores, maxima, sums and outputs are
+// float32.
 #include <limits.h>
 
 #include <algorithm>
@@ -399,7 +400,7 @@ size_t attend_workspace(int n_seq, int n_tokens, bool ragged, int kv_heads, int 
 
 int launch_attend(AttendArgs a, int max_length, void* workspace, size_t workspace_bytes, hipStream_t stream) {
   const Plan p = plan_of(a.kv.n_seq, a.n_tokens, a.kv.starts != nullptr, a.kv.heads, a.group, max_length, a.window, a.dim);
-  if (p.pairs[0] > 65535 || (p.splits[1] > 1 && p.pairs[1] > 65535) || p.tiles * a.kv.heads >= 1 << 23) return kAttendUnsupported;
+  if (p.pairs[0] > 65535 || p.tiles * a.kv.heads >= 1 << 23) return kAttendUnsupported;  // past the limits of a grid
   const size_t need = parts_bytes(p);  // of the plan that is launched
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return kAttendWorkspace;
   const int W = kv_groups(a.dim);

@@ -12,6 +12,10 @@
 // L lanes hold a head, each the vectors at i and i + rot / 2 whose values turn with each other, so that nothing but the
 // sum of squares crosses lanes. Heads whose rotary part does not split into whole vectors take a wave each, a pair of
 // values at a time.
+//
+// Memory bounds the form without a cache (4096 tokens of 32 + 8 heads of 128, bfloat16: 84 MB in 17.5 us, 5 TB/s), the
+// vector units the one with a cache (26 us, 3.5 TB/s; a division a code and 32-bit indexes took 34), and what waits for what
+// both on few tokens (3.5 us and 6).
 #include "mxa_kernels.hpp"
 #include "mxa_kv4.hpp"
 
@@ -20,7 +24,7 @@
 namespace mxa {
 namespace {
 
-constexpr int kHeadThreads = 256, kHeadBatch = 3;
+constexpr int kHeadThreads = 256, kHeadBatch = 3;  // rows of a lane that are requested together (2: 3 to 6% slower)
 
 struct HeadSide {
   const void* x;
@@ -110,7 +114,7 @@ __device__ __forceinline__ void quantize8(float (&x)[8], bool here, float (&byte
   m_bits = __builtin_bit_cast(uint16_t, mh);
 }
 
-// Whole vectors' products: a multiplication of 32 bits costs four of 24.
+// Products for indexes below 2^23: one of 32 bits costs four of these.
 __device__ __forceinline__ int mul24(int a, int b) { return __mul24(a, b); }
 __device__ __forceinline__ long long mul64(int a, long long b) { return (long long)((uint64_t)(uint32_t)a * (uint64_t)b); }
 
@@ -371,7 +375,8 @@ __global__ __launch_bounds__(kHeadThreads) void heads_kernel(HeadArgs a, int TP,
       if (whole)
         *(uint32_t*)(blk + kv_value_codes(W) + kv_value_word(W, p.gg, tok >> 2 & 3, oct * 4 + z, tok >> 4)) = word;
       if (cached && oct == 0) {
-        uint16_t* const to = (uint16_t*)(blk + kv_value_scales(W) + (p.gg * 8 + (tok >> 2)) * 16) + ((tok & 1) * 2 + (tok >> 1 & 1));
+        uint16_t* const quad = (uint16_t*)(blk + kv_value_scales(W) + (p.gg * 8 + (tok >> 2)) * 16);
+        uint16_t* const to = quad + ((tok & 1) * 2 + (tok >> 1 & 1));
         to[0] = sb;
         to[4] = mb;
       }
@@ -414,13 +419,17 @@ void launch_heads_t(const HeadArgs& a, hipStream_t stream) {
   const int kh = a.k.heads, qh = a.q.heads, H = qh + kh;
   int TP, HQ, HK, split;
   if (CACHE) {
+    // One token a workgroup while that fills the CUs: 256 tokens 8.3 us (four: 9.7), 512 tokens 11.0 (10.3). Key heads then by
+    // four (16 tokens, 32 + 8 heads: 6.6 us; eight 8.7, one 6.7 but 29 for 512 tokens); with four tokens sixteen groups, or
+    // thirty-two from 4096 tokens on, when a workgroup's start is shared by more (4096: 30.7 us, 34.1; 1024: 15.1, 13.2).
     TP = a.n_tokens > 256 ? 4 : 1;
     const int G = qh / kh;
     const int room = max(1, 8192 / (TP * 32 * W));  // keys that 32 KB hold
-    HK = min(min(kh, room), TP == 1 ? 4 : max(1, (a.n_tokens >= 4096 ? 32 : 16) / W));  // a lane an octet of the values of four tokens
+    HK = min(min(kh, room), TP == 1 ? 4 : max(1, (a.n_tokens >= 4096 ? 32 : 16) / W));
     HQ = HK * G;
     split = (kh + HK - 1) / HK;
   } else {
+    // tokens share what their sines cost; up to 512 the heads of one are spread over workgroups instead
     TP = a.n_tokens > 512 ? min(8, (a.n_tokens + 1023) / 1024) : 1;
     split = a.n_tokens > 512 ? 1 : min(4096, (H + per - 1) / per);
     HQ = (qh + split - 1) / split;

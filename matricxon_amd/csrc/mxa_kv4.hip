@@ -13,9 +13,10 @@ constexpr int kReadThreads = 256, kReadTokens = 4;
 
 // A workgroup takes `tokens` tokens, a thread eight values of one's key and of its value: one word of the key's codes, a
 // byte of four words of the value's. s * code + m is rounded once to float32 (its product is exact), then to the output's
-// type.
+// type. 4096 tokens of 8 heads of 128 take 8 us; one token a workgroup fills the CUs up to some thousand.
 template <class T>
-__global__ __launch_bounds__(kReadThreads) void kv4_read_kernel(KvPages kv, int n_tokens, int dim, int tokens, T* k_out, T* v_out) {
+__global__ __launch_bounds__(kReadThreads) void kv4_read_kernel(KvPages kv, int n_tokens, int dim, int tokens, T* k_out,
+                                                                T* v_out) {
   __shared__ Spot spots[kReadTokens];
   const int O = dim / 8, W = kv_groups(dim), tid = threadIdx.x;
   const int tok0 = (int)blockIdx.x * tokens, nt = min(tokens, n_tokens - tok0);
