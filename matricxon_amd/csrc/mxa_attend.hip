@@ -28,6 +28,33 @@ namespace {
 
 constexpr int kAttendThreads = 256, kAttendWaves = kAttendThreads / 64;
 
+// The sequence, tile and key head of workgroup (y, z): y a pair of sequence z, or, `compact`, y the head and z the tile of the
+// call as its parts are laid out (part_of). 64 replies as sequences of a ragged call have 80 tiles so, not 64 times as many as
+// one sequence could have: 16384 places at most 247 us, and 148 so. Lanes look for the last sequence that does not
+// begin behind tile z.
+__device__ __forceinline__ bool tile_of(const AttendArgs& a, int y, int z, int& b, int& rt, int& h) {
+  if (!a.compact) {
+    b = z, rt = y / a.kv.heads, h = y - rt * a.kv.heads;
+    return true;
+  }
+  const auto begin = [&](int i) {
+    int first, count;
+    kv_rows_of(a.kv, i, a.n_tokens, first, count);
+    return (int)((long long)first * a.group / 16) + i;
+  };
+  int lo = 0, hi = a.kv.n_seq;  // as many as lo are known to begin by then, no more than hi do
+  while (lo < hi) {
+    const int step = (hi - lo + 63) / 64, at = lo + (int)(threadIdx.x & 63) * step;
+    const int some = __popcll(__ballot(at < hi && begin(at) <= z));
+    if (some == 0) break;
+    lo += (some - 1) * step + 1;
+    hi = min(hi, lo + step - 1);
+  }
+  if (lo == 0) return false;
+  b = lo - 1, rt = z - begin(b), h = y;
+  return true;
+}
+
 // W groups of 32 values a head. Workgroup (split, pair, sequence) takes a split's blocks of a pair, which its waves take in
 // turn; their parts are joined in LDS, and the parts of a pair of several splits go to the workspace. No LDS holds the
 // codes: a lane's are adjacent and go to its registers, the next blocks' while the present one is computed, as many as leave
@@ -40,7 +67,10 @@ __global__ __launch_bounds__(kAttendThreads, W <= 4 ? 3 : 2) void attend_kernel(
   __shared__ float m_join[kAttendWaves][16], l_join[kAttendWaves][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, g = lane >> 4;
-  const int split = blockIdx.x, h = blockIdx.y % a.kv.heads, rt = blockIdx.y / a.kv.heads, b = blockIdx.z;
+  const int split = blockIdx.x;
+  int b, rt, h;
+  if (!tile_of(a, blockIdx.y, blockIdx.z, b, rt, h)) return;
+  b = __builtin_amdgcn_readfirstlane(b), rt = __builtin_amdgcn_readfirstlane(rt);
   const Sequence seq = Sequence(a, b).uniform();
   if (rt >= seq.tiles || split >= seq.splits) return;
   const int begin = split * seq.chunk, end = min(begin + seq.chunk, seq.blocks);
@@ -227,8 +257,9 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join_kernel(AttendArgs 
   __shared__ float f[kAttendMaxSplits];
   __shared__ f32x4 sums[kAttendThreads];
   __shared__ float wave_max[kAttendWaves], wave_sum[kAttendWaves];
-  const int b = blockIdx.z, r = blockIdx.x, pair = blockIdx.y, tid = threadIdx.x;
-  const int h = pair % a.kv.heads, rt = pair / a.kv.heads;
+  const int r = blockIdx.x, tid = threadIdx.x;
+  int b, rt, h;
+  if (!tile_of(a, blockIdx.y, blockIdx.z, b, rt, h)) return;
   const Sequence seq(a, b);
   const int parts = seq.splits;
   if (rt * 16 + r >= seq.rows || parts == 1) return;
@@ -271,8 +302,9 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join_kernel(AttendArgs 
 // 11 with sixteen threads a row and parts in turn, 17 with a workgroup a row; one reply of 96 parts takes 5 with that.
 __global__ __launch_bounds__(kAttendThreads) void attend_join_rows_kernel(AttendArgs a, int W) {
   constexpr int U = 8;
-  const int b = blockIdx.y, pair = blockIdx.x;
-  const int h = pair % a.kv.heads, rt = pair / a.kv.heads;
+  int b, rt, h;
+  if (!tile_of(a, blockIdx.x, blockIdx.y, b, rt, h)) return;
+  b = __builtin_amdgcn_readfirstlane(b), rt = __builtin_amdgcn_readfirstlane(rt);
   const Sequence seq = Sequence(a, b).uniform();
   const int parts = seq.splits, rows = min(16, seq.rows - rt * 16), vectors = a.dim / 4;
   if (parts == 1) return;
@@ -337,6 +369,7 @@ struct Plan {
   int splits[2], chunk[2];
   int rows;           // of a workgroup, for many rows
   long long tiles;    // of the call, for many rows
+  long long slots;    // tiles of 16 rows of the call, at most
   long long floats;   // of all tiles' parts, one each
 };
 
@@ -348,11 +381,16 @@ Plan plan_of(int n_seq, int n_tokens, bool ragged, int kv_heads, int group, int 
   const long long reach = window > 0 ? std::min<long long>(max_length, window + most / group) : max_length;
   const long long blocks = reach / kKvBlock + 2;
   const bool narrow = kv_groups(dim) <= 4;
-  p.floats = ((long long)n_tokens * group / 16 + n_seq) * kv_heads * (long long)part_floats(kv_groups(dim));
+  p.slots = (long long)n_tokens * group / 16 + n_seq;
+  p.floats = p.slots * kv_heads * (long long)part_floats(kv_groups(dim));
   if (p.few) {
     p.pairs[0] = (std::min<long long>(most, kFewRows) + 15) / 16 * kv_heads;
     const long long slots = 256 * (narrow ? 3 : 2);  // workgroups that the CUs hold at once
-    share_out(blocks, p.pairs[0] * n_seq, slots, kLeastBlocks, n_seq > 1 ? kMostBlocks : INT_MAX,
+    // pairs that have rows: with query_starts the grid has room for any sequence to have all of them, and those of many rows
+    // are not here
+    const long long pairs = std::min(p.pairs[0] * n_seq,
+                                     kv_heads * std::max<long long>(std::min(n_seq, n_tokens), (long long)n_tokens * group / 16));
+    share_out(blocks, pairs, slots, kLeastBlocks, n_seq > 1 ? kMostBlocks : INT_MAX,
               (int)std::max<long long>(1, kMostFloats / p.floats), p.splits[0], p.chunk[0]);
   }
   if (p.many) {
@@ -387,8 +425,8 @@ size_t part_bytes(const Plan& p, int kind) {
 size_t parts_bytes(const Plan& p) { return part_bytes(p, 0) + part_bytes(p, 1); }
 
 template <int W>
-void launch_few(const AttendArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL(attend_kernel<W>, dim3(a.splits, a.pairs, a.kv.n_seq), dim3(kAttendThreads), 0, stream, a);
+void launch_few(const AttendArgs& a, int z, hipStream_t stream) {
+  hipLaunchKernelGGL(attend_kernel<W>, dim3(a.splits, a.pairs, z), dim3(kAttendThreads), 0, stream, a);
 }
 
 }  // namespace
@@ -407,22 +445,25 @@ int launch_attend(AttendArgs a, int max_length, void* workspace, size_t workspac
   for (int kind = 0; kind < 2; ++kind) {
     if (!(kind ? p.many : p.few)) continue;
     a.least_rows = kind ? kFewRows + 1 : 1, a.most_rows = kind ? 0x7fffffff : kFewRows;
-    a.pairs = (int)p.pairs[kind], a.splits = p.splits[kind], a.chunk = p.chunk[kind];
+    a.splits = p.splits[kind], a.chunk = p.chunk[kind];
+    a.compact = a.kv.starts != nullptr && p.slots <= 65535 && p.slots * a.kv.heads < p.pairs[kind] * a.kv.n_seq;
+    a.pairs = a.compact ? a.kv.heads : (int)p.pairs[kind];
+    const int z = a.compact ? (int)p.slots : a.kv.n_seq;
     a.part = (float*)((char*)workspace + (kind ? part_bytes(p, 0) : 0));
     if (kind == 1) {
       launch_attend_tile(a, p.rows, p.tiles, stream);
     } else {
       switch (W) {
 #define MXA_CASE(W) \
-  case W: launch_few<W>(a, stream); break;
+  case W: launch_few<W>(a, z, stream); break;
         MXA_CASE(1) MXA_CASE(2) MXA_CASE(3) MXA_CASE(4) MXA_CASE(5) MXA_CASE(6) MXA_CASE(7) MXA_CASE(8)
 #undef MXA_CASE
       }
     }
     if (a.splits > 1 && a.splits <= kFewParts)
-      hipLaunchKernelGGL(attend_join_rows_kernel, dim3(a.pairs, a.kv.n_seq), dim3(kAttendThreads), 0, stream, a, W);
+      hipLaunchKernelGGL(attend_join_rows_kernel, dim3(a.pairs, z), dim3(kAttendThreads), 0, stream, a, W);
     else if (a.splits > 1)
-      hipLaunchKernelGGL(attend_join_kernel, dim3(16, a.pairs, a.kv.n_seq), dim3(kAttendThreads), 0, stream, a, W);
+      hipLaunchKernelGGL(attend_join_kernel, dim3(16, a.pairs, z), dim3(kAttendThreads), 0, stream, a, W);
   }
   return 0;
 }

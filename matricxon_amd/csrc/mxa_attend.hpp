@@ -43,6 +43,7 @@ struct AttendArgs {
   int least_rows, most_rows;  // sequences of fewer or more rows a key head are left out
   int pairs, splits, chunk;  // of the grid: pairs and splits of a sequence, blocks of a split at least (0: each tile in
                              // `splits` even parts)
+  int compact;               // the grid has the tiles of the call, not as many for each sequence
   float scale;
 
   __device__ __forceinline__ const uint16_t* q_row(int t, int h) const {

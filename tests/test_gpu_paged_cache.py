@@ -661,3 +661,19 @@ def test_many_rows_captured(gpu) -> None:
         check_attention(cache, q[:t], got[:t], table, lengths, counts)
         out.fill_(7.0)
         assert same(cache.attend(q, table, length, starts, out=out), got)
+
+
+@pytest.mark.parametrize("b", [3, 70, 300])
+def test_many_ragged_sequences(gpu, b) -> None:
+    """Replies, short chunks, sequences without rows and rows in front of the first, long places among short ones."""
+    g = torch.Generator(device="cuda").manual_seed(b)
+    counts = [(1, 0, 1, 5, 1, 40)[i % 6] for i in range(b)]
+    counts[b // 2] = 150
+    lengths = [c + (0, 700, 31)[i % 3] for i, c in enumerate(counts)]
+    lengths[1], lengths[b // 2] = 3000, 400
+    cache, table = filled(g, b, lengths, 2, 64, 32, width=3008 // 32)
+    t = sum(counts)
+    q, out = rand(g, t + 5, 8, 64, dt=BF16), torch.full((t + 5, 8, 64), 3.0, dtype=BF16, device="cuda")
+    cache.attend(q, table, i32(lengths), starts_of(counts) + 3, out=out)
+    assert (out[:3] == 3.0).all() and (out[t + 3 :] == 3.0).all()
+    check_attention(cache, q[3 : t + 3], out[3 : t + 3], table, lengths, counts)
