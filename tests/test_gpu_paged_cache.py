@@ -677,3 +677,15 @@ def test_many_ragged_sequences(gpu, b) -> None:
     cache.attend(q, table, i32(lengths), starts_of(counts) + 3, out=out)
     assert (out[:3] == 3.0).all() and (out[t + 3 :] == 3.0).all()
     check_attention(cache, q[3 : t + 3], out[3 : t + 3], table, lengths, counts)
+
+
+@pytest.mark.parametrize("n", [1, 130])
+def test_as_many_heads_as_there_may_be(gpu, n) -> None:
+    g = torch.Generator(device="cuda").manual_seed(31)
+    heads, lengths = 4096, [n + 40]
+    cache, table = filled(g, 1, lengths, heads, 8, 32)
+    q, k, v = (rand(g, n, heads, 8, dt=BF16) for _ in range(3))
+    q2 = cache.append(q, k, v, table, i32(lengths))
+    k2, v2 = cache.read(n, table, i32(lengths), dtype=F32)
+    assert same(q2, q) and same(k2, held(k)) and same(v2, held(v))
+    check_attention(cache, q, cache.attend(q, table, i32(lengths)), table, lengths, [n])
