@@ -16,6 +16,7 @@
 // Memory bounds the form without a cache (4096 tokens of 32 + 8 heads of 128, bfloat16: 84 MB in 17.5 us, 5 TB/s), the
 // vector units the one with a cache (26 us, 3.5 TB/s; a division a code and 32-bit indexes took 34), and what waits for what
 // both on few tokens (3.5 us and 6).
+#include "mxa_heads_grid.hpp"
 #include "mxa_kernels.hpp"
 #include "mxa_kv4.hpp"
 
@@ -24,7 +25,7 @@
 namespace mxa {
 namespace {
 
-constexpr int kHeadThreads = 256, kHeadBatch = 3;  // rows of a lane that are requested together (2: 3 to 6% slower)
+constexpr int kHeadBatch = 3;  // rows of a lane that are requested together (2: 3 to 6% slower)
 
 struct HeadSide {
   const void* x;
@@ -118,7 +119,8 @@ __device__ __forceinline__ void quantize8(float (&x)[8], bool here, float (&byte
 __device__ __forceinline__ int mul24(int a, int b) { return __mul24(a, b); }
 __device__ __forceinline__ long long mul64(int a, long long b) { return (long long)((uint64_t)(uint32_t)a * (uint64_t)b); }
 
-// T the element type; FAST: vectors of V values. A workgroup takes TP tokens and, from grid.y, HQ heads of q and HK of k.
+// T the element type; FAST: vectors of V values. A workgroup takes TP tokens and, from grid.y, HQ heads of q and HK of k, one
+// head at least (heads_grid).
 template <class T, bool INTER, bool FAST, bool CACHE>
 __global__ __launch_bounds__(kHeadThreads) void heads_kernel(HeadArgs a, int TP, int L, int HQ, int HK) {
   constexpr int V = FAST ? 16 / (int)sizeof(T) : 1;
@@ -156,7 +158,7 @@ __global__ __launch_bounds__(kHeadThreads) void heads_kernel(HeadArgs a, int TP,
     int t, hh, h;
     bool live, isq;
   };
-  const int step_t = per / max(H, 1), step_h = per - step_t * max(H, 1);
+  const int step_t = per / H, step_h = per - step_t * H;
   const auto row_at = [&](int t, int hh) {
     Row w;
     w.live = t < nt;
@@ -170,7 +172,7 @@ __global__ __launch_bounds__(kHeadThreads) void heads_kernel(HeadArgs a, int TP,
     t += step_t, hh += step_h;
     if (hh >= H) hh -= H, ++t;
   };
-  int now_t = tid / L / max(H, 1), now_h = tid / L - now_t * H;
+  int now_t = tid / L / H, now_h = tid / L - now_t * H;
   // The rows of a batch, and a quad's values, are requested before what depends on the page table and the positions.
   Piece x[kHeadBatch], y[kHeadBatch];
   const auto load_rows = [&] {
@@ -408,39 +410,14 @@ __global__ __launch_bounds__(kHeadThreads) void heads_kernel(HeadArgs a, int TP,
 
 template <class T, bool INTER, bool CACHE>
 void launch_heads_t(const HeadArgs& a, hipStream_t stream) {
-  constexpr int V = 16 / sizeof(T);
-  const int half = a.rot / 2;
-  const int CR = INTER ? a.rot / V : half / V, C = CR + (a.dim - a.rot) / V;
-  const bool fast = (INTER ? a.rot : half) % V == 0 && (a.dim - a.rot) % V == 0 && C <= 64;
-  int L = 64;
-  if (fast)
-    for (L = 1; L < C;) L *= 2;
-  const int per = kHeadThreads / L, W = kv_groups(a.dim);
-  const int kh = a.k.heads, qh = a.q.heads, H = qh + kh;
-  int TP, HQ, HK, split;
-  if (CACHE) {
-    // One token a workgroup while that fills the CUs: 256 tokens 8.3 us (four: 9.7), 512 tokens 11.0 (10.3). Key heads then by
-    // four (16 tokens, 32 + 8 heads: 6.6 us; eight 8.7, one 6.7 but 29 for 512 tokens); with four tokens sixteen groups, or
-    // thirty-two from 4096 tokens on, when a workgroup's start is shared by more (4096: 30.7 us, 34.1; 1024: 15.1, 13.2).
-    TP = a.n_tokens > 256 ? 4 : 1;
-    const int G = qh / kh;
-    const int room = max(1, 8192 / (TP * 32 * W));  // keys that 32 KB hold
-    HK = min(min(kh, room), TP == 1 ? 4 : max(1, (a.n_tokens >= 4096 ? 32 : 16) / W));
-    HQ = HK * G;
-    split = (kh + HK - 1) / HK;
-  } else {
-    // tokens share what their sines cost; up to 512 the heads of one are spread over workgroups instead
-    TP = a.n_tokens > 512 ? min(8, (a.n_tokens + 1023) / 1024) : 1;
-    split = a.n_tokens > 512 ? 1 : min(4096, (H + per - 1) / per);
-    HQ = (qh + split - 1) / split;
-    HK = (kh + split - 1) / split;
-  }
-  const size_t lds = (CACHE ? TP * sizeof(Spot) + (size_t)TP * HK * 32 * W * 4 : 0) + (size_t)TP * a.rot * sizeof(float);
-  const dim3 grid((a.n_tokens + TP - 1) / TP, split);
-  if (fast)
-    hipLaunchKernelGGL((heads_kernel<T, INTER, true, CACHE>), grid, dim3(kHeadThreads), lds, stream, a, TP, L, HQ, HK);
+  const HeadGrid g = heads_grid(CACHE, sizeof(T), INTER, a.q.heads, a.k.heads, a.n_tokens, a.dim, a.rot);
+  const size_t keys = CACHE ? g.TP * sizeof(Spot) + (size_t)g.TP * g.HK * 32 * kv_groups(a.dim) * 4 : 0;
+  const size_t lds = keys + (size_t)g.TP * a.rot * sizeof(float);
+  const dim3 grid((a.n_tokens + g.TP - 1) / g.TP, g.split);
+  if (g.fast)
+    hipLaunchKernelGGL((heads_kernel<T, INTER, true, CACHE>), grid, dim3(kHeadThreads), lds, stream, a, g.TP, g.L, g.HQ, g.HK);
   else
-    hipLaunchKernelGGL((heads_kernel<T, INTER, false, CACHE>), grid, dim3(kHeadThreads), lds, stream, a, TP, L, HQ, HK);
+    hipLaunchKernelGGL((heads_kernel<T, INTER, false, CACHE>), grid, dim3(kHeadThreads), lds, stream, a, g.TP, g.L, g.HQ, g.HK);
 }
 
 template <bool CACHE>

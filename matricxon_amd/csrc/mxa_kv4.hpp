@@ -15,14 +15,12 @@
 #pragma once
 
 #include "mxa_device.hpp"
+#include "mxa_kv4_shape.hpp"
 
 namespace mxa {
 
-constexpr int kKvBlock = 32;           // tokens of a block
-constexpr int kKvMaxDim = 256;         // values of a head
 constexpr float kKvHeld = 65000.0f;    // values beyond are held as this: s * 15 + m then stays a finite float16
 
-__host__ __device__ constexpr int kv_groups(int dim) { return (dim + 31) / 32; }
 __host__ __device__ constexpr int kv_block_bytes(int w) { return 1280 * w; }
 __host__ __device__ constexpr int kv_key_scales(int w) { return 512 * w; }
 __host__ __device__ constexpr int kv_value_codes(int w) { return 640 * w; }

@@ -163,3 +163,27 @@ def test_refusals(gpu) -> None:
         rot(q, None, pos, k_weight=w)
     empty, _ = rot(q[:0], None, pos[:0], q_weight=w)
     assert empty.shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("t", [1, 2, 512])
+@pytest.mark.parametrize("hq, hk, dim, dt, interleaved",
+                         [(64, 8, 128, F32, True), (64, 8, 256, BF16, True), (64, 8, 256, F32, False), (32, 8, 256, F32, True),
+                          (8, 64, 128, F32, True), (33, 65, 64, BF16, False)])
+def test_heads_that_share_out_unevenly(gpu, hq, hk, dim, dt, interleaved, t) -> None:
+    """Heads of q and k whose shares are rounded up (test_host_grids.py), k the last of its buffer."""
+    g = torch.Generator(device="cuda").manual_seed(hq + t)
+    rot = HipRotary(dim, interleaved=interleaved)
+    q, k = rand(g, t, hq, dim, dt=dt), rand(g, t, hk, dim, dt=dt)
+    qw, kw = (1 + 0.3 * rand(g, dim)).to(dt), (1 + 0.3 * rand(g, dim)).to(dt)
+    pos = torch.randint(0, 5000, (t,), device="cuda", generator=g)
+    q2, k2 = rot(q, k, pos, q_weight=qw, k_weight=kw)
+    check(rot, q, q2, pos, qw)
+    check(rot, k, k2, pos, kw)
+
+
+def test_more_heads_than_shares(gpu) -> None:
+    """q alone, of as many heads as are shared out over 4096 workgroups a token by ten."""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    rot = HipRotary(256, interleaved=True)
+    q, w, pos = rand(g, 1, 40000, 256, dt=BF16), (1 + 0.3 * rand(g, 256)).to(BF16), torch.tensor([77], device="cuda")
+    check(rot, q, rot(q, None, pos, q_weight=w)[0], pos, w)
