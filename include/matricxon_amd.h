@@ -414,8 +414,9 @@ int mxa_norm_rope(const void *q, const long long *q_strides, int q_heads, const 
  * Sequence b (of n_seq) has lengths[b] tokens, place p of it in page table[b * table_stride + p / page_size]; a place
  * whose page number is outside [0, n_pages), and one at or behind table_width * page_size, is not cached: nothing is
  * written for it, it reads as zeros and is not attended to. The call's rows are the last tokens of the sequences: rows
- * [query_starts[b], query_starts[b + 1]) those of b (n_seq + 1 ascending values; rows outside all belong to none), or
- * with query_starts NULL n_tokens / n_seq of each. table, lengths and query_starts are DEVICE int32.
+ * [query_starts[b], query_starts[b + 1]) those of b (n_seq + 1 ascending values; rows outside all belong to none; values
+ * that descend give results without a meaning, within the call's memory), or with query_starts NULL n_tokens / n_seq of
+ * each. table, lengths and query_starts are DEVICE int32.
  * kv_heads <= MXA_KV4_MAX_HEADS, page_size a multiple of 32 up to MXA_KV4_MAX_PAGE, head_dim a multiple of 8 up to
  * MXA_KV4_MAX_DIM, table_width * page_size <= MXA_KV4_MAX_PLACES, n_seq <= MXA_KV4_MAX_SEQ, n_tokens <= MXA_MAX_TOKENS,
  * of mxa_kv4_attend n_tokens * q_heads <= MXA_KV4_MAX_ROWS; else -1. */

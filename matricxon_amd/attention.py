@@ -13,7 +13,8 @@ call moves on with them:
   [0, n_pages) is no page: what would lie there is neither written nor attended to, and reads as zeros.
 * `lengths` (B,): tokens of each sequence, those of this call among them.
 * `query_starts` (B + 1,), ascending, or None: rows [query_starts[b], query_starts[b + 1]) of q, k and v are the last
-  tokens of sequence b; rows behind the last sequence belong to none. None: the same number of rows for each.
+  tokens of sequence b; rows behind the last sequence belong to none. None: the same number of rows for each. (Of starts
+  that descend the results mean nothing; no memory outside the tensors is touched.)
 
 q, k and v are (T, heads, head_dim), or (B, T, heads, head_dim) without `query_starts`, of any strides with adjacent
 values in a head, as the columns of a q | k | v buffer. The reference keeps its cache in tensors of the layer's dtype

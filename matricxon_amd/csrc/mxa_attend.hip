@@ -31,7 +31,7 @@ constexpr int kAttendThreads = 256, kAttendWaves = kAttendThreads / 64;
 // The sequence, tile and key head of workgroup (y, z): y a pair of sequence z, or, `compact`, y the head and z the tile of the
 // call as its parts are laid out (part_of). 64 replies as sequences of a ragged call have 80 tiles so, not 64 times as many as
 // one sequence could have: 16384 places at most 247 us, and 148 so. Lanes look for the last sequence that does not
-// begin behind tile z.
+// begin behind tile z. (Starts that descend may find one that does; its tile would be before its first, and is none.)
 __device__ __forceinline__ bool tile_of(const AttendArgs& a, int y, int z, int& b, int& rt, int& h) {
   if (!a.compact) {
     b = z, rt = y / a.kv.heads, h = y - rt * a.kv.heads;
@@ -52,7 +52,7 @@ __device__ __forceinline__ bool tile_of(const AttendArgs& a, int y, int z, int& 
   }
   if (lo == 0) return false;
   b = lo - 1, rt = z - begin(b), h = y;
-  return true;
+  return rt >= 0;
 }
 
 // W groups of 32 values a head. Workgroup (split, pair, sequence) takes a split's blocks of a pair, which its waves take in

@@ -689,3 +689,21 @@ def test_as_many_heads_as_there_may_be(gpu, n) -> None:
     k2, v2 = cache.read(n, table, i32(lengths), dtype=F32)
     assert same(q2, q) and same(k2, held(k)) and same(v2, held(v))
     check_attention(cache, q, cache.attend(q, table, i32(lengths)), table, lengths, [n])
+
+
+@pytest.mark.parametrize("starts", [[6, 0, 3], [6, 6, 0], [9, 2, -1], [-3, 6, 2]])
+def test_starts_that_descend_touch_nothing_else(gpu, starts) -> None:
+    """What the rows then get means nothing, but it lies in the rows, and an ascending call behind it is right."""
+    g = torch.Generator(device="cuda").manual_seed(32)
+    heads, group, dim, lengths = 2, 32, 32, [90, 80]
+    cache, table = filled(g, 2, lengths, heads, dim, 32)
+    pages = cache.pages.clone()
+    q = rand(g, 6, heads * group, dim, dt=BF16)
+    for most in (96, None):
+        around = torch.full((8, heads * group, dim), 7.0, dtype=BF16, device="cuda")
+        cache.attend(q, table, i32(lengths), i32(starts), max_length=most, out=around[1:7])
+        assert (around[0] == 7).all() and (around[7] == 7).all()
+        assert cache.append(q, q[:, :heads], q[:, :heads], i32([[-1] * 3] * 2), i32(lengths), i32(starts)).isfinite().all()
+        assert same(cache.pages, pages)
+        got = cache.attend(q, table, i32(lengths), starts_of([2, 4]), max_length=most)
+        check_attention(cache, q, got, table, lengths, [2, 4])
