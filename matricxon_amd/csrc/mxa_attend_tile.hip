@@ -110,9 +110,11 @@ __global__ __launch_bounds__(64 * NW, W <= 4 ? 2 : 1) void attend_tile_kernel(At
       for (int j = 0; j < 8; ++j) v[j] = bf16_to_float(raw[k][j]);
       q[k] = key_order(v, -e);
     }
-    if (a.scale < 0.0f)  // its sign goes to q: the largest product is the largest score
+    if (!(a.scale >= 0.0f)) {  // its sign goes to q: the largest product is the largest score; so does what is no number
+      const _Float16 by = a.scale < 0.0f ? -1.0f : a.scale;
 #pragma unroll
-      for (int k = 0; k < 2 * W; ++k) q[k] = -q[k];
+      for (int k = 0; k < 2 * W; ++k) q[k] *= by;
+    }
     back = fmaxf(ldexpf(fabsf(a.scale) * kLog2e, e), 1e-37f);  // not 0, with which a place left out would be no number
   }
   f32x16 o[W];

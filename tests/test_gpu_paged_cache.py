@@ -707,3 +707,18 @@ def test_starts_that_descend_touch_nothing_else(gpu, starts) -> None:
         assert same(cache.pages, pages)
         got = cache.attend(q, table, i32(lengths), starts_of([2, 4]), max_length=most)
         check_attention(cache, q, got, table, lengths, [2, 4])
+
+
+@pytest.mark.parametrize("n", [1, 70, 300])
+@pytest.mark.parametrize("dim", [64, 200])
+def test_a_scale_that_is_no_number(gpu, n, dim) -> None:
+    """Few rows and many: not-a-number in every row that attends to something, zeros in the others."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    lengths = [2000, 0, n // 2]
+    cache, table = filled(g, 3, lengths, 2, dim, 32)
+    q = rand(g, 3 * n, 8, dim, dt=BF16)
+    for window in (0, 20):
+        got = cache.attend(q, table, i32(lengths), scale=math.nan, window=window)
+        some = torch.zeros(3 * n, dtype=torch.bool, device="cuda")
+        some[:n] = some[3 * n - n // 2 :] = True
+        assert got[some].isnan().all() and (got[~some] == 0).all()
