@@ -14,10 +14,6 @@
 // float16 exactly (an or of its bits into a float16's, less that float16), then s * code + m rounded once; q is brought by a
 // power of two into float16's range, exactly but for values below 2^-24 of its largest. Scores, maxima, sums and outputs are
 // float32.
-#include <limits.h>
-
-#include <algorithm>
-
 #include "mxa_attend.hpp"
 #include "mxa_kernels.hpp"
 
@@ -341,89 +337,6 @@ __global__ __launch_bounds__(kAttendThreads) void attend_join_rows_kernel(Attend
   }
 }
 
-// (std::min and std::max here: on the host, HIP's own of that name take ints.)
-// Shares of `least` to `most` blocks for the workgroups that the CUs hold at once. At least two blocks a wave: 1000 places
-// of one reply took 13.8 us in shares of 4 blocks, 11.8 of 8, 12.2 of 16 (9.5 since their join is faster). At most 128
-// blocks where several sequences end at places that the host does not know: 64 replies of up to 16384 places 188 us without,
-// 149 us with that bound, 160 of 96. More of them where the parts would not fit into kMostFloats.
-void share_out(long long blocks, long long workgroups, long long slots, int least, int most, int most_splits, int& splits,
-               int& chunk) {
-  const long long want = std::max<long long>(1, slots / workgroups);
-  chunk = (int)std::max<long long>(least, std::min<long long>(most, (blocks + want - 1) / want));
-  most_splits = std::min<int>(most_splits, kAttendMaxSplits);
-  chunk = (int)std::max<long long>(chunk, (blocks + most_splits - 1) / most_splits);
-  splits = (int)((blocks + chunk - 1) / chunk);
-  chunk = (int)((blocks + splits - 1) / splits);
-}
-
-// How the places of up to `most` tokens of each sequence are shared out. Sequences of up to kFewRows rows a key head go in
-// tiles of 16 rows (attend_kernel), others in those of attend_tile_kernel, which widens a place once for
-// all of them; a call without query_starts has one kind. 16 sequences of 2048 places take, of 64 rows a key head, 32 us in
-// tiles of 16 and 41 in the others; of 96 rows 39 and 43; of 128 rows 51 and 45, and with lengths of all sizes up to 2048
-// 36 and 43.
-constexpr int kFewRows = 128, kTileSplits = 16, kFewParts = 16, kLeastBlocks = 8, kMostBlocks = 128;
-constexpr long long kMostFloats = 64 << 20;  // of a workspace
-struct Plan {
-  bool few, many;     // the kinds that there may be
-  long long pairs[2]; // (tile of 16 rows, key head) of a sequence
-  int splits[2], chunk[2];
-  int rows;           // of a workgroup, for many rows
-  long long tiles;    // of the call, for many rows
-  long long slots;    // tiles of 16 rows of the call, at most
-  long long floats;   // of all tiles' parts, one each
-};
-
-Plan plan_of(int n_seq, int n_tokens, bool ragged, int kv_heads, int group, int max_length, long long window, int dim) {
-  Plan p{};
-  const long long most = (long long)(ragged ? n_tokens : n_tokens / n_seq) * group;
-  p.few = ragged || most <= kFewRows;
-  p.many = most > kFewRows;
-  const long long reach = window > 0 ? std::min<long long>(max_length, window + most / group) : max_length;
-  const long long blocks = reach / kKvBlock + 2;
-  const bool narrow = kv_groups(dim) <= 4;
-  p.slots = (long long)n_tokens * group / 16 + n_seq;
-  p.floats = p.slots * kv_heads * (long long)part_floats(kv_groups(dim));
-  if (p.few) {
-    p.pairs[0] = (std::min<long long>(most, kFewRows) + 15) / 16 * kv_heads;
-    const long long slots = 256 * (narrow ? 3 : 2);  // workgroups that the CUs hold at once
-    // pairs that have rows: with query_starts the grid has room for any sequence to have all of them, and those of many rows
-    // are not here
-    const long long pairs = std::min(p.pairs[0] * n_seq,
-                                     kv_heads * std::max<long long>(std::min(n_seq, n_tokens), (long long)n_tokens * group / 16));
-    share_out(blocks, pairs, slots, kLeastBlocks, n_seq > 1 ? kMostBlocks : INT_MAX,
-              (int)std::max<long long>(1, kMostFloats / p.floats), p.splits[0], p.chunk[0]);
-  }
-  if (p.many) {
-    p.pairs[1] = (most + 15) / 16 * kv_heads;
-    // Workgroups of 256 rows widen a place once for all; where they are too few for the CUs and their places few as well,
-    // two of 128 rows hide each other's waits: 128 tokens x 32 heads of 128, window 1024: 27.9 and 22.3 us; without, over
-    // 8192 places, 52.7 and 57.2.
-    const auto span_of = [&](int rows) {
-      return window > 0 ? std::min<long long>(max_length, (long long)window + rows / group) / kKvBlock + 2 : blocks;
-    };
-    const bool fill = (most + 255) / 256 * kv_heads * (ragged ? 1 : n_seq) >= 256;
-    p.rows = narrow && most > 128 && (fill || span_of(256) > 48) ? 256 : 128;
-    p.tiles = ragged ? most / p.rows + std::min<long long>(n_seq, most / (kFewRows + 1)) : (most + p.rows - 1) / p.rows * n_seq;
-    const long long span = span_of(p.rows);
-    const long long groups = p.tiles * kv_heads, slots = narrow && p.rows == 128 ? 512 : 256;
-    // Parts of a tile's places, by what they cost: as many rounds of the CUs as the workgroups take, each a part's blocks
-    // and some 10 blocks' time to begin and end, and the join
-    double least = 0;
-    for (int n = 1; n <= kTileSplits && (n == 1 || span / n >= 8); ++n) {
-      const double cost = (double)((groups * n + slots - 1) / slots) * ((double)span / n + 10) + (n > 1 ? 8 : 0);
-      if (n == 1 || cost < 0.95 * least) least = cost, p.splits[1] = n;
-    }
-    if (p.floats * p.splits[1] > kMostFloats) p.splits[1] = 1;
-    p.chunk[1] = 0;
-  }
-  return p;
-}
-
-size_t part_bytes(const Plan& p, int kind) {
-  return p.splits[kind] <= 1 ? 0 : (size_t)(p.floats * p.splits[kind]) * sizeof(float);
-}
-size_t parts_bytes(const Plan& p) { return part_bytes(p, 0) + part_bytes(p, 1); }
-
 template <int W>
 void launch_few(const AttendArgs& a, int z, hipStream_t stream) {
   hipLaunchKernelGGL(attend_kernel<W>, dim3(a.splits, a.pairs, z), dim3(kAttendThreads), 0, stream, a);
@@ -447,6 +360,7 @@ int launch_attend(AttendArgs a, int max_length, void* workspace, size_t workspac
     a.least_rows = kind ? kFewRows + 1 : 1, a.most_rows = kind ? 0x7fffffff : kFewRows;
     a.splits = p.splits[kind], a.chunk = p.chunk[kind];
     a.compact = a.kv.starts != nullptr && p.slots <= 65535 && p.slots * a.kv.heads < p.pairs[kind] * a.kv.n_seq;
+    a.per = p.per[kind];
     a.pairs = a.compact ? a.kv.heads : (int)p.pairs[kind];
     const int z = a.compact ? (int)p.slots : a.kv.n_seq;
     a.part = (float*)((char*)workspace + (kind ? part_bytes(p, 0) : 0));

@@ -1,6 +1,7 @@
 // What the attention kernels over the 4-bit cache share: their arguments, which rows a workgroup has, operands from codes.
 #pragma once
 
+#include "mxa_attend_plan.hpp"
 #include "mxa_kv4.hpp"
 
 namespace mxa {
@@ -23,15 +24,11 @@ typedef uint16_t u16x8 __attribute__((ext_vector_type(8), aligned(2)));
 
 __device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
 
-constexpr int kAttendMaxSplits = 768;
-
 // A split's part of a pair's rows, unnormalised.
 struct AttendPart {
   float* o;   // 16 rows of 32 W values
   float* ml;  // 16 references of log2 p, 16 sums
 };
-
-inline size_t part_floats(int w) { return 16 * 32 * (size_t)w + 32; }
 
 struct AttendArgs {
   const uint16_t* q;
@@ -44,6 +41,7 @@ struct AttendArgs {
   int pairs, splits, chunk;  // of the grid: pairs and splits of a sequence, blocks of a split at least (0: each tile in
                              // `splits` even parts)
   int compact;               // the grid has the tiles of the call, not as many for each sequence
+  int per;                   // tiles that the parts have room for of each sequence; 0: as they lie in the call
   float scale;
 
   __device__ __forceinline__ const uint16_t* q_row(int t, int h) const {
@@ -51,10 +49,10 @@ struct AttendArgs {
     return q + (long long)b * q_batch + (long long)(t - b * seq) * q_tok + (long long)h * q_head;
   }
   __device__ __forceinline__ uint16_t* out_row(int t, int h) const { return out + ((long long)t * heads + h) * dim; }
-  // Of tile rt of sequence b, whose rows begin at `first`: as each sequence has one tile of 16 rows more than its rows' share
-  // of the call's at most, the tiles of those before it are first * group / 16 + b and fewer.
+  // Of tile rt of sequence b, whose rows begin at `first`. As they lie in the call: as each sequence has one tile of 16 rows
+  // more than its rows' share of the call's at most, the tiles of those before it are first * group / 16 + b and fewer.
   __device__ __forceinline__ AttendPart part_of(int b, int first, int rt, int h, int split, int w) const {
-    const long long tile = (long long)first * group / 16 + b + rt;
+    const long long tile = per > 0 ? (long long)b * per + rt : (long long)first * group / 16 + b + rt;
     float* const p = part + ((tile * kv.heads + h) * splits + split) * (16 * 32 * w + 32);
     return AttendPart{p, p + 16 * 32 * w};
   }

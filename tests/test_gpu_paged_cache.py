@@ -722,3 +722,15 @@ def test_a_scale_that_is_no_number(gpu, n, dim) -> None:
         some = torch.zeros(3 * n, dtype=torch.bool, device="cuda")
         some[:n] = some[3 * n - n // 2 :] = True
         assert got[some].isnan().all() and (got[~some] == 0).all()
+
+
+@pytest.mark.parametrize("chunk", [130, 700, 2100])
+def test_long_replies_beside_a_chunk(gpu, chunk) -> None:
+    """Replies whose places are shared out, between and behind sequences of many rows, and one of few rows of its own."""
+    g = torch.Generator(device="cuda").manual_seed(chunk)
+    counts, lengths = [1, chunk, 0, 1, 20, 2], [20000, chunk + 300, 40, 5, 9000, 13000]
+    cache, table = filled(g, 6, lengths, 2, 64, 64)
+    q = rand(g, sum(counts), 8, 64, dt=BF16)
+    for most in (None, 3000):
+        got = cache.attend(q, table, i32(lengths), starts_of(counts), max_length=most)
+        check_attention(cache, q, got, table, lengths, counts)

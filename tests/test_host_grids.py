@@ -10,10 +10,16 @@ from tests.conftest import REPO
 
 CSRC = REPO / "matricxon_amd" / "csrc"
 SOURCE = """
+#include "mxa_attend_plan.hpp"
 #include "mxa_heads_grid.hpp"
 extern "C" void heads(int cache, int size, int interleaved, int qh, int kh, int n, int dim, int rot, int* out) {
   const mxa::HeadGrid g = mxa::heads_grid(cache, size, interleaved, qh, kh, n, dim, rot);
   out[0] = g.fast, out[1] = g.L, out[2] = g.TP, out[3] = g.HQ, out[4] = g.HK, out[5] = g.split;
+}
+extern "C" void plan(int n_seq, int n, int ragged, int kv_heads, int group, int most, int window, int dim, long long* out) {
+  const mxa::Plan p = mxa::plan_of(n_seq, n, ragged != 0, kv_heads, group, most, window, dim);
+  out[0] = p.few ? p.splits[0] : 0, out[1] = p.chunk[0], out[2] = p.many ? p.splits[1] : 0, out[3] = p.per[0];
+  out[4] = p.floats[0], out[5] = p.slots, out[6] = (long long)mxa::parts_bytes(p), out[7] = (long long)mxa::part_bytes(p, 0);
 }
 """
 
@@ -62,3 +68,21 @@ def test_every_workgroup_of_an_append_has_a_key_head(grids, dim, rot, size) -> N
                 _, _, tokens, hq, hk, split = out
                 assert hq == hk * group and split * hk >= kh > (split - 1) * hk
                 assert tokens * (16 + 4 * (hk * -(-dim // 32) * 32 + rot)) <= 65536
+
+
+def plan(grids, n_seq, n, ragged, kv_heads, group, most, window=0, dim=128):
+    out = (ctypes.c_longlong * 8)()
+    grids.plan(n_seq, n, ragged, kv_heads, group, most, window, dim, out)
+    return list(out)
+
+
+@pytest.mark.parametrize("most", [4096, 131072, 1 << 20])
+@pytest.mark.parametrize("replies", [1, 3, 15])
+def test_replies_keep_their_shares_beside_a_chunk(grids, replies, most) -> None:
+    """However long the chunk: a reply's places go in shares of 128 blocks at most, or as many as the room for parts allows, of
+    which a chunk's rows take none of this kind."""
+    tiles = (replies + 1) * 8 * 8  # of 16 rows, of sequences of up to 128 rows
+    for chunk in (40, 512, 2048, 4096, 8192, 60000, 1 << 20):
+        splits, blocks = plan(grids, replies + 1, replies + chunk, 1, 8, 4, most)[:2]
+        assert splits * blocks >= most // 32
+        assert blocks <= 128 or splits > (32 << 20) // (tiles * 2080) * 0.95, (chunk, splits, blocks)
