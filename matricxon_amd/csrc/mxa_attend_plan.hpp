@@ -36,7 +36,7 @@ inline void share_out(long long blocks, long long workgroups, long long slots, i
 // tiles of 16 and 41 in the others; of 96 rows 39 and 43; of 128 rows 51 and 45, and with lengths of all sizes up to 2048
 // 36 and 43.
 constexpr int kFewRows = 128, kTileSplits = 16, kFewParts = 16, kLeastBlocks = 8, kMostBlocks = 128;
-constexpr long long kMostFloats = 64 << 20;  // of a workspace
+constexpr long long kMostFloats = 64 << 20;  // of a call's parts, of both kinds together
 struct Plan {
   bool few, many;       // the kinds that there may be
   long long pairs[2];   // (tile of 16 rows, key head) of a sequence
@@ -74,13 +74,13 @@ inline Plan plan_of(int n_seq, int n_tokens, bool ragged, int kv_heads, int grou
     const long long span = span_of(p.rows);
     const long long groups = p.tiles * kv_heads, slots = narrow && p.rows == 128 ? 512 : 256;
     // Parts of a tile's places, by what they cost: as many rounds of the CUs as the workgroups take, each a part's blocks
-    // and some 10 blocks' time to begin and end, and the join
+    // and some 10 blocks' time to begin and end, and the join. Half of the room, where there may be few rows as well.
+    const long long room = p.few ? kMostFloats / 2 : kMostFloats;
     double least = 0;
-    for (int n = 1; n <= kTileSplits && (n == 1 || span / n >= 8); ++n) {
+    for (int n = 1; n <= kTileSplits && (n == 1 || (span / n >= 8 && p.floats[1] * n <= room)); ++n) {
       const double cost = (double)((groups * n + slots - 1) / slots) * ((double)span / n + 10) + (n > 1 ? 8 : 0);
       if (n == 1 || cost < 0.95 * least) least = cost, p.splits[1] = n;
     }
-    if (p.floats[1] * p.splits[1] > kMostFloats) p.splits[1] = 1;
     p.chunk[1] = 0;
   }
   if (p.few) {
@@ -91,13 +91,14 @@ inline Plan plan_of(int n_seq, int n_tokens, bool ragged, int kv_heads, int grou
     // of the call there would be one share of all 4098).
     p.per[0] = tiles * n_seq <= p.slots ? (int)tiles : 0;
     p.floats[0] = std::min<long long>(tiles * n_seq, p.slots) * part;
+    const long long room = kMostFloats - (p.many && p.splits[1] > 1 ? p.floats[1] * p.splits[1] : 0);
     const long long slots = 256 * (narrow ? 3 : 2);  // workgroups that the CUs hold at once
     // pairs that have rows: with query_starts the grid has room for any sequence to have all of them, and those of many rows
     // are not here
     const long long pairs = std::min<long long>(p.pairs[0] * n_seq,
                                                 kv_heads * std::max<long long>(std::min(n_seq, n_tokens), (long long)n_tokens * group / 16));
     share_out(blocks, pairs, slots, kLeastBlocks, n_seq > 1 ? kMostBlocks : INT_MAX,
-              (int)std::max<long long>(1, kMostFloats / p.floats[0]), p.splits[0], p.chunk[0]);
+              (int)std::max<long long>(1, room / p.floats[0]), p.splits[0], p.chunk[0]);
   }
   return p;
 }

@@ -83,6 +83,23 @@ def test_replies_keep_their_shares_beside_a_chunk(grids, replies, most) -> None:
     which a chunk's rows take none of this kind."""
     tiles = (replies + 1) * 8 * 8  # of 16 rows, of sequences of up to 128 rows
     for chunk in (40, 512, 2048, 4096, 8192, 60000, 1 << 20):
-        splits, blocks = plan(grids, replies + 1, replies + chunk, 1, 8, 4, most)[:2]
-        assert splits * blocks >= most // 32
+        splits, blocks, _, _, _, _, total, _ = plan(grids, replies + 1, replies + chunk, 1, 8, 4, most)
+        assert splits * blocks >= most // 32 and total <= 1 << 28
         assert blocks <= 128 or splits > (32 << 20) // (tiles * 2080) * 0.95, (chunk, splits, blocks)
+
+
+def test_parts_of_both_kinds_fit_together(grids) -> None:
+    """256 MiB a call, whichever kinds of rows it may have."""
+    for n_seq in (1, 2, 4, 33, 64, 300, 1000, 65535):
+        for more in (0, 1, 31, 515, 4000, 70000):
+            for heads, group, dim in ((8, 4, 128), (1, 1, 8), (8, 8, 256), (4096, 1, 64), (2, 20, 96)):
+                for most in (64, 4096, 131072, 1 << 30):
+                    n = n_seq + more
+                    if n * heads * group > 1 << 28:
+                        continue
+                    few, _, many, per, floats, slots, total, _ = plan(grids, n_seq, n, 1, heads, group, most, 0, dim)
+                    assert total <= 1 << 28 and few >= 1
+                    # room for every tile that the call may have, by either way of counting them
+                    part = heads * (512 * -(-dim // 32) + 32)
+                    assert floats == part * (per * n_seq if per else slots)
+                    assert per == 0 or per >= min(8, -(-n * group // 16))
