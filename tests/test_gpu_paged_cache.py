@@ -734,3 +734,127 @@ def test_long_replies_beside_a_chunk(gpu, chunk) -> None:
     for most in (None, 3000):
         got = cache.attend(q, table, i32(lengths), starts_of(counts), max_length=most)
         check_attention(cache, q, got, table, lengths, counts)
+
+
+# ---- what a copy, a wider table and 4 bits do to the values
+def test_queries_whose_values_are_not_adjacent(gpu) -> None:
+    """attend makes a copy of such a q: the bits of the call with a contiguous one, of three and of four dimensions."""
+    g = torch.Generator(device="cuda").manual_seed(33)
+    lengths = [100, 77]
+    cache, table = filled(g, 2, lengths, 2, 64, 32)
+    every = rand(g, 2, 6, 4, 64, 2, dt=BF16)[..., 1]
+    turned = rand(g, 2, 6, 64, 4, dt=BF16).transpose(2, 3)
+    for q in (every, turned):
+        assert q.stride(-1) != 1
+        want = cache.attend(q.contiguous(), table, i32(lengths))
+        got = cache.attend(q, table, i32(lengths))
+        assert same(got, want) and got.is_contiguous()
+        assert same(cache.attend(q.flatten(0, 1), table, i32(lengths), starts_of([6, 6])), want.flatten(0, 1))
+        check_attention(cache, q, got, table, lengths, [6, 6])
+
+
+def test_keys_and_values_that_are_not_adjacent(gpu) -> None:
+    g = torch.Generator(device="cuda").manual_seed(34)
+    q, k, v = rand(g, 9, 4, 64, 2), rand(g, 9, 64, 2).transpose(1, 2), rand(g, 9, 2, 128)[..., ::2]
+    q, w, rot = q[..., 0], 1 + 0.2 * rand(g, 128), HipRotary(64)
+    caches = [HipPagedCache(1, 32, 2, 64) for _ in range(2)]
+    out = [c.append(*x, i32([[0]]), i32([9]), rotary=rot, q_weight=y, k_weight=y)
+           for c, x, y in ((caches[0], (q, k, v), w[::2]),
+                           (caches[1], (q.contiguous(), k.contiguous(), v.contiguous()), w[::2].contiguous()))]
+    assert same(*out) and same(caches[0].pages, caches[1].pages) and bool((caches[0].pages != 0).any())
+    assert same(caches[0].read(9, i32([[0]]), i32([9]), dtype=F32)[1], held(v))
+
+
+def test_a_table_that_is_part_of_a_wider_one(gpu) -> None:
+    """Columns from the middle of rows whose other entries name other pages."""
+    g = torch.Generator(device="cuda").manual_seed(35)
+    wide = i32([[5, 0, 2, 4, 4], [5, 1, 3, 4, 5]])
+    table, lengths, counts = wide[:, 1:3], [64, 50], [64, 50]
+    assert table.stride(0) > table.shape[1]
+    caches = [HipPagedCache(6, 32, 2, 64) for _ in range(2)]
+    k, v, q = rand(g, 114, 2, 64), rand(g, 114, 2, 64), rand(g, 114, 4, 64, dt=BF16)
+    for cache, t in zip(caches, (table, table.contiguous())):
+        cache.append(None, k, v, t, i32(lengths), starts_of(counts))
+    assert same(caches[0].pages, caches[1].pages)
+    assert (caches[0].pages[4:] == 0).all() and (caches[0].pages[:4] != 0).any()
+    read = caches[0].read(114, table, i32(lengths), starts_of(counts), dtype=F32)
+    assert same(read[0], held(k)) and same(read[1], held(v))
+    for n in (1, 50):
+        x = q[: 2 * n]
+        got = caches[0].attend(x, table, i32(lengths))
+        assert same(got, caches[1].attend(x, table.contiguous(), i32(lengths)))
+        check_attention(caches[0], x, got, table, lengths, [n, n])
+
+
+def test_against_values_that_were_never_held(gpu) -> None:
+    """Prompts and replies as test_prompt_and_replies_as_a_model_runs_them has them, against attention in 64 bits over the
+    float32 keys and values that were given to the cache.
+
+    A held value is within half a step of its group, s / 2 with s = f16((max - min) / 15), and what the roundings of s and of
+    the minimum leave at the group's ends: 15 |s - (max - min) / 15| and |m - min|, half a step of float16 each (2^-11 of
+    themselves, 2^-25 where subnormal): |dx| <= (max - min) (1/30 + 2^-10) + 2^-11 |min| + 2^-20. With E_t = scale sum |q dk_t|
+    and E the largest of them a probability is off by e^(2 E) - 1 of itself, so that the output is within
+    (e^(2 E) - 1) sum p |v| + e^(2 E) sum p |dv| of attention over what was given, and the kernel's own error besides, for which
+    check_attention's bound on each step is taken with 0.03 of the largest |v|: 2^-8 for the output and e^(2 e) - 1 + 2.1 h for
+    e = scale sum |q k| (h + 66 2^-24) up to 5e-3."""
+    g = torch.Generator(device="cuda").manual_seed(36)
+    hq, hk, dim, page = 8, 2, 64, 32
+    rot = HipRotary(dim, base=500000.0)
+    table, n = a_table(g, 3, 6)
+    cache = HipPagedCache(n, page, hk, dim)
+    qw, kw = (1 + 0.2 * rand(g, dim)).to(BF16), (1 + 0.2 * rand(g, dim)).to(BF16)
+    lengths, given = [0, 0, 0], [([], []) for _ in range(3)]
+    for counts in ([64, 33, 64], [6, 0, 65], [1, 1, 1], [1, 1, 1]):
+        lengths = [a + c for a, c in zip(lengths, counts)]
+        t = sum(counts)
+        qkv = rand(g, t, (hq + 2 * hk) * dim, dt=BF16)
+        q, k, v = (x.unflatten(-1, (-1, dim)) for x in torch.split(qkv, [hq * dim, hk * dim, hk * dim], dim=-1))
+        where = (table, i32(lengths), starts_of(counts))
+        q2 = cache.append(q, k, v, *where, rotary=rot, q_weight=qw, k_weight=kw)
+        got = cache.attend(q2, *where)
+        places = torch.tensor([p for _, p in rows_of(counts, lengths)], device="cuda")
+        turned = rot(k.float(), None, places, q_weight=kw.float())[0]
+        at = 0
+        for b, c in enumerate(counts):
+            if c == 0:
+                continue
+            given[b][0].append(turned[at : at + c]), given[b][1].append(v[at : at + c].float())
+            x, y = (z[at : at + c].double().transpose(0, 1) for z in (q2, got))
+            at += c
+            keys, values = (torch.cat(z) for z in given[b])
+            off = []
+            for z, kept in zip((keys, values), cache.read(lengths[b], table[b : b + 1], i32([lengths[b]]), dtype=F32)):
+                low, high = (f(z.unflatten(-1, (-1, 32)), -1, keepdim=True).expand(-1, -1, -1, 32).flatten(2)
+                             for f in (torch.amin, torch.amax))
+                off.append((kept.double() - z.double()).abs())
+                assert (off[-1] <= (high - low) * (1 / 30 + 2.0 ** -10) + low.abs() * H16 + 2.0 ** -20).all()
+            keys, values, dk, dv = (z.double().repeat_interleave(hq // hk, 1).transpose(0, 1) for z in (keys, values, *off))
+            place = torch.arange(lengths[b] - c, lengths[b], device="cuda")[:, None]
+            seen = torch.arange(lengths[b], device="cuda") <= place
+            scores = (x @ keys.transpose(1, 2) * dim ** -0.5).masked_fill(~seen, -math.inf)
+            p = torch.softmax(scores, -1)
+            e = torch.where(seen, x.abs() @ dk.transpose(1, 2) * dim ** -0.5, 0.0).amax(-1, keepdim=True)
+            own = torch.where(seen, x.abs() @ keys.abs().transpose(1, 2) * dim ** -0.5, 0.0).amax()
+            assert float(own) * (H16 + 66 * E32) < 5e-3
+            bound = (torch.exp(2 * e) - 1) * (p @ values.abs()) + torch.exp(2 * e) * (p @ dv) + 0.03 * values.abs().amax()
+            assert ((y - p @ values).abs() <= bound).all()
+
+
+def test_more_tiles_than_a_grid_takes_one_by_one(gpu) -> None:
+    """With query_starts, so many sequences that the grid is one of every sequence's most; one of them a chunk."""
+    g = torch.Generator(device="cuda").manual_seed(37)
+    b = 60000
+    lengths = torch.randint(1, 60, (b,), generator=torch.Generator().manual_seed(1)).tolist()
+    lengths[b // 2], lengths[b - 2] = 60, 33
+    cache, table = filled(g, b, lengths, 1, 8, 32, width=2)
+    q = rand(g, b, 4, 8, dt=BF16)
+    want = cache.attend(q, table, i32(lengths))
+    assert same(cache.attend(q, table, i32(lengths), torch.arange(b + 1, device="cuda").int()), want)
+    counts = [1] * b
+    counts[5], counts[b // 2], counts[b - 2] = 0, 50, 3
+    q = rand(g, sum(counts), 4, 8, dt=BF16)
+    got = cache.attend(q, table, i32(lengths), starts_of(counts))
+    for s in (0, 5, 6, b // 2 - 1, b // 2, b // 2 + 1, b - 2, b - 1):
+        first = sum(counts[:s])
+        rows = slice(first, first + counts[s])
+        check_attention(cache, q[rows], got[rows], table[s : s + 1], [lengths[s]], [counts[s]])
