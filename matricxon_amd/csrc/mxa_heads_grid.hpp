@@ -31,10 +31,13 @@ inline HeadGrid heads_grid(bool cache, int size, bool interleaved, int qh, int k
   if (cache) {
     // One token a workgroup while that fills the CUs: 256 tokens 8.3 us (four: 9.7), 512 tokens 11.0 (10.3). Key heads then by
     // four (16 tokens, 32 + 8 heads: 6.6 us; eight 8.7, one 6.7 but 29 for 512 tokens); with four tokens sixteen groups, or
-    // thirty-two from 4096 tokens on, when a workgroup's start is shared by more (4096: 30.7 us, 34.1; 1024: 15.1, 13.2).
+    // thirty-two where the call has 80000 groups of keys and more (some five workgroups of sixteen a CU), when a workgroup's
+    // start is shared by more. us of a captured call, sixteen and thirty-two: 32 + 8 heads of 128, 2048 tokens 17.3 and 18.4,
+    // 2500 21.7 and 21.5, 3500 27.5 and 25.1, 8192 49 and 43; 64 + 16 of 64 the same; 16 + 8 of 256, 1024 tokens 14.8 and 15.4,
+    // 1536 21.3 and 19.0, 4096 44.9 and 38.9.
     g.TP = n_tokens > 256 ? 4 : 1;
     const int room = std::max(1, 8192 / (g.TP * 32 * W));  // keys that 32 KB hold
-    g.HK = std::min(std::min(kh, room), g.TP == 1 ? 4 : std::max(1, (n_tokens >= 4096 ? 32 : 16) / W));
+    g.HK = std::min(std::min(kh, room), g.TP == 1 ? 4 : std::max(1, ((long long)n_tokens * kh * W >= 80000 ? 32 : 16) / W));
     g.HQ = g.HK * (qh / kh);
   } else {
     // tokens share what their sines cost; up to 512 the heads of one are spread over workgroups instead

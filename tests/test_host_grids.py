@@ -61,7 +61,7 @@ def test_every_workgroup_of_head_norms_has_a_head(grids, dim, rot, size, interle
 def test_every_workgroup_of_an_append_has_a_key_head(grids, dim, rot, size) -> None:
     """Its LDS within 64 KB, and the query heads of its key heads beside them."""
     out = (ctypes.c_int * 6)()
-    for n in (1, 256, 257, 4095, 4096):
+    for n in (1, 256, 257, 2499, 2500, 4096, 1 << 24):
         for kh in (1, 2, 3, 5, 8, 17, 100, 4096):
             for group in (0, 1, 3, 4, 16):
                 grids.heads(1, size, 0, kh * group, kh, n, dim, rot, out)
