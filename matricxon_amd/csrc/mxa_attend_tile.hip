@@ -8,9 +8,10 @@
 // A tile's packed bytes are copied into a ring of LDS slots by copies that no wave waits for until they are widened, some
 // tiles later.
 //
-// Matrix instructions bound it from below: 2048 tokens of 32 heads of 128 behind 6144 places take 290 us, 830 TFLOP/s, of
-// which they alone would take some 200. A place is widened once for 256 rows (128 rows: 350 us); four slots of copies on
-// their way took 306 us to 290, and two waves of a SIMD a step apart 347 to 306.
+// Matrix instructions bound it from below: 2048 tokens of 32 heads of 128 behind 6144 places take 297 us, 810 TFLOP/s, of
+// which they alone would take some 200. A place is widened once for 256 rows (128 rows: 350 us, beside 290); two waves of a
+// SIMD a step apart took 347 us to 306, and four slots of copies on their way that to 290, measured in one session on a
+// card a little faster.
 #include "mxa_attend.hpp"
 #include "mxa_kernels.hpp"
 

@@ -13,9 +13,9 @@
 // sum of squares crosses lanes. Heads whose rotary part does not split into whole vectors take a wave each, a pair of
 // values at a time.
 //
-// Memory bounds the form without a cache (4096 tokens of 32 + 8 heads of 128, bfloat16: 84 MB in 17.5 us, 5 TB/s), the
-// vector units the one with a cache (26 us, 3.5 TB/s; a division a code and 32-bit indexes took 34), and what waits for what
-// both on few tokens (3.5 us and 6).
+// Memory bounds the form without a cache (4096 tokens of 32 + 8 heads of 128, bfloat16: 84 MB in 16 us of a stream of calls,
+// 5.2 TB/s), the vector units the one with a cache (a launch of 28 us, 3.1 TB/s; a division a code and 32-bit indexes took
+// 34), and what waits for what both on few tokens (3.6 us and 6.8).
 #include "mxa_heads_grid.hpp"
 #include "mxa_kernels.hpp"
 #include "mxa_kv4.hpp"
